@@ -592,6 +592,164 @@ int sf_gemm_frag(const sf_frag_gemm_desc* desc, void* stream);
  * w_dtype are read). */
 int32_t sf_gemm_frag_ss_tiles(const sf_frag_gemm_desc* desc);
 
+/* ---------------------------------------------------------------------------
+ * Projections over 4-bit weights with group scales.
+ *
+ * C[m][n] = act(sum_k A[m][k] * scale[n][k / group] * (code[n][k]
+ * - zero[n][k / group]) + bias[n]): the weight form below the reference's
+ * weight-only int8 (quantization.cu:18-51 ahead of gemm_bias_act,
+ * cuda_backend.cu:337-467), which has no 4-bit form.  Codes are 0..15, group
+ * 32, 64 or 128 inputs, K a multiple of the group, any N, any M.
+ *
+ * sf_w4_pack lays a checkpoint's codes and scales out once, in the order the
+ * matrix operands are read; sf_gemm_w4 reads that.
+ * ------------------------------------------------------------------------- */
+typedef struct sf_w4_pack_desc {
+    int32_t N, K, group;
+    const uint8_t* codes;    /* [N][ldc] bytes: inputs 2 i (low half) and 2 i + 1 (high half) in byte i */
+    int64_t ldc;             /* bytes, >= K / 2 */
+    const void* scales;      /* [N][lds], K / group a row */
+    int64_t lds;
+    int32_t scale_dtype;     /* SF_F16 or SF_BF16, kept bit for bit */
+    const uint8_t* zeros;    /* [N][ldz], one byte a group (0..255), or NULL: 8 */
+    int64_t ldz;
+} sf_w4_pack_desc;
+
+/* Bytes of the packed form (0 for a shape that is not supported). */
+size_t sf_w4_bytes(int32_t N, int32_t K, int32_t group);
+/* out: sf_w4_bytes() bytes, 16-byte aligned. */
+int sf_w4_pack(const sf_w4_pack_desc* desc, void* out, void* stream);
+
+typedef struct sf_gemm_w4_desc {
+    int32_t M, N, K, group;
+    const void* A;           /* [M][lda] bf16 or fp16, rows 16-byte aligned (lda a multiple of 8) */
+    int64_t lda;
+    int32_t a_dtype;
+    const void* W;           /* sf_w4_pack's output for the same N, K, group */
+    int32_t scale_dtype;     /* as packed */
+    const float* bias;       /* [N] or NULL */
+    int32_t act;             /* sf_act */
+    void* C;                 /* [M][ldc] */
+    int64_t ldc;
+    int32_t c_dtype;         /* SF_F32, SF_BF16 or SF_F16 */
+    int32_t accumulate;      /* SF_F32 only: C += act(...) */
+} sf_gemm_w4_desc;
+/* One launch, no workspace.  Codes and activations meet exactly in fp32
+ * accumulators; scale and zero point are applied to each group's sum in fp32.
+ * C must not overlap A. */
+int sf_gemm_w4(const sf_gemm_w4_desc* desc, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * 4-bit key / value cache: head norm + rotation into it, and attention over it.
+ *
+ * Format.  For every batch element, key head, token and group of 64 channels:
+ * mid = bf16((max + min) / 2), a = max |x - mid|, s = (a rounded up to bf16)
+ * / 8, code = clamp(floor((x - mid) / s) + 8, 0, 15); a code stands for
+ * s (code - 7.5) + mid, so |value - x| <= s / 2.  s below 2^-126 counts as 0
+ * (every code then stands for mid); a group with an infinity or a NaN reads
+ * back as NaN, and only that group.  36 bytes for 64 channels of K or V,
+ * against 128 in 16 bits.  The reference caches no keys: it projects them
+ * again on every call (dit_block.cu:288-293).
+ *
+ * data: sf_kv4_bytes(B, H, capacity, D) bytes, 16-byte aligned, D 64 or 128;
+ * it needs no initialisation.  Tokens are written one by one or many at a
+ * time, each into its own bytes: writes to other slots never disturb a token,
+ * so appending needs no order.
+ * ------------------------------------------------------------------------- */
+typedef struct sf_kv4_cache {
+    void* data;
+    int32_t B, H, capacity, D;
+} sf_kv4_cache;
+/* 0 for a shape that is not supported. */
+size_t sf_kv4_bytes(int32_t B, int32_t H, int32_t capacity, int32_t D);
+
+/* Query, key and value heads of B * S tokens: RMSNorm over each query and key
+ * head's D channels (gamma[0], gamma[1]; NULL: none) -- apply_qk_norm,
+ * dit_block.cu:185-196, 262-272 -- then the rotation of their first `rot`
+ * channels by the token's position: channels (i, i + rot / 2), or (2 i,
+ * 2 i + 1) with interleaved, turn by positions[m] * inv_freq[i] radians,
+ * i < rot / 2 (the angle is formed in 64 bits).  rot a multiple of 16, 0 for
+ * none.  Values pass unchanged.  All arithmetic in fp32, one rounding at the
+ * end.
+ *
+ * Section j (0 query, 1 key, 2 value) has heads[j] heads (0: left out), reads
+ * src[j] and writes out[j], both addressed as [B][heads][S][D] through element
+ * strides {b, h, s}, channels contiguous: pointers 16-byte aligned, strides
+ * non-negative multiples of 8.  A projection's output rows are three such
+ * views (h stride D, s stride the row's).  out[j] may be src[j] itself (same
+ * strides and type); otherwise they must not overlap.
+ *
+ * cache.data != NULL: keys and values go into the cache instead of out[1] and
+ * out[2] (heads[1] == heads[2] == cache.H, cache.B == B, cache.D == D), token m
+ * at slot slots[m], or at its position if slots is NULL.  A slot outside
+ * [0, capacity) leaves the cache as it was.  The slots of one batch element
+ * have to differ within a call; two tokens at one slot leave a mixture there,
+ * and only there.
+ * positions, slots: DEVICE [B * S]; positions NULL: token s of each batch
+ * element is at s.  A token with a negative position is padding: nothing of it
+ * is written. */
+typedef struct sf_heads_rope_desc {
+    int32_t B, S, D;
+    int32_t heads[3];
+    int32_t in_dtype, out_dtype;      /* SF_F32, SF_BF16 or SF_F16 */
+    const void* src[3];
+    int64_t src_stride[3][3];
+    void* out[3];
+    int64_t out_stride[3][3];
+    const float* gamma[2];            /* [D] or NULL */
+    float eps;
+    const int32_t* positions;
+    const double* inv_freq;           /* DEVICE [rot / 2] */
+    int32_t rot, interleaved;
+    sf_kv4_cache cache;               /* data NULL: none */
+    const int32_t* slots;             /* only with a cache */
+} sf_heads_rope_desc;
+int sf_heads_rope(const sf_heads_rope_desc* desc, void* stream);
+
+/* The values that cached tokens stand for: k and v [B][H][S][D] through
+ * element strides {b, h, s} (as above) in out_dtype, token (b, s) from slot
+ * slots[b * S + s] (DEVICE; NULL: slot s).  Zeros for a slot outside
+ * [0, capacity). */
+int sf_kv4_read(const sf_kv4_cache* cache, const int32_t* slots, int32_t S, void* k, const int64_t* k_stride, void* v,
+                const int64_t* v_stride, int32_t out_dtype, void* stream);
+
+/* out = softmax(Q K^T scale) V over the cache (IBackend::attention,
+ * backend.h:105-110, on the values that the codes stand for).  Q and out
+ * [B][Hq][Sq][D] through element strides {b, h, s}, channels contiguous,
+ * pointers 16-byte aligned, strides non-negative multiples of 8; Hq a multiple
+ * of cache.H, query head h reads key head h / (Hq / cache.H).
+ * Sk: keys [0, Sk) are read at most (<= cache.capacity).  kv_valid_len: NULL
+ * or DEVICE [B]: keys from there on are not seen (clamped to [0, Sk]).
+ * kv_mask: NULL or DEVICE bytes, [B] rows of Sk kv_mask_stride apart, nonzero
+ * = seen.  is_causal: query s of Sq is the token at valid_len - Sq + s, and
+ * sees the keys up to itself -- one new token, or a chunk behind what is
+ * cached.  (sf_attn_fwd aligns causal rows at the other end, as
+ * attention.cu:117 does.)  A row that sees nothing yields zeros.  Slots that
+ * no row sees may hold anything.
+ * scale 0: 1 / sqrt(D); negative: SF_ENOTSUP.  in_dtype SF_BF16 or SF_F16.
+ * The softmax's maximum and sum are fp32; its weights enter the product with V
+ * as bf16 (hi, lo) pairs, 2^-17 relative.
+ * num_splits: 0 chooses; n > 0 forces n key splits (at most 64). */
+typedef struct sf_attn_kv4_desc {
+    int32_t B, Hq, Sq, Sk;
+    float scale;
+    int32_t in_dtype, out_dtype;
+    int32_t is_causal;
+    int32_t num_splits;
+    const int32_t* kv_valid_len;
+    const uint8_t* kv_mask;
+    int64_t kv_mask_stride;
+    int64_t q_stride[3];
+    int64_t o_stride[3];
+    sf_kv4_cache cache;
+} sf_attn_kv4_desc;
+/* Bytes of device workspace (the splits' partial sums), 0 where none is
+ * needed.  No initialisation; calls that may run concurrently need separate
+ * workspaces. */
+size_t sf_attn_kv4_workspace_bytes(const sf_attn_kv4_desc* desc);
+int sf_attn_kv4(const sf_attn_kv4_desc* desc, const void* q, void* out, void* workspace, size_t workspace_bytes,
+                void* stream);
+
 /* Static text for a status code. */
 const char* sf_strerror(int status);
 

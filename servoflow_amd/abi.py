@@ -170,6 +170,59 @@ class AbsmaxJob(ctypes.Structure):
 SF_ABSMAX_MAX_JOBS = 64
 
 
+class W4PackDesc(ctypes.Structure):
+    """Mirror of `sf_w4_pack_desc`."""
+
+    _fields_ = [("N", ctypes.c_int32), ("K", ctypes.c_int32), ("group", ctypes.c_int32),
+                ("codes", ctypes.c_void_p), ("ldc", ctypes.c_int64),
+                ("scales", ctypes.c_void_p), ("lds", ctypes.c_int64), ("scale_dtype", ctypes.c_int32),
+                ("zeros", ctypes.c_void_p), ("ldz", ctypes.c_int64)]
+
+
+class GemmW4Desc(ctypes.Structure):
+    """Mirror of `sf_gemm_w4_desc`."""
+
+    _fields_ = [("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("group", ctypes.c_int32),
+                ("A", ctypes.c_void_p), ("lda", ctypes.c_int64), ("a_dtype", ctypes.c_int32),
+                ("W", ctypes.c_void_p), ("scale_dtype", ctypes.c_int32),
+                ("bias", ctypes.c_void_p), ("act", ctypes.c_int32),
+                ("C", ctypes.c_void_p), ("ldc", ctypes.c_int64), ("c_dtype", ctypes.c_int32),
+                ("accumulate", ctypes.c_int32)]
+
+
+class Kv4CacheDesc(ctypes.Structure):
+    """Mirror of `sf_kv4_cache`."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("B", ctypes.c_int32), ("H", ctypes.c_int32),
+                ("capacity", ctypes.c_int32), ("D", ctypes.c_int32)]
+
+
+class HeadsRopeDesc(ctypes.Structure):
+    """Mirror of `sf_heads_rope_desc`."""
+
+    _fields_ = [("B", ctypes.c_int32), ("S", ctypes.c_int32), ("D", ctypes.c_int32),
+                ("heads", ctypes.c_int32 * 3),
+                ("in_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
+                ("src", ctypes.c_void_p * 3), ("src_stride", (ctypes.c_int64 * 3) * 3),
+                ("out", ctypes.c_void_p * 3), ("out_stride", (ctypes.c_int64 * 3) * 3),
+                ("gamma", ctypes.c_void_p * 2), ("eps", ctypes.c_float),
+                ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+                ("rot", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("cache", Kv4CacheDesc), ("slots", ctypes.c_void_p)]
+
+
+class AttnKv4Desc(ctypes.Structure):
+    """Mirror of `sf_attn_kv4_desc`."""
+
+    _fields_ = [("B", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Sq", ctypes.c_int32), ("Sk", ctypes.c_int32),
+                ("scale", ctypes.c_float),
+                ("in_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
+                ("is_causal", ctypes.c_int32), ("num_splits", ctypes.c_int32),
+                ("kv_valid_len", ctypes.c_void_p), ("kv_mask", ctypes.c_void_p), ("kv_mask_stride", ctypes.c_int64),
+                ("q_stride", ctypes.c_int64 * 3), ("o_stride", ctypes.c_int64 * 3),
+                ("cache", Kv4CacheDesc)]
+
+
 class SfError(RuntimeError):
     def __init__(self, status: int, what: str):
         super().__init__(f"{what}: {strerror(status)} (status {status})")
@@ -246,6 +299,23 @@ def lib() -> ctypes.CDLL:
     L.sf_bf16_to_f16_below.restype = ctypes.c_int
     L.sf_gemm_set_algo_timing.argtypes = [i32]
     L.sf_gemm_set_algo_timing.restype = ctypes.c_int
+    L.sf_w4_bytes.argtypes = [i32, i32, i32]
+    L.sf_w4_bytes.restype = ctypes.c_size_t
+    L.sf_w4_pack.argtypes = [ctypes.POINTER(W4PackDesc), vp, vp]
+    L.sf_w4_pack.restype = ctypes.c_int
+    L.sf_gemm_w4.argtypes = [ctypes.POINTER(GemmW4Desc), vp]
+    L.sf_gemm_w4.restype = ctypes.c_int
+    L.sf_kv4_bytes.argtypes = [i32, i32, i32, i32]
+    L.sf_kv4_bytes.restype = ctypes.c_size_t
+    L.sf_heads_rope.argtypes = [ctypes.POINTER(HeadsRopeDesc), vp]
+    L.sf_heads_rope.restype = ctypes.c_int
+    L.sf_kv4_read.argtypes = [ctypes.POINTER(Kv4CacheDesc), vp, i32, vp, ctypes.POINTER(i64), vp,
+                              ctypes.POINTER(i64), i32, vp]
+    L.sf_kv4_read.restype = ctypes.c_int
+    L.sf_attn_kv4_workspace_bytes.argtypes = [ctypes.POINTER(AttnKv4Desc)]
+    L.sf_attn_kv4_workspace_bytes.restype = ctypes.c_size_t
+    L.sf_attn_kv4.argtypes = [ctypes.POINTER(AttnKv4Desc), vp, vp, vp, ctypes.c_size_t, vp]
+    L.sf_attn_kv4.restype = ctypes.c_int
     L.sf_strerror.argtypes = [ctypes.c_int]
     L.sf_strerror.restype = ctypes.c_char_p
     _lib = L

@@ -1,4 +1,5 @@
-"""Torch-tensor front end for `sf_attn_fwd` (tests and bench plumbing).
+"""Torch-tensor front ends for `sf_attn_fwd` and for the 4-bit key / value
+cache with `sf_attn_kv4` (tests and bench plumbing).
 
 torch supplies device memory and the current HIP stream; the arithmetic runs
 in libsf_hip_kernels.so.  Mirrors IBackend::attention
@@ -12,7 +13,7 @@ import ctypes
 
 import torch
 
-from . import abi
+from . import abi, kernels
 
 _DT = {torch.bfloat16: abi.SF_BF16, torch.float32: abi.SF_F32, torch.float16: abi.SF_F16}
 
@@ -101,4 +102,92 @@ def attention(q, k, v, out=None, scale=0.0, is_causal=False, valid_len=None, num
     st = abi.lib().sf_attn_fwd(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                out.data_ptr(), ws_ptr, ws_n, s.cuda_stream)
     abi.check(st, "sf_attn_fwd")
+    return out
+
+
+class Kv4Cache:
+    """Keys and values of B batch elements, H heads of D channels (64 or 128)
+    and up to `capacity` tokens in 4 bits (sf_kv4_cache)."""
+
+    def __init__(self, B, H, capacity, D, device="cuda"):
+        n = abi.lib().sf_kv4_bytes(B, H, capacity, D)
+        if n == 0:
+            raise ValueError(f"no cache of B {B}, H {H}, capacity {capacity}, D {D}: positive sizes, D 64 or 128")
+        self.B, self.H, self.capacity, self.D = B, H, capacity, D
+        self.data = torch.empty(n, dtype=torch.uint8, device=device)   # needs no init
+
+    def desc(self):
+        c = abi.Kv4CacheDesc()
+        c.data, c.B, c.H, c.capacity, c.D = self.data.data_ptr(), self.B, self.H, self.capacity, self.D
+        return c
+
+    def write(self, k, v, slots=None):
+        """Tokens k, v [B, H, S, D] into slots (int32 [B, S], one outside
+        [0, capacity) is left out; None: 0 .. S - 1)."""
+        kernels.heads_rope_strided((None, k, v), (None, None, None), cache=self, slots=slots)
+
+    def read(self, slots=None, dtype=torch.bfloat16):
+        """(k, v) [B, H, S, D]: the values of the tokens in slots (int32
+        [B, S]; None: all of them), zeros for a slot outside [0, capacity)."""
+        S = self.capacity
+        if slots is not None:
+            if slots.dtype != torch.int32 or slots.dim() != 2 or slots.shape[0] != self.B or \
+                    not slots.is_contiguous() or slots.device != self.data.device:
+                raise ValueError(f"slots must be a contiguous int32 [{self.B}, S] on {self.data.device}")
+            S = slots.shape[1]
+        k, v = (torch.empty(self.B, self.H, S, self.D, dtype=dtype, device=self.data.device) for _ in range(2))
+        st = (ctypes.c_int64 * 3)(*k.stride()[:3])
+        with torch.cuda.device(self.data.device):
+            s = abi.lib().sf_kv4_read(ctypes.byref(self.desc()), slots.data_ptr() if slots is not None else None, S,
+                                      k.data_ptr(), st, v.data_ptr(), st, _DT[dtype],
+                                      torch.cuda.current_stream().cuda_stream)
+        abi.check(s, "sf_kv4_read")
+        return k, v
+
+
+def attention_kv4(q, cache, out=None, scale=0.0, is_causal=False, valid_len=None, kv_mask=None, keys=None,
+                  num_splits=0, out_dtype=None, workspace=None):
+    """softmax(q K^T scale) V over a Kv4Cache: q [B, Hq, Sq, D] bf16 or fp16
+    (any strides with a contiguous last axis), Hq a multiple of the cache's H.
+    keys: how many slots are read at most (the capacity); valid_len: device
+    int32 [B] lengths; kv_mask: device bool [B, keys] (True = attend);
+    is_causal: query s is the token at valid_len - Sq + s.  Runs on torch's
+    current stream; a row that sees nothing is zeros."""
+    if q.dim() != 4 or q.shape[0] != cache.B or q.shape[3] != cache.D or q.shape[1] % cache.H:
+        raise ValueError(f"q{tuple(q.shape)} over a cache of B {cache.B}, H {cache.H}, D {cache.D}")
+    if q.device != cache.data.device or q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"q must be bfloat16 or float16 on {cache.data.device}")
+    B, Hq, Sq, D = q.shape
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+    if out.shape != q.shape or out.device != q.device or out.dtype not in _DT or \
+            (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f"out{tuple(out.shape)} {out.dtype} for q{tuple(q.shape)}")
+    d = abi.AttnKv4Desc()
+    d.B, d.Hq, d.Sq, d.Sk = B, Hq, Sq, cache.capacity if keys is None else int(keys)
+    d.scale, d.in_dtype, d.out_dtype = float(scale), _DT[q.dtype], _DT[out.dtype]
+    d.is_causal, d.num_splits = 1 if is_causal else 0, int(num_splits)
+    if valid_len is not None:
+        if valid_len.dtype != torch.int32 or valid_len.numel() != B or not valid_len.is_contiguous() or \
+                valid_len.device != q.device:
+            raise ValueError("valid_len must be a device int32 tensor of B elements")
+        d.kv_valid_len = valid_len.data_ptr()
+    if kv_mask is not None:
+        if kv_mask.dtype not in (torch.bool, torch.uint8) or kv_mask.shape != (B, d.Sk) or \
+                (d.Sk > 1 and kv_mask.stride(1) != 1) or kv_mask.device != q.device:
+            raise ValueError(f"kv_mask must be a device bool/uint8 tensor [{B}, {d.Sk}] with contiguous rows")
+        d.kv_mask, d.kv_mask_stride = kv_mask.data_ptr(), kv_mask.stride(0) if B > 1 else 0
+    for name, t in (("q", q), ("out", out)):
+        if t.shape[3] > 1 and t.stride(3) != 1:
+            raise ValueError(f"{name} must have a contiguous last axis")
+    d.q_stride[:], d.o_stride[:] = kernels._strides_bhs(q), kernels._strides_bhs(out)
+    d.cache = cache.desc()
+    with torch.cuda.device(q.device):
+        need = int(abi.lib().sf_attn_kv4_workspace_bytes(ctypes.byref(d)))
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)   # needs no init
+        ws, n = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
+        st = abi.lib().sf_attn_kv4(ctypes.byref(d), q.data_ptr(), out.data_ptr(), ws, n,
+                                   torch.cuda.current_stream().cuda_stream)
+    abi.check(st, "sf_attn_kv4")
     return out

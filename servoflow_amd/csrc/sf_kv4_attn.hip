@@ -1,0 +1,506 @@
+// Attention over the 4-bit key / value cache (gfx950).
+//
+// A cached value is s (c - 7.5) + mid with s and mid of its token, head and
+// 64-channel group, so both contractions run on the codes themselves and the
+// parameters meet the scores in fp32:
+//   S_j = s_j sum_d q_d (16 + c_jd) + (mid_j - 23.5 s_j) sum_d q_d
+//   O_d = sum_j p_j s_j (16 + c_jd) - 23.5 sum_j p_j s_j + sum_j p_j mid_j
+// (16 + c: see sf_nibble.h).  p_j s_j enters the matrix unit as a bf16 (hi, lo)
+// pair, 2^-17 relative, and sum_j p_j s_j is taken over the same rounded pair
+// by an operand of ones, so the offset of 23.5 cancels exactly what the codes'
+// offset added.
+//
+// One wave takes blocks of 32 tokens against QT tiles of 16 query rows; query
+// heads that share a key head are rows of one tile, so a cached token is read
+// and unpacked once for all of them.  S^T = K Q^T puts a row's scores in the
+// lanes that the second product wants them in as P^T (the cache's value order,
+// sf_kv4.h): nothing passes through LDS inside the loop.  The running maximum
+// moves only when a score exceeds it by 2^8: p stays below 2^8, far inside
+// bf16 and fp32, and the common block has neither a cross-lane maximum nor a
+// rescale.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "sf_device.h"
+#include "sf_hip.h"
+#include "sf_kv4.h"
+#include "sf_nibble.h"
+
+namespace sfk {
+
+constexpr int kKvWaves = 4;
+constexpr int kKvMaxSplits = 64;
+constexpr float kKvSlack = 8.f;       // log2
+constexpr float kKvNoMax = -1e30f;    // a row that has seen nothing
+
+struct KvAttnArgs {
+    const uint16_t* q;
+    const uint8_t* cache;
+    void* out;
+    float* part;          // [splits][rows][D + 2], rows = B * Hq * Sq: O, then max and sum
+    const int32_t* valid;
+    const uint8_t* mask;
+    int64_t mask_stride, cache_blocks;
+    int64_t qs[3], os[3];
+    int64_t rows;
+    int B, H, G, Sq, Sk, splits, qgroups, causal, out_kind;
+    float scale_log2;
+};
+
+// Four channels to out: kind 0 fp32, 1 bf16, 2 fp16.
+__device__ __forceinline__ void kv_store4(void* out, int64_t at, int kind, f32x4 o) {
+    if (kind == 0) *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = o;
+    else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) =
+            kind == 1 ? uint2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])}
+                      : uint2{pack_f16x2_rn(o[0], o[1]), pack_f16x2_rn(o[2], o[3])};
+}
+
+__device__ __forceinline__ float lanes4_sum(float x) {   // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+__device__ __forceinline__ float lanes4_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+
+// What a wave holds of a block of 32 tokens.
+template <int D>
+struct KvBlock {
+    static constexpr int G = D / 64;
+    u32x4 k[G], v[G];                       // codes
+    u32x4 kp[G][2], vp[G][2];               // parameters of tokens 4 g .. + 3 and 16 + 4 g .. + 3
+    __device__ __forceinline__ void load(const uint8_t* blk, int lane) {
+        const int g = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            k[i] = *reinterpret_cast<const u32x4*>(blk + i * 1024 + lane * 16);
+            v[i] = *reinterpret_cast<const u32x4*>(blk + Kv4<D>::kV + i * 1024 + lane * 16);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                kp[i][t] = *reinterpret_cast<const u32x4*>(blk + Kv4<D>::key_par(16 * t + 4 * g, i));
+                vp[i][t] = *reinterpret_cast<const u32x4*>(blk + Kv4<D>::value_par(16 * t + 4 * g, i));
+            }
+        }
+    }
+    // Key code dword of tile t, group i, step ks.
+    __device__ __forceinline__ uint32_t key(int t, int i, int ks) const {
+        return D == 64 ? k[0][2 * t + ks] : k[t][2 * i + ks];
+    }
+};
+
+template <bool F16, int D, int QT>
+__global__ __launch_bounds__(64 * kKvWaves) void attn_kv4_kernel(const KvAttnArgs p) {
+    constexpr int GR = D / 64, DT = D / 16;   // 64-channel groups, tiles of 16 channels
+    constexpr int kRow = DT * 4;              // floats of O per lane and tile
+    __shared__ float xm[kKvWaves][QT][16], xl[kKvWaves][QT][16];
+    __shared__ float xo[2][QT * kRow][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, g = lane >> 4;
+    const int split = blockIdx.x % p.splits;
+    const int qg = (blockIdx.x / p.splits) % p.qgroups;
+    const int bh = blockIdx.x / p.splits / p.qgroups;
+    const int b = bh / p.H, h = bh % p.H;
+    const int R = p.G * p.Sq, q0 = qg * 16 * QT;
+
+    const int len = p.valid ? min(max(p.valid[b], 0), p.Sk) : p.Sk;
+    // Query s sees keys below len - Sq + s + 1 (causal) or len; the smallest and largest limit of the group's rows.
+    int lim_lo = len, lim_hi = len;
+    if (p.causal) {
+        const int q1 = min(q0 + 16 * QT, R) - 1;
+        const bool one = q0 / p.Sq == q1 / p.Sq;
+        lim_lo = len - p.Sq + 1 + (one ? q0 % p.Sq : 0);
+        lim_hi = len - p.Sq + 1 + (one ? q1 % p.Sq : p.Sq - 1);
+    }
+    const int nblk = (max(lim_hi, 0) + kKvBlock - 1) / kKvBlock;
+    const int b0 = (int)((int64_t)nblk * split / p.splits), b1 = (int)((int64_t)nblk * (split + 1) / p.splits);
+
+    u32x4 q[QT][GR][2];
+    float qs[QT][GR];
+    int limit[QT];
+    int64_t qrow[QT];   // the row's place in [B][Hq][Sq]
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int r = min(q0 + 16 * t + col, R - 1);
+        const int hq = h * p.G + r / p.Sq, s = r % p.Sq;
+        const uint16_t* src = p.q + b * p.qs[0] + hq * p.qs[1] + s * p.qs[2];
+        qrow[t] = ((int64_t)b * p.H * p.G + hq) * p.Sq + s;
+        limit[t] = p.causal ? len - p.Sq + 1 + s : len;
+#pragma unroll
+        for (int i = 0; i < GR; ++i) {
+            float sum = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                q[t][i][ks] = *reinterpret_cast<const u32x4*>(src + 64 * i + 16 * g + 8 * ks);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t u = q[t][i][ks][e];
+                    sum += F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)u) +
+                                     (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16))
+                               : __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
+                }
+            }
+            qs[t][i] = lanes4_sum(sum);
+        }
+    }
+
+    f32x4 o[QT][DT], one[QT][GR];   // O^T without the parameters' part; sum of the rounded p s
+    float m[QT], l[QT], pm[QT][GR];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        m[t] = kKvNoMax, l[t] = 0.f;
+#pragma unroll
+        for (int i = 0; i < GR; ++i) pm[t][i] = 0.f, one[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    const uint8_t* base = p.cache + (int64_t)bh * p.cache_blocks * Kv4<D>::kBytes;
+
+    KvBlock<D> nx;
+    if (b0 + wave < b1) nx.load(base + (int64_t)(b0 + wave) * Kv4<D>::kBytes, lane);
+    for (int blk = b0 + wave; blk < b1; blk += kKvWaves) {
+        const KvBlock<D> kv = nx;
+        if (blk + kKvWaves < b1) nx.load(base + (int64_t)(blk + kKvWaves) * Kv4<D>::kBytes, lane);
+        const int key0 = kKvBlock * blk;
+        const bool masked = p.mask || key0 + kKvBlock > lim_lo;
+        float ks[GR][8], ko[GR][8], vs[GR][8], vm[GR][8];
+        uint32_t see = 0xffu;   // the lane's 8 tokens, by length and mask
+        if (masked) {
+            see = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int key = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
+                if (key < len && (!p.mask || p.mask[b * p.mask_stride + key])) see |= 1u << e;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < GR; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                uint32_t kp = kv.kp[i][e >> 2][e & 3], vp = kv.vp[i][e >> 2][e & 3];
+                if (masked && !(see >> e & 1u)) kp = vp = 0u;   // tokens behind the last hold anything
+                ks[i][e] = __uint_as_float(kp << 16) * p.scale_log2;
+                ko[i][e] = __uint_as_float(kp & 0xffff0000u) * p.scale_log2 - 23.5f * ks[i][e];
+                vs[i][e] = __uint_as_float(vp << 16);
+                vm[i][e] = __uint_as_float(vp & 0xffff0000u);
+            }
+        u32x4 ka[2][GR][2], va[DT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < GR; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) ka[t][i][k] = nibbles_plus16<F16>(kv.key(t, i, k));
+#pragma unroll
+        for (int t = 0; t < DT / 2; ++t) {
+            const uint32_t w0 = kv.v[t >> 1][2 * (t & 1)], w1 = kv.v[t >> 1][2 * (t & 1) + 1];
+            va[2 * t] = u32x4{nibble_pair_plus16<false, 0>(w0), nibble_pair_plus16<false, 2>(w0),
+                              nibble_pair_plus16<false, 0>(w1), nibble_pair_plus16<false, 2>(w1)};
+            va[2 * t + 1] = u32x4{nibble_pair_plus16<false, 1>(w0), nibble_pair_plus16<false, 3>(w0),
+                                  nibble_pair_plus16<false, 1>(w1), nibble_pair_plus16<false, 3>(w1)};
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < GR; ++i)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+                    s = mfma_16b<F16>(ka[kt][i][0], q[t][i][0], s);
+                    s = mfma_16b<F16>(ka[kt][i][1], q[t][i][1], s);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x[4 * kt + e] = __builtin_fmaf(
+                            ks[i][4 * kt + e], s[e], __builtin_fmaf(ko[i][4 * kt + e], qs[t][i], x[4 * kt + e]));
+                }
+            uint32_t row = see;
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) >= limit[t]) row &= ~(1u << e);
+                    if (!(row >> e & 1u)) x[e] = -INFINITY;
+                }
+            }
+            const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            if (__any(mx > m[t] + kKvSlack)) {
+                const float nm = fmaxf(m[t], lanes4_max(mx)), al = __builtin_amdgcn_exp2f(m[t] - nm);
+                m[t] = nm;
+                l[t] *= al;
+#pragma unroll
+                for (int i = 0; i < GR; ++i) pm[t][i] *= al, one[t][i] *= al;
+#pragma unroll
+                for (int i = 0; i < DT; ++i) o[t][i] *= al;
+            }
+            float pr[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                pr[e] = __builtin_amdgcn_exp2f(x[e] - m[t]);
+                l[t] += pr[e];
+            }
+#pragma unroll
+            for (int i = 0; i < GR; ++i) {
+                u32x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float a = pr[2 * e] * vs[i][2 * e], c = pr[2 * e + 1] * vs[i][2 * e + 1];
+                    float ma = pr[2 * e] * vm[i][2 * e], mc = pr[2 * e + 1] * vm[i][2 * e + 1];
+                    if (masked) {   // a token only later rows see may hold NaN parameters
+                        if (!(row >> (2 * e) & 1u)) a = ma = 0.f;
+                        if (!(row >> (2 * e + 1) & 1u)) c = mc = 0.f;
+                    }
+                    pm[t][i] += ma + mc;
+                    hi[e] = pack_bf16x2(a, c);
+                    lo[e] = pack_bf16x2(a - __uint_as_float(hi[e] << 16), c - __uint_as_float(hi[e] & 0xffff0000u));
+                }
+                one[t][i] = mfma_16b<false>(ones, hi, one[t][i]);
+                one[t][i] = mfma_16b<false>(ones, lo, one[t][i]);
+#pragma unroll
+                for (int d = 4 * i; d < 4 * i + 4; ++d) {
+                    o[t][d] = mfma_16b<false>(va[d], hi, o[t][d]);
+                    o[t][d] = mfma_16b<false>(va[d], lo, o[t][d]);
+                }
+            }
+        }
+    }
+
+    // The waves' rows meet: common maximum, then two rounds of adds through LDS.
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        l[t] = lanes4_sum(l[t]);
+#pragma unroll
+        for (int i = 0; i < GR; ++i) {
+            const float add = lanes4_sum(pm[t][i]) - 23.5f * one[t][i][0];
+#pragma unroll
+            for (int d = 4 * i; d < 4 * i + 4; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[t][d][e] += add;
+        }
+        if (g == 0) xm[wave][t][col] = m[t];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        float mm = xm[0][t][col];
+#pragma unroll
+        for (int w = 1; w < kKvWaves; ++w) mm = fmaxf(mm, xm[w][t][col]);
+        const float al = __builtin_amdgcn_exp2f(m[t] - mm);
+        m[t] = mm;
+        l[t] *= al;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[t][d] *= al;
+        if (g == 0) xl[wave][t][col] = l[t];
+        if (wave >= 2) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) xo[wave - 2][t * kRow + 4 * d + e][lane] = o[t][d][e];
+        }
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[t][d][e] += xo[wave][t * kRow + 4 * d + e][lane];
+    }
+    __syncthreads();
+    if (wave == 1) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) xo[0][t * kRow + 4 * d + e][lane] = o[t][d][e];
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        if (q0 + 16 * t + col >= R) continue;
+        const float sum = xl[0][t][col] + xl[1][t][col] + xl[2][t][col] + xl[3][t][col];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][d][e] += xo[0][t * kRow + 4 * d + e][lane];
+        if (p.splits > 1) {
+            float* dst = p.part + ((int64_t)split * p.rows + qrow[t]) * (D + 2);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dst[16 * d + 4 * g + e] = o[t][d][e];
+            if (g == 0) dst[D] = m[t], dst[D + 1] = sum;
+            continue;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
+        const int r = q0 + 16 * t + col;
+        const int64_t at = b * p.os[0] + (h * p.G + r / p.Sq) * p.os[1] + r % p.Sq * p.os[2];
+#pragma unroll
+        for (int d = 0; d < DT; ++d) kv_store4(p.out, at + 16 * d + 4 * g, p.out_kind, o[t][d] * inv);
+    }
+}
+
+// out = sum_splits O 2^(m - M) / sum_splits l 2^(m - M), one wave per row.
+template <int D>
+__global__ __launch_bounds__(256) void attn_kv4_merge_kernel(const KvAttnArgs p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= p.rows) return;
+    const float* src = p.part + row * (D + 2);
+    const int64_t step = p.rows * (D + 2);
+    float m = kKvNoMax, l = 0.f;
+    if (lane < p.splits) m = src[lane * step + D], l = src[lane * step + D + 1];
+    float mm = m;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
+    const float w = __builtin_amdgcn_exp2f(m - mm);
+    float sum = l * w;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    constexpr int E = D / 64;
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+        const float ws = __shfl(w, s, 64);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += ws * src[s * step + 64 * e + lane];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int s = (int)(row % p.Sq);
+    const int64_t bh = row / p.Sq, Hq = (int64_t)p.H * p.G;
+    const int64_t at = bh / Hq * p.os[0] + bh % Hq * p.os[1] + s * p.os[2];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float y = acc[e] * inv;
+        const int64_t i = at + 64 * e + lane;
+        if (p.out_kind == 0) static_cast<float*>(p.out)[i] = y;
+        else if (p.out_kind == 1) static_cast<uint16_t*>(p.out)[i] = (uint16_t)f32_to_bf16_bits(y);
+        else static_cast<_Float16*>(p.out)[i] = (_Float16)y;
+    }
+}
+
+// Tiles of 16 query rows a workgroup takes, of those the kernel is built for:
+// the fewest passes over the keys first, then the fewest idle rows.
+static int kv_tiles(int rows) {
+    const int tiles = (rows + 15) / 16;
+    const int most = 2;
+    const int per = (tiles + (tiles + most - 1) / most - 1) / ((tiles + most - 1) / most);
+    return per;
+}
+
+struct KvPlan {
+    int qt, qgroups, splits;
+    int64_t wgs, rows;
+};
+
+static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
+    KvPlan k;
+    const int R = d->Hq / d->cache.H * d->Sq;
+    k.qt = kv_tiles(R);
+    k.qgroups = (R + 16 * k.qt - 1) / (16 * k.qt);
+    k.rows = (int64_t)d->B * d->Hq * d->Sq;
+    const int64_t base = (int64_t)d->B * d->cache.H * k.qgroups;
+    if (d->num_splits > 0) {
+        k.splits = d->num_splits;
+    } else {
+        // about two workgroups a CU, and at least two blocks a wave
+        const int64_t want = (512 + base - 1) / base, most = (d->Sk + 255) / 256;
+        k.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kKvMaxSplits}));
+    }
+    k.wgs = base * k.splits;
+    return k;
+}
+
+static int kv_attn_check(const sf_attn_kv4_desc* d) {
+    if (!d || d->B < 0 || d->Hq < 0 || d->Sq < 0 || d->Sk < 0 || d->cache.B <= 0 || d->cache.H <= 0 ||
+        d->cache.capacity <= 0)
+        return SF_EINVAL;
+    if (d->cache.D != 64 && d->cache.D != 128) return SF_ENOTSUP;
+    if (d->Hq % d->cache.H || d->B != d->cache.B || d->Sk > d->cache.capacity) return SF_EINVAL;
+    if (d->num_splits < 0 || d->num_splits > kKvMaxSplits) return SF_EINVAL;
+    if ((int64_t)d->Hq / d->cache.H * d->Sq > 0x7fffff00LL) return SF_ENOTSUP;
+    return SF_OK;
+}
+
+}  // namespace sfk
+
+extern "C" size_t sf_attn_kv4_workspace_bytes(const sf_attn_kv4_desc* d) {
+    if (sfk::kv_attn_check(d) != SF_OK || !d->B || !d->Hq || !d->Sq) return 0;
+    const sfk::KvPlan k = sfk::kv_plan(d);
+    return k.splits > 1 ? (size_t)k.splits * (size_t)k.rows * (d->cache.D + 2) * sizeof(float) : 0;
+}
+
+extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+    const int st = sfk::kv_attn_check(d);
+    if (st != SF_OK) return st;
+    if (!d->B || !d->Hq || !d->Sq) return SF_OK;
+    if (d->in_dtype != SF_BF16 && d->in_dtype != SF_F16) return SF_ENOTSUP;
+    if (d->out_dtype != SF_BF16 && d->out_dtype != SF_F16 && d->out_dtype != SF_F32) return SF_ENOTSUP;
+    if (d->scale < 0.f) return SF_ENOTSUP;
+    if (!q || !out || !d->cache.data) return SF_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(d->cache.data)) & 15)
+        return SF_EINVAL;
+    for (int i = 0; i < 3; ++i)
+        if (d->q_stride[i] < 0 || (d->q_stride[i] & 7) || d->o_stride[i] < 0 || (d->o_stride[i] & 7)) return SF_EINVAL;
+    if (d->kv_mask && d->kv_mask_stride < 0) return SF_EINVAL;
+    const sfk::KvPlan k = sfk::kv_plan(d);
+    if (k.wgs > 0x7fffffffLL || (k.rows + 3) / 4 > 0x7fffffffLL) return SF_ENOTSUP;
+    if (k.splits > 1 && (!workspace || workspace_bytes < sf_attn_kv4_workspace_bytes(d))) return SF_EWORKSPACE;
+    if (k.splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 3)) return SF_EINVAL;
+    sfk::KvAttnArgs p = {};
+    p.q = static_cast<const uint16_t*>(q);
+    p.cache = static_cast<const uint8_t*>(d->cache.data);
+    p.out = out;
+    p.part = static_cast<float*>(workspace);
+    p.valid = d->kv_valid_len;
+    p.mask = d->kv_mask;
+    p.mask_stride = d->kv_mask_stride;
+    p.cache_blocks = sfk::kv4_blocks(d->cache.capacity);
+    for (int i = 0; i < 3; ++i) p.qs[i] = d->q_stride[i], p.os[i] = d->o_stride[i];
+    p.rows = k.rows;
+    p.B = d->B;
+    p.H = d->cache.H;
+    p.G = d->Hq / d->cache.H;
+    p.Sq = d->Sq;
+    p.Sk = d->Sk;
+    p.splits = k.splits;
+    p.qgroups = k.qgroups;
+    p.causal = d->is_causal != 0;
+    p.out_kind = d->out_dtype == SF_BF16 ? 1 : (d->out_dtype == SF_F16 ? 2 : 0);
+    p.scale_log2 = (d->scale == 0.f ? 1.f / sqrtf((float)d->cache.D) : d->scale) * 1.4426950408889634f;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const dim3 grid((unsigned)k.wgs), block(64 * sfk::kKvWaves);
+    const bool f16 = d->in_dtype == SF_F16;
+#define SF_KV4_LAUNCH(DD, QT)                                                                       \
+    do {                                                                                            \
+        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT>), grid, block, 0, s, p);    \
+        else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT>), grid, block, 0, s, p);       \
+    } while (0)
+    if (d->cache.D == 64) {
+        if (k.qt == 1) SF_KV4_LAUNCH(64, 1);
+        else SF_KV4_LAUNCH(64, 2);
+    } else {
+        if (k.qt == 1) SF_KV4_LAUNCH(128, 1);
+        else SF_KV4_LAUNCH(128, 2);
+    }
+#undef SF_KV4_LAUNCH
+    if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
+    if (k.splits > 1) {
+        const dim3 mg((unsigned)((k.rows + 3) / 4));
+        if (d->cache.D == 64) hipLaunchKernelGGL(sfk::attn_kv4_merge_kernel<64>, mg, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL(sfk::attn_kv4_merge_kernel<128>, mg, dim3(256), 0, s, p);
+        if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
+    }
+    return SF_OK;
+}

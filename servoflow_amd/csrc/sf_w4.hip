@@ -1,0 +1,261 @@
+// Projections over 4-bit weights with group scales (gfx950).
+//
+// C[m][n] = act(sum_k A[m][k] s[n][k / g] (c[n][k] - z[n][k / g]) + bias[n]),
+// codes c in 0..15.  A code goes into a 16-bit matrix operand without an
+// arithmetic conversion: its four bits are placed at the top of the mantissa
+// of 16.0, which makes the operand 16 + c exactly (bf16 0x4180 | c << 3, fp16
+// 0x4C00 | c << 6), two codes for one shift and one and-or.  The products with
+// A are exact in the fp32 accumulator, and a group ends with
+//   acc += s (sum_k (16 + c) A - (16 + z) sum_k A),
+// sum_k A of the group from one more matrix product with an operand of ones.
+// Scale and zero point never round to 16 bits; the offset of 16 costs the
+// accumulator about two bits (the sums are of 16..31 instead of -8..7).
+//
+// Layout (sf_w4_pack): blocks of 16 rows x 128 columns, 1 KB each, lane
+// l = 16 g + r of a wave holding row r's codes k = 32 j + 8 g + e in dword j,
+// code e at nibble (e >> 1) + 4 (e & 1): one 16-byte load per lane is the
+// operand of four v_mfma_f32_16x16x32.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "sf_act.h"
+#include "sf_device.h"
+#include "sf_hip.h"
+#include "sf_nibble.h"
+
+namespace sfk {
+
+struct W4Args {
+    const uint16_t* a;     // [M][lda]
+    int64_t lda;
+    const uint8_t* w;      // packed codes, then params
+    const uint32_t* par;   // [N16][groups][16]: scale bits << 16 | zero
+    const float* bias;
+    void* c;
+    int64_t ldc;
+    int M, N, K, KB, groups, n16;
+    int scale_f16, act, c_kind, accumulate;
+};
+
+__device__ __forceinline__ float w4_scale(uint32_t u, int f16) {
+    return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16)) : __uint_as_float(u & 0xffff0000u);
+}
+
+// One workgroup: 16 NT columns of C (rows of W) x 16 MB rows, K blocks of 128
+// dealt to its WK waves, whose sums meet in LDS.
+template <bool F16, int MB, int NT, int WK, int GROUP>
+__global__ __launch_bounds__(64 * WK) void gemm_w4_kernel(const W4Args p) {
+    constexpr int kSteps = GROUP / 32, kGroups = 4 / kSteps;   // per block of 128
+    __shared__ f32x4 red[WK][MB * NT][64];
+    const int lane = threadIdx.x & 63, wk = threadIdx.x >> 6;
+    const int r = lane & 15, g = lane >> 4;
+    const int nb0 = blockIdx.x * NT;
+    const int m0 = blockIdx.y * 16 * MB;
+
+    const uint16_t* arow[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) arow[b] = p.a + (int64_t)min(m0 + 16 * b + r, p.M - 1) * p.lda + 8 * g;
+    f32x4 acc[NT][MB];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const u32x4 ones = F16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
+                           : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    for (int kb = wk; kb < p.KB; kb += WK) {
+        u32x4 x[MB][4], code[NT], par[NT][kGroups];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int nb = min(nb0 + t, p.n16 - 1);
+            code[t] = *reinterpret_cast<const u32x4*>(p.w + ((int64_t)nb * p.KB + kb) * 1024 + 16 * lane);
+#pragma unroll
+            for (int q = 0; q < kGroups; ++q)
+                par[t][q] = *reinterpret_cast<const u32x4*>(
+                    p.par + ((int64_t)nb * p.groups + kb * kGroups + q) * 16 + 4 * g);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = 128 * kb + 32 * j;   // K is a multiple of 32: a step is inside or outside as a whole
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+                x[b][j] = k < p.K ? *reinterpret_cast<const u32x4*>(arow[b] + k) : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) {
+            f32x4 sx[MB], pr[NT][MB];
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+                sx[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) pr[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int j = q * kSteps; j < (q + 1) * kSteps; ++j) {
+#pragma unroll
+                for (int b = 0; b < MB; ++b) sx[b] = mfma_16b<F16>(ones, x[b][j], sx[b]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const u32x4 w = nibbles_plus16<F16>(code[t][j]);
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) pr[t][b] = mfma_16b<F16>(w, x[b][j], pr[t][b]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float s = w4_scale(par[t][q][i], p.scale_f16);
+                    const float z = -s * (16.f + (float)(par[t][q][i] & 0xffu));
+#pragma unroll
+                    for (int b = 0; b < MB; ++b)
+                        acc[t][b][i] = __builtin_fmaf(z, sx[b][0], __builtin_fmaf(s, pr[t][b][i], acc[t][b][i]));
+                }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) red[wk][t * MB + b][lane] = acc[t][b];
+    __syncthreads();
+    for (int u = wk; u < NT * MB; u += WK) {
+        f32x4 v = red[0][u][lane];
+#pragma unroll
+        for (int w = 1; w < WK; ++w) v += red[w][u][lane];
+        const int m = m0 + 16 * (u % MB) + r, n = 16 * (nb0 + u / MB) + 4 * g;
+        if (m >= p.M) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (n + i >= p.N) break;
+            const float y = apply_act(p.act, v[i] + (p.bias ? p.bias[n + i] : 0.f));
+            const int64_t at = (int64_t)m * p.ldc + n + i;
+            if (p.c_kind == 0) {
+                float* c = static_cast<float*>(p.c) + at;
+                *c = p.accumulate ? *c + y : y;
+            } else if (p.c_kind == 1) {
+                static_cast<uint16_t*>(p.c)[at] = (uint16_t)f32_to_bf16_bits(y);
+            } else {
+                static_cast<_Float16*>(p.c)[at] = (_Float16)y;
+            }
+        }
+    }
+}
+
+// One thread per dword of the packed codes, then one per parameter.
+__global__ __launch_bounds__(256) void w4_pack_kernel(const sf_w4_pack_desc d, uint32_t* out, int n16, int KB,
+                                                      int groups) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t codes = (int64_t)n16 * KB * 256;
+    if (i < codes) {
+        const int j = i & 3, l = (i >> 2) & 63;
+        const int64_t blk = i >> 8;
+        const int64_t n = blk / KB * 16 + (l & 15);
+        const int k = (int)(blk % KB) * 128 + 32 * j + 8 * (l >> 4);
+        uint32_t v = 0;
+        if (n < d.N && k < d.K) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {   // byte b: codes 2 b and 2 b + 1, at nibbles b and b + 4
+                const uint32_t two = d.codes[n * d.ldc + (k >> 1) + b];
+                v |= (two & 15u) << (4 * b) | (two >> 4) << (16 + 4 * b);
+            }
+        }
+        out[i] = v;
+    } else if (i < codes + (int64_t)n16 * groups * 16) {
+        const int64_t q = i - codes;
+        const int64_t n = q / ((int64_t)groups * 16) * 16 + (q & 15);
+        const int gr = (int)((q >> 4) % groups);
+        uint32_t v = 0;
+        if (n < d.N && gr < d.K / d.group) {
+            const uint32_t s = static_cast<const uint16_t*>(d.scales)[n * d.lds + gr];
+            v = s << 16 | (d.zeros ? d.zeros[n * d.ldz + gr] : 8u);
+        }
+        out[i] = v;
+    }
+}
+
+static inline bool w4_shape_ok(int32_t N, int32_t K, int32_t group) {
+    return N > 0 && K > 0 && (group == 32 || group == 64 || group == 128) && K % group == 0;
+}
+static inline int w4_kb(int K) { return (K + 127) / 128; }
+static inline int w4_groups(int K, int group) { return w4_kb(K) * (128 / group); }
+
+template <bool F16, int MB>
+static void launch_w4_group(const W4Args& p, int group, hipStream_t s) {
+    constexpr int NT = 1, WK = 8;
+    const dim3 grid((unsigned)((p.n16 + NT - 1) / NT), (unsigned)((p.M + 16 * MB - 1) / (16 * MB)));
+    if (group == 32) hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, 32>), grid, dim3(64 * WK), 0, s, p);
+    else if (group == 64) hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, 64>), grid, dim3(64 * WK), 0, s, p);
+    else hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, 128>), grid, dim3(64 * WK), 0, s, p);
+}
+
+template <bool F16>
+static void launch_w4(const W4Args& p, int group, hipStream_t s) {
+    if (p.M <= 16) launch_w4_group<F16, 1>(p, group, s);
+    else if (p.M <= 32) launch_w4_group<F16, 2>(p, group, s);
+    else launch_w4_group<F16, 5>(p, group, s);
+}
+
+}  // namespace sfk
+
+extern "C" size_t sf_w4_bytes(int32_t N, int32_t K, int32_t group) {
+    if (!sfk::w4_shape_ok(N, K, group)) return 0;
+    const size_t n16 = ((size_t)N + 15) / 16;
+    return n16 * sfk::w4_kb(K) * 1024 + n16 * sfk::w4_groups(K, group) * 64;
+}
+
+extern "C" int sf_w4_pack(const sf_w4_pack_desc* desc, void* out, void* stream) {
+    if (!desc || !sfk::w4_shape_ok(desc->N, desc->K, desc->group)) return SF_EINVAL;
+    if (!desc->codes || !desc->scales || !out || (reinterpret_cast<uintptr_t>(out) & 15)) return SF_EINVAL;
+    if (desc->ldc < desc->K / 2 || desc->lds < desc->K / desc->group ||
+        (desc->zeros && desc->ldz < desc->K / desc->group) || (reinterpret_cast<uintptr_t>(desc->scales) & 1))
+        return SF_EINVAL;
+    if (desc->scale_dtype != SF_F16 && desc->scale_dtype != SF_BF16) return SF_ENOTSUP;
+    const int64_t words = (int64_t)(sf_w4_bytes(desc->N, desc->K, desc->group) / 4);
+    const int64_t blocks = (words + 255) / 256;
+    if (blocks > 0x7fffffffLL) return SF_ENOTSUP;
+    hipLaunchKernelGGL(sfk::w4_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       *desc, static_cast<uint32_t*>(out), (int)(((int64_t)desc->N + 15) / 16), sfk::w4_kb(desc->K),
+                       sfk::w4_groups(desc->K, desc->group));
+    return hipGetLastError() == hipSuccess ? SF_OK : SF_ELAUNCH;
+}
+
+extern "C" int sf_gemm_w4(const sf_gemm_w4_desc* desc, void* stream) {
+    if (!desc || desc->M < 0 || !sfk::w4_shape_ok(desc->N, desc->K, desc->group)) return SF_EINVAL;
+    if (desc->M == 0) return SF_OK;
+    if (!desc->A || !desc->W || !desc->C) return SF_EINVAL;
+    if (((reinterpret_cast<uintptr_t>(desc->A) | reinterpret_cast<uintptr_t>(desc->W)) & 15) || desc->lda < desc->K ||
+        (desc->lda & 7) || desc->ldc < desc->N)
+        return SF_EINVAL;
+    const uintptr_t calign = desc->c_dtype == SF_F32 ? 3 : 1;
+    if ((reinterpret_cast<uintptr_t>(desc->C) & calign) || (reinterpret_cast<uintptr_t>(desc->bias) & 3))
+        return SF_EINVAL;
+    if (desc->a_dtype != SF_F16 && desc->a_dtype != SF_BF16) return SF_ENOTSUP;
+    if (desc->scale_dtype != SF_F16 && desc->scale_dtype != SF_BF16) return SF_ENOTSUP;
+    if (desc->c_dtype != SF_F32 && desc->c_dtype != SF_F16 && desc->c_dtype != SF_BF16) return SF_ENOTSUP;
+    if (desc->act < SF_ACT_NONE || desc->act > SF_ACT_SILU) return SF_ENOTSUP;
+    if (desc->accumulate && desc->c_dtype != SF_F32) return SF_ENOTSUP;
+    if ((desc->M + 79) / 80 > 65535) return SF_ENOTSUP;   // the grid's second dimension
+    sfk::W4Args p = {};
+    p.a = static_cast<const uint16_t*>(desc->A);
+    p.lda = desc->lda;
+    p.KB = sfk::w4_kb(desc->K);
+    p.groups = sfk::w4_groups(desc->K, desc->group);
+    p.n16 = (int)(((int64_t)desc->N + 15) / 16);
+    p.w = static_cast<const uint8_t*>(desc->W);
+    p.par = reinterpret_cast<const uint32_t*>(p.w + (int64_t)p.n16 * p.KB * 1024);
+    p.bias = desc->bias;
+    p.c = desc->C;
+    p.ldc = desc->ldc;
+    p.M = desc->M;
+    p.N = desc->N;
+    p.K = desc->K;
+    p.scale_f16 = desc->scale_dtype == SF_F16;
+    p.act = desc->act;
+    p.c_kind = desc->c_dtype == SF_BF16 ? 1 : (desc->c_dtype == SF_F16 ? 2 : 0);
+    p.accumulate = desc->accumulate != 0;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (desc->a_dtype == SF_F16) sfk::launch_w4<true>(p, desc->group, s);
+    else sfk::launch_w4<false>(p, desc->group, s);
+    return hipGetLastError() == hipSuccess ? SF_OK : SF_ELAUNCH;
+}

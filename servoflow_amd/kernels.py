@@ -1,9 +1,11 @@
-"""Torch-tensor front ends for sf_gemm, sf_rmsnorm, sf_add_rmsnorm and
-sf_dequant_int8 (test and bench plumbing: torch supplies device memory and
-the stream; the arithmetic runs in libsf_hip_kernels.so)."""
+"""Torch-tensor front ends for sf_gemm, sf_rmsnorm, sf_add_rmsnorm,
+sf_dequant_int8, sf_gemm_w4 and sf_heads_rope (test and bench plumbing: torch
+supplies device memory and the stream; the arithmetic runs in
+libsf_hip_kernels.so)."""
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 
 import torch
 
@@ -280,3 +282,170 @@ def dequant_int8(q, scale, per_channel=True, out_dtype=torch.float32):
                                    out.data_ptr(), _DT[out_dtype], N, K, _stream(q))
     abi.check(st, "sf_dequant_int8")
     return out
+
+
+def _check(t, name, dtypes, like=None, dim=None):
+    """t is a device tensor of one of dtypes (on like's device, with dim axes and a contiguous last one)."""
+    if not t.is_cuda or (like is not None and t.device != like.device):
+        raise ValueError(f"{name} must be a device tensor" + ("" if like is None else f" on {like.device}"))
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} is {t.dtype}: {' or '.join(str(d) for d in dtypes)} expected")
+    if dim is not None and (t.dim() != dim or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1)):
+        raise ValueError(f"{name}{tuple(t.shape)}: {dim} axes with a contiguous last one expected")
+
+
+_B16 = (torch.bfloat16, torch.float16)
+
+
+def _strides_bhs(t):
+    """Element strides of [B, H, S, D], 0 for an axis of one (torch leaves any number there)."""
+    return tuple(st if n > 1 else 0 for st, n in zip(t.stride()[:3], t.shape[:3]))
+
+
+@dataclasses.dataclass(frozen=True)
+class W4:
+    """4-bit weights [N, K] as sf_gemm_w4 reads them (w4_pack)."""
+
+    data: torch.Tensor
+    N: int
+    K: int
+    group: int
+    scale_dtype: torch.dtype
+
+
+def w4_pack(codes, scales, zeros=None, group=128):
+    """Lays 4-bit weights out once for gemm_w4.  codes: uint8 [N, K / 2], input
+    2 i of a row in the low half of byte i, 2 i + 1 in the high half; scales:
+    fp16 or bf16 [N, K / group]; zeros: uint8 [N, K / group] or None (8).  The
+    weight is scale * (code - zero)."""
+    _check(codes, "codes", (torch.uint8,), dim=2)
+    _check(scales, "scales", _B16, codes, 2)
+    N, K = codes.shape[0], 2 * codes.shape[1]
+    if zeros is not None:
+        _check(zeros, "zeros", (torch.uint8,), codes, 2)
+    for name, t in (("scales", scales), ("zeros", zeros)):
+        if t is not None and (K % group or t.shape != (N, K // group)):
+            raise ValueError(f"{name}{tuple(t.shape)}: [{N}, {K} / {group}] expected")
+    d = abi.W4PackDesc()
+    d.N, d.K, d.group = N, K, group
+    d.codes, d.ldc = codes.data_ptr(), max(codes.stride(0), K // 2)
+    d.scales, d.lds, d.scale_dtype = scales.data_ptr(), max(scales.stride(0), scales.shape[1]), _DT[scales.dtype]
+    if zeros is not None:
+        d.zeros, d.ldz = zeros.data_ptr(), max(zeros.stride(0), zeros.shape[1])
+    with torch.cuda.device(codes.device):
+        out = torch.empty(abi.lib().sf_w4_bytes(N, K, group), dtype=torch.uint8, device=codes.device)
+        abi.check(abi.lib().sf_w4_pack(ctypes.byref(d), out.data_ptr(), _stream(codes)), "sf_w4_pack")
+    return W4(out, N, K, group, scales.dtype)
+
+
+def gemm_w4(a, w, bias=None, act=abi.SF_ACT_NONE, out=None, out_dtype=None, accumulate=False):
+    """out[M, N] = act(a[M, K] W^T + bias) with 4-bit weights w (w4_pack); a
+    bf16 or fp16, out_dtype a's unless given.  accumulate adds into an fp32
+    `out`."""
+    _check(a, "a", _B16, w.data, 2)
+    M, K = a.shape
+    if K != w.K:
+        raise ValueError(f"a{tuple(a.shape)} against weights [{w.N}, {w.K}]")
+    if bias is not None:
+        _check(bias, "bias", (torch.float32,), a, 1)
+        if bias.numel() != w.N:
+            raise ValueError(f"bias{tuple(bias.shape)}: {w.N} elements expected")
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate adds into out: give one")
+        out = torch.empty(M, w.N, dtype=out_dtype or a.dtype, device=a.device)
+    _check(out, "out", tuple(_DT)[:3], a, 2)
+    if out.shape != (M, w.N) or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f"out{tuple(out.shape)} {out.dtype}: [{M}, {w.N}] of {out_dtype or out.dtype} expected")
+    d = abi.GemmW4Desc()
+    d.M, d.N, d.K, d.group = M, w.N, K, w.group
+    d.A, d.lda, d.a_dtype = a.data_ptr(), a.stride(0) if M > 1 else max(a.stride(0), (K + 7) // 8 * 8), _DT[a.dtype]
+    d.W, d.scale_dtype = w.data.data_ptr(), _DT[w.scale_dtype]
+    d.bias, d.act = _p(bias), act
+    d.C, d.ldc, d.c_dtype = out.data_ptr(), out.stride(0) if M > 1 else max(out.stride(0), w.N), _DT[out.dtype]
+    d.accumulate = 1 if accumulate else 0
+    with torch.cuda.device(a.device):
+        abi.check(abi.lib().sf_gemm_w4(ctypes.byref(d), _stream(a)), "sf_gemm_w4")
+    return out
+
+
+def heads_rope_strided(srcs, outs, gammas=(None, None), positions=None, inv_freq=None, interleaved=False, eps=1e-6,
+                       cache=None, slots=None):
+    """sf_heads_rope on query, key and value views [B, heads, S, D] (None: left
+    out), written to outs (views of the same shapes; key and value None with a
+    cache, attention.Kv4Cache)."""
+    like = next((t for t in srcs if t is not None), None)
+    if like is None or len(srcs) != 3 or len(outs) != 3:
+        raise ValueError("three sources and outputs, query, key and value, not all of them None")
+    F = tuple(_DT)[:3]
+    d = abi.HeadsRopeDesc()
+    B, _, S, D = like.shape if like.dim() == 4 else (0, 0, 0, 0)
+    out_like = None
+    for j, (t, o) in enumerate(zip(srcs, outs)):
+        if t is None:
+            if o is not None:
+                raise ValueError("an output without its source")
+            continue
+        _check(t, "source", F, like, 4)
+        if t.dtype != like.dtype or (t.shape[0], t.shape[2], t.shape[3]) != (B, S, D):
+            raise ValueError(f"source {tuple(t.shape)} {t.dtype} beside {tuple(like.shape)} {like.dtype}")
+        d.heads[j], d.src[j] = t.shape[1], t.data_ptr()
+        d.src_stride[j][:] = _strides_bhs(t)
+        if (o is None) != (cache is not None and j > 0):
+            raise ValueError("an output for every source; none for keys and values that go into a cache")
+        if o is not None:
+            out_like = o if out_like is None else out_like
+            _check(o, "output", (out_like.dtype,) if out_like.dtype in F else F, like, 4)
+            if o.shape != t.shape:
+                raise ValueError(f"output {tuple(o.shape)} for a source {tuple(t.shape)}")
+            d.out[j] = o.data_ptr()
+            d.out_stride[j][:] = _strides_bhs(o)
+    d.B, d.S, d.D = B, S, D
+    d.in_dtype, d.out_dtype = _DT[like.dtype], _DT[like.dtype if out_like is None else out_like.dtype]
+    for j, gm in enumerate(gammas):
+        if gm is not None:
+            _check(gm, "gamma", (torch.float32,), like, 1)
+            if gm.numel() != D:
+                raise ValueError(f"gamma{tuple(gm.shape)}: {D} elements expected")
+            d.gamma[j] = gm.data_ptr()
+    d.eps = eps
+    for name, t in (("positions", positions), ("slots", slots)):
+        if t is not None:
+            _check(t, name, (torch.int32,), like)
+            if t.numel() != B * S or not t.is_contiguous():
+                raise ValueError(f"{name}{tuple(t.shape)}: {B * S} contiguous elements expected")
+            setattr(d, name, t.data_ptr())
+    if inv_freq is not None:
+        _check(inv_freq, "inv_freq", (torch.float64,), like, 1)
+        d.inv_freq, d.rot, d.interleaved = inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0
+    if cache is not None:
+        if cache.data.device != like.device:
+            raise ValueError(f"the cache must be on {like.device}")
+        d.cache = cache.desc()
+    with torch.cuda.device(like.device):
+        abi.check(abi.lib().sf_heads_rope(ctypes.byref(d), _stream(like)), "sf_heads_rope")
+
+
+def heads_rope(p, S, heads, D, gammas=(None, None), positions=None, inv_freq=None, interleaved=False, eps=1e-6,
+               out_dtype=None, cache=None, slots=None):
+    """Splits a projection's rows p [B * S, (Hq + Hk + Hv) * D] into query, key
+    and value heads [B, heads, S, D] (heads = (Hq, Hk, Hv), 0 leaves one out),
+    with the RMSNorm of each query and key head (gammas, fp32 [D] or None) and
+    the rotation of their first 2 * len(inv_freq) channels by the token's
+    position (positions: int32 [B * S]; inv_freq: float64 radians a position;
+    pairs (i, i + half), or (2 i, 2 i + 1) with interleaved).  A token with a
+    negative position is padding and is not written.  With a cache
+    (attention.Kv4Cache) keys and values go there, at `slots` (int32) or the
+    positions.  Returns (q, k, v), None for what is left out or cached."""
+    _check(p, "p", tuple(_DT)[:3], dim=2)
+    if len(heads) != 3 or min(heads) < 0 or p.shape[1] != sum(heads) * D or S <= 0 or p.shape[0] % S:
+        raise ValueError(f"p{tuple(p.shape)}: rows of {sum(heads)} x {D} for tokens in groups of {S} expected")
+    B, srcs, outs, at = p.shape[0] // S, [], [], 0
+    for j, h in enumerate(heads):
+        t = p[:, at * D:(at + h) * D].unflatten(0, (B, S)).unflatten(2, (h, D)).transpose(1, 2) if h else None
+        cached = t is None or (cache is not None and j > 0)
+        srcs.append(t)
+        outs.append(None if cached else torch.empty(B, h, S, D, dtype=out_dtype or p.dtype, device=p.device))
+        at += h
+    heads_rope_strided(srcs, outs, gammas, positions, inv_freq, interleaved, eps, cache, slots)
+    return tuple(outs)

@@ -1,0 +1,336 @@
+"""Head norm + rotation, the 4-bit key / value cache and the attention over it
+against plain forms in 64 bits.
+
+Tolerances, from the arithmetic.
+  norm + rotation: fp32; a norm takes D / 8 + 4 additions, a root, a division
+  and two products (24 roundings), a rotation 3 and an angle whose fraction of
+  a turn is held to 2^-26 (2 pi 2^-26 radians) with sine and cosine to 2 units:
+  40 roundings of 2^-24 of |x1| + |x2| cover both; then half a step of the
+  output type.
+  cache: keys and values as given are quantised exactly as the format says, so
+  the read values are equal.
+  attention, against the values that the cache stands for: a score is off by
+  the roundings of its sums (24 of 2^-24 of scale * sum |q| (|k| + 40 s)); p by
+  that and by exp2's 2^-22; the (hi, lo) pair by 2^-17; sums over tokens by
+  (32 + tokens / 32) 2^-24 of 55 s / max |v| <= 16 times the largest value."""
+import math
+
+import pytest
+import torch
+
+from servoflow_amd import kernels
+from servoflow_amd.attention import Kv4Cache, attention_kv4
+
+from _quant4 import attend, half_step, kv4_levels, rms, rotate
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _randn(seed, *shape, dtype=F32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def _freq(rot, base=10000.0):
+    return base ** (-torch.arange(rot // 2, dtype=torch.float64) / (rot // 2))
+
+
+def _rope_check(got, ref, x, dtype, what=""):
+    """x: the normed values before the rotation, 64 bits."""
+    tol = 40 * 2.0 ** -24 * (x.abs().amax(-1, keepdim=True) * 2 + 1e-30) + half_step(dtype) * ref.abs()
+    if dtype == FP:
+        tol = tol + 2.0 ** -25
+    err = (got.cpu().double() - ref).abs()
+    assert torch.isfinite(got).all(), what
+    assert (err <= tol).all(), f"{what}: {float((err / tol).max())} of the tolerance"
+
+
+# --- norm + rotation -------------------------------------------------------
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype,out_dtype", [(BF, BF), (FP, FP), (F32, F32), (BF, F32), (F32, BF)])
+@pytest.mark.parametrize("rot,interleaved", [(0, False), (16, False), (16, True), (48, False), (48, True), ("D", False),
+                                             ("D", True)])
+def test_heads_rope(D, dtype, out_dtype, rot, interleaved):
+    rot = D if rot == "D" else rot
+    B, S, Hq, Hk = 2, 5, 6, 3
+    p = _randn(1, B * S, (Hq + 2 * Hk) * D, dtype=dtype)
+    gq, gk = 1 + 0.2 * _randn(2, D), 1 + 0.2 * _randn(3, D)
+    pos = torch.tensor([[0, 1, 7, 1000, 999999], [3, 2 ** 31 - 1, 65536, 12, 1]], dtype=torch.int32)
+    f = _freq(rot) if rot else None
+    q, k, v = kernels.heads_rope(p.to(DEV), S, (Hq, Hk, Hk), D, (gq.to(DEV), gk.to(DEV)), pos.to(DEV),
+                                 None if f is None else f.to(DEV), interleaved, 1e-6, out_dtype)
+    x = p.double().reshape(B, S, -1, D).transpose(1, 2)
+    for name, got, part, gm in (("q", q, x[:, :Hq], gq), ("k", k, x[:, Hq:Hq + Hk], gk)):
+        n = rms(part, gm, 1e-6)
+        _rope_check(got, rotate(n, pos, f, interleaved) if rot else n, n, out_dtype, name)
+    assert torch.equal(v.cpu(), x[:, Hq + Hk:].to(dtype).to(out_dtype))
+
+
+@pytest.mark.parametrize("B,S,Hq,Hk,Hv", [(1, 1, 1, 0, 0), (1, 1, 0, 1, 1), (3, 1, 0, 0, 2), (1, 2049, 3, 1, 1),
+                                          (2049, 1, 5, 0, 0), (7, 9, 33, 2, 1)])
+def test_heads_rope_shapes(B, S, Hq, Hk, Hv):
+    D, dtype = 64, FP
+    p = _randn(4, B * S, (Hq + Hk + Hv) * D, dtype=dtype)
+    out = kernels.heads_rope(p.to(DEV), S, (Hq, Hk, Hv), D, inv_freq=_freq(D).to(DEV))
+    x = p.double().reshape(B, S, -1, D).transpose(1, 2)
+    pos = torch.arange(S).expand(B, S)
+    for got, part, turn in ((out[0], x[:, :Hq], True), (out[1], x[:, Hq:Hq + Hk], True), (out[2], x[:, Hq + Hk:], False)):
+        assert (got is None) == (part.shape[1] == 0)
+        if got is not None:
+            _rope_check(got, rotate(part, pos, _freq(D), False) if turn else part, part, dtype)
+
+
+def test_padding_rows_and_strided_in_place():
+    """Padding tokens stay as they were; rows rotated where they lie, behind other columns."""
+    B, S, H, D = 2, 6, 4, 64
+    wide = _randn(5, B * S, 3 * H * D + 40, dtype=BF).to(DEV)
+    was = wide.clone()
+    x = wide[:, 16:16 + H * D].unflatten(0, (B, S)).unflatten(2, (H, D)).transpose(1, 2)
+    pos = torch.tensor([[0, 1, 2, 3, -1, -5], [9, -1, 11, 12, 13, 14]], dtype=torch.int32)
+    ref = rotate(x.cpu().double(), pos.clamp_min(0), _freq(D), True)
+    before = x.cpu().double()
+    kernels.heads_rope_strided((x, None, None), (x, None, None), positions=pos.to(DEV), inv_freq=_freq(D).to(DEV),
+                               interleaved=True)
+    real = (pos >= 0)[:, None, :, None]
+    _rope_check(x, torch.where(real, ref, before), before, BF)
+    assert torch.equal(torch.masked_select(x.cpu().double(), ~real), torch.masked_select(before, ~real))
+    same = torch.ones(wide.shape[1], dtype=torch.bool)
+    same[16:16 + H * D] = False
+    assert torch.equal(wide[:, same], was[:, same])
+
+
+# --- the cache --------------------------------------------------------------
+
+
+def _levels(x):
+    return kv4_levels(x.cpu())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("S", [1, 31, 32, 33, 100])
+def test_cache_round_trip(D, dtype, S):
+    B, H = 2, 3
+    k, v = (_randn(6 + i, B, H, S, D, dtype=dtype) * (1 + 3 * i) + 0.3 for i in range(2))
+    c = Kv4Cache(B, H, S, D, DEV)
+    c.write(k.to(DEV), v.to(DEV))
+    rk, rv = c.read(dtype=F32)
+    assert torch.equal(rk.cpu(), _levels(k).float()) and torch.equal(rv.cpu(), _levels(v).float())
+
+
+def test_cache_slots_leave_the_rest():
+    """Ragged slots, slots out of range, and what other slots held."""
+    B, H, D, cap = 3, 2, 64, 70
+    c = Kv4Cache(B, H, cap, D, DEV)
+    k, v = _randn(8, B, H, cap, D, dtype=BF), _randn(9, B, H, cap, D, dtype=BF)
+    c.write(k.to(DEV), v.to(DEV))
+    nk, nv = _randn(10, B, H, 4, D, dtype=BF), _randn(11, B, H, 4, D, dtype=BF)
+    slots = torch.tensor([[69, 0, 33, -1], [70, 5, 2 ** 31 - 1, 6], [31, 32, 63, 64]], dtype=torch.int32)
+    c.write(nk.to(DEV), nv.to(DEV), slots.to(DEV))
+    ek, ev = k.clone(), v.clone()
+    for b in range(B):
+        for j, s in enumerate(slots[b].tolist()):
+            if 0 <= s < cap:
+                ek[b, :, s], ev[b, :, s] = nk[b, :, j], nv[b, :, j]
+    rk, rv = c.read(dtype=F32)
+    assert torch.equal(rk.cpu(), _levels(ek).float()) and torch.equal(rv.cpu(), _levels(ev).float())
+    gk, gv = c.read(slots.to(DEV), F32)
+    inside = ((slots >= 0) & (slots < cap))[:, None, :, None]
+    assert torch.equal(gk.cpu(), torch.where(inside, _levels(nk).float(), torch.zeros(())))
+    assert torch.equal(gv.cpu(), torch.where(inside, _levels(nv).float(), torch.zeros(())))
+
+
+def test_cache_extreme_values():
+    """Constant groups, outliers, the largest and smallest numbers; an infinity or NaN spoils its group alone."""
+    D = 128
+    x = _randn(12, 1, 1, 12, D)
+    x[0, 0, 0] = 0
+    x[0, 0, 1] = -3.25
+    x[0, 0, 2, 5] = 3e38
+    x[0, 0, 3] *= 1e-37
+    x[0, 0, 4] *= 1e-30
+    x[0, 0, 5, :] = 3.3895e38
+    x[0, 0, 5, 1::2] = -3.3895e38
+    x[0, 0, 6, 70] = 1e5
+    x[0, 0, 7, 3] = float("inf")
+    x[0, 0, 8, 100] = float("nan")
+    x[0, 0, 9] = 2.0 ** torch.arange(D).remainder(16).float()
+    c = Kv4Cache(1, 1, 12, D, DEV)
+    c.write(x.to(DEV), x.to(DEV))
+    bad = torch.zeros(12, 2, dtype=torch.bool)
+    bad[7, 0] = bad[8, 1] = True
+    y = x.clone()
+    y[0, 0].unflatten(-1, (2, 64))[bad] = 0
+    ref = _levels(y).float()[0, 0].unflatten(-1, (2, 64))
+    for got in c.read(dtype=F32):
+        got = got.cpu()[0, 0].unflatten(-1, (2, 64))
+        assert torch.isnan(got[bad]).all()
+        keep = ~bad
+        keep[3] = False   # steps near the normal range's end: only how far they are from the input
+        assert torch.equal(got[keep], ref[keep])
+        assert ((got[3] - x[0, 0, 3].unflatten(-1, (2, 64))).abs() <= 1e-37).all()
+
+
+def test_rope_into_cache():
+    """Normed, rotated keys and plain values at given slots; queries to a tensor."""
+    B, S, Hq, H, D = 2, 37, 4, 2, 128
+    p = _randn(13, B * S, (Hq + 2 * H) * D, dtype=BF)
+    gk = 1 + 0.2 * _randn(14, D)
+    pos = (torch.arange(S) + torch.tensor([[5], [60]])).to(torch.int32)
+    pos[1, 3] = -1
+    c = Kv4Cache(B, H, 100, D, DEV)
+    c.data.zero_()
+    q, k, v = kernels.heads_rope(p.to(DEV), S, (Hq, H, H), D, (None, gk.to(DEV)), pos.to(DEV), _freq(D).to(DEV),
+                                 cache=c)
+    assert k is None and v is None
+    x = p.double().reshape(B, S, -1, D).transpose(1, 2)
+    n = rms(x[:, Hq:Hq + H], gk, 1e-6)
+    ref = rotate(n, pos.clamp_min(0), _freq(D), False)
+    rk, rv = (t.cpu().double() for t in c.read(pos.to(DEV), F32))
+    real = pos >= 0
+    assert torch.equal(rv, torch.where(real[:, None, :, None], kv4_levels(x[:, Hq + H:]), torch.zeros((), dtype=rv.dtype)))
+    # a key's code may fall on the other side of a border by the rounding before it: half a step more
+    step = (ref.unflatten(-1, (2, 64)).amax(-1) - ref.unflatten(-1, (2, 64)).amin(-1)) / 16 * 1.02
+    err = (rk - ref).abs().unflatten(-1, (2, 64)).amax(-1)
+    assert (err <= torch.where(real[:, None, :, None], step * 0.5 + 1e-4, math.inf)).all()
+    same = (rk - kv4_levels(ref.float())).abs() < 1e-6
+    assert same[real[:, None, :, None].expand_as(same)].float().mean() > 0.999
+
+
+# --- attention ----------------------------------------------------------------
+
+
+def _filled(B, H, Sk, D, dtype, seed, cap=None):
+    k = _randn(seed, B, H, Sk, D, dtype=dtype) + 0.5 * _randn(seed + 1, 1, H, 1, D).to(dtype)
+    v = _randn(seed + 2, B, H, Sk, D, dtype=dtype)
+    c = Kv4Cache(B, H, cap or Sk, D, DEV)
+    c.data.fill_(0xff)   # NaN parameters everywhere: what is not written must not be seen
+    c.write(k.to(DEV), v.to(DEV))
+    return c, kv4_levels(k), kv4_levels(v)
+
+
+def _attn_check(got, q, k, v, dtype, scale=0.0, what="", **kw):
+    ref = attend(q, k, v, scale=scale, **kw)
+    D, Sk = q.shape[-1], k.shape[2]
+    sc = scale or 1 / math.sqrt(D)
+    # |k| + 40 s: s is at most a sixteenth of a row's spread, itself at most twice its largest value
+    dx = 24 * 2.0 ** -24 * sc * float(q.double().abs().sum(-1).max()) * float(k.abs().max()) * 6 if k.numel() else 0.0
+    rel = 2 * (dx + 2.0 ** -22) + 2.0 ** -16 + (32 + Sk / 32) * 2.0 ** -24 * 16
+    tol = rel * float(v.abs().max()) + half_step(dtype) * ref.abs()
+    if dtype == FP:
+        tol = tol + 2.0 ** -25
+    err = (got.cpu().double() - ref).abs()
+    assert torch.isfinite(got).all(), what
+    assert (err <= tol).all(), f"{what}: {float((err / tol).max())} of the tolerance"
+    return ref
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("Hq,H,Sq", [(1, 1, 1), (8, 2, 1), (4, 4, 1), (6, 2, 5), (2, 2, 16), (4, 2, 17), (2, 2, 67),
+                                     (8, 1, 33)])
+@pytest.mark.parametrize("Sk", [1, 31, 32, 33, 257, 700])
+def test_attention(D, dtype, Hq, H, Sq, Sk):
+    B = 2
+    c, k, v = _filled(B, H, Sk, D, dtype, 20)
+    q = _randn(23, B, Hq, Sq, D, dtype=dtype)
+    for out_dtype in (F32, dtype):
+        got = attention_kv4(q.to(DEV), c, out_dtype=out_dtype)
+        _attn_check(got, q, k, v, out_dtype, what=f"out {out_dtype}")
+
+
+@pytest.mark.parametrize("splits", [1, 2, 7, 64])
+@pytest.mark.parametrize("Sq,causal", [(1, False), (3, True), (40, True), (200, True)])
+def test_splits_and_causal(splits, Sq, causal):
+    B, Hq, H, Sk, D = 3, 4, 2, 190, 64
+    c, k, v = _filled(B, H, Sk, D, BF, 30, cap=201)
+    q = _randn(33, B, Hq, Sq, D, dtype=BF)
+    valid = torch.tensor([190, 0, 77], dtype=torch.int32)
+    got = attention_kv4(q.to(DEV), c, keys=Sk, is_causal=causal, valid_len=valid.to(DEV), num_splits=splits,
+                        out_dtype=F32)
+    ref = _attn_check(got, q, k, v, F32, valid=valid, causal=causal)
+    assert (ref[1] == 0).all() and (got[1] == 0).all()   # no key at all
+    if causal and Sq == 200:
+        assert (got[2, :, :123] == 0).all()               # rows before the first token
+
+
+@pytest.mark.parametrize("Sq", [1, 67])
+def test_masks(Sq):
+    """Masks with rows of nothing, lengths out of range, and a NaN key behind the mask."""
+    B, Hq, H, Sk, D = 4, 4, 2, 150, 128
+    c, k, v = _filled(B, H, Sk, D, FP, 40, cap=160)
+    mask = torch.rand(B, Sk, generator=torch.Generator().manual_seed(4)) < 0.6
+    mask[0] = False
+    mask[1, :64] = False
+    mask[2, 77] = False
+    bad = torch.full((B, H, 1, D), float("nan"), dtype=FP, device=DEV)
+    c.write(bad, bad, torch.tensor([[-1], [3], [77], [159]], dtype=torch.int32, device=DEV))
+    valid = torch.tensor([150, 1000, 149, -3], dtype=torch.int32)
+    q = _randn(43, B, Hq, Sq, D, dtype=FP)
+    for dt in (torch.bool, torch.uint8):
+        got = attention_kv4(q.to(DEV), c, keys=Sk, valid_len=valid.to(DEV), kv_mask=mask.to(dt).to(DEV), out_dtype=FP)
+        _attn_check(got, q, k, v, FP, valid=valid, mask=mask)
+        assert (got[0] == 0).all() and (got[3] == 0).all()
+
+
+def test_causal_nan_is_seen_by_later_rows_only():
+    B, H, Sk, D = 1, 1, 40, 64
+    c, k, v = _filled(B, H, Sk, D, BF, 50)
+    bad = torch.full((1, 1, 1, D), float("nan"), dtype=BF, device=DEV)
+    c.write(bad, bad, torch.tensor([[30]], dtype=torch.int32, device=DEV))
+    q = _randn(53, B, H, Sk, D, dtype=BF)
+    got = attention_kv4(q.to(DEV), c, is_causal=True, out_dtype=F32)
+    _attn_check(got[:, :, :30], q[:, :, :30], k[:, :, :30], v[:, :, :30], F32, causal=True)
+    assert torch.isnan(got[:, :, 30:]).all()
+
+
+@pytest.mark.parametrize("scale", [0.02, 1.0, 8.0])
+def test_scales_and_peaks(scale):
+    """Nearly uniform weights up to one key's taking all, with maxima that rise along the keys."""
+    B, H, Sk, D = 1, 2, 300, 64
+    k = _randn(60, B, H, Sk, D, dtype=BF) * torch.linspace(0.1, 3, Sk)[:, None].to(BF)
+    v = _randn(61, B, H, Sk, D, dtype=BF)
+    c = Kv4Cache(B, H, Sk, D, DEV)
+    c.write(k.to(DEV), v.to(DEV))
+    q = _randn(62, B, H, 3, D, dtype=BF)
+    got = attention_kv4(q.to(DEV), c, scale=scale, out_dtype=F32)
+    _attn_check(got, q, kv4_levels(k), kv4_levels(v), F32, scale=scale)
+
+
+def test_values_of_unequal_size():
+    """Tokens whose values differ by 2^40, the large ones all but unseen."""
+    B, H, Sk, D = 1, 1, 96, 64
+    k = _randn(63, B, H, Sk, D, dtype=BF)
+    v = _randn(64, B, H, Sk, D, dtype=BF)
+    v[:, :, ::7] *= 2.0 ** 20
+    v[:, :, 1::7] *= 2.0 ** -20
+    c = Kv4Cache(B, H, Sk, D, DEV)
+    c.write(k.to(DEV), v.to(DEV))
+    q = _randn(65, B, H, 2, D, dtype=BF)
+    _attn_check(attention_kv4(q.to(DEV), c, out_dtype=F32), q, kv4_levels(k), kv4_levels(v), F32)
+
+
+def test_strides_and_neighbours():
+    """Queries as columns of a projection's rows, output as rows [B, S, H * D] inside a wider buffer."""
+    B, Hq, H, Sq, Sk, D = 2, 6, 3, 9, 65, 64
+    c, k, v = _filled(B, H, Sk, D, BF, 70)
+    rows = _randn(73, B, Sq, 2 * Hq * D, dtype=BF).to(DEV)
+    q = rows[..., Hq * D:].unflatten(2, (Hq, D)).transpose(1, 2)
+    wide = torch.full((B, Sq, Hq * D + 16), 7.0, dtype=F32, device=DEV)
+    out = wide[..., 8:8 + Hq * D].unflatten(2, (Hq, D)).transpose(1, 2)
+    attention_kv4(q, c, out=out)
+    _attn_check(out, q.cpu(), k, v, F32)
+    assert (wide[..., :8] == 7).all() and (wide[..., 8 + Hq * D:] == 7).all()
+
+
+def test_runs_are_equal_and_splits_agree():
+    B, Hq, H, Sk, D = 2, 8, 2, 3000, 128
+    c, k, v = _filled(B, H, Sk, D, BF, 80)
+    q = _randn(83, B, Hq, 1, D, dtype=BF).to(DEV)
+    one = attention_kv4(q, c, out_dtype=F32)
+    for _ in range(3):
+        assert torch.equal(one, attention_kv4(q, c, out_dtype=F32))
+    _attn_check(attention_kv4(q, c, num_splits=5, out_dtype=F32), q.cpu(), k, v, F32)
