@@ -10,6 +10,7 @@ semantics as documented on `sf_attn_desc`.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -116,10 +117,9 @@ class Kv4Cache:
         self.B, self.H, self.capacity, self.D = B, H, capacity, D
         self.data = torch.empty(n, dtype=torch.uint8, device=device)   # needs no init
 
-    def desc(self):
-        c = abi.Kv4CacheDesc()
-        c.data, c.B, c.H, c.capacity, c.D = self.data.data_ptr(), self.B, self.H, self.capacity, self.D
-        return c
+    def fields(self):
+        """The members of sf_kv4_cache."""
+        return self.data.data_ptr(), self.B, self.H, self.capacity, self.D
 
     def write(self, k, v, slots=None):
         """Tokens k, v [B, H, S, D] into slots (int32 [B, S], one outside
@@ -129,20 +129,23 @@ class Kv4Cache:
     def read(self, slots=None, dtype=torch.bfloat16):
         """(k, v) [B, H, S, D]: the values of the tokens in slots (int32
         [B, S]; None: all of them), zeros for a slot outside [0, capacity)."""
-        S = self.capacity
+        S, dev, ptr = self.capacity, self.data.device, None
         if slots is not None:
-            if slots.dtype != torch.int32 or slots.dim() != 2 or slots.shape[0] != self.B or \
-                    not slots.is_contiguous() or slots.device != self.data.device:
-                raise ValueError(f"slots must be a contiguous int32 [{self.B}, S] on {self.data.device}")
-            S = slots.shape[1]
-        k, v = (torch.empty(self.B, self.H, S, self.D, dtype=dtype, device=self.data.device) for _ in range(2))
+            if slots.dtype is not torch.int32 or slots.dim() != 2 or slots.shape[0] != self.B or \
+                    not slots.is_contiguous() or slots.device != dev:
+                raise ValueError(f"slots must be a contiguous int32 [{self.B}, S] on {dev}")
+            S, ptr = slots.shape[1], slots.data_ptr()
+        k = torch.empty(self.B, self.H, S, self.D, dtype=dtype, device=dev)
+        v = torch.empty(self.B, self.H, S, self.D, dtype=dtype, device=dev)
         st = (ctypes.c_int64 * 3)(*k.stride()[:3])
-        with torch.cuda.device(self.data.device):
-            s = abi.lib().sf_kv4_read(ctypes.byref(self.desc()), slots.data_ptr() if slots is not None else None, S,
-                                      k.data_ptr(), st, v.data_ptr(), st, _DT[dtype],
-                                      torch.cuda.current_stream().cuda_stream)
-        abi.check(s, "sf_kv4_read")
+        kernels.call_on(dev, "sf_kv4_read", abi.lib().sf_kv4_read, ctypes.byref(abi.Kv4CacheDesc(*self.fields())), ptr,
+                        S, k.data_ptr(), st, v.data_ptr(), st, _DT[dtype])
         return k, v
+
+
+# sf_attn_kv4_desc in one pack.
+_KV4_DESC = struct.Struct("@4if4i4x2Pq3q3qP4i")
+assert _KV4_DESC.size == ctypes.sizeof(abi.AttnKv4Desc)
 
 
 def attention_kv4(q, cache, out=None, scale=0.0, is_causal=False, valid_len=None, kv_mask=None, keys=None,
@@ -153,41 +156,40 @@ def attention_kv4(q, cache, out=None, scale=0.0, is_causal=False, valid_len=None
     int32 [B] lengths; kv_mask: device bool [B, keys] (True = attend);
     is_causal: query s is the token at valid_len - Sq + s.  Runs on torch's
     current stream; a row that sees nothing is zeros."""
-    if q.dim() != 4 or q.shape[0] != cache.B or q.shape[3] != cache.D or q.shape[1] % cache.H:
-        raise ValueError(f"q{tuple(q.shape)} over a cache of B {cache.B}, H {cache.H}, D {cache.D}")
-    if q.device != cache.data.device or q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"q must be bfloat16 or float16 on {cache.data.device}")
-    B, Hq, Sq, D = q.shape
+    dev, shape = cache.data.device, q.shape
+    if len(shape) != 4 or shape[0] != cache.B or shape[3] != cache.D or shape[1] % cache.H:
+        raise ValueError(f"q{tuple(shape)} over a cache of B {cache.B}, H {cache.H}, D {cache.D}")
+    if not q.is_cuda or q.device != dev or q.dtype not in (torch.bfloat16, torch.float16) or q.stride(3) != 1:
+        raise ValueError(f"q must be bfloat16 or float16 on {dev}, a device, with a contiguous last axis")
+    B, Hq, Sq, D = shape
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
-    if out.shape != q.shape or out.device != q.device or out.dtype not in _DT or \
+        out = torch.empty(shape, dtype=out_dtype or q.dtype, device=dev)
+    elif out.shape != shape or out.device != dev or out.dtype not in _DT or out.stride(3) != 1 or \
             (out_dtype is not None and out.dtype != out_dtype):
-        raise ValueError(f"out{tuple(out.shape)} {out.dtype} for q{tuple(q.shape)}")
-    d = abi.AttnKv4Desc()
-    d.B, d.Hq, d.Sq, d.Sk = B, Hq, Sq, cache.capacity if keys is None else int(keys)
-    d.scale, d.in_dtype, d.out_dtype = float(scale), _DT[q.dtype], _DT[out.dtype]
-    d.is_causal, d.num_splits = 1 if is_causal else 0, int(num_splits)
+        raise ValueError(f"out{tuple(out.shape)} {out.dtype} for q{tuple(shape)}")
+    Sk = cache.capacity if keys is None else int(keys)
+    valid_ptr = mask_ptr = mask_st = 0
     if valid_len is not None:
-        if valid_len.dtype != torch.int32 or valid_len.numel() != B or not valid_len.is_contiguous() or \
-                valid_len.device != q.device:
+        if valid_len.dtype is not torch.int32 or valid_len.numel() != B or not valid_len.is_contiguous() or \
+                valid_len.device != dev:
             raise ValueError("valid_len must be a device int32 tensor of B elements")
-        d.kv_valid_len = valid_len.data_ptr()
+        valid_ptr = valid_len.data_ptr()
     if kv_mask is not None:
-        if kv_mask.dtype not in (torch.bool, torch.uint8) or kv_mask.shape != (B, d.Sk) or \
-                (d.Sk > 1 and kv_mask.stride(1) != 1) or kv_mask.device != q.device:
-            raise ValueError(f"kv_mask must be a device bool/uint8 tensor [{B}, {d.Sk}] with contiguous rows")
-        d.kv_mask, d.kv_mask_stride = kv_mask.data_ptr(), kv_mask.stride(0) if B > 1 else 0
-    for name, t in (("q", q), ("out", out)):
-        if t.shape[3] > 1 and t.stride(3) != 1:
-            raise ValueError(f"{name} must have a contiguous last axis")
-    d.q_stride[:], d.o_stride[:] = kernels._strides_bhs(q), kernels._strides_bhs(out)
-    d.cache = cache.desc()
-    with torch.cuda.device(q.device):
-        need = int(abi.lib().sf_attn_kv4_workspace_bytes(ctypes.byref(d)))
-        if need and workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)   # needs no init
-        ws, n = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
-        st = abi.lib().sf_attn_kv4(ctypes.byref(d), q.data_ptr(), out.data_ptr(), ws, n,
-                                   torch.cuda.current_stream().cuda_stream)
-    abi.check(st, "sf_attn_kv4")
+        if kv_mask.dtype not in (torch.bool, torch.uint8) or kv_mask.shape != (B, Sk) or \
+                (Sk > 1 and kv_mask.stride(1) != 1) or kv_mask.device != dev:
+            raise ValueError(f"kv_mask must be a device bool/uint8 tensor [{B}, {Sk}] with contiguous rows")
+        mask_ptr, mask_st = kv_mask.data_ptr(), kv_mask.stride(0) if B > 1 else 0
+    raw = _KV4_DESC.pack(B, Hq, Sq, Sk, scale, _DT[q.dtype], _DT[out.dtype], 1 if is_causal else 0, int(num_splits),
+                         valid_ptr, mask_ptr, mask_st, *kernels.strides_bhs(q), *kernels.strides_bhs(out),
+                         *cache.fields())
+    d = ctypes.byref(abi.AttnKv4Desc.from_buffer_copy(raw))
+    ws, n = None, 0
+    if workspace is None:
+        n = abi.lib().sf_attn_kv4_workspace_bytes(d)
+        if n:
+            workspace = torch.empty(n, dtype=torch.uint8, device=dev)   # needs no init
+            ws = workspace.data_ptr()
+    else:
+        ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    kernels.call_on(dev, "sf_attn_kv4", abi.lib().sf_attn_kv4, d, q.data_ptr(), out.data_ptr(), ws, n)
     return out

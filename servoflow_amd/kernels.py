@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import struct
 
 import torch
 
@@ -284,22 +285,50 @@ def dequant_int8(q, scale, per_channel=True, out_dtype=torch.float32):
     return out
 
 
-def _check(t, name, dtypes, like=None, dim=None):
-    """t is a device tensor of one of dtypes (on like's device, with dim axes and a contiguous last one)."""
-    if not t.is_cuda or (like is not None and t.device != like.device):
-        raise ValueError(f"{name} must be a device tensor" + ("" if like is None else f" on {like.device}"))
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} is {t.dtype}: {' or '.join(str(d) for d in dtypes)} expected")
-    if dim is not None and (t.dim() != dim or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1)):
-        raise ValueError(f"{name}{tuple(t.shape)}: {dim} axes with a contiguous last one expected")
+def _raw_stream(device):
+    """The raw handle of torch's current stream on `device`, without building a Stream object (2 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def call_on(device, what, fn, *args):
+    """fn(*args, stream) on torch's current stream of `device`, with that device current (kernels are loaded and
+    launched on the current one); raises on an error status."""
+    if device.index == torch.cuda.current_device():
+        st = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, _raw_stream(device))
+    if st:
+        abi.check(st, what)
 
 
 _B16 = (torch.bfloat16, torch.float16)
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def _strides_bhs(t):
+def _check(t, name, dtypes, device=None, dim=None):
+    """t is a device tensor of one of dtypes (on `device`, with dim axes and a contiguous last one)."""
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{name} must be a device tensor" + ("" if device is None else f" on {device}"))
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} is {t.dtype}: {' or '.join(str(d) for d in dtypes)} expected")
+    if dim is not None and (t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel())):
+        raise ValueError(f"{name}{tuple(t.shape)}: {dim} axes with a contiguous last one expected")
+
+
+def _vector(t, name, dtype, n, device):
+    """The pointer of a contiguous device tensor of n elements (0 for None)."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.device != device or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}{tuple(t.shape)} {t.dtype}: {n} contiguous {dtype} on {device} expected")
+    return t.data_ptr()
+
+
+def strides_bhs(t):
     """Element strides of [B, H, S, D], 0 for an axis of one (torch leaves any number there)."""
-    return tuple(st if n > 1 else 0 for st, n in zip(t.stride()[:3], t.shape[:3]))
+    n, st = t.shape, t.stride()
+    return (st[0] if n[0] > 1 else 0, st[1] if n[1] > 1 else 0, st[2] if n[2] > 1 else 0)
 
 
 @dataclasses.dataclass(frozen=True)
@@ -319,22 +348,25 @@ def w4_pack(codes, scales, zeros=None, group=128):
     fp16 or bf16 [N, K / group]; zeros: uint8 [N, K / group] or None (8).  The
     weight is scale * (code - zero)."""
     _check(codes, "codes", (torch.uint8,), dim=2)
-    _check(scales, "scales", _B16, codes, 2)
-    N, K = codes.shape[0], 2 * codes.shape[1]
+    dev, (N, half) = codes.device, codes.shape
+    K = 2 * half
+    need = abi.lib().sf_w4_bytes(N, K, group)
+    if need == 0:
+        raise ValueError(f"no 4-bit weights [{N}, {K}] in groups of {group}: 32, 64 or 128, K a multiple")
+    _check(scales, "scales", _B16, dev, 2)
     if zeros is not None:
-        _check(zeros, "zeros", (torch.uint8,), codes, 2)
+        _check(zeros, "zeros", (torch.uint8,), dev, 2)
     for name, t in (("scales", scales), ("zeros", zeros)):
-        if t is not None and (K % group or t.shape != (N, K // group)):
-            raise ValueError(f"{name}{tuple(t.shape)}: [{N}, {K} / {group}] expected")
+        if t is not None and t.shape != (N, K // group):
+            raise ValueError(f"{name}{tuple(t.shape)}: [{N}, {K // group}] expected")
     d = abi.W4PackDesc()
     d.N, d.K, d.group = N, K, group
-    d.codes, d.ldc = codes.data_ptr(), max(codes.stride(0), K // 2)
-    d.scales, d.lds, d.scale_dtype = scales.data_ptr(), max(scales.stride(0), scales.shape[1]), _DT[scales.dtype]
+    d.codes, d.ldc = codes.data_ptr(), codes.stride(0) if N > 1 else half
+    d.scales, d.lds, d.scale_dtype = scales.data_ptr(), scales.stride(0) if N > 1 else K, _DT[scales.dtype]
     if zeros is not None:
-        d.zeros, d.ldz = zeros.data_ptr(), max(zeros.stride(0), zeros.shape[1])
-    with torch.cuda.device(codes.device):
-        out = torch.empty(abi.lib().sf_w4_bytes(N, K, group), dtype=torch.uint8, device=codes.device)
-        abi.check(abi.lib().sf_w4_pack(ctypes.byref(d), out.data_ptr(), _stream(codes)), "sf_w4_pack")
+        d.zeros, d.ldz = zeros.data_ptr(), zeros.stride(0) if N > 1 else K
+    out = torch.empty(need, dtype=torch.uint8, device=dev)
+    call_on(dev, "sf_w4_pack", abi.lib().sf_w4_pack, ctypes.byref(d), out.data_ptr())
     return W4(out, N, K, group, scales.dtype)
 
 
@@ -342,31 +374,44 @@ def gemm_w4(a, w, bias=None, act=abi.SF_ACT_NONE, out=None, out_dtype=None, accu
     """out[M, N] = act(a[M, K] W^T + bias) with 4-bit weights w (w4_pack); a
     bf16 or fp16, out_dtype a's unless given.  accumulate adds into an fp32
     `out`."""
-    _check(a, "a", _B16, w.data, 2)
-    M, K = a.shape
-    if K != w.K:
-        raise ValueError(f"a{tuple(a.shape)} against weights [{w.N}, {w.K}]")
-    if bias is not None:
-        _check(bias, "bias", (torch.float32,), a, 1)
-        if bias.numel() != w.N:
-            raise ValueError(f"bias{tuple(bias.shape)}: {w.N} elements expected")
+    dev, N, K = w.data.device, w.N, w.K
+    _check(a, "a", _B16, dev, 2)
+    M = a.shape[0]
+    if a.shape[1] != K:
+        raise ValueError(f"a{tuple(a.shape)} against weights [{N}, {K}]")
     if out is None:
         if accumulate:
             raise ValueError("accumulate adds into out: give one")
-        out = torch.empty(M, w.N, dtype=out_dtype or a.dtype, device=a.device)
-    _check(out, "out", tuple(_DT)[:3], a, 2)
-    if out.shape != (M, w.N) or (out_dtype is not None and out.dtype != out_dtype):
-        raise ValueError(f"out{tuple(out.shape)} {out.dtype}: [{M}, {w.N}] of {out_dtype or out.dtype} expected")
-    d = abi.GemmW4Desc()
-    d.M, d.N, d.K, d.group = M, w.N, K, w.group
-    d.A, d.lda, d.a_dtype = a.data_ptr(), a.stride(0) if M > 1 else max(a.stride(0), (K + 7) // 8 * 8), _DT[a.dtype]
-    d.W, d.scale_dtype = w.data.data_ptr(), _DT[w.scale_dtype]
-    d.bias, d.act = _p(bias), act
-    d.C, d.ldc, d.c_dtype = out.data_ptr(), out.stride(0) if M > 1 else max(out.stride(0), w.N), _DT[out.dtype]
-    d.accumulate = 1 if accumulate else 0
-    with torch.cuda.device(a.device):
-        abi.check(abi.lib().sf_gemm_w4(ctypes.byref(d), _stream(a)), "sf_gemm_w4")
+        out = torch.empty(M, N, dtype=out_dtype or a.dtype, device=dev)
+    else:
+        _check(out, "out", _FLOATS, dev, 2)
+        if out.shape != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError(f"out{tuple(out.shape)} {out.dtype}: [{M}, {N}] of {out_dtype or out.dtype} expected")
+    d = abi.GemmW4Desc(M, N, K, w.group, a.data_ptr(), a.stride(0) if M > 1 else K, _DT[a.dtype], w.data.data_ptr(),
+                       _DT[w.scale_dtype], _vector(bias, "bias", torch.float32, N, dev), act, out.data_ptr(),
+                       out.stride(0) if M > 1 else N, _DT[out.dtype], 1 if accumulate else 0)
+    call_on(dev, "sf_gemm_w4", abi.lib().sf_gemm_w4, ctypes.byref(d))
     return out
+
+
+# sf_heads_rope_desc in one pack (a ctypes structure of nested arrays takes 3 us to fill).
+_ROPE_DESC = struct.Struct("@8i3P9q3P9q2Pf4x2P2iP4iP")
+assert _ROPE_DESC.size == ctypes.sizeof(abi.HeadsRopeDesc)
+_NO_CACHE = (0, 0, 0, 0, 0)
+
+
+def _heads_rope(dev, n, head, src, src_st, out, out_st, D, gammas, positions, inv_freq, interleaved, eps, cache, slots):
+    """The call: head = (B, S, D, Hq, Hk, Hv, in_dtype, out_dtype), pointers and strides flat, n = B * S tokens."""
+    gq, gk = gammas
+    rot = 0 if inv_freq is None else 2 * inv_freq.numel()
+    if cache is not None and cache.data.device != dev:
+        raise ValueError(f"the cache must be on {dev}")
+    raw = _ROPE_DESC.pack(
+        *head, *src, *src_st, *out, *out_st, _vector(gq, "gamma", torch.float32, D, dev),
+        _vector(gk, "gamma", torch.float32, D, dev), eps, _vector(positions, "positions", torch.int32, n, dev),
+        _vector(inv_freq, "inv_freq", torch.float64, rot // 2, dev), rot, 1 if interleaved else 0,
+        *(_NO_CACHE if cache is None else cache.fields()), _vector(slots, "slots", torch.int32, n, dev))
+    call_on(dev, "sf_heads_rope", abi.lib().sf_heads_rope, ctypes.byref(abi.HeadsRopeDesc.from_buffer_copy(raw)))
 
 
 def heads_rope_strided(srcs, outs, gammas=(None, None), positions=None, inv_freq=None, interleaved=False, eps=1e-6,
@@ -377,53 +422,27 @@ def heads_rope_strided(srcs, outs, gammas=(None, None), positions=None, inv_freq
     like = next((t for t in srcs if t is not None), None)
     if like is None or len(srcs) != 3 or len(outs) != 3:
         raise ValueError("three sources and outputs, query, key and value, not all of them None")
-    F = tuple(_DT)[:3]
-    d = abi.HeadsRopeDesc()
-    B, _, S, D = like.shape if like.dim() == 4 else (0, 0, 0, 0)
-    out_like = None
+    _check(like, "source", _FLOATS, None, 4)
+    dev, (B, _, S, D) = like.device, like.shape
+    heads, src, src_st, out, out_st, out_dtype = [0, 0, 0], [0, 0, 0], [], [0, 0, 0], [], None
     for j, (t, o) in enumerate(zip(srcs, outs)):
-        if t is None:
-            if o is not None:
-                raise ValueError("an output without its source")
-            continue
-        _check(t, "source", F, like, 4)
-        if t.dtype != like.dtype or (t.shape[0], t.shape[2], t.shape[3]) != (B, S, D):
-            raise ValueError(f"source {tuple(t.shape)} {t.dtype} beside {tuple(like.shape)} {like.dtype}")
-        d.heads[j], d.src[j] = t.shape[1], t.data_ptr()
-        d.src_stride[j][:] = _strides_bhs(t)
-        if (o is None) != (cache is not None and j > 0):
+        if (o is None) != (t is None or (cache is not None and j > 0)):
             raise ValueError("an output for every source; none for keys and values that go into a cache")
+        if t is not None:
+            _check(t, "source", (like.dtype,), dev, 4)
+            if (t.shape[0], t.shape[2], t.shape[3]) != (B, S, D):
+                raise ValueError(f"source {tuple(t.shape)} beside {tuple(like.shape)}")
+            heads[j], src[j] = t.shape[1], t.data_ptr()
         if o is not None:
-            out_like = o if out_like is None else out_like
-            _check(o, "output", (out_like.dtype,) if out_like.dtype in F else F, like, 4)
+            out_dtype = out_dtype or o.dtype
+            _check(o, "output", (out_dtype,) if out_dtype in _FLOATS else _FLOATS, dev, 4)
             if o.shape != t.shape:
                 raise ValueError(f"output {tuple(o.shape)} for a source {tuple(t.shape)}")
-            d.out[j] = o.data_ptr()
-            d.out_stride[j][:] = _strides_bhs(o)
-    d.B, d.S, d.D = B, S, D
-    d.in_dtype, d.out_dtype = _DT[like.dtype], _DT[like.dtype if out_like is None else out_like.dtype]
-    for j, gm in enumerate(gammas):
-        if gm is not None:
-            _check(gm, "gamma", (torch.float32,), like, 1)
-            if gm.numel() != D:
-                raise ValueError(f"gamma{tuple(gm.shape)}: {D} elements expected")
-            d.gamma[j] = gm.data_ptr()
-    d.eps = eps
-    for name, t in (("positions", positions), ("slots", slots)):
-        if t is not None:
-            _check(t, name, (torch.int32,), like)
-            if t.numel() != B * S or not t.is_contiguous():
-                raise ValueError(f"{name}{tuple(t.shape)}: {B * S} contiguous elements expected")
-            setattr(d, name, t.data_ptr())
-    if inv_freq is not None:
-        _check(inv_freq, "inv_freq", (torch.float64,), like, 1)
-        d.inv_freq, d.rot, d.interleaved = inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0
-    if cache is not None:
-        if cache.data.device != like.device:
-            raise ValueError(f"the cache must be on {like.device}")
-        d.cache = cache.desc()
-    with torch.cuda.device(like.device):
-        abi.check(abi.lib().sf_heads_rope(ctypes.byref(d), _stream(like)), "sf_heads_rope")
+            out[j] = o.data_ptr()
+        src_st += (0, 0, 0) if t is None else strides_bhs(t)
+        out_st += (0, 0, 0) if o is None else strides_bhs(o)
+    _heads_rope(dev, B * S, (B, S, D, *heads, _DT[like.dtype], _DT[out_dtype or like.dtype]), src, src_st, out, out_st, D,
+                gammas, positions, inv_freq, interleaved, eps, cache, slots)
 
 
 def heads_rope(p, S, heads, D, gammas=(None, None), positions=None, inv_freq=None, interleaved=False, eps=1e-6,
@@ -437,15 +456,18 @@ def heads_rope(p, S, heads, D, gammas=(None, None), positions=None, inv_freq=Non
     negative position is padding and is not written.  With a cache
     (attention.Kv4Cache) keys and values go there, at `slots` (int32) or the
     positions.  Returns (q, k, v), None for what is left out or cached."""
-    _check(p, "p", tuple(_DT)[:3], dim=2)
-    if len(heads) != 3 or min(heads) < 0 or p.shape[1] != sum(heads) * D or S <= 0 or p.shape[0] % S:
+    _check(p, "p", _FLOATS, None, 2)
+    dev, (n, cols) = p.device, p.shape
+    Hq, Hk, Hv = heads
+    if min(heads) < 0 or cols != (Hq + Hk + Hv) * D or S <= 0 or n % S:
         raise ValueError(f"p{tuple(p.shape)}: rows of {sum(heads)} x {D} for tokens in groups of {S} expected")
-    B, srcs, outs, at = p.shape[0] // S, [], [], 0
-    for j, h in enumerate(heads):
-        t = p[:, at * D:(at + h) * D].unflatten(0, (B, S)).unflatten(2, (h, D)).transpose(1, 2) if h else None
-        cached = t is None or (cache is not None and j > 0)
-        srcs.append(t)
-        outs.append(None if cached else torch.empty(B, h, S, D, dtype=out_dtype or p.dtype, device=p.device))
-        at += h
-    heads_rope_strided(srcs, outs, gammas, positions, inv_freq, interleaved, eps, cache, slots)
-    return tuple(outs)
+    B, ld, base, dtype = n // S, p.stride(0) if n > 1 else 0, p.data_ptr(), out_dtype or p.dtype
+    step = D * p.element_size()
+    q, k, v = (torch.empty(B, h, S, D, dtype=dtype, device=dev) if h and (cache is None or j == 0) else None
+               for j, h in enumerate(heads))
+    _heads_rope(dev, n, (B, S, D, Hq, Hk, Hv, _DT[p.dtype], _DT[dtype]),
+                (base, base + Hq * step, base + (Hq + Hk) * step), (S * ld, D, ld) * 3,
+                tuple(0 if t is None else t.data_ptr() for t in (q, k, v)),
+                (Hq * S * D, S * D, D, Hk * S * D, S * D, D, Hv * S * D, S * D, D),
+                D, gammas, positions, inv_freq, interleaved, eps, cache, slots)
+    return q, k, v
