@@ -4,11 +4,11 @@
 // 64-channel group, so both contractions run on the codes themselves and the
 // parameters meet the scores in fp32:
 //   S_j = s_j sum_d q_d (16 + c_jd) + (mid_j - 23.5 s_j) sum_d q_d
-//   O_d = sum_j p_j s_j (16 + c_jd) - 23.5 sum_j p_j s_j + sum_j p_j mid_j
+//   O_d = sum_j p_j s_j (16 + c_jd) + sum_j p_j (mid_j - 23.5 s_j)
 // (16 + c: see sf_nibble.h).  p_j s_j enters the matrix unit as a bf16 (hi, lo)
-// pair, 2^-17 relative, and sum_j p_j s_j is taken over the same rounded pair
-// by an operand of ones, so the offset of 23.5 cancels exactly what the codes'
-// offset added.
+// pair, 2^-18 relative: the codes' offset triples what that rounding does to a
+// value, which one bf16 would make visible in a 16-bit output and the pair
+// keeps near fp32's own error.
 //
 // One wave takes blocks of 32 tokens against QT tiles of 16 query rows; query
 // heads that share a key head are rows of one tile, so a cached token is read
@@ -23,6 +23,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "sf_device.h"
 #include "sf_hip.h"
@@ -34,7 +35,7 @@ namespace sfk {
 constexpr int kKvWaves = 4;
 constexpr int kKvMaxSplits = 64;
 constexpr float kKvSlack = 8.f;       // log2
-constexpr float kKvNoMax = -1e30f;    // a row that has seen nothing
+constexpr float kKvNoMax = -1.5e38f;  // the maximum of a row that has seen nothing
 
 struct KvAttnArgs {
     const uint16_t* q;
@@ -93,12 +94,27 @@ struct KvBlock {
     }
 };
 
-template <bool F16, int D, int QT>
-__global__ __launch_bounds__(64 * kKvWaves) void attn_kv4_kernel(const KvAttnArgs p) {
+// The rare step of the running maximum: a row's scores x (less the old maximum
+// m, or as they are in a row that has seen nothing) exceed it by the slack.
+// Returns what the row's sums are to be scaled by.
+__device__ __forceinline__ float kv_raise(float (&x)[8], float mx, float& m) {
+    const bool first = m == kKvNoMax;
+    const float top = lanes4_max(mx), up = first ? (top == -INFINITY ? 0.f : top) : fmaxf(0.f, top);
+    m = first ? (top == -INFINITY ? kKvNoMax : top) : m + up;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] -= up;
+    return first ? 1.f : __builtin_amdgcn_exp2f(-up);   // first: nothing to scale
+}
+
+// PAIR: p s enters the second product as a bf16 (hi, lo) pair; otherwise p and
+// V as fp16.
+template <bool F16, int D, int QT, bool PAIR>
+__global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel(const KvAttnArgs p) {
     constexpr int GR = D / 64, DT = D / 16;   // 64-channel groups, tiles of 16 channels
     constexpr int kRow = DT * 4;              // floats of O per lane and tile
     __shared__ float xm[kKvWaves][QT][16], xl[kKvWaves][QT][16];
     __shared__ float xo[2][QT * kRow][64];
+    __shared__ u32x4 ql[QT > 1 ? QT * GR * 2 : 1][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, g = lane >> 4;
     const int split = blockIdx.x % p.splits;
@@ -119,56 +135,53 @@ __global__ __launch_bounds__(64 * kKvWaves) void attn_kv4_kernel(const KvAttnArg
     const int nblk = (max(lim_hi, 0) + kKvBlock - 1) / kKvBlock;
     const int b0 = (int)((int64_t)nblk * split / p.splits), b1 = (int)((int64_t)nblk * (split + 1) / p.splits);
 
-    u32x4 q[QT][GR][2];
+    // Query fragments: B operands, in registers for one tile, else in LDS for all four waves.
+    u32x4 qr[GR][2];
     float qs[QT][GR];
-    int limit[QT];
-    int64_t qrow[QT];   // the row's place in [B][Hq][Sq]
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int r = min(q0 + 16 * t + col, R - 1);
-        const int hq = h * p.G + r / p.Sq, s = r % p.Sq;
-        const uint16_t* src = p.q + b * p.qs[0] + hq * p.qs[1] + s * p.qs[2];
-        qrow[t] = ((int64_t)b * p.H * p.G + hq) * p.Sq + s;
-        limit[t] = p.causal ? len - p.Sq + 1 + s : len;
+        const uint16_t* src = p.q + b * p.qs[0] + (h * p.G + r / p.Sq) * p.qs[1] + r % p.Sq * p.qs[2];
 #pragma unroll
         for (int i = 0; i < GR; ++i) {
             float sum = 0.f;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                q[t][i][ks] = *reinterpret_cast<const u32x4*>(src + 64 * i + 16 * g + 8 * ks);
+                const u32x4 v = *reinterpret_cast<const u32x4*>(src + 64 * i + 16 * g + 8 * ks);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t u = q[t][i][ks][e];
-                    sum += F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)u) +
-                                     (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16))
-                               : __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
-                }
+                for (int e = 0; e < 4; ++e)
+                    sum += F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v[e]) +
+                                     (float)__builtin_bit_cast(_Float16, (uint16_t)(v[e] >> 16))
+                               : __uint_as_float(v[e] << 16) + __uint_as_float(v[e] & 0xffff0000u);
+                if (QT == 1) qr[i][ks] = v;
+                else if (wave == ((t * GR + i) & 3)) ql[(t * GR + i) * 2 + ks][lane] = v;
             }
             qs[t][i] = lanes4_sum(sum);
         }
     }
+    if (QT > 1) __syncthreads();
 
-    f32x4 o[QT][DT], one[QT][GR];   // O^T without the parameters' part; sum of the rounded p s
-    float m[QT], l[QT], pm[QT][GR];
+    f32x4 o[QT][DT];   // O^T; PAIR: without the parameters' part pm
+    float m[QT], l[QT], pm[QT][PAIR ? GR : 1];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         m[t] = kKvNoMax, l[t] = 0.f;
 #pragma unroll
-        for (int i = 0; i < GR; ++i) pm[t][i] = 0.f, one[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < (PAIR ? GR : 1); ++i) pm[t][i] = 0.f;
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    // fp16 form: values are held times `vdown`, a power of two that keeps every one seen below 2^15, fp16's top
+    // binade (the smaller ones then stay normal over a range of 2^29); `vcap` = 2^15 / vdown.
+    float vdown = 1.f, vcap = 0.f;
     const uint8_t* base = p.cache + (int64_t)bh * p.cache_blocks * Kv4<D>::kBytes;
 
     KvBlock<D> nx;
     if (b0 + wave < b1) nx.load(base + (int64_t)(b0 + wave) * Kv4<D>::kBytes, lane);
-    for (int blk = b0 + wave; blk < b1; blk += kKvWaves) {
-        const KvBlock<D> kv = nx;
-        if (blk + kKvWaves < b1) nx.load(base + (int64_t)(blk + kKvWaves) * Kv4<D>::kBytes, lane);
+
+    auto block = [&](const int blk, auto masked_c) __attribute__((always_inline)) {
+        constexpr bool masked = decltype(masked_c)::value;
         const int key0 = kKvBlock * blk;
-        const bool masked = p.mask || key0 + kKvBlock > lim_lo;
-        float ks[GR][8], ko[GR][8], vs[GR][8], vm[GR][8];
         uint32_t see = 0xffu;   // the lane's 8 tokens, by length and mask
         if (masked) {
             see = 0;
@@ -178,16 +191,19 @@ __global__ __launch_bounds__(64 * kKvWaves) void attn_kv4_kernel(const KvAttnArg
                 if (key < len && (!p.mask || p.mask[b * p.mask_stride + key])) see |= 1u << e;
             }
         }
+        float ks[GR][8], ko[GR][8], vs[GR][8], vm[GR][8];
 #pragma unroll
         for (int i = 0; i < GR; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                uint32_t kp = kv.kp[i][e >> 2][e & 3], vp = kv.vp[i][e >> 2][e & 3];
+                uint32_t kp = nx.kp[i][e >> 2][e & 3], vp = nx.vp[i][e >> 2][e & 3];
                 if (masked && !(see >> e & 1u)) kp = vp = 0u;   // tokens behind the last hold anything
+                if (masked && !PAIR && (vp & 0x7f80u) == 0x7f80u) kp |= 0x7fc07fc0u, vp = 0u;   // see below
                 ks[i][e] = __uint_as_float(kp << 16) * p.scale_log2;
                 ko[i][e] = __uint_as_float(kp & 0xffff0000u) * p.scale_log2 - 23.5f * ks[i][e];
                 vs[i][e] = __uint_as_float(vp << 16);
                 vm[i][e] = __uint_as_float(vp & 0xffff0000u);
+                if (PAIR) vm[i][e] -= 23.5f * vs[i][e];
             }
         u32x4 ka[2][GR][2], va[DT];
 #pragma unroll
@@ -195,80 +211,137 @@ __global__ __launch_bounds__(64 * kKvWaves) void attn_kv4_kernel(const KvAttnArg
 #pragma unroll
             for (int i = 0; i < GR; ++i)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) ka[t][i][k] = nibbles_plus16<F16>(kv.key(t, i, k));
+                for (int k = 0; k < 2; ++k) ka[t][i][k] = nibbles_plus16<F16>(nx.key(t, i, k));
 #pragma unroll
         for (int t = 0; t < DT / 2; ++t) {
-            const uint32_t w0 = kv.v[t >> 1][2 * (t & 1)], w1 = kv.v[t >> 1][2 * (t & 1) + 1];
-            va[2 * t] = u32x4{nibble_pair_plus16<false, 0>(w0), nibble_pair_plus16<false, 2>(w0),
-                              nibble_pair_plus16<false, 0>(w1), nibble_pair_plus16<false, 2>(w1)};
-            va[2 * t + 1] = u32x4{nibble_pair_plus16<false, 1>(w0), nibble_pair_plus16<false, 3>(w0),
-                                  nibble_pair_plus16<false, 1>(w1), nibble_pair_plus16<false, 3>(w1)};
+            const uint32_t w0 = nx.v[t >> 1][2 * (t & 1)], w1 = nx.v[t >> 1][2 * (t & 1) + 1];
+            va[2 * t] = u32x4{nibble_pair_plus16<!PAIR, 0>(w0), nibble_pair_plus16<!PAIR, 2>(w0),
+                              nibble_pair_plus16<!PAIR, 0>(w1), nibble_pair_plus16<!PAIR, 2>(w1)};
+            va[2 * t + 1] = u32x4{nibble_pair_plus16<!PAIR, 1>(w0), nibble_pair_plus16<!PAIR, 3>(w0),
+                                  nibble_pair_plus16<!PAIR, 1>(w1), nibble_pair_plus16<!PAIR, 3>(w1)};
         }
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        if (!PAIR) {
+            float big = 0.f;
 #pragma unroll
             for (int i = 0; i < GR; ++i)
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-                    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-                    s = mfma_16b<F16>(ka[kt][i][0], q[t][i][0], s);
-                    s = mfma_16b<F16>(ka[kt][i][1], q[t][i][1], s);
+                for (int e = 0; e < 8; ++e) big = fmaxf(big, __builtin_fmaf(8.f, vs[i][e], fabsf(vm[i][e])));
+            if (__any(big > vcap)) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x[4 * kt + e] = __builtin_fmaf(
-                            ks[i][4 * kt + e], s[e], __builtin_fmaf(ko[i][4 * kt + e], qs[t][i], x[4 * kt + e]));
+                for (int w = 1; w < 64; w <<= 1) big = fmaxf(big, __shfl_xor(big, w, 64));
+                const int ex = max((int)(__float_as_uint(big) >> 23) - 127 - 14, -100);   // big < 2^(ex + 15)
+                const float nd = __uint_as_float((uint32_t)(127 - ex) << 23), al = nd / vdown;
+                vcap = __uint_as_float((uint32_t)(127 + ex) << 23) * 32768.f;
+                vdown = nd;
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int i = 0; i < DT; ++i) o[t][i] *= al;
+            }
+#pragma unroll
+            for (int i = 0; i < GR; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {   // pairs of tokens: (c - 7.5) s + mid, one rounding
+                    const f16x2v sp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vs[i][2 * e] * vdown, vs[i][2 * e + 1] * vdown));
+                    const f16x2v mp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vm[i][2 * e] * vdown, vm[i][2 * e + 1] * vdown));
+#pragma unroll
+                    for (int t = 4 * i; t < 4 * i + 4; ++t) {
+                        const uint32_t w = va[t][e];   // a value: bit_cast of a vector's element reads its first one
+                        const f16x2v c = __builtin_bit_cast(f16x2v, w) - f16x2v{(_Float16)23.5f, (_Float16)23.5f};
+                        va[t][e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, sp, mp));
+                    }
+                }
+        }
+        // the raw block is spent: fetch the wave's next one
+        if (blk + kKvWaves < b1) nx.load(base + (int64_t)(blk + kKvWaves) * Kv4<D>::kBytes, lane);
+
+        f32x4 s[2][2][GR];   // this tile's raw scores and the next one's, issued a tile ahead
+        auto scores = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < GR; ++i) {
+                const u32x4 qa = QT == 1 ? qr[i][0] : ql[(t * GR + i) * 2][lane];
+                const u32x4 qb = QT == 1 ? qr[i][1] : ql[(t * GR + i) * 2 + 1][lane];
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+                    s[t & 1][kt][i] = mfma_16b<F16>(ka[kt][i][1], qb, mfma_16b<F16>(ka[kt][i][0], qa, f32x4{0.f, 0.f, 0.f, 0.f}));
+            }
+        };
+        scores(0);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            if (t + 1 < QT) scores(t + 1);
+            float x[8];   // scores less the row's maximum, base 2
+            const float neg = m[t] == kKvNoMax ? 0.f : -m[t];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float u = neg;
+#pragma unroll
+                    for (int i = 0; i < GR; ++i)
+                        u = __builtin_fmaf(ks[i][4 * kt + e], s[t & 1][kt][i][e], __builtin_fmaf(ko[i][4 * kt + e], qs[t][i], u));
+                    x[4 * kt + e] = u;
                 }
             uint32_t row = see;
             if (masked) {
+                const int limit = p.causal ? len - p.Sq + 1 + min(q0 + 16 * t + col, R - 1) % p.Sq : len;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) >= limit[t]) row &= ~(1u << e);
+                    if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) >= limit) row &= ~(1u << e);
                     if (!(row >> e & 1u)) x[e] = -INFINITY;
                 }
             }
             const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            if (__any(mx > m[t] + kKvSlack)) {
-                const float nm = fmaxf(m[t], lanes4_max(mx)), al = __builtin_amdgcn_exp2f(m[t] - nm);
-                m[t] = nm;
+            if (__any(mx > (m[t] == kKvNoMax ? -INFINITY : kKvSlack))) {
+                const float al = kv_raise(x, mx, m[t]);
                 l[t] *= al;
 #pragma unroll
-                for (int i = 0; i < GR; ++i) pm[t][i] *= al, one[t][i] *= al;
+                for (int i = 0; i < (PAIR ? GR : 1); ++i) pm[t][i] *= al;
 #pragma unroll
                 for (int i = 0; i < DT; ++i) o[t][i] *= al;
             }
-            float pr[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                pr[e] = __builtin_amdgcn_exp2f(x[e] - m[t]);
-                l[t] += pr[e];
-            }
+            for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(x[e]);
+            if (PAIR) {
 #pragma unroll
-            for (int i = 0; i < GR; ++i) {
-                u32x4 hi, lo;
+                for (int e = 0; e < 8; ++e) l[t] += x[e];
+#pragma unroll
+                for (int i = 0; i < GR; ++i) {
+                    u32x4 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float a = x[2 * e] * vs[i][2 * e], c = x[2 * e + 1] * vs[i][2 * e + 1];
+                        float ma = x[2 * e] * vm[i][2 * e], mc = x[2 * e + 1] * vm[i][2 * e + 1];
+                        if (masked) {   // a token that only later rows see may hold NaN parameters
+                            if (!(row >> (2 * e) & 1u)) a = ma = 0.f;
+                            if (!(row >> (2 * e + 1) & 1u)) c = mc = 0.f;
+                        }
+                        pm[t][i] += ma + mc;
+                        hi[e] = pack_bf16x2(a, c);
+                        lo[e] = pack_bf16x2(a - __uint_as_float(hi[e] << 16), c - __uint_as_float(hi[e] & 0xffff0000u));
+                    }
+#pragma unroll
+                    for (int d = 4 * i; d < 4 * i + 4; ++d) {
+                        o[t][d] = mfma_16b<false>(va[d], hi, o[t][d]);
+                        o[t][d] = mfma_16b<false>(va[d], lo, o[t][d]);
+                    }
+                }
+            } else {   // the sum is taken over the rounded p, as the product is
+                u32x4 ph;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float a = pr[2 * e] * vs[i][2 * e], c = pr[2 * e + 1] * vs[i][2 * e + 1];
-                    float ma = pr[2 * e] * vm[i][2 * e], mc = pr[2 * e + 1] * vm[i][2 * e + 1];
-                    if (masked) {   // a token only later rows see may hold NaN parameters
-                        if (!(row >> (2 * e) & 1u)) a = ma = 0.f;
-                        if (!(row >> (2 * e + 1) & 1u)) c = mc = 0.f;
-                    }
-                    pm[t][i] += ma + mc;
-                    hi[e] = pack_bf16x2(a, c);
-                    lo[e] = pack_bf16x2(a - __uint_as_float(hi[e] << 16), c - __uint_as_float(hi[e] & 0xffff0000u));
+                    const uint32_t w = pack_f16x2_rn(x[2 * e], x[2 * e + 1]);
+                    ph[e] = w;
+                    l[t] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2v, w), f16x2v{(_Float16)1.f, (_Float16)1.f}, l[t], false);
                 }
-                one[t][i] = mfma_16b<false>(ones, hi, one[t][i]);
-                one[t][i] = mfma_16b<false>(ones, lo, one[t][i]);
 #pragma unroll
-                for (int d = 4 * i; d < 4 * i + 4; ++d) {
-                    o[t][d] = mfma_16b<false>(va[d], hi, o[t][d]);
-                    o[t][d] = mfma_16b<false>(va[d], lo, o[t][d]);
-                }
+                for (int d = 0; d < DT; ++d) o[t][d] = mfma_16b<true>(va[d], ph, o[t][d]);
             }
         }
+    };
+    for (int blk = b0 + wave; blk < b1; blk += kKvWaves) {
+        if (p.mask || kKvBlock * (blk + 1) > lim_lo) block(blk, std::true_type{});
+        else block(blk, std::false_type{});
     }
 
     // The waves' rows meet: common maximum, then two rounds of adds through LDS.
@@ -277,11 +350,11 @@ __global__ __launch_bounds__(64 * kKvWaves) void attn_kv4_kernel(const KvAttnArg
         l[t] = lanes4_sum(l[t]);
 #pragma unroll
         for (int i = 0; i < GR; ++i) {
-            const float add = lanes4_sum(pm[t][i]) - 23.5f * one[t][i][0];
+            const float add = PAIR ? lanes4_sum(pm[t][PAIR ? i : 0]) : 0.f, by = PAIR ? 1.f : 1.f / vdown;
 #pragma unroll
             for (int d = 4 * i; d < 4 * i + 4; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[t][d][e] += add;
+                for (int e = 0; e < 4; ++e) o[t][d][e] = o[t][d][e] * by + add;
         }
         if (g == 0) xm[wave][t][col] = m[t];
     }
@@ -333,7 +406,9 @@ __global__ __launch_bounds__(64 * kKvWaves) void attn_kv4_kernel(const KvAttnArg
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[t][d][e] += xo[0][t * kRow + 4 * d + e][lane];
         if (p.splits > 1) {
-            float* dst = p.part + ((int64_t)split * p.rows + qrow[t]) * (D + 2);
+            const int r = q0 + 16 * t + col;
+            const int64_t row = ((int64_t)b * p.H * p.G + h * p.G + r / p.Sq) * p.Sq + r % p.Sq;
+            float* dst = p.part + ((int64_t)split * p.rows + row) * (D + 2);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -391,11 +466,11 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(const KvAttnArgs p)
 
 // Tiles of 16 query rows a workgroup takes, of those the kernel is built for:
 // the fewest passes over the keys first, then the fewest idle rows.
-static int kv_tiles(int rows) {
+static int kv_tiles(int D, int rows) {
     const int tiles = (rows + 15) / 16;
-    const int most = 2;
+    const int most = D == 64 ? 5 : 2;
     const int per = (tiles + (tiles + most - 1) / most - 1) / ((tiles + most - 1) / most);
-    return per;
+    return per <= 2 ? per : most;
 }
 
 struct KvPlan {
@@ -406,7 +481,7 @@ struct KvPlan {
 static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
     KvPlan k;
     const int R = d->Hq / d->cache.H * d->Sq;
-    k.qt = kv_tiles(R);
+    k.qt = kv_tiles(d->cache.D, R);
     k.qgroups = (R + 16 * k.qt - 1) / (16 * k.qt);
     k.rows = (int64_t)d->B * d->Hq * d->Sq;
     const int64_t base = (int64_t)d->B * d->cache.H * k.qgroups;
@@ -482,17 +557,22 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)k.wgs), block(64 * sfk::kKvWaves);
     const bool f16 = d->in_dtype == SF_F16;
-#define SF_KV4_LAUNCH(DD, QT)                                                                       \
-    do {                                                                                            \
-        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT>), grid, block, 0, s, p);    \
-        else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT>), grid, block, 0, s, p);       \
+#define SF_KV4_LAUNCH(DD, QT, PAIR)                                                                      \
+    do {                                                                                                 \
+        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT, PAIR>), grid, block, 0, s, p);   \
+        else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT, PAIR>), grid, block, 0, s, p);      \
     } while (0)
+    const bool pair = d->out_dtype != SF_BF16;
     if (d->cache.D == 64) {
-        if (k.qt == 1) SF_KV4_LAUNCH(64, 1);
-        else SF_KV4_LAUNCH(64, 2);
+        if (k.qt == 1) SF_KV4_LAUNCH(64, 1, true);
+        else if (k.qt == 2 && pair) SF_KV4_LAUNCH(64, 2, true);
+        else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, false);
+        else if (pair) SF_KV4_LAUNCH(64, 5, true);
+        else SF_KV4_LAUNCH(64, 5, false);
     } else {
-        if (k.qt == 1) SF_KV4_LAUNCH(128, 1);
-        else SF_KV4_LAUNCH(128, 2);
+        if (k.qt == 1) SF_KV4_LAUNCH(128, 1, true);
+        else if (pair) SF_KV4_LAUNCH(128, 2, true);
+        else SF_KV4_LAUNCH(128, 2, false);
     }
 #undef SF_KV4_LAUNCH
     if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;

@@ -12,7 +12,10 @@ Tolerances, from the arithmetic.
   attention, against the values that the cache stands for: a score is off by
   the roundings of its sums (24 of 2^-24 of scale * sum |q| (|k| + 40 s)); p by
   that and by exp2's 2^-22; the (hi, lo) pair by 2^-17; sums over tokens by
-  (32 + tokens / 32) 2^-24 of 55 s / max |v| <= 16 times the largest value."""
+  (32 + tokens / 32) 2^-24 of 55 s / max |v| <= 16 times the largest value.  A
+  bf16 output of more than 16 rows to a key head takes p and V in fp16 instead
+  of the pair: p, its sum and V round by 2^-12 each, 3 2^-12 of the largest
+  value together."""
 import math
 
 import pytest
@@ -219,6 +222,8 @@ def _attn_check(got, q, k, v, dtype, scale=0.0, what="", **kw):
     # |k| + 40 s: s is at most a sixteenth of a row's spread, itself at most twice its largest value
     dx = 24 * 2.0 ** -24 * sc * float(q.double().abs().sum(-1).max()) * float(k.abs().max()) * 6 if k.numel() else 0.0
     rel = 2 * (dx + 2.0 ** -22) + 2.0 ** -16 + (32 + Sk / 32) * 2.0 ** -24 * 16
+    if dtype == BF and q.shape[1] // k.shape[1] * q.shape[2] > 16:
+        rel += 3 * 2.0 ** -12
     tol = rel * float(v.abs().max()) + half_step(dtype) * ref.abs()
     if dtype == FP:
         tol = tol + 2.0 ** -25
@@ -334,3 +339,40 @@ def test_runs_are_equal_and_splits_agree():
     for _ in range(3):
         assert torch.equal(one, attention_kv4(q, c, out_dtype=F32))
     _attn_check(attention_kv4(q, c, num_splits=5, out_dtype=F32), q.cpu(), k, v, F32)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_bf16_rows_of_many_tiles(D):
+    """Many query rows with a bf16 output: V in fp16 under a common power of two, p in fp16 (2^-11 together)."""
+    B, Hq, H, Sq, Sk = 2, 4, 2, 67, 333
+    k = _randn(90, B, H, Sk, D, dtype=BF)
+    v = _randn(91, B, H, Sk, D, dtype=BF)
+    v[0] *= 2.0 ** 100          # beyond fp16's range, a head at a time
+    v[1, 1] *= 2.0 ** -100
+    v[0, 0, ::5] *= 2.0 ** -20  # and within one
+    v[1, 0, 200:] *= 2.0 ** 30  # a common power that has to move
+    c = Kv4Cache(B, H, Sk, D, DEV)
+    c.write(k.to(DEV), v.to(DEV))
+    q = _randn(92, B, Hq, Sq, D, dtype=BF)
+    got = attention_kv4(q.to(DEV), c).cpu().double()
+    lk, lv = kv4_levels(k), kv4_levels(v)
+    ref = attend(q, lk, lv)
+    for b in range(B):
+        for h in range(Hq):
+            tol = 2.0 ** -10 * float(lv[b, h // 2].abs().max()) + half_step(BF) * ref[b, h].abs()
+            assert ((got[b, h] - ref[b, h]).abs() <= tol).all(), (b, h)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_causal_nan_with_bf16_output(D):
+    B, H, Sk = 1, 1, 70
+    c, k, v = _filled(B, H, Sk, D, BF, 93)
+    good = _randn(94, 1, 1, 1, D, dtype=BF)
+    bad = good.clone()
+    bad[..., 5] = float("inf")
+    c.write(good.to(DEV), bad.to(DEV), torch.tensor([[30]], dtype=torch.int32, device=DEV))
+    q = _randn(95, B, H, Sk, D, dtype=BF)
+    got = attention_kv4(q.to(DEV), c, is_causal=True)
+    ref = attend(q[:, :, :30], k[:, :, :30], v[:, :, :30], causal=True)
+    assert ((got[:, :, :30].cpu().double() - ref).abs() <= 2.0 ** -10 * 5 + half_step(BF) * ref.abs()).all()
+    assert torch.isnan(got[:, :, 30:, :64]).all()
