@@ -176,6 +176,7 @@ __global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel
     float vdown = 1.f, vcap = 0.f;
     const uint8_t* base = p.cache + (int64_t)bh * p.cache_blocks * Kv4<D>::kBytes;
 
+    const NibbleMask kmask = nibble_mask<F16>(), vmask = nibble_mask<!PAIR>();
     KvBlock<D> nx;
     if (b0 + wave < b1) nx.load(base + (int64_t)(b0 + wave) * Kv4<D>::kBytes, lane);
 
@@ -211,14 +212,14 @@ __global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel
 #pragma unroll
             for (int i = 0; i < GR; ++i)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) ka[t][i][k] = nibbles_plus16<F16>(nx.key(t, i, k));
+                for (int k = 0; k < 2; ++k) ka[t][i][k] = nibbles_plus16<F16>(nx.key(t, i, k), kmask);
 #pragma unroll
         for (int t = 0; t < DT / 2; ++t) {
             const uint32_t w0 = nx.v[t >> 1][2 * (t & 1)], w1 = nx.v[t >> 1][2 * (t & 1) + 1];
-            va[2 * t] = u32x4{nibble_pair_plus16<!PAIR, 0>(w0), nibble_pair_plus16<!PAIR, 2>(w0),
-                              nibble_pair_plus16<!PAIR, 0>(w1), nibble_pair_plus16<!PAIR, 2>(w1)};
-            va[2 * t + 1] = u32x4{nibble_pair_plus16<!PAIR, 1>(w0), nibble_pair_plus16<!PAIR, 3>(w0),
-                                  nibble_pair_plus16<!PAIR, 1>(w1), nibble_pair_plus16<!PAIR, 3>(w1)};
+            va[2 * t] = u32x4{nibble_pair_plus16<!PAIR, 0>(w0, vmask), nibble_pair_plus16<!PAIR, 2>(w0, vmask),
+                              nibble_pair_plus16<!PAIR, 0>(w1, vmask), nibble_pair_plus16<!PAIR, 2>(w1, vmask)};
+            va[2 * t + 1] = u32x4{nibble_pair_plus16<!PAIR, 1>(w0, vmask), nibble_pair_plus16<!PAIR, 3>(w0, vmask),
+                                  nibble_pair_plus16<!PAIR, 1>(w1, vmask), nibble_pair_plus16<!PAIR, 3>(w1, vmask)};
         }
         if (!PAIR) {
             float big = 0.f;
@@ -437,7 +438,7 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(const KvAttnArgs p)
     float mm = m;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
-    const float w = __builtin_amdgcn_exp2f(m - mm);
+    const float w = lane < p.splits ? __builtin_amdgcn_exp2f(m - mm) : 0.f;
     float sum = l * w;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -445,10 +446,18 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(const KvAttnArgs p)
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float ws = __shfl(w, s, 64);
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {   // eight splits' loads in flight
+        float v[8][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += ws * src[s * step + 64 * e + lane];
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[j][e] = s0 + j < p.splits ? src[(s0 + j) * step + 64 * e + lane] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float ws = __shfl(w, s0 + j, 64);   // 0 behind the last split
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += ws * v[j][e];
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int s = (int)(row % p.Sq);
@@ -488,8 +497,8 @@ static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
     if (d->num_splits > 0) {
         k.splits = d->num_splits;
     } else {
-        // about two workgroups a CU, and at least two blocks a wave
-        const int64_t want = (512 + base - 1) / base, most = (d->Sk + 255) / 256;
+        // about two workgroups a CU (one of five tiles), and at least two blocks a wave
+        const int64_t want = ((k.qt > 2 ? 256 : 512) + base - 1) / base, most = (d->Sk + 255) / 256;
         k.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kKvMaxSplits}));
     }
     k.wgs = base * k.splits;

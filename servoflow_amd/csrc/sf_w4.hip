@@ -62,6 +62,7 @@ __global__ __launch_bounds__(64 * WK) void gemm_w4_kernel(const W4Args p) {
 #pragma unroll
         for (int b = 0; b < MB; ++b) acc[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    const NibbleMask nmask = nibble_mask<F16>();
     const u32x4 ones = F16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
                            : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
     for (int kb = wk; kb < p.KB; kb += WK) {
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(64 * WK) void gemm_w4_kernel(const W4Args p) {
                 for (int b = 0; b < MB; ++b) sx[b] = mfma_16b<F16>(ones, x[b][j], sx[b]);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const u32x4 w = nibbles_plus16<F16>(code[t][j]);
+                    const u32x4 w = nibbles_plus16<F16>(code[t][j], nmask);
 #pragma unroll
                     for (int b = 0; b < MB; ++b) pr[t][b] = mfma_16b<F16>(w, x[b][j], pr[t][b]);
                 }
