@@ -32,7 +32,6 @@
 
 namespace sfk {
 
-constexpr int kKvWaves = 4;
 constexpr int kKvMaxSplits = 64;
 constexpr float kKvSlack = 8.f;       // log2
 constexpr float kKvNoMax = -1.5e38f;  // the maximum of a row that has seen nothing
@@ -51,13 +50,23 @@ struct KvAttnArgs {
     float scale_log2;
 };
 
-// Four channels to out: kind 0 fp32, 1 bf16, 2 fp16.
-__device__ __forceinline__ void kv_store4(void* out, int64_t at, int kind, f32x4 o) {
-    if (kind == 0) *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = o;
-    else
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) =
-            kind == 1 ? uint2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])}
-                      : uint2{pack_f16x2_rn(o[0], o[1]), pack_f16x2_rn(o[2], o[3])};
+// N consecutive channels to out: kind 0 fp32, 1 bf16, 2 fp16 (stores of 2 N and 4 N bytes, N even).
+template <int N>
+__device__ __forceinline__ void kv_store(void* out, int64_t at, int kind, const float (&y)[N]) {
+    typedef float fv __attribute__((ext_vector_type(N)));
+    typedef uint32_t uv __attribute__((ext_vector_type(N / 2)));
+    if (kind == 0) {
+        fv v;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = y[e];
+        *reinterpret_cast<fv*>(static_cast<float*>(out) + at) = v;
+        return;
+    }
+    uv u;
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e)
+        u[e] = kind == 1 ? pack_bf16x2(y[2 * e], y[2 * e + 1]) : pack_f16x2_rn(y[2 * e], y[2 * e + 1]);
+    *reinterpret_cast<uv*>(static_cast<uint16_t*>(out) + at) = u;
 }
 
 __device__ __forceinline__ float lanes4_sum(float x) {   // over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -67,6 +76,11 @@ __device__ __forceinline__ float lanes4_sum(float x) {   // over lanes l, l ^ 16
 __device__ __forceinline__ float lanes4_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16, 64));
     return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+
+// mid - 23.5 s of a parameter dword (both exact in the dot product's operands).
+__device__ __forceinline__ float kv_offset(uint32_t par) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v, par), bf16x2v{(__bf16)-23.5f, (__bf16)1.f}, 0.f, false);
 }
 
 // What a wave holds of a block of 32 tokens.
@@ -108,12 +122,11 @@ __device__ __forceinline__ float kv_raise(float (&x)[8], float mx, float& m) {
 
 // PAIR: p s enters the second product as a bf16 (hi, lo) pair; otherwise p and
 // V as fp16.
-template <bool F16, int D, int QT, bool PAIR>
-__global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel(const KvAttnArgs p) {
+template <bool F16, int D, int QT, bool PAIR, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     constexpr int GR = D / 64, DT = D / 16;   // 64-channel groups, tiles of 16 channels
-    constexpr int kRow = DT * 4;              // floats of O per lane and tile
-    __shared__ float xm[kKvWaves][QT][16], xl[kKvWaves][QT][16];
-    __shared__ float xo[2][QT * kRow][64];
+    __shared__ float xm[NW][QT * 16], xl[NW][QT * 16], xf[NW][QT * 16], xs[QT * 16];
+    __shared__ float xo[NW][16][D + 4];
     __shared__ u32x4 ql[QT > 1 ? QT * GR * 2 : 1][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, g = lane >> 4;
@@ -135,30 +148,39 @@ __global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel
     const int nblk = (max(lim_hi, 0) + kKvBlock - 1) / kKvBlock;
     const int b0 = (int)((int64_t)nblk * split / p.splits), b1 = (int)((int64_t)nblk * (split + 1) / p.splits);
 
-    // Query fragments: B operands, in registers for one tile, else in LDS for all four waves.
-    u32x4 qr[GR][2];
+    const uint8_t* base = p.cache + (int64_t)bh * p.cache_blocks * Kv4<D>::kBytes;
+    KvBlock<D> nx;
+    if (b0 + wave < b1) nx.load(base + (int64_t)(b0 + wave) * Kv4<D>::kBytes, lane);
+
+    // Query fragments: B operands, in registers for one tile, else in LDS for all waves.
+    u32x4 qr[QT][GR][2];
     float qs[QT][GR];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int r = min(q0 + 16 * t + col, R - 1);
         const uint16_t* src = p.q + b * p.qs[0] + (h * p.G + r / p.Sq) * p.qs[1] + r % p.Sq * p.qs[2];
 #pragma unroll
+        for (int i = 0; i < GR; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) qr[t][i][k] = *reinterpret_cast<const u32x4*>(src + 64 * i + 16 * g + 8 * k);
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
         for (int i = 0; i < GR; ++i) {
             float sum = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(src + 64 * i + 16 * g + 8 * ks);
+            for (int k = 0; k < 2; ++k) {
+                const u32x4 v = qr[t][i][k];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     sum += F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v[e]) +
                                      (float)__builtin_bit_cast(_Float16, (uint16_t)(v[e] >> 16))
                                : __uint_as_float(v[e] << 16) + __uint_as_float(v[e] & 0xffff0000u);
-                if (QT == 1) qr[i][ks] = v;
-                else if (wave == ((t * GR + i) & 3)) ql[(t * GR + i) * 2 + ks][lane] = v;
+                if (QT > 1 && wave == (t * GR + i) % NW) ql[(t * GR + i) * 2 + k][lane] = v;
             }
-            qs[t][i] = lanes4_sum(sum);
+            qs[t][i] = lanes4_sum(sum) * p.scale_log2;
         }
-    }
     if (QT > 1) __syncthreads();
 
     f32x4 o[QT][DT];   // O^T; PAIR: without the parameters' part pm
@@ -171,14 +193,11 @@ __global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // fp16 form: values are held times `vdown`, a power of two that keeps every one seen below 2^15, fp16's top
-    // binade (the smaller ones then stay normal over a range of 2^29); `vcap` = 2^15 / vdown.
+    // fp16 form: values are held times `vdown`, a power of two that keeps |mid - 23.5 s| + 31 s, and with it both terms
+    // and the value, below 2^15 for every token seen: 1 where they fit as they are, else such that the largest is in
+    // fp16's upper binades and smaller ones stay normal over 2^29.  `vcap` = 2^15 / vdown.
     float vdown = 1.f, vcap = 0.f;
-    const uint8_t* base = p.cache + (int64_t)bh * p.cache_blocks * Kv4<D>::kBytes;
-
     const NibbleMask kmask = nibble_mask<F16>(), vmask = nibble_mask<!PAIR>();
-    KvBlock<D> nx;
-    if (b0 + wave < b1) nx.load(base + (int64_t)(b0 + wave) * Kv4<D>::kBytes, lane);
 
     auto block = [&](const int blk, auto masked_c) __attribute__((always_inline)) {
         constexpr bool masked = decltype(masked_c)::value;
@@ -201,10 +220,9 @@ __global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel
                 if (masked && !(see >> e & 1u)) kp = vp = 0u;   // tokens behind the last hold anything
                 if (masked && !PAIR && (vp & 0x7f80u) == 0x7f80u) kp |= 0x7fc07fc0u, vp = 0u;   // see below
                 ks[i][e] = __uint_as_float(kp << 16) * p.scale_log2;
-                ko[i][e] = __uint_as_float(kp & 0xffff0000u) * p.scale_log2 - 23.5f * ks[i][e];
+                ko[i][e] = kv_offset(kp);
                 vs[i][e] = __uint_as_float(vp << 16);
-                vm[i][e] = __uint_as_float(vp & 0xffff0000u);
-                if (PAIR) vm[i][e] -= 23.5f * vs[i][e];
+                vm[i][e] = kv_offset(vp);
             }
         u32x4 ka[2][GR][2], va[DT];
 #pragma unroll
@@ -226,11 +244,13 @@ __global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel
 #pragma unroll
             for (int i = 0; i < GR; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) big = fmaxf(big, __builtin_fmaf(8.f, vs[i][e], fabsf(vm[i][e])));
+                for (int e = 0; e < 8; ++e) big = fmaxf(big, __builtin_fmaf(31.f, vs[i][e], fabsf(vm[i][e])));
             if (__any(big > vcap)) {
 #pragma unroll
                 for (int w = 1; w < 64; w <<= 1) big = fmaxf(big, __shfl_xor(big, w, 64));
-                const int ex = max((int)(__float_as_uint(big) >> 23) - 127 - 14, -100);   // big < 2^(ex + 15)
+                int ex = (int)(__float_as_uint(big) >> 23) - 127 - 14;   // big < 2^(ex + 15)
+                if (vcap == 0.f && ex <= 0 && ex >= -16) ex = 0;         // fp16 holds them as they are
+                ex = __builtin_amdgcn_readfirstlane(max(ex, -100));
                 const float nd = __uint_as_float((uint32_t)(127 - ex) << 23), al = nd / vdown;
                 vcap = __uint_as_float((uint32_t)(127 + ex) << 23) * 32768.f;
                 vdown = nd;
@@ -239,29 +259,34 @@ __global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel
 #pragma unroll
                     for (int i = 0; i < DT; ++i) o[t][i] *= al;
             }
+            if (vdown != 1.f) {
+#pragma unroll
+                for (int i = 0; i < GR; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) vs[i][e] *= vdown, vm[i][e] *= vdown;
+            }
 #pragma unroll
             for (int i = 0; i < GR; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {   // pairs of tokens: (c - 7.5) s + mid, one rounding
-                    const f16x2v sp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vs[i][2 * e] * vdown, vs[i][2 * e + 1] * vdown));
-                    const f16x2v mp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vm[i][2 * e] * vdown, vm[i][2 * e + 1] * vdown));
+                for (int e = 0; e < 4; ++e) {   // pairs of tokens: (16 + c) s + (mid - 23.5 s)
+                    const f16x2v sp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vs[i][2 * e], vs[i][2 * e + 1]));
+                    const f16x2v mp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vm[i][2 * e], vm[i][2 * e + 1]));
 #pragma unroll
                     for (int t = 4 * i; t < 4 * i + 4; ++t) {
                         const uint32_t w = va[t][e];   // a value: bit_cast of a vector's element reads its first one
-                        const f16x2v c = __builtin_bit_cast(f16x2v, w) - f16x2v{(_Float16)23.5f, (_Float16)23.5f};
-                        va[t][e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, sp, mp));
+                        va[t][e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2v, w), sp, mp));
                     }
                 }
         }
         // the raw block is spent: fetch the wave's next one
-        if (blk + kKvWaves < b1) nx.load(base + (int64_t)(blk + kKvWaves) * Kv4<D>::kBytes, lane);
+        if (blk + NW < b1) nx.load(base + (int64_t)(blk + NW) * Kv4<D>::kBytes, lane);
 
         f32x4 s[2][2][GR];   // this tile's raw scores and the next one's, issued a tile ahead
         auto scores = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < GR; ++i) {
-                const u32x4 qa = QT == 1 ? qr[i][0] : ql[(t * GR + i) * 2][lane];
-                const u32x4 qb = QT == 1 ? qr[i][1] : ql[(t * GR + i) * 2 + 1][lane];
+                const u32x4 qa = QT == 1 ? qr[0][i][0] : ql[(t * GR + i) * 2][lane];
+                const u32x4 qb = QT == 1 ? qr[0][i][1] : ql[(t * GR + i) * 2 + 1][lane];
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
                     s[t & 1][kt][i] = mfma_16b<F16>(ka[kt][i][1], qb, mfma_16b<F16>(ka[kt][i][0], qa, f32x4{0.f, 0.f, 0.f, 0.f}));
@@ -340,88 +365,74 @@ __global__ __launch_bounds__(64 * kKvWaves, QT > 1 ? 2 : 1) void attn_kv4_kernel
             }
         }
     };
-    for (int blk = b0 + wave; blk < b1; blk += kKvWaves) {
+    for (int blk = b0 + wave; blk < b1; blk += NW) {
         if (p.mask || kKvBlock * (blk + 1) > lim_lo) block(blk, std::true_type{});
         else block(blk, std::false_type{});
     }
 
-    // The waves' rows meet: common maximum, then two rounds of adds through LDS.
+    // The waves' rows meet: what each wave's sums count of a row, then tile by tile through LDS, every thread a
+    // piece of a row.
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         l[t] = lanes4_sum(l[t]);
 #pragma unroll
         for (int i = 0; i < GR; ++i) {
-            const float add = PAIR ? lanes4_sum(pm[t][PAIR ? i : 0]) : 0.f, by = PAIR ? 1.f : 1.f / vdown;
+            const float add = PAIR ? lanes4_sum(pm[t][PAIR ? i : 0]) : 0.f;
 #pragma unroll
             for (int d = 4 * i; d < 4 * i + 4; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[t][d][e] = o[t][d][e] * by + add;
+                for (int e = 0; e < 4; ++e) o[t][d][e] += add;
         }
-        if (g == 0) xm[wave][t][col] = m[t];
+        if (g == 0) xm[wave][16 * t + col] = m[t], xl[wave][16 * t + col] = l[t];
     }
     __syncthreads();
+    for (int i = threadIdx.x; i < QT * 16; i += 64 * NW) {
+        float mm = xm[0][i], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < NW; ++w) mm = fmaxf(mm, xm[w][i]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float f = __builtin_amdgcn_exp2f(xm[w][i] - mm);
+            xf[w][i] = f;
+            sum += f * xl[w][i];
+        }
+        xs[i] = sum;
+        xm[0][i] = mm;   // this thread's alone
+    }
+    __syncthreads();
+    constexpr int E = D / (4 * NW);   // channels a thread finishes
+    const int row = (int)threadIdx.x / (4 * NW), d0 = E * ((int)threadIdx.x % (4 * NW));
+    const float undo = PAIR ? 1.f : 1.f / vdown;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        float mm = xm[0][t][col];
+        const float f = xf[wave][16 * t + col] * undo;
 #pragma unroll
-        for (int w = 1; w < kKvWaves; ++w) mm = fmaxf(mm, xm[w][t][col]);
-        const float al = __builtin_amdgcn_exp2f(m[t] - mm);
-        m[t] = mm;
-        l[t] *= al;
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&xo[wave][col][16 * d + 4 * g]) = o[t][d] * f;
+        __syncthreads();
+        const int r = q0 + 16 * t + row;
+        if (r < R) {
+            float y[E];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[t][d] *= al;
-        if (g == 0) xl[wave][t][col] = l[t];
-        if (wave >= 2) {
+            for (int e = 0; e < E; ++e) y[e] = xo[0][row][d0 + e];
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int w = 1; w < NW; ++w)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) xo[wave - 2][t * kRow + 4 * d + e][lane] = o[t][d][e];
+                for (int e = 0; e < E; ++e) y[e] += xo[w][row][d0 + e];
+            const float sum = xs[16 * t + row];
+            const int hq = h * p.G + r / p.Sq, s = r % p.Sq;
+            if (p.splits > 1) {
+                float* dst = p.part + ((int64_t)split * p.rows + ((int64_t)b * p.H * p.G + hq) * p.Sq + s) * (D + 2);
+#pragma unroll
+                for (int e = 0; e < E; ++e) dst[d0 + e] = y[e];
+                if (d0 == 0) dst[D] = xm[0][16 * t + row], dst[D + 1] = sum;
+            } else {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[e] *= inv;
+                kv_store<E>(p.out, b * p.os[0] + hq * p.os[1] + s * p.os[2] + d0, p.out_kind, y);
+            }
         }
-    }
-    __syncthreads();
-    if (wave < 2) {
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[t][d][e] += xo[wave][t * kRow + 4 * d + e][lane];
-    }
-    __syncthreads();
-    if (wave == 1) {
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) xo[0][t * kRow + 4 * d + e][lane] = o[t][d][e];
-    }
-    __syncthreads();
-    if (wave != 0) return;
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        if (q0 + 16 * t + col >= R) continue;
-        const float sum = xl[0][t][col] + xl[1][t][col] + xl[2][t][col] + xl[3][t][col];
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[t][d][e] += xo[0][t * kRow + 4 * d + e][lane];
-        if (p.splits > 1) {
-            const int r = q0 + 16 * t + col;
-            const int64_t row = ((int64_t)b * p.H * p.G + h * p.G + r / p.Sq) * p.Sq + r % p.Sq;
-            float* dst = p.part + ((int64_t)split * p.rows + row) * (D + 2);
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) dst[16 * d + 4 * g + e] = o[t][d][e];
-            if (g == 0) dst[D] = m[t], dst[D + 1] = sum;
-            continue;
-        }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
-        const int r = q0 + 16 * t + col;
-        const int64_t at = b * p.os[0] + (h * p.G + r / p.Sq) * p.os[1] + r % p.Sq * p.os[2];
-#pragma unroll
-        for (int d = 0; d < DT; ++d) kv_store4(p.out, at + 16 * d + 4 * g, p.out_kind, o[t][d] * inv);
+        if (t + 1 < QT) __syncthreads();
     }
 }
 
@@ -564,24 +575,24 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
     p.out_kind = d->out_dtype == SF_BF16 ? 1 : (d->out_dtype == SF_F16 ? 2 : 0);
     p.scale_log2 = (d->scale == 0.f ? 1.f / sqrtf((float)d->cache.D) : d->scale) * 1.4426950408889634f;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)k.wgs), block(64 * sfk::kKvWaves);
+    const dim3 grid((unsigned)k.wgs);
     const bool f16 = d->in_dtype == SF_F16;
-#define SF_KV4_LAUNCH(DD, QT, PAIR)                                                                      \
-    do {                                                                                                 \
-        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT, PAIR>), grid, block, 0, s, p);   \
-        else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT, PAIR>), grid, block, 0, s, p);      \
+#define SF_KV4_LAUNCH(DD, QT, PAIR, NW)                                                                                       \
+    do {                                                                                                                      \
+        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT, PAIR, NW>), grid, dim3(64 * NW), 0, s, p);            \
+        else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT, PAIR, NW>), grid, dim3(64 * NW), 0, s, p);               \
     } while (0)
     const bool pair = d->out_dtype != SF_BF16;
     if (d->cache.D == 64) {
-        if (k.qt == 1) SF_KV4_LAUNCH(64, 1, true);
-        else if (k.qt == 2 && pair) SF_KV4_LAUNCH(64, 2, true);
-        else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, false);
-        else if (pair) SF_KV4_LAUNCH(64, 5, true);
-        else SF_KV4_LAUNCH(64, 5, false);
+        if (k.qt == 1) SF_KV4_LAUNCH(64, 1, true, 8);
+        else if (k.qt == 2 && pair) SF_KV4_LAUNCH(64, 2, true, 8);
+        else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, false, 8);
+        else if (pair) SF_KV4_LAUNCH(64, 5, true, 8);
+        else SF_KV4_LAUNCH(64, 5, false, 8);
     } else {
-        if (k.qt == 1) SF_KV4_LAUNCH(128, 1, true);
-        else if (pair) SF_KV4_LAUNCH(128, 2, true);
-        else SF_KV4_LAUNCH(128, 2, false);
+        if (k.qt == 1) SF_KV4_LAUNCH(128, 1, true, 8);
+        else if (pair) SF_KV4_LAUNCH(128, 2, true, 4);
+        else SF_KV4_LAUNCH(128, 2, false, 4);
     }
 #undef SF_KV4_LAUNCH
     if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
