@@ -126,7 +126,8 @@ template <bool F16, int D, int QT, bool PAIR, int NW>
 __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     constexpr int GR = D / 64, DT = D / 16;   // 64-channel groups, tiles of 16 channels
     __shared__ float xm[NW][QT * 16], xl[NW][QT * 16], xf[NW][QT * 16], xs[QT * 16];
-    __shared__ float xo[NW][16][D + 4];
+    constexpr int kJoin = QT == 5 ? 3 : QT;   // tiles that meet at a time
+    __shared__ float xo[NW][kJoin * 16][D + 4], xq[GR][QT * 16];
     __shared__ u32x4 ql[QT > 1 ? QT * GR * 2 : 1][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, g = lane >> 4;
@@ -152,36 +153,50 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     KvBlock<D> nx;
     if (b0 + wave < b1) nx.load(base + (int64_t)(b0 + wave) * Kv4<D>::kBytes, lane);
 
-    // Query fragments: B operands, in registers for one tile, else in LDS for all waves.
-    u32x4 qr[QT][GR][2];
+    // Query fragments (B operands) and row sums: in registers for one tile, else each tile's by one wave into LDS.
+    u32x4 qr[GR][2];
     float qs[QT][GR];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
+    auto load_q = [&](int t, float (&sums)[GR]) __attribute__((always_inline)) {
         const int r = min(q0 + 16 * t + col, R - 1);
         const uint16_t* src = p.q + b * p.qs[0] + (h * p.G + r / p.Sq) * p.qs[1] + r % p.Sq * p.qs[2];
 #pragma unroll
         for (int i = 0; i < GR; ++i)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) qr[t][i][k] = *reinterpret_cast<const u32x4*>(src + 64 * i + 16 * g + 8 * k);
-    }
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
+            for (int k = 0; k < 2; ++k) qr[i][k] = *reinterpret_cast<const u32x4*>(src + 64 * i + 16 * g + 8 * k);
 #pragma unroll
         for (int i = 0; i < GR; ++i) {
             float sum = 0.f;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const u32x4 v = qr[t][i][k];
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    sum += F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v[e]) +
-                                     (float)__builtin_bit_cast(_Float16, (uint16_t)(v[e] >> 16))
-                               : __uint_as_float(v[e] << 16) + __uint_as_float(v[e] & 0xffff0000u);
-                if (QT > 1 && wave == (t * GR + i) % NW) ql[(t * GR + i) * 2 + k][lane] = v;
-            }
-            qs[t][i] = lanes4_sum(sum) * p.scale_log2;
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t v = qr[i][k][e];
+                    sum += F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v) + (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16))
+                               : __uint_as_float(v << 16) + __uint_as_float(v & 0xffff0000u);
+                }
+            sums[i] = lanes4_sum(sum) * p.scale_log2;
         }
-    if (QT > 1) __syncthreads();
+    };
+    if (QT == 1) {
+        load_q(0, qs[0]);
+    } else {
+        static_assert(QT == 1 || QT <= NW, "a wave for each tile");
+        if (wave < QT) {
+            float sums[GR];
+            load_q(wave, sums);
+#pragma unroll
+            for (int i = 0; i < GR; ++i) {
+                ql[(wave * GR + i) * 2][lane] = qr[i][0];
+                ql[(wave * GR + i) * 2 + 1][lane] = qr[i][1];
+                if (g == 0) xq[i][16 * wave + col] = sums[i];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int i = 0; i < GR; ++i) qs[t][i] = xq[i][16 * t + col];
+    }
 
     f32x4 o[QT][DT];   // O^T; PAIR: without the parameters' part pm
     float m[QT], l[QT], pm[QT][PAIR ? GR : 1];
@@ -281,21 +296,28 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
         // the raw block is spent: fetch the wave's next one
         if (blk + NW < b1) nx.load(base + (int64_t)(blk + NW) * Kv4<D>::kBytes, lane);
 
-        f32x4 s[2][2][GR];   // this tile's raw scores and the next one's, issued a tile ahead
-        auto scores = [&](int t) __attribute__((always_inline)) {
+        // Raw scores of a tile; the next one's products are issued before this one's exponentials, its operands
+        // read before this one's maximum.
+        f32x4 s[2][GR];
+        u32x4 qf[GR][2];
+        auto operands = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < GR; ++i) {
-                const u32x4 qa = QT == 1 ? qr[0][i][0] : ql[(t * GR + i) * 2][lane];
-                const u32x4 qb = QT == 1 ? qr[0][i][1] : ql[(t * GR + i) * 2 + 1][lane];
+            for (int i = 0; i < GR; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) qf[i][k] = QT == 1 ? qr[i][k] : ql[(t * GR + i) * 2 + k][lane];
+        };
+        auto scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < GR; ++i)
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
-                    s[t & 1][kt][i] = mfma_16b<F16>(ka[kt][i][1], qb, mfma_16b<F16>(ka[kt][i][0], qa, f32x4{0.f, 0.f, 0.f, 0.f}));
-            }
+                    s[kt][i] = mfma_16b<F16>(ka[kt][i][1], qf[i][1], mfma_16b<F16>(ka[kt][i][0], qf[i][0], f32x4{0.f, 0.f, 0.f, 0.f}));
         };
-        scores(0);
+        operands(0);
+        scores();
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            if (t + 1 < QT) scores(t + 1);
+            if (t + 1 < QT) operands(t + 1);
             float x[8];   // scores less the row's maximum, base 2
             const float neg = m[t] == kKvNoMax ? 0.f : -m[t];
 #pragma unroll
@@ -305,7 +327,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                     float u = neg;
 #pragma unroll
                     for (int i = 0; i < GR; ++i)
-                        u = __builtin_fmaf(ks[i][4 * kt + e], s[t & 1][kt][i][e], __builtin_fmaf(ko[i][4 * kt + e], qs[t][i], u));
+                        u = __builtin_fmaf(ks[i][4 * kt + e], s[kt][i][e], __builtin_fmaf(ko[i][4 * kt + e], qs[t][i], u));
                     x[4 * kt + e] = u;
                 }
             uint32_t row = see;
@@ -326,6 +348,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 #pragma unroll
                 for (int i = 0; i < DT; ++i) o[t][i] *= al;
             }
+            if (t + 1 < QT) scores();
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(x[e]);
             if (PAIR) {
@@ -365,7 +388,19 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
             }
         }
     };
+    // Two waves of a workgroup share a SIMD, and the older one wins every tie: it would end first and leave the other
+    // to run alone.  A wave's priority falls as it gets on, so the one behind goes first.
+    int pace = 3;
+    __builtin_amdgcn_s_setprio(3);
     for (int blk = b0 + wave; blk < b1; blk += NW) {
+        const int left = b1 - __builtin_amdgcn_readfirstlane(blk), all = b1 - b0;   // priority 3 for 40% of the way, 2 to 70%, 1 to 90%
+        const int now = 10 * left > 6 * all ? 3 : 10 * left > 3 * all ? 2 : 10 * left > all ? 1 : 0;
+        if (now != pace) {
+            if (now == 2) __builtin_amdgcn_s_setprio(2);
+            else if (now == 1) __builtin_amdgcn_s_setprio(1);
+            else __builtin_amdgcn_s_setprio(0);
+            pace = now;
+        }
         if (p.mask || kKvBlock * (blk + 1) > lim_lo) block(blk, std::true_type{});
         else block(blk, std::false_type{});
     }
@@ -400,31 +435,38 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
         xm[0][i] = mm;   // this thread's alone
     }
     __syncthreads();
-    constexpr int E = D / (4 * NW);   // channels a thread finishes
+    constexpr int E = D / (4 * NW);   // channels a thread finishes of a row of each tile
     const int row = (int)threadIdx.x / (4 * NW), d0 = E * ((int)threadIdx.x % (4 * NW));
     const float undo = PAIR ? 1.f : 1.f / vdown;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const float f = xf[wave][16 * t + col] * undo;
+    for (int t0 = 0; t0 < QT; t0 += kJoin) {
+        if (t0) __syncthreads();
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&xo[wave][col][16 * d + 4 * g]) = o[t][d] * f;
+        for (int j = 0; j < kJoin; ++j) {
+            if (t0 + j >= QT) continue;
+            const float f = xf[wave][16 * (t0 + j) + col] * undo;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                *reinterpret_cast<f32x4*>(&xo[wave][16 * j + col][16 * d + 4 * g]) = o[t0 + j][d] * f;
+        }
         __syncthreads();
-        const int r = q0 + 16 * t + row;
-        if (r < R) {
+        for (int j = 0; j < kJoin && t0 + j < QT; ++j) {
+            const int r = q0 + 16 * (t0 + j) + row;
+            if (r >= R) break;
             float y[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) y[e] = xo[0][row][d0 + e];
+            for (int e = 0; e < E; ++e) y[e] = xo[0][16 * j + row][d0 + e];
 #pragma unroll
             for (int w = 1; w < NW; ++w)
 #pragma unroll
-                for (int e = 0; e < E; ++e) y[e] += xo[w][row][d0 + e];
-            const float sum = xs[16 * t + row];
+                for (int e = 0; e < E; ++e) y[e] += xo[w][16 * j + row][d0 + e];
+            const float sum = xs[16 * (t0 + j) + row];
             const int hq = h * p.G + r / p.Sq, s = r % p.Sq;
             if (p.splits > 1) {
                 float* dst = p.part + ((int64_t)split * p.rows + ((int64_t)b * p.H * p.G + hq) * p.Sq + s) * (D + 2);
 #pragma unroll
                 for (int e = 0; e < E; ++e) dst[d0 + e] = y[e];
-                if (d0 == 0) dst[D] = xm[0][16 * t + row], dst[D + 1] = sum;
+                if (d0 == 0) dst[D] = xm[0][16 * (t0 + j) + row], dst[D + 1] = sum;
             } else {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
 #pragma unroll
@@ -432,7 +474,6 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 kv_store<E>(p.out, b * p.os[0] + hq * p.os[1] + s * p.os[2] + d0, p.out_kind, y);
             }
         }
-        if (t + 1 < QT) __syncthreads();
     }
 }
 
@@ -507,10 +548,20 @@ static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
     const int64_t base = (int64_t)d->B * d->cache.H * k.qgroups;
     if (d->num_splits > 0) {
         k.splits = d->num_splits;
+    } else if (k.qt == 1) {
+        // Four waves to a workgroup.  Up to 512 keys a wave has four blocks at most and a merge costs as much as it
+        // saves (8 heads x 512 keys: 8.0 us with one split, 7.9 with four); beyond, about two workgroups a CU of at
+        // least a block to a wave, and no split over 2048 keys, so that batches of unequal lengths spread (16 x 8
+        // heads, 4096..16384 keys: 61 us with 8 splits, 65 with 4, 132 with 1).
+        const int64_t want = std::max<int64_t>((512 + base - 1) / base, (d->Sk + 2047) / 2048), most = (d->Sk + 127) / 128;
+        k.splits = d->Sk <= 512 ? 1 : (int)std::min<int64_t>({want, most, (int64_t)kKvMaxSplits});
     } else {
-        // about two workgroups a CU (one of five tiles), and at least two blocks a wave
-        const int64_t want = ((k.qt > 2 ? 256 : 512) + base - 1) / base, most = (d->Sk + 255) / 256;
-        k.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kKvMaxSplits}));
+        // Eight waves to a workgroup and one workgroup a CU.  A split has to save the merge's 7 us at about 1.5 us a
+        // block: 32 heads x 67 rows x 4374 keys 41 -> 19 us with 8 splits, 12 heads x 520 rows x 1537 keys (causal)
+        // 23 us with one split, 30 with four.
+        const int64_t s = std::min<int64_t>(256 / base, kKvMaxSplits), waves = d->cache.D == 64 ? 8 : 4;
+        const int64_t blocks = (d->Sk + kKvBlock * waves - 1) / (kKvBlock * waves);
+        k.splits = s > 1 && blocks * (s - 1) >= 5 * s ? (int)std::min(s, blocks) : 1;
     }
     k.wgs = base * k.splits;
     return k;
@@ -584,13 +635,13 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
     } while (0)
     const bool pair = d->out_dtype != SF_BF16;
     if (d->cache.D == 64) {
-        if (k.qt == 1) SF_KV4_LAUNCH(64, 1, true, 8);
+        if (k.qt == 1) SF_KV4_LAUNCH(64, 1, true, 4);
         else if (k.qt == 2 && pair) SF_KV4_LAUNCH(64, 2, true, 8);
         else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, false, 8);
         else if (pair) SF_KV4_LAUNCH(64, 5, true, 8);
         else SF_KV4_LAUNCH(64, 5, false, 8);
     } else {
-        if (k.qt == 1) SF_KV4_LAUNCH(128, 1, true, 8);
+        if (k.qt == 1) SF_KV4_LAUNCH(128, 1, true, 4);
         else if (pair) SF_KV4_LAUNCH(128, 2, true, 4);
         else SF_KV4_LAUNCH(128, 2, false, 4);
     }
