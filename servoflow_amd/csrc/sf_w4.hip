@@ -36,46 +36,55 @@ struct W4Args {
     int64_t ldc;
     int M, N, K, KB, groups, n16;
     int scale_f16, act, c_kind, accumulate;
+    int vec4;              // four columns of C fit one aligned store
 };
 
 __device__ __forceinline__ float w4_scale(uint32_t u, int f16) {
     return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16)) : __uint_as_float(u & 0xffff0000u);
 }
 
-// One workgroup: 16 NT columns of C (rows of W) x 16 MB rows, K blocks of 128
-// dealt to its WK waves, whose sums meet in LDS.
-template <bool F16, int MB, int NT, int WK, int GROUP>
-__global__ __launch_bounds__(64 * WK) void gemm_w4_kernel(const W4Args p) {
+// A wave's operands of one block of 128 columns: codes and parameters of its NT
+// tiles of 16 rows of W.
+template <int NT, int GROUPS>
+struct W4Block {
+    u32x4 code[NT], par[NT][GROUPS];
+};
+
+// One workgroup: 16 NT WN columns of C (rows of W) x 16 MB rows.  Its WN x WK
+// waves take NT tiles of columns each and deal the blocks of 128 inputs among
+// WK; the WK sums meet in LDS.  Weights are fetched PF blocks ahead (each byte
+// once, from memory), activations one block ahead (from the caches).
+template <bool F16, int MB, int NT, int WK, int WN, int PF, int GROUP>
+__global__ __launch_bounds__(64 * WK * WN) void gemm_w4_kernel(const W4Args p) {
     constexpr int kSteps = GROUP / 32, kGroups = 4 / kSteps;   // per block of 128
-    __shared__ f32x4 red[WK][MB * NT][64];
-    const int lane = threadIdx.x & 63, wk = threadIdx.x >> 6;
+    __shared__ f32x4 red[WK > 1 ? WK : 1][WN][WK > 1 ? MB * NT : 1][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wk = wave % WK, wn = wave / WK;
     const int r = lane & 15, g = lane >> 4;
-    const int nb0 = blockIdx.x * NT;
+    const int nb0 = (blockIdx.x * WN + wn) * NT;
     const int m0 = blockIdx.y * 16 * MB;
 
     const uint16_t* arow[MB];
 #pragma unroll
     for (int b = 0; b < MB; ++b) arow[b] = p.a + (int64_t)min(m0 + 16 * b + r, p.M - 1) * p.lda + 8 * g;
-    f32x4 acc[NT][MB];
+    const uint8_t* wtile[NT];
+    const uint32_t* ptile[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int b = 0; b < MB; ++b) acc[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    const NibbleMask nmask = nibble_mask<F16>();
-    const u32x4 ones = F16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
-                           : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-    for (int kb = wk; kb < p.KB; kb += WK) {
-        u32x4 x[MB][4], code[NT], par[NT][kGroups];
+    for (int t = 0; t < NT; ++t) {   // tiles behind the last one repeat it; they are not stored
+        const int64_t nb = min(nb0 + t, p.n16 - 1);
+        wtile[t] = p.w + nb * p.KB * 1024 + 16 * lane;
+        ptile[t] = p.par + nb * p.groups * 16 + 4 * g;
+    }
+    auto load_w = [&](W4Block<NT, kGroups>& o, int kb) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int nb = min(nb0 + t, p.n16 - 1);
-            code[t] = *reinterpret_cast<const u32x4*>(p.w + ((int64_t)nb * p.KB + kb) * 1024 + 16 * lane);
+            o.code[t] = *reinterpret_cast<const u32x4*>(wtile[t] + (int64_t)kb * 1024);
 #pragma unroll
             for (int q = 0; q < kGroups; ++q)
-                par[t][q] = *reinterpret_cast<const u32x4*>(
-                    p.par + ((int64_t)nb * p.groups + kb * kGroups + q) * 16 + 4 * g);
+                o.par[t][q] = *reinterpret_cast<const u32x4*>(ptile[t] + (int64_t)(kb * kGroups + q) * 16);
         }
+    };
+    auto load_x = [&](u32x4 (&x)[MB][4], int kb) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int k = 128 * kb + 32 * j;   // K is a multiple of 32: a step is inside or outside as a whole
@@ -83,63 +92,125 @@ __global__ __launch_bounds__(64 * WK) void gemm_w4_kernel(const W4Args p) {
             for (int b = 0; b < MB; ++b)
                 x[b][j] = k < p.K ? *reinterpret_cast<const u32x4*>(arow[b] + k) : u32x4{0, 0, 0, 0};
         }
-#pragma unroll
-        for (int q = 0; q < kGroups; ++q) {
-            f32x4 sx[MB], pr[NT][MB];
-#pragma unroll
-            for (int b = 0; b < MB; ++b) {
-                sx[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int t = 0; t < NT; ++t) pr[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-#pragma unroll
-            for (int j = q * kSteps; j < (q + 1) * kSteps; ++j) {
-#pragma unroll
-                for (int b = 0; b < MB; ++b) sx[b] = mfma_16b<F16>(ones, x[b][j], sx[b]);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const u32x4 w = nibbles_plus16<F16>(code[t][j], nmask);
-#pragma unroll
-                    for (int b = 0; b < MB; ++b) pr[t][b] = mfma_16b<F16>(w, x[b][j], pr[t][b]);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float s = w4_scale(par[t][q][i], p.scale_f16);
-                    const float z = -s * (16.f + (float)(par[t][q][i] & 0xffu));
-#pragma unroll
-                    for (int b = 0; b < MB; ++b)
-                        acc[t][b][i] = __builtin_fmaf(z, sx[b][0], __builtin_fmaf(s, pr[t][b][i], acc[t][b][i]));
-                }
-        }
-    }
+    };
+
+    f32x4 acc[NT][MB];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int b = 0; b < MB; ++b) red[wk][t * MB + b][lane] = acc[t][b];
-    __syncthreads();
-    for (int u = wk; u < NT * MB; u += WK) {
-        f32x4 v = red[0][u][lane];
+        for (int b = 0; b < MB; ++b) acc[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const NibbleMask nmask = nibble_mask<F16>();
+    const u32x4 ones = F16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
+                           : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    W4Block<NT, kGroups> st[PF];
+    constexpr bool kAhead = MB <= 2;   // activations a block ahead, where registers allow
+    u32x4 x[MB][4], xn[kAhead ? MB : 1][4];
 #pragma unroll
-        for (int w = 1; w < WK; ++w) v += red[w][u][lane];
-        const int m = m0 + 16 * (u % MB) + r, n = 16 * (nb0 + u / MB) + 4 * g;
-        if (m >= p.M) continue;
+    for (int s = 0; s < PF; ++s)
+        if (wk + s * WK < p.KB) load_w(st[s], wk + s * WK);
+    if (kAhead && wk < p.KB) load_x(x, wk);
+    for (int kb0 = wk; kb0 < p.KB; kb0 += PF * WK) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (n + i >= p.N) break;
-            const float y = apply_act(p.act, v[i] + (p.bias ? p.bias[n + i] : 0.f));
-            const int64_t at = (int64_t)m * p.ldc + n + i;
-            if (p.c_kind == 0) {
-                float* c = static_cast<float*>(p.c) + at;
-                *c = p.accumulate ? *c + y : y;
-            } else if (p.c_kind == 1) {
-                static_cast<uint16_t*>(p.c)[at] = (uint16_t)f32_to_bf16_bits(y);
+        for (int s = 0; s < PF; ++s) {
+            const int kb = kb0 + s * WK;
+            if (kb >= p.KB) break;
+            if constexpr (kAhead) {
+                if (kb + WK < p.KB) load_x(xn, kb + WK);
             } else {
-                static_cast<_Float16*>(p.c)[at] = (_Float16)y;
+                load_x(x, kb);
+            }
+#pragma unroll
+            for (int q = 0; q < kGroups; ++q) {
+                f32x4 sx[MB], pr[NT][MB];
+#pragma unroll
+                for (int b = 0; b < MB; ++b) {
+                    sx[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) pr[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll
+                for (int j = q * kSteps; j < (q + 1) * kSteps; ++j) {
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) sx[b] = mfma_16b<F16>(ones, x[b][j], sx[b]);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const u32x4 w = nibbles_plus16<F16>(st[s].code[t][j], nmask);
+#pragma unroll
+                        for (int b = 0; b < MB; ++b) pr[t][b] = mfma_16b<F16>(w, x[b][j], pr[t][b]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t par = st[s].par[t][q][i];
+                        const float sc = w4_scale(par, p.scale_f16);
+                        const float z = -sc * (16.f + (float)(par & 0xffu));
+#pragma unroll
+                        for (int b = 0; b < MB; ++b)
+                            acc[t][b][i] = __builtin_fmaf(z, sx[b][0], __builtin_fmaf(sc, pr[t][b][i], acc[t][b][i]));
+                    }
+            }
+            if (kb + PF * WK < p.KB) load_w(st[s], kb + PF * WK);
+            if constexpr (kAhead) {
+#pragma unroll
+                for (int b = 0; b < MB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[b][j] = xn[b][j];
             }
         }
+    }
+    if (WK > 1) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) red[wk][wn][t * MB + b][lane] = acc[t][b];
+        __syncthreads();
+    }
+    auto finish = [&](int t, int b, f32x4 v) __attribute__((always_inline)) {
+        const int m = m0 + 16 * b + r, n = 16 * (nb0 + t) + 4 * g;
+        if (m >= p.M || n >= p.N) return;
+        const int64_t at = (int64_t)m * p.ldc + n;
+        const int cols = min(4, p.N - n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < cols) v[i] = apply_act(p.act, v[i] + (p.bias ? p.bias[n + i] : 0.f));
+        if (cols == 4 && p.vec4) {
+            if (p.c_kind == 0) {
+                f32x4* c = reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at);
+                *c = p.accumulate ? *c + v : v;
+            } else {
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.c) + at) =
+                    p.c_kind == 1 ? uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}
+                                  : uint2{pack_f16x2_rn(v[0], v[1]), pack_f16x2_rn(v[2], v[3])};
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i >= cols) continue;
+            if (p.c_kind == 0) {
+                float* c = static_cast<float*>(p.c) + at + i;
+                *c = p.accumulate ? *c + v[i] : v[i];
+            } else if (p.c_kind == 1) {
+                static_cast<uint16_t*>(p.c)[at + i] = (uint16_t)f32_to_bf16_bits(v[i]);
+            } else {
+                static_cast<_Float16*>(p.c)[at + i] = (_Float16)v[i];
+            }
+        }
+    };
+    if (WK > 1) {
+        for (int u = wk; u < NT * MB; u += WK) {
+            f32x4 v = red[0][wn][u][lane];
+#pragma unroll
+            for (int w = 1; w < WK; ++w) v += red[w][wn][u][lane];
+            finish(u / MB, u % MB, v);
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) finish(t, b, acc[t][b]);
     }
 }
 
@@ -181,20 +252,20 @@ static inline bool w4_shape_ok(int32_t N, int32_t K, int32_t group) {
 static inline int w4_kb(int K) { return (K + 127) / 128; }
 static inline int w4_groups(int K, int group) { return w4_kb(K) * (128 / group); }
 
-template <bool F16, int MB>
-static void launch_w4_group(const W4Args& p, int group, hipStream_t s) {
-    constexpr int NT = 1, WK = 8;
-    const dim3 grid((unsigned)((p.n16 + NT - 1) / NT), (unsigned)((p.M + 16 * MB - 1) / (16 * MB)));
-    if (group == 32) hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, 32>), grid, dim3(64 * WK), 0, s, p);
-    else if (group == 64) hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, 64>), grid, dim3(64 * WK), 0, s, p);
-    else hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, 128>), grid, dim3(64 * WK), 0, s, p);
+template <bool F16, int MB, int NT, int WK, int WN, int PF>
+static void launch_w4_shape(const W4Args& p, int group, hipStream_t s) {
+    const dim3 grid((unsigned)((p.n16 + NT * WN - 1) / (NT * WN)), (unsigned)((p.M + 16 * MB - 1) / (16 * MB)));
+    const dim3 block(64 * WK * WN);
+    if (group == 32) hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, WN, PF, 32>), grid, block, 0, s, p);
+    else if (group == 64) hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, WN, PF, 64>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, WN, PF, 128>), grid, block, 0, s, p);
 }
 
 template <bool F16>
 static void launch_w4(const W4Args& p, int group, hipStream_t s) {
-    if (p.M <= 16) launch_w4_group<F16, 1>(p, group, s);
-    else if (p.M <= 32) launch_w4_group<F16, 2>(p, group, s);
-    else launch_w4_group<F16, 5>(p, group, s);
+    if (p.M <= 16) launch_w4_shape<F16, 1, 1, 8, 1, 2>(p, group, s);
+    else if (p.M <= 32) launch_w4_shape<F16, 2, 1, 8, 1, 2>(p, group, s);
+    else launch_w4_shape<F16, 5, 1, 4, 2, 2>(p, group, s);
 }
 
 }  // namespace sfk
@@ -255,6 +326,7 @@ extern "C" int sf_gemm_w4(const sf_gemm_w4_desc* desc, void* stream) {
     p.act = desc->act;
     p.c_kind = desc->c_dtype == SF_BF16 ? 1 : (desc->c_dtype == SF_F16 ? 2 : 0);
     p.accumulate = desc->accumulate != 0;
+    p.vec4 = desc->ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(desc->C) & (p.c_kind == 0 ? 15 : 7)) == 0;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (desc->a_dtype == SF_F16) sfk::launch_w4<true>(p, desc->group, s);
     else sfk::launch_w4<false>(p, desc->group, s);
