@@ -64,9 +64,19 @@ __global__ __launch_bounds__(64 * WK * WN) void gemm_w4_kernel(const W4Args p) {
     const int nb0 = (blockIdx.x * WN + wn) * NT;
     const int m0 = blockIdx.y * 16 * MB;
 
-    const uint16_t* arow[MB];
+    // Activations: lane l reads 16 bytes of row l / 16 (+ 4 i), so an instruction covers four rows' 256 bytes, and the
+    // operand's order is made in LDS, by each wave for itself.  (Read in operand order an instruction takes the same
+    // 64 bytes of 16 rows, which meet in the cache's banks: 67 x 6144 x 2048 took 15.7 us, and 13.4 with rows 16 bytes
+    // longer.)
+    __shared__ __attribute__((aligned(16))) uint16_t xs[WK * WN][16][136];
+    const int xc = 8 * (lane & 15), xr = lane >> 4;
+    const char* abase = reinterpret_cast<const char*>(p.a + (int64_t)m0 * p.lda);
+    uint32_t arow[MB][4];   // bytes: lda is at most 2^24
 #pragma unroll
-    for (int b = 0; b < MB; ++b) arow[b] = p.a + (int64_t)min(m0 + 16 * b + r, p.M - 1) * p.lda + 8 * g;
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            arow[b][i] = 2u * ((uint32_t)min(16 * b + 4 * i + xr, p.M - 1 - m0) * (uint32_t)p.lda + xc);
     const uint8_t* wtile[NT];
     const uint32_t* ptile[NT];
 #pragma unroll
@@ -85,13 +95,23 @@ __global__ __launch_bounds__(64 * WK * WN) void gemm_w4_kernel(const W4Args p) {
         }
     };
     auto load_x = [&](u32x4 (&x)[MB][4], int kb) __attribute__((always_inline)) {
+        const bool in = 128 * kb + xc < p.K;   // K is a multiple of 32
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = 128 * kb + 32 * j;   // K is a multiple of 32: a step is inside or outside as a whole
+        for (int b = 0; b < MB; ++b)
 #pragma unroll
-            for (int b = 0; b < MB; ++b)
-                x[b][j] = k < p.K ? *reinterpret_cast<const u32x4*>(arow[b] + k) : u32x4{0, 0, 0, 0};
-        }
+            for (int i = 0; i < 4; ++i)
+                if (m0 + 16 * b + 4 * i < p.M)   // rows behind the last are other columns of the product, not stored
+                    x[b][i] = in ? *reinterpret_cast<const u32x4*>(abase + 256 * (int64_t)kb + arow[b][i]) : u32x4{0, 0, 0, 0};
+    };
+    auto order_x = [&](u32x4 (&f)[4], const u32x4 (&x)[4]) __attribute__((always_inline)) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(&xs[wave][4 * i + xr][xc]) = x[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const u32x4*>(&xs[wave][r][32 * j + 8 * g]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     };
 
     f32x4 acc[NT][MB];
@@ -104,21 +124,24 @@ __global__ __launch_bounds__(64 * WK * WN) void gemm_w4_kernel(const W4Args p) {
                            : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
     W4Block<NT, kGroups> st[PF];
     constexpr bool kAhead = MB <= 2;   // activations a block ahead, where registers allow
-    u32x4 x[MB][4], xn[kAhead ? MB : 1][4];
+    u32x4 x[MB][4], xahead[kAhead ? MB : 1][4] = {};
+    auto& xn = [&]() -> u32x4(&)[MB][4] {
+        if constexpr (kAhead) return xahead;
+        else return x;
+    }();
 #pragma unroll
     for (int s = 0; s < PF; ++s)
         if (wk + s * WK < p.KB) load_w(st[s], wk + s * WK);
-    if (kAhead && wk < p.KB) load_x(x, wk);
+    if (kAhead && wk < p.KB) load_x(xn, wk);
     for (int kb0 = wk; kb0 < p.KB; kb0 += PF * WK) {
 #pragma unroll
         for (int s = 0; s < PF; ++s) {
             const int kb = kb0 + s * WK;
             if (kb >= p.KB) break;
-            if constexpr (kAhead) {
-                if (kb + WK < p.KB) load_x(xn, kb + WK);
-            } else {
-                load_x(x, kb);
-            }
+            if (!kAhead) load_x(xn, kb);
+#pragma unroll
+            for (int b = 0; b < MB; ++b) order_x(x[b], xn[b]);
+            if (kAhead && kb + WK < p.KB) load_x(xn, kb + WK);
 #pragma unroll
             for (int q = 0; q < kGroups; ++q) {
                 f32x4 sx[MB], pr[NT][MB];
@@ -152,12 +175,6 @@ __global__ __launch_bounds__(64 * WK * WN) void gemm_w4_kernel(const W4Args p) {
                     }
             }
             if (kb + PF * WK < p.KB) load_w(st[s], kb + PF * WK);
-            if constexpr (kAhead) {
-#pragma unroll
-                for (int b = 0; b < MB; ++b)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[b][j] = xn[b][j];
-            }
         }
     }
     if (WK > 1) {
@@ -252,20 +269,48 @@ static inline bool w4_shape_ok(int32_t N, int32_t K, int32_t group) {
 static inline int w4_kb(int K) { return (K + 127) / 128; }
 static inline int w4_groups(int K, int group) { return w4_kb(K) * (128 / group); }
 
-template <bool F16, int MB, int NT, int WK, int WN, int PF>
-static void launch_w4_shape(const W4Args& p, int group, hipStream_t s) {
+template <bool F16, int MB, int NT, int WK, int WN, int PF, int GROUP>
+static void launch_w4_shape(const W4Args& p, hipStream_t s) {
     const dim3 grid((unsigned)((p.n16 + NT * WN - 1) / (NT * WN)), (unsigned)((p.M + 16 * MB - 1) / (16 * MB)));
-    const dim3 block(64 * WK * WN);
-    if (group == 32) hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, WN, PF, 32>), grid, block, 0, s, p);
-    else if (group == 64) hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, WN, PF, 64>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, WN, PF, 128>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, WN, PF, GROUP>), grid, dim3(64 * WK * WN), 0, s, p);
+}
+
+// Shapes by rows and tiles of 16 columns; us with weights from memory, groups of 128, MB,NT,WK,WN,PF:
+//   up to 16 rows: 16 x 2048 x 8192 8.5 with 1,1,16,1,1 and 12.2 with 1,2,8,1,2; 16 x 8192 x 8192 12.8 with
+//   1,2,16,1,2 and 16.5 with 1,1,16,1,1 (a second tile of columns halves the activations' reads; the first fills
+//   the card with few columns).
+//   up to 32 rows: 32 x 8192 x 8192 16.4 with 2,2,8,1,2 and 25 with 2,1,8,1,2.
+//   beyond, in slabs of 80 rows: 67 x 2048 x 2048 7.3 with 5,1,8,1,2 and 12.3 with 5,2,4,1,2; 67 x 6144 x 2048 14.0
+//   with 5,2,4,1,2 and 24 with 5,1,8,1,2; 268 x 8192 x 8192 107 with 5,4,2,2,2 and 151 with 5,1,4,1,2.
+// Groups of 64 keep twice the parameters, one block ahead; groups of 32 four times, and one tile of columns.
+template <bool F16, int GROUP>
+static void launch_w4(const W4Args& p, hipStream_t s) {
+    constexpr int PF = GROUP == 128 ? 2 : 1;
+    const int64_t tiles = (int64_t)p.n16 * ((p.M + 79) / 80);
+    if constexpr (GROUP == 32) {
+        if (p.M <= 16) launch_w4_shape<F16, 1, 1, 16, 1, 1, GROUP>(p, s);
+        else if (p.M <= 32) launch_w4_shape<F16, 2, 1, 8, 1, 1, GROUP>(p, s);
+        else launch_w4_shape<F16, 5, 1, 4, 1, 1, GROUP>(p, s);
+    } else if (p.M <= 16) {
+        if (tiles <= 256) launch_w4_shape<F16, 1, 1, 16, 1, 1, GROUP>(p, s);
+        else launch_w4_shape<F16, 1, 2, 16, 1, PF, GROUP>(p, s);
+    } else if (p.M <= 32) {
+        if (tiles <= 256) launch_w4_shape<F16, 2, 1, 8, 1, PF, GROUP>(p, s);
+        else launch_w4_shape<F16, 2, 2, 8, 1, PF, GROUP>(p, s);
+    } else if (tiles <= 256) {
+        launch_w4_shape<F16, 5, 1, 8, 1, PF, GROUP>(p, s);
+    } else if (tiles < 1024) {
+        launch_w4_shape<F16, 5, 2, 4, 1, PF, GROUP>(p, s);
+    } else {
+        launch_w4_shape<F16, 5, 4, 2, 2, PF, GROUP>(p, s);
+    }
 }
 
 template <bool F16>
-static void launch_w4(const W4Args& p, int group, hipStream_t s) {
-    if (p.M <= 16) launch_w4_shape<F16, 1, 1, 8, 1, 2>(p, group, s);
-    else if (p.M <= 32) launch_w4_shape<F16, 2, 1, 8, 1, 2>(p, group, s);
-    else launch_w4_shape<F16, 5, 1, 4, 2, 2>(p, group, s);
+static void launch_w4_group(const W4Args& p, int group, hipStream_t s) {
+    if (group == 32) launch_w4<F16, 32>(p, s);
+    else if (group == 64) launch_w4<F16, 64>(p, s);
+    else launch_w4<F16, 128>(p, s);
 }
 
 }  // namespace sfk
@@ -307,7 +352,8 @@ extern "C" int sf_gemm_w4(const sf_gemm_w4_desc* desc, void* stream) {
     if (desc->c_dtype != SF_F32 && desc->c_dtype != SF_F16 && desc->c_dtype != SF_BF16) return SF_ENOTSUP;
     if (desc->act < SF_ACT_NONE || desc->act > SF_ACT_SILU) return SF_ENOTSUP;
     if (desc->accumulate && desc->c_dtype != SF_F32) return SF_ENOTSUP;
-    if ((desc->M + 79) / 80 > 65535) return SF_ENOTSUP;   // the grid's second dimension
+    if (((int64_t)desc->M + 79) / 80 > 65535) return SF_ENOTSUP;   // the grid's second dimension
+    if (desc->lda > 1 << 24) return SF_ENOTSUP;                     // a workgroup's rows are addressed in 32 bits
     sfk::W4Args p = {};
     p.a = static_cast<const uint16_t*>(desc->A);
     p.lda = desc->lda;
@@ -328,7 +374,7 @@ extern "C" int sf_gemm_w4(const sf_gemm_w4_desc* desc, void* stream) {
     p.accumulate = desc->accumulate != 0;
     p.vec4 = desc->ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(desc->C) & (p.c_kind == 0 ? 15 : 7)) == 0;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (desc->a_dtype == SF_F16) sfk::launch_w4<true>(p, desc->group, s);
-    else sfk::launch_w4<false>(p, desc->group, s);
+    if (desc->a_dtype == SF_F16) sfk::launch_w4_group<true>(p, desc->group, s);
+    else sfk::launch_w4_group<false>(p, desc->group, s);
     return hipGetLastError() == hipSuccess ? SF_OK : SF_ELAUNCH;
 }
