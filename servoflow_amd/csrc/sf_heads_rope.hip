@@ -18,11 +18,15 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "sf_device.h"
 #include "sf_hip.h"
 #include "sf_kv4.h"
 
 namespace sfk {
+
+constexpr int kRopeTokens = kKvBlock;   // tokens of a workgroup, at most
 
 struct RopeArgs {
     const void* src[3];
@@ -37,29 +41,40 @@ struct RopeArgs {
     int64_t cache_blocks;   // per (b, h)
     int heads[3];
     int S, cap, rot, interleaved, in_kind, out_kind;
-    int64_t tokens;         // B * S
     float eps;
-    int tok_per_wg, heads_per_wg;
+    int tok_per_wg, windows;           // a batch element's tokens in windows
+    int heads_per_wg;
+    int heads_magic;                   // ceil(2^16 / heads_per_wg): (i * this) >> 16 is i / heads_per_wg, i < 2048
 };
 
-// kind: 0 fp32, 1 bf16, 2 fp16
-__device__ __forceinline__ void load8(const void* p, int64_t at, int kind, float v[8]) {
+// Eight channels as loaded.  kind: 0 fp32, 1 bf16, 2 fp16
+struct Raw8 {
+    u32x4 a, b;   // b: fp32 only
+};
+__device__ __forceinline__ Raw8 load8(const void* p, int64_t at, int kind) {
+    Raw8 r = {};
     if (kind == 0) {
-        const f32x4* q = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
-        const f32x4 a = q[0], b = q[1];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
-        return;
+        const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const float*>(p) + at);
+        r.a = q[0];
+        r.b = q[1];
+    } else {
+        r.a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
     }
-    const u32x4 u = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
+    return r;
+}
+__device__ __forceinline__ void widen8(const Raw8& r, int kind, float v[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        if (kind == 1) {
-            v[2 * e] = __uint_as_float(u[e] << 16);
-            v[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+        const uint32_t u = r.a[e], w = r.b[e];
+        if (kind == 0) {
+            v[e] = __uint_as_float(u);
+            v[4 + e] = __uint_as_float(w);
+        } else if (kind == 1) {
+            v[2 * e] = __uint_as_float(u << 16);
+            v[2 * e + 1] = __uint_as_float(u & 0xffff0000u);
         } else {
-            v[2 * e] = (float)__builtin_bit_cast(_Float16, (uint16_t)u[e]);
-            v[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u[e] >> 16));
+            v[2 * e] = (float)__builtin_bit_cast(_Float16, (uint16_t)u);
+            v[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
         }
     }
 }
@@ -132,17 +147,47 @@ __device__ __forceinline__ uint32_t nibbles_to_pairs(uint32_t c) {
     return o;
 }
 
-template <int D>
+// One workgroup: up to tok_per_wg tokens of a batch element and heads_per_wg of
+// the query, key and value heads in a row.  Into a cache the windows of tokens
+// follow the cache's blocks, as far as the slots count up from the element's
+// first one: a window of 32 tokens that fills a block is put together in LDS
+// and stored as it lies there, 16 bytes a lane; other tokens are stored piece by
+// piece (a token's codes are 4-byte and 1-byte pieces of its block: 4374 tokens
+// of 32 heads took 45 us that way).
+template <int D, bool CACHE>
 __global__ __launch_bounds__(256) void heads_rope_kernel(const RopeArgs p) {
-    constexpr int L = D / 8, kRows = 256 / L;
-    extern __shared__ float2 cs[];   // [tok_per_wg][rot / 2]: cosine, sine
-    const int64_t t0 = (int64_t)blockIdx.x * p.tok_per_wg;
-    const int nt = (int)min((int64_t)p.tok_per_wg, p.tokens - t0);
-    const int half = p.rot >> 1;
+    constexpr int L = D / 8, kRows = 256 / L, kAhead = 4;   // rows in flight a thread
+    constexpr int kImage = 16 * D + 2 * D;                  // a head's codes and parameters of 32 tokens, keys or values
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    float2* cs = reinterpret_cast<float2*>(lds);                                      // [tok_per_wg][rot / 2]
+    uint8_t* image = lds + sizeof(float2) * (size_t)p.tok_per_wg * (p.rot >> 1);      // [heads_per_wg][kImage]
+    __shared__ int tpos[kRopeTokens], tslot[kRopeTokens], odd;
+    const int b = blockIdx.x / p.windows, win = blockIdx.x % p.windows;
+    const int64_t m0 = (int64_t)b * p.S;
+    int s0 = win * p.tok_per_wg, s1 = min(s0 + p.tok_per_wg, p.S);
+    const int32_t* slots = p.slots ? p.slots : p.positions;
+    if (CACHE && p.tok_per_wg == kKvBlock) {
+        const int off = slots ? slots[m0] & (kKvBlock - 1) : 0;
+        s1 = min(s0 + kKvBlock - off, p.S);   // the last window ends at S or behind it
+        s0 = max(s0 - off, 0);
+    }
+    const int nt = s1 - s0, half = p.rot >> 1;
+    if (nt <= 0) return;
+    if (threadIdx.x == 0) odd = nt != kKvBlock;
+    __syncthreads();
+    if ((int)threadIdx.x < nt) {
+        const int s = s0 + (int)threadIdx.x, pos = p.positions ? p.positions[m0 + s] : s;
+        const int slot = slots ? slots[m0 + s] : s;
+        tpos[threadIdx.x] = pos;
+        tslot[threadIdx.x] = slot;
+        const int first = slots ? slots[m0 + s0] : s0;
+        if (CACHE && (pos < 0 || first < 0 || (first & (kKvBlock - 1)) || slot != first + (int)threadIdx.x || slot >= p.cap))
+            odd = 1;
+    }
+    __syncthreads();
+    const bool whole = CACHE && !odd;
     for (int i = threadIdx.x; i < nt * half; i += 256) {
-        const int64_t m = t0 + i / half;
-        const int pos = p.positions ? p.positions[m] : (int)(m % p.S);
-        const double turns = (double)pos * (p.inv_freq[i % half] * 0.15915494309189533577);
+        const double turns = (double)tpos[i / half] * (p.inv_freq[i % half] * 0.15915494309189533577);
         float c, s;
         sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
         cs[i] = float2{c, s};
@@ -152,83 +197,110 @@ __global__ __launch_bounds__(256) void heads_rope_kernel(const RopeArgs p) {
     const int j = threadIdx.x & (L - 1), sub = threadIdx.x / L;
     const int h0 = blockIdx.y * p.heads_per_wg;
     const int nh = min(p.heads_per_wg, p.heads[0] + p.heads[1] + p.heads[2] - h0);
-    for (int base = 0; base < nt * nh; base += kRows) {
-        const int i = base + sub;
-        if (i >= nt * nh) continue;   // whole groups of L lanes
-        const int ti = i / nh;
-        const int64_t m = t0 + ti;
-        int h = h0 + i % nh, sec = 0;
-        if (h >= p.heads[0]) h -= p.heads[0], sec = 1;
-        if (sec == 1 && h >= p.heads[1]) h -= p.heads[1], sec = 2;
-        const int64_t b = m / p.S;
-        const int s = (int)(m % p.S);
-        const int pos = p.positions ? p.positions[m] : s;
-        if (pos < 0) continue;   // a padding row
-        float v[8];
-        load8(p.src[sec], b * p.ss[sec][0] + h * p.ss[sec][1] + s * p.ss[sec][2] + 8 * j, p.in_kind, v);
-        const float* gm = sec < 2 ? p.gamma[sec] : nullptr;
-        if (gm) {
-            float q = 0.f;
+    const int rows = nt * p.heads_per_wg;
+    for (int base = sub; base - sub < rows; base += kRows * kAhead) {
+        Raw8 raw[kAhead];
+        int where[kAhead];   // token << 20 | section << 18 | head; -1: none
 #pragma unroll
-            for (int e = 0; e < 8; ++e) q += v[e] * v[e];
-            q = L == 8 ? row8_sum(q) : row16_sum(q);
-            const float r = 1.f / sqrtf(q / (float)D + p.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = v[e] * r * gm[8 * j + e];
+        for (int a = 0; a < kAhead; ++a) {
+            const int i = base + a * kRows, ti = (i * p.heads_magic) >> 16, hi = i - ti * p.heads_per_wg;
+            where[a] = -1;
+            if (i >= rows || hi >= nh || tpos[ti] < 0) continue;   // a padding token is not written
+            int h = h0 + hi, sec = 0;
+            if (h >= p.heads[0]) h -= p.heads[0], sec = 1;
+            if (sec == 1 && h >= p.heads[1]) h -= p.heads[1], sec = 2;
+            where[a] = ti << 20 | sec << 18 | h;
+            raw[a] = load8(p.src[sec], b * p.ss[sec][0] + h * p.ss[sec][1] + (s0 + ti) * p.ss[sec][2] + 8 * j, p.in_kind);
         }
-        if (sec < 2 && half) {
-            const float2* t = cs + ti * half;
-            if (p.interleaved) {
-                if (8 * j < p.rot) {
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            if (where[a] < 0) continue;   // whole groups of L lanes
+            const int ti = where[a] >> 20, sec = where[a] >> 18 & 3, h = where[a] & 0x3ffff;
+            float v[8];
+            widen8(raw[a], p.in_kind, v);
+            const float* gm = sec == 0 ? p.gamma[0] : sec == 1 ? p.gamma[1] : nullptr;
+            if (gm) {
+                float q = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q += v[e] * v[e];
+                q = L == 8 ? row8_sum(q) : row16_sum(q);
+                const float r = 1.f / sqrtf(q / (float)D + p.eps);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = v[e] * r * gm[8 * j + e];
+            }
+            if (sec < 2 && half) {
+                const float2* t = cs + ti * half;
+                if (p.interleaved) {
+                    if (8 * j < p.rot) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 w = t[4 * j + e];
+                            const float x = v[2 * e], y = v[2 * e + 1];
+                            v[2 * e] = x * w.x - y * w.y;
+                            v[2 * e + 1] = y * w.x + x * w.y;
+                        }
+                    }
+                } else {   // the partner's 8 channels are rot / 16 lanes away
+                    const int step = p.rot >> 4;
+                    const bool low = j < step, in = j < 2 * step;
+                    const int lane = (int)(threadIdx.x & 63);
+                    const int from = in ? (low ? lane + step : lane - step) : lane;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float y = __shfl(v[e], from, 64);
+                        if (in) {
+                            const float2 w = t[8 * (low ? j : j - step) + e];
+                            v[e] = low ? v[e] * w.x - y * w.y : v[e] * w.x + y * w.y;
+                        }
+                    }
+                }
+            }
+            if (sec == 0 || !CACHE) {
+                store8(p.out[sec], b * p.os[sec][0] + h * p.os[sec][1] + (s0 + ti) * p.os[sec][2] + 8 * j, p.out_kind, v);
+                continue;
+            }
+            if constexpr (CACHE) {
+                uint32_t par;
+                const uint32_t c = kv4_quantise(v, &par);
+                const uint32_t other = (uint32_t)__shfl_xor((int)c, 2, 64);
+                const int slot = tslot[ti];
+                if (slot < 0 || slot >= p.cap) continue;
+                // where the block's codes and parameters lie: in the cache, or in this head's image
+                const int tok = slot % kKvBlock, head = (int)(sec == 1 ? p.heads[0] + h : p.heads[0] + p.heads[1] + h) - h0;
+                uint8_t* blk = whole ? image + head * kImage
+                                     : p.cache + (((int64_t)b * p.heads[1] + h) * p.cache_blocks + slot / kKvBlock) * Kv4<D>::kBytes;
+                uint8_t* pars = blk + (whole ? 16 * D : sec == 1 ? Kv4<D>::kPar : Kv4<D>::kVPar);
+                if ((j & 7) == 0) *reinterpret_cast<uint32_t*>(pars + ((j >> 3) * kKvBlock + tok) * 4) = par;
+                if (sec == 1) {
+                    *reinterpret_cast<uint32_t*>(blk + Kv4<D>::key_dword(tok, j)) = nibbles_to_pairs(c);
+                } else {
+                    // lanes j and j ^ 2 hold channels 16 apart: each writes four of the eight bytes they share
+                    const bool hi = j & 2;
+                    const uint32_t lo = hi ? other : c, up = hi ? c : other;
+                    const int first = hi ? 4 : 0, at = whole ? Kv4<D>::kV : 0;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float2 a = t[4 * j + e];
-                        const float x = v[2 * e], y = v[2 * e + 1];
-                        v[2 * e] = x * a.x - y * a.y;
-                        v[2 * e + 1] = y * a.x + x * a.y;
-                    }
-                }
-            } else {   // the partner's 8 channels are rot / 16 lanes away
-                const int step = p.rot >> 4;
-                const bool low = j < step, in = j < 2 * step;
-                const int lane = (int)(threadIdx.x & 63);
-                const int from = in ? (low ? lane + step : lane - step) : lane;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float y = __shfl(v[e], from, 64);
-                    if (in) {
-                        const float2 a = t[8 * (low ? j : j - step) + e];
-                        v[e] = low ? v[e] * a.x - y * a.y : v[e] * a.x + y * a.y;
+                        const int sh = 4 * (first + e);
+                        blk[Kv4<D>::value_byte(tok, j >> 2, 8 * (j & 1) + first + e) - at] =
+                            (uint8_t)(((lo >> sh) & 15u) | ((up >> sh) & 15u) << 4);
                     }
                 }
             }
         }
-        if (sec == 0 || !p.cache) {
-            store8(p.out[sec], b * p.os[sec][0] + h * p.os[sec][1] + s * p.os[sec][2] + 8 * j, p.out_kind, v);
-            continue;
-        }
-        const int slot = p.slots ? p.slots[m] : pos;
-        uint32_t par;
-        const uint32_t c = kv4_quantise(v, &par);
-        const uint32_t other = (uint32_t)__shfl_xor((int)c, 2, 64);
-        if (slot < 0 || slot >= p.cap) continue;
-        uint8_t* blk = p.cache + ((b * p.heads[1] + h) * p.cache_blocks + slot / kKvBlock) * Kv4<D>::kBytes;
-        const int tok = slot % kKvBlock;
-        if (sec == 1) {
-            *reinterpret_cast<uint32_t*>(blk + Kv4<D>::key_dword(tok, j)) = nibbles_to_pairs(c);
-            if ((j & 7) == 0) *reinterpret_cast<uint32_t*>(blk + Kv4<D>::key_par(tok, j >> 3)) = par;
-        } else {
-            // lanes j and j ^ 2 hold channels 16 apart: each writes four of the eight bytes they share
-            const bool hi = j & 2;
-            const uint32_t lo = hi ? other : c, up = hi ? c : other;
-            const int first = hi ? 4 : 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int sh = 4 * (first + e);
-                blk[Kv4<D>::value_byte(tok, j >> 2, 8 * (j & 1) + first + e)] =
-                    (uint8_t)(((lo >> sh) & 15u) | ((up >> sh) & 15u) << 4);
-            }
-            if ((j & 7) == 0) *reinterpret_cast<uint32_t*>(blk + Kv4<D>::value_par(tok, j >> 3)) = par;
+    }
+    if constexpr (CACHE) {
+        if (!whole) return;
+        __syncthreads();
+        constexpr int kPieces = kImage / 16, kCodes = 16 * D / 16;
+        for (int i = threadIdx.x; i < nh * kPieces; i += 256) {
+            const int hi = i / kPieces, piece = i % kPieces, g = h0 + hi - p.heads[0];
+            if (g < 0) continue;   // a query head
+            const bool val = g >= p.heads[1];
+            const int h = val ? g - p.heads[1] : g;
+            uint8_t* blk = p.cache + (((int64_t)b * p.heads[1] + h) * p.cache_blocks + tslot[0] / kKvBlock) * Kv4<D>::kBytes;
+            const int to = piece < kCodes ? (val ? Kv4<D>::kV : 0) + 16 * piece
+                                          : (val ? Kv4<D>::kVPar : Kv4<D>::kPar) + 16 * (piece - kCodes);
+            *reinterpret_cast<u32x4*>(blk + to) = *reinterpret_cast<const u32x4*>(image + hi * kImage + 16 * piece);
         }
     }
 }
@@ -349,17 +421,28 @@ extern "C" int sf_heads_rope(const sf_heads_rope_desc* d, void* stream) {
     p.interleaved = d->interleaved != 0;
     p.in_kind = sfk::rope_kind(d->in_dtype);
     p.out_kind = sfk::rope_kind(d->out_dtype);
-    p.tokens = tokens;
     p.eps = d->eps;
+    // A few hundred rows to a workgroup where there are many, one pass of its threads where there are few.
     const int rows = 256 / (d->D / 8);
-    p.tok_per_wg = tokens >= 2048 ? 8 : 1;
-    p.heads_per_wg = p.tok_per_wg == 1 ? rows : (int)heads;
-    const dim3 grid((unsigned)((tokens + p.tok_per_wg - 1) / p.tok_per_wg),
-                    (unsigned)((heads + p.heads_per_wg - 1) / p.heads_per_wg));
-    const size_t lds = sizeof(float2) * (size_t)p.tok_per_wg * (size_t)(d->rot / 2);
+    const bool many = tokens >= 512;
+    p.tok_per_wg = cached ? (d->S >= sfk::kKvBlock ? sfk::kKvBlock : 1) : many ? 8 : 1;
+    p.windows = (int)((d->S + (int64_t)p.tok_per_wg - 1) / p.tok_per_wg);
+    if (p.tok_per_wg == sfk::kKvBlock && (d->positions || d->slots)) ++p.windows;   // the first one may be cut short
+    p.heads_per_wg = (int)std::min<int64_t>(heads, p.tok_per_wg == sfk::kKvBlock ? 8 : many ? 32 : rows);
+    p.heads_magic = (65536 + p.heads_per_wg - 1) / p.heads_per_wg;
+    const int64_t wgs = (int64_t)d->B * p.windows;
+    if (wgs > 0x7fffffffLL) return SF_ENOTSUP;
+    const dim3 grid((unsigned)wgs, (unsigned)((heads + p.heads_per_wg - 1) / p.heads_per_wg));
+    size_t lds = sizeof(float2) * (size_t)p.tok_per_wg * (size_t)(d->rot / 2);
+    if (p.tok_per_wg == sfk::kKvBlock) lds += (size_t)p.heads_per_wg * 18 * d->D;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (d->D == 64) hipLaunchKernelGGL(sfk::heads_rope_kernel<64>, grid, dim3(256), lds, s, p);
-    else hipLaunchKernelGGL(sfk::heads_rope_kernel<128>, grid, dim3(256), lds, s, p);
+    if (d->D == 64) {
+        if (cached) hipLaunchKernelGGL((sfk::heads_rope_kernel<64, true>), grid, dim3(256), lds, s, p);
+        else hipLaunchKernelGGL((sfk::heads_rope_kernel<64, false>), grid, dim3(256), lds, s, p);
+    } else {
+        if (cached) hipLaunchKernelGGL((sfk::heads_rope_kernel<128, true>), grid, dim3(256), lds, s, p);
+        else hipLaunchKernelGGL((sfk::heads_rope_kernel<128, false>), grid, dim3(256), lds, s, p);
+    }
     return hipGetLastError() == hipSuccess ? SF_OK : SF_ELAUNCH;
 }
 

@@ -148,6 +148,47 @@ def test_cache_slots_leave_the_rest():
     assert torch.equal(gv.cpu(), torch.where(inside, _levels(nv).float(), torch.zeros(())))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S", [32, 40, 64, 70, 95, 131])
+@pytest.mark.parametrize("first", [0, 1, 10, 31, 33])
+def test_cache_runs_of_tokens(D, S, first):
+    """Prompts whose slots count up from anywhere in a block, whole blocks and ragged ends; one batch element with a
+    gap, one that runs out of the cache, and what lay beside them."""
+    B, H = 3, 5
+    cap = first + S + 3
+    c = Kv4Cache(B, H, cap, D, DEV)
+    old = _randn(100, B, H, cap, D, dtype=BF)
+    c.write(old.to(DEV), old.to(DEV))
+    k, v = _randn(101, B, H, S, D, dtype=BF), _randn(102, B, H, S, D, dtype=BF)
+    slots = (torch.arange(S) + torch.tensor([[first], [first], [first + 8]])).to(torch.int32)
+    slots[1, S // 2:] += 2
+    c.write(k.to(DEV), v.to(DEV), slots.to(DEV))
+    ek, ev = old.clone(), old.clone()
+    for b in range(B):
+        for j, s in enumerate(slots[b].tolist()):
+            if s < cap:
+                ek[b, :, s], ev[b, :, s] = k[b, :, j], v[b, :, j]
+    rk, rv = c.read(dtype=F32)
+    assert torch.equal(rk.cpu(), _levels(ek).float()) and torch.equal(rv.cpu(), _levels(ev).float())
+
+
+def test_rope_prompt_into_cache_at_an_offset():
+    """A prompt's queries, keys and values together, behind cached tokens, with padding at its end."""
+    B, S, Hq, H, D = 2, 77, 3, 2, 64
+    p = _randn(110, B * S, (Hq + 2 * H) * D, dtype=FP)
+    pos = (torch.arange(S) + torch.tensor([[19], [64]])).to(torch.int32)
+    pos[0, 70:] = -1
+    c = Kv4Cache(B, H, 150, D, DEV)
+    q, _, _ = kernels.heads_rope(p.to(DEV), S, (Hq, H, H), D, positions=pos.to(DEV), inv_freq=_freq(D).to(DEV), cache=c)
+    x = p.double().reshape(B, S, -1, D).transpose(1, 2)
+    real = (pos >= 0)[:, None, :, None]
+    ref = rotate(x[:, :Hq], pos.clamp_min(0), _freq(D), False)
+    keep = real.expand_as(ref)
+    _rope_check(torch.where(keep, q.cpu().double(), 0.0), torch.where(keep, ref, 0.0), x[:, :Hq], FP)
+    _, rv = c.read(pos.to(DEV), F32)
+    assert torch.equal(rv.cpu().double(), torch.where(real, kv4_levels(x[:, Hq + H:].float()), torch.zeros(()).double()))
+
+
 def test_cache_extreme_values():
     """Constant groups, outliers, the largest and smallest numbers; an infinity or NaN spoils its group alone."""
     D = 128

@@ -62,6 +62,15 @@ def test_columns_and_groups(N, group, K):
         _check(out, a.double() @ ref_w.t(), big, K, dtype, what=f"N {N} K {K} group {group}")
 
 
+@pytest.mark.parametrize("M,N", [(5, 4113), (20, 4113), (40, 4113), (90, 2100), (321, 3300)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_many_columns(M, N, group):
+    """More tiles of columns and rows than one shape of workgroup takes."""
+    K, dtype = 384, BF if M & 1 else FP
+    a, w, ref_w, big = _case(M, N, K, group, dtype, True, M)
+    _check(kernels.gemm_w4(a.to(DEV), w, out_dtype=F32), a.double() @ ref_w.t(), big, K, F32, what=f"{M} x {N}")
+
+
 @pytest.mark.parametrize("M", [1, 67])
 @pytest.mark.parametrize("out_dtype", [F32, BF, FP])
 @pytest.mark.parametrize("act", [abi.SF_ACT_NONE, abi.SF_ACT_GELU_TANH, abi.SF_ACT_SILU])
