@@ -93,27 +93,34 @@ __device__ __forceinline__ void store8(void* p, int64_t at, int kind, const floa
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + at) = u;
 }
 
+// max over the 8 lanes of half a DPP row (row8_sum's steps).
+__device__ __forceinline__ float row8_max(float x) {
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xB1, 0xF, 0xF, true)));
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x4E, 0xF, 0xF, true)));
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x141, 0xF, 0xF, true)));
+}
+__device__ __forceinline__ uint32_t row8_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));
+    return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, true));
+}
+
 // Step and middle of a group of 64 channels held by 8 lanes, and the lane's
-// eight codes (channel e at nibble e).  The step is a power of two times a
-// bf16, so step * integer and x - n * step below carry one rounding at most
-// and the code is the floor of the exact quotient, whatever the reciprocal's
-// last bit.
+// eight codes, channel e at nibble (e >> 1) + 4 (e & 1).  The step is a power of
+// two times a bf16, so t * step is exact for the whole t next to the approximate
+// quotient, and comparing with it gives the floor of the exact quotient.
 __device__ __forceinline__ uint32_t kv4_quantise(const float v[8], uint32_t* par) {
-    float mx = v[0], mn = v[0];
+    float mx = v[0], mn = -v[0];
     uint32_t big = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         mx = fmaxf(mx, v[e]);
-        mn = fminf(mn, v[e]);
+        mn = fmaxf(mn, -v[e]);
         big = max(big, __float_as_uint(v[e]) & 0x7fffffffu);
     }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-        mn = fminf(mn, __shfl_xor(mn, o, 64));
-        big = max(big, (uint32_t)__shfl_xor((int)big, o, 64));
-    }
-    if (big >= 0x7f800000u) {   // an infinity or a NaN: the group reads back as NaN
+    mx = row8_max(mx);
+    mn = -row8_max(mn);
+    if (row8_max(big) >= 0x7f800000u) {   // an infinity or a NaN: the group reads back as NaN
         *par = 0x7fc07fc0u;
         return 0;
     }
@@ -129,22 +136,35 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float v[8], uint32_t* par
     uint32_t c = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float d = v[e] - mid;
-        float n = floorf(d * inv);
-        const float left = __builtin_fmaf(-n, s, d);
-        if (left < 0.f) n -= 1.f;
-        else if (left >= s) n += 1.f;
-        c |= (uint32_t)(int)(fminf(fmaxf(n, -8.f), 7.f) + 8.f) << (4 * e);
+        const float d = v[e] - mid, t = rintf(d * inv);
+        const int n = (int)t + (d < t * s ? 7 : 8);
+        c |= (uint32_t)min(max(n, 0), 15) << (4 * ((e >> 1) + 4 * (e & 1)));
     }
     return c;
 }
 
-// Nibble e -> nibble (e >> 1) + 4 (e & 1), and back.
-__device__ __forceinline__ uint32_t nibbles_to_pairs(uint32_t c) {
-    uint32_t o = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o |= ((c >> (4 * e)) & 15u) << (4 * ((e >> 1) + 4 * (e & 1)));
-    return o;
+// A lane's codes of token `tok` to `codes`, the start of its head's key or value
+// codes, with the parameters `par_at` bytes on.  Inlined with a pointer that is
+// known to be of global memory or of LDS: one that may be either would be
+// addressed by flat instructions, which tell the two apart by the address before
+// the instruction's own offset is added.
+template <int D, typename P>
+__device__ __forceinline__ void kv4_put(P codes, int par_at, int tok, bool value, int j, uint32_t c, uint32_t other,
+                                        uint32_t par) {
+    if ((j & 7) == 0) *reinterpret_cast<uint32_t*>(codes + par_at + ((j >> 3) * kKvBlock + tok) * 4) = par;
+    if (!value) {
+        *reinterpret_cast<uint32_t*>(codes + Kv4<D>::key_dword(tok, j)) = c;
+        return;
+    }
+    // Lanes j and j ^ 2 hold channels 16 apart, the low and the high halves of eight bytes: the first writes those of
+    // channels 0, 4, 1, 5, as its nibbles lie, the other 2, 6, 3, 7.
+    const bool hi = j & 2;
+    const uint32_t w = hi ? (other >> 4 & 0x0f0f0f0fu) | (c & 0xf0f0f0f0u) : (c & 0x0f0f0f0fu) | (other << 4 & 0xf0f0f0f0u);
+    P to = codes + Kv4<D>::value_byte(tok, j >> 2, 8 * (j & 1) + (hi ? 2 : 0));
+    to[0] = (uint8_t)w;
+    to[4 * 16] = (uint8_t)(w >> 8);
+    to[16] = (uint8_t)(w >> 16);
+    to[5 * 16] = (uint8_t)(w >> 24);
 }
 
 // One workgroup: up to tok_per_wg tokens of a batch element and heads_per_wg of
@@ -162,6 +182,7 @@ __global__ __launch_bounds__(256) void heads_rope_kernel(const RopeArgs p) {
     float2* cs = reinterpret_cast<float2*>(lds);                                      // [tok_per_wg][rot / 2]
     uint8_t* image = lds + sizeof(float2) * (size_t)p.tok_per_wg * (p.rot >> 1);      // [heads_per_wg][kImage]
     __shared__ int tpos[kRopeTokens], tslot[kRopeTokens], odd;
+    __shared__ __attribute__((aligned(16))) float gamma[2][D];
     const int b = blockIdx.x / p.windows, win = blockIdx.x % p.windows;
     const int64_t m0 = (int64_t)b * p.S;
     int s0 = win * p.tok_per_wg, s1 = min(s0 + p.tok_per_wg, p.S);
@@ -174,6 +195,7 @@ __global__ __launch_bounds__(256) void heads_rope_kernel(const RopeArgs p) {
     const int nt = s1 - s0, half = p.rot >> 1;
     if (nt <= 0) return;
     if (threadIdx.x == 0) odd = nt != kKvBlock;
+    if (threadIdx.x < 2 * D && p.gamma[threadIdx.x / D]) gamma[threadIdx.x / D][threadIdx.x % D] = p.gamma[threadIdx.x / D][threadIdx.x % D];
     __syncthreads();
     if ((int)threadIdx.x < nt) {
         const int s = s0 + (int)threadIdx.x, pos = p.positions ? p.positions[m0 + s] : s;
@@ -218,15 +240,14 @@ __global__ __launch_bounds__(256) void heads_rope_kernel(const RopeArgs p) {
             const int ti = where[a] >> 20, sec = where[a] >> 18 & 3, h = where[a] & 0x3ffff;
             float v[8];
             widen8(raw[a], p.in_kind, v);
-            const float* gm = sec == 0 ? p.gamma[0] : sec == 1 ? p.gamma[1] : nullptr;
-            if (gm) {
+            if (sec == 0 ? p.gamma[0] != nullptr : sec == 1 && p.gamma[1]) {
                 float q = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) q += v[e] * v[e];
                 q = L == 8 ? row8_sum(q) : row16_sum(q);
-                const float r = 1.f / sqrtf(q / (float)D + p.eps);
+                const float r = __builtin_amdgcn_rsqf(q * (1.f / (float)D) + p.eps);   // one unit
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = v[e] * r * gm[8 * j + e];
+                for (int e = 0; e < 8; ++e) v[e] = v[e] * r * gamma[sec][8 * j + e];
             }
             if (sec < 2 && half) {
                 const float2* t = cs + ti * half;
@@ -265,25 +286,14 @@ __global__ __launch_bounds__(256) void heads_rope_kernel(const RopeArgs p) {
                 const uint32_t other = (uint32_t)__shfl_xor((int)c, 2, 64);
                 const int slot = tslot[ti];
                 if (slot < 0 || slot >= p.cap) continue;
-                // where the block's codes and parameters lie: in the cache, or in this head's image
-                const int tok = slot % kKvBlock, head = (int)(sec == 1 ? p.heads[0] + h : p.heads[0] + p.heads[1] + h) - h0;
-                uint8_t* blk = whole ? image + head * kImage
-                                     : p.cache + (((int64_t)b * p.heads[1] + h) * p.cache_blocks + slot / kKvBlock) * Kv4<D>::kBytes;
-                uint8_t* pars = blk + (whole ? 16 * D : sec == 1 ? Kv4<D>::kPar : Kv4<D>::kVPar);
-                if ((j & 7) == 0) *reinterpret_cast<uint32_t*>(pars + ((j >> 3) * kKvBlock + tok) * 4) = par;
-                if (sec == 1) {
-                    *reinterpret_cast<uint32_t*>(blk + Kv4<D>::key_dword(tok, j)) = nibbles_to_pairs(c);
+                const int tok = slot % kKvBlock;
+                if (whole) {   // the head's image in LDS: codes, then parameters
+                    const int head = (sec == 1 ? p.heads[0] + h : p.heads[0] + p.heads[1] + h) - h0;
+                    kv4_put<D>(image + head * kImage, 16 * D, tok, sec == 2, j, c, other, par);
                 } else {
-                    // lanes j and j ^ 2 hold channels 16 apart: each writes four of the eight bytes they share
-                    const bool hi = j & 2;
-                    const uint32_t lo = hi ? other : c, up = hi ? c : other;
-                    const int first = hi ? 4 : 0, at = whole ? Kv4<D>::kV : 0;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int sh = 4 * (first + e);
-                        blk[Kv4<D>::value_byte(tok, j >> 2, 8 * (j & 1) + first + e) - at] =
-                            (uint8_t)(((lo >> sh) & 15u) | ((up >> sh) & 15u) << 4);
-                    }
+                    uint8_t* blk = p.cache + (((int64_t)b * p.heads[1] + h) * p.cache_blocks + slot / kKvBlock) * Kv4<D>::kBytes;
+                    if (sec == 1) kv4_put<D>(blk, Kv4<D>::kPar, tok, false, j, c, other, par);
+                    else kv4_put<D>(blk + Kv4<D>::kV, Kv4<D>::kVPar - Kv4<D>::kV, tok, true, j, c, other, par);
                 }
             }
         }
@@ -305,46 +315,79 @@ __global__ __launch_bounds__(256) void heads_rope_kernel(const RopeArgs p) {
     }
 }
 
+// Eight channels of a token's key (sec 0) or value out of its block (in global
+// memory or in LDS: see kv4_put).
+template <int D, typename P>
+__device__ __forceinline__ void kv4_get(P blk, int tok, int sec, int j, float v[8]) {
+    const uint32_t par = *reinterpret_cast<const uint32_t*>(
+        blk + (sec ? Kv4<D>::value_par(tok, j >> 3) : Kv4<D>::key_par(tok, j >> 3)));
+    const float st = __uint_as_float(par << 16), mid = __uint_as_float(par & 0xffff0000u);
+    if (sec) {
+        P from = blk + Kv4<D>::kV + Kv4<D>::value_byte(tok, j >> 2, 8 * (j & 1));
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = __builtin_fmaf((float)((uint32_t)from[16 * e] >> (j & 2 ? 4 : 0) & 15u) - 7.5f, st, mid);
+    } else {
+        const uint32_t c = *reinterpret_cast<const uint32_t*>(blk + Kv4<D>::key_dword(tok, j));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf((float)(c >> (4 * ((e >> 1) + 4 * (e & 1))) & 15u) - 7.5f, st, mid);
+    }
+}
+
 struct Kv4ReadArgs {
     const uint8_t* cache;
     int64_t cache_blocks;
     const int32_t* slots;
     void* out[2];
     int64_t os[2][3];
-    int H, S, cap, out_kind;
-    int64_t rows;   // B * S * H * 2
+    int H, S, cap, out_kind, windows;
 };
 
-// The values of given slots: one row of D / 8 lanes per (token, head, K or V).
+constexpr int kReadHeads = 4;   // heads of a workgroup
+
+// The values of given slots, 32 tokens of four heads to a workgroup.  Tokens
+// that fill a block are read through LDS, whole blocks at 16 bytes a lane; others
+// piece by piece.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4ReadArgs p) {
-    constexpr int L = D / 8, kRows = 256 / L;
-    const int j = threadIdx.x & (L - 1);
-    const int64_t i = (int64_t)blockIdx.x * kRows + threadIdx.x / L;
-    if (i >= p.rows) return;
-    const int sec = (int)(i & 1), h = (int)((i >> 1) % p.H);
-    const int64_t m = (i >> 1) / p.H, b = m / p.S;
-    const int s = (int)(m % p.S);
-    const int slot = p.slots ? p.slots[m] : s;
-    float v[8];
-    if (slot < 0 || slot >= p.cap) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    } else {
-        const uint8_t* blk = p.cache + ((b * p.H + h) * p.cache_blocks + slot / kKvBlock) * Kv4<D>::kBytes;
-        const int tok = slot % kKvBlock;
-        const uint32_t par = *reinterpret_cast<const uint32_t*>(
-            blk + (sec ? Kv4<D>::value_par(tok, j >> 3) : Kv4<D>::key_par(tok, j >> 3)));
-        const float st = __uint_as_float(par << 16), mid = __uint_as_float(par & 0xffff0000u);
-        const uint32_t c = sec ? 0u : *reinterpret_cast<const uint32_t*>(blk + Kv4<D>::key_dword(tok, j));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            uint32_t n = (c >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u;
-            if (sec) n = ((uint32_t)blk[Kv4<D>::value_byte(tok, j >> 2, 8 * (j & 1) + e)] >> (j & 2 ? 4 : 0)) & 15u;
-            v[e] = __builtin_fmaf((float)n - 7.5f, st, mid);
-        }
+    constexpr int L = D / 8, kRows = 256 / L, kBlk = Kv4<D>::kBytes;
+    __shared__ __attribute__((aligned(16))) uint8_t image[kReadHeads * kBlk];
+    __shared__ int tslot[kKvBlock], odd;
+    const int b = blockIdx.x / p.windows, win = blockIdx.x % p.windows, h0 = blockIdx.y * kReadHeads;
+    const int nh = min(kReadHeads, p.H - h0);
+    const int64_t m0 = (int64_t)b * p.S;
+    const int off = p.slots ? p.slots[m0] & (kKvBlock - 1) : 0;
+    const int s0 = max(win * kKvBlock - off, 0), s1 = min((win + 1) * kKvBlock - off, p.S), nt = s1 - s0;
+    if (nt <= 0) return;
+    if (threadIdx.x == 0) odd = nt != kKvBlock;
+    __syncthreads();
+    if ((int)threadIdx.x < nt) {
+        const int s = s0 + (int)threadIdx.x, slot = p.slots ? p.slots[m0 + s] : s, first = p.slots ? p.slots[m0 + s0] : s0;
+        tslot[threadIdx.x] = slot;
+        if (first < 0 || (first & (kKvBlock - 1)) || slot != first + (int)threadIdx.x || slot >= p.cap) odd = 1;
     }
-    store8(p.out[sec], b * p.os[sec][0] + h * p.os[sec][1] + s * p.os[sec][2] + 8 * j, p.out_kind, v);
+    __syncthreads();
+    const bool whole = !odd;
+    const uint8_t* heads = p.cache + ((int64_t)b * p.H + h0) * p.cache_blocks * kBlk;
+    if (whole) {
+        for (int i = threadIdx.x; i < nh * (kBlk / 16); i += 256) {
+            const int hi = i / (kBlk / 16), piece = i % (kBlk / 16);
+            *reinterpret_cast<u32x4*>(image + hi * kBlk + 16 * piece) = *reinterpret_cast<const u32x4*>(
+                heads + (hi * p.cache_blocks + tslot[0] / kKvBlock) * kBlk + 16 * piece);
+        }
+        __syncthreads();
+    }
+    const int j = threadIdx.x & (L - 1);
+    for (int i = threadIdx.x / L; i < nt * nh * 2; i += kRows) {
+        const int sec = i & 1, hi = (i >> 1) % nh, ti = (i >> 1) / nh, slot = tslot[ti];
+        float v[8] = {};
+        if (slot >= 0 && slot < p.cap) {
+            const int tok = slot % kKvBlock;
+            if (whole) kv4_get<D>(image + hi * kBlk, tok, sec, j, v);
+            else kv4_get<D>(heads + (hi * p.cache_blocks + slot / kKvBlock) * kBlk, tok, sec, j, v);
+        }
+        store8(p.out[sec], b * p.os[sec][0] + (h0 + hi) * p.os[sec][1] + (s0 + ti) * p.os[sec][2] + 8 * j, p.out_kind, v);
+    }
 }
 
 static inline int rope_kind(int32_t dt) { return dt == SF_BF16 ? 1 : (dt == SF_F16 ? 2 : 0); }
@@ -465,12 +508,13 @@ extern "C" int sf_kv4_read(const sf_kv4_cache* cache, const int32_t* slots, int3
     p.S = S;
     p.cap = cache->capacity;
     p.out_kind = sfk::rope_kind(out_dtype);
-    p.rows = (int64_t)cache->B * S * cache->H * 2;
-    const int rows = 256 / (cache->D / 8);
-    const int64_t blocks = (p.rows + rows - 1) / rows;
-    if ((int64_t)cache->B * S > 0x7fffffffLL || blocks > 0x7fffffffLL) return SF_ENOTSUP;
+    if ((int64_t)cache->B * S > 0x7fffffffLL || (cache->H + sfk::kReadHeads - 1) / sfk::kReadHeads > 65535) return SF_ENOTSUP;
+    // with slots the first window may be cut short
+    p.windows = (int)((S + (int64_t)sfk::kKvBlock - 1) / sfk::kKvBlock) + (slots ? 1 : 0);
+    if ((int64_t)cache->B * p.windows > 0x7fffffffLL) return SF_ENOTSUP;
+    const dim3 grid((unsigned)(cache->B * p.windows), (unsigned)((cache->H + sfk::kReadHeads - 1) / sfk::kReadHeads));
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (cache->D == 64) hipLaunchKernelGGL(sfk::kv4_read_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL(sfk::kv4_read_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, s, p);
+    if (cache->D == 64) hipLaunchKernelGGL(sfk::kv4_read_kernel<64>, grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(sfk::kv4_read_kernel<128>, grid, dim3(256), 0, s, p);
     return hipGetLastError() == hipSuccess ? SF_OK : SF_ELAUNCH;
 }

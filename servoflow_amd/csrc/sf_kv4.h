@@ -40,10 +40,10 @@ struct Kv4 {
         const int grp = j >> 3, g = (j >> 1) & 3, lane = 16 * g + (tok & 15), tile = tok >> 4;
         return D == 64 ? lane * 16 + tile * 8 + (j & 1) * 4 : tile * 1024 + lane * 16 + grp * 8 + (j & 1) * 4;
     }
-    // Byte of token `tok`'s value codes of channels 32 t + dl (low nibble) and 32 t + 16 + dl (high).
+    // Byte, from kV on, of token `tok`'s value codes of channels 32 t + dl (low nibble) and 32 t + 16 + dl (high).
     __device__ static int value_byte(int tok, int t, int dl) {
         const int g = (tok & 15) >> 2, e = tok & 3;
-        return kV + (t >> 1) * 1024 + (16 * g + dl) * 16 + (t & 1) * 8 + (tok >> 4) * 4 + ((e & 1) << 1 | e >> 1);
+        return (t >> 1) * 1024 + (16 * g + dl) * 16 + (t & 1) * 8 + (tok >> 4) * 4 + ((e & 1) << 1 | e >> 1);
     }
     __device__ static int key_par(int tok, int grp) { return kPar + (grp * kKvBlock + tok) * 4; }
     __device__ static int value_par(int tok, int grp) { return kVPar + (grp * kKvBlock + tok) * 4; }
