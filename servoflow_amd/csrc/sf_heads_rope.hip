@@ -47,29 +47,20 @@ struct RopeArgs {
     int heads_magic;                   // ceil(2^16 / heads_per_wg): (i * this) >> 16 is i / heads_per_wg, i < 2048
 };
 
-// Eight channels as loaded.  kind: 0 fp32, 1 bf16, 2 fp16
-struct Raw8 {
-    u32x4 a, b;   // b: fp32 only
-};
-__device__ __forceinline__ Raw8 load8(const void* p, int64_t at, int kind) {
-    Raw8 r = {};
+// kind: 0 fp32, 1 bf16, 2 fp16
+__device__ __forceinline__ void load8(const void* p, int64_t at, int kind, float v[8]) {
     if (kind == 0) {
-        const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const float*>(p) + at);
-        r.a = q[0];
-        r.b = q[1];
-    } else {
-        r.a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
+        const f32x4* q = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
+        const f32x4 a = q[0], b = q[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+        return;
     }
-    return r;
-}
-__device__ __forceinline__ void widen8(const Raw8& r, int kind, float v[8]) {
+    const u32x4 r = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const uint32_t u = r.a[e], w = r.b[e];
-        if (kind == 0) {
-            v[e] = __uint_as_float(u);
-            v[4 + e] = __uint_as_float(w);
-        } else if (kind == 1) {
+        const uint32_t u = r[e];
+        if (kind == 1) {
             v[2 * e] = __uint_as_float(u << 16);
             v[2 * e + 1] = __uint_as_float(u & 0xffff0000u);
         } else {
@@ -176,7 +167,7 @@ __device__ __forceinline__ void kv4_put(P codes, int par_at, int tok, bool value
 // of 32 heads took 45 us that way).
 template <int D, bool CACHE>
 __global__ __launch_bounds__(256) void heads_rope_kernel(const RopeArgs p) {
-    constexpr int L = D / 8, kRows = 256 / L, kAhead = 4;   // rows in flight a thread
+    constexpr int L = D / 8, kRows = 256 / L;
     constexpr int kImage = 16 * D + 2 * D;                  // a head's codes and parameters of 32 tokens, keys or values
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     float2* cs = reinterpret_cast<float2*>(lds);                                      // [tok_per_wg][rot / 2]
@@ -220,81 +211,68 @@ __global__ __launch_bounds__(256) void heads_rope_kernel(const RopeArgs p) {
     const int h0 = blockIdx.y * p.heads_per_wg;
     const int nh = min(p.heads_per_wg, p.heads[0] + p.heads[1] + p.heads[2] - h0);
     const int rows = nt * p.heads_per_wg;
-    for (int base = sub; base - sub < rows; base += kRows * kAhead) {
-        Raw8 raw[kAhead];
-        int where[kAhead];   // token << 20 | section << 18 | head; -1: none
+    for (int i = sub; i < rows; i += kRows) {
+        const int ti = (i * p.heads_magic) >> 16, hi = i - ti * p.heads_per_wg;
+        if (hi >= nh || tpos[ti] < 0) continue;   // whole groups of L lanes; a padding token is not written
+        int h = h0 + hi, sec = 0;
+        if (h >= p.heads[0]) h -= p.heads[0], sec = 1;
+        if (sec == 1 && h >= p.heads[1]) h -= p.heads[1], sec = 2;
+        float v[8];
+        load8(p.src[sec], b * p.ss[sec][0] + h * p.ss[sec][1] + (s0 + ti) * p.ss[sec][2] + 8 * j, p.in_kind, v);
+        if (sec == 0 ? p.gamma[0] != nullptr : sec == 1 && p.gamma[1]) {
+            float q = 0.f;
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-            const int i = base + a * kRows, ti = (i * p.heads_magic) >> 16, hi = i - ti * p.heads_per_wg;
-            where[a] = -1;
-            if (i >= rows || hi >= nh || tpos[ti] < 0) continue;   // a padding token is not written
-            int h = h0 + hi, sec = 0;
-            if (h >= p.heads[0]) h -= p.heads[0], sec = 1;
-            if (sec == 1 && h >= p.heads[1]) h -= p.heads[1], sec = 2;
-            where[a] = ti << 20 | sec << 18 | h;
-            raw[a] = load8(p.src[sec], b * p.ss[sec][0] + h * p.ss[sec][1] + (s0 + ti) * p.ss[sec][2] + 8 * j, p.in_kind);
+            for (int e = 0; e < 8; ++e) q += v[e] * v[e];
+            q = L == 8 ? row8_sum(q) : row16_sum(q);
+            const float r = __builtin_amdgcn_rsqf(q * (1.f / (float)D) + p.eps);   // one unit
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] * r * gamma[sec][8 * j + e];
         }
+        if (sec < 2 && half) {
+            const float2* t = cs + ti * half;
+            if (p.interleaved) {
+                if (8 * j < p.rot) {
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-            if (where[a] < 0) continue;   // whole groups of L lanes
-            const int ti = where[a] >> 20, sec = where[a] >> 18 & 3, h = where[a] & 0x3ffff;
-            float v[8];
-            widen8(raw[a], p.in_kind, v);
-            if (sec == 0 ? p.gamma[0] != nullptr : sec == 1 && p.gamma[1]) {
-                float q = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) q += v[e] * v[e];
-                q = L == 8 ? row8_sum(q) : row16_sum(q);
-                const float r = __builtin_amdgcn_rsqf(q * (1.f / (float)D) + p.eps);   // one unit
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = v[e] * r * gamma[sec][8 * j + e];
-            }
-            if (sec < 2 && half) {
-                const float2* t = cs + ti * half;
-                if (p.interleaved) {
-                    if (8 * j < p.rot) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 w = t[4 * j + e];
-                            const float x = v[2 * e], y = v[2 * e + 1];
-                            v[2 * e] = x * w.x - y * w.y;
-                            v[2 * e + 1] = y * w.x + x * w.y;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 w = t[4 * j + e];
+                        const float x = v[2 * e], y = v[2 * e + 1];
+                        v[2 * e] = x * w.x - y * w.y;
+                        v[2 * e + 1] = y * w.x + x * w.y;
                     }
-                } else {   // the partner's 8 channels are rot / 16 lanes away
-                    const int step = p.rot >> 4;
-                    const bool low = j < step, in = j < 2 * step;
-                    const int lane = (int)(threadIdx.x & 63);
-                    const int from = in ? (low ? lane + step : lane - step) : lane;
+                }
+            } else {   // the partner's 8 channels are rot / 16 lanes away
+                const int step = p.rot >> 4;
+                const bool low = j < step, in = j < 2 * step;
+                const int lane = (int)(threadIdx.x & 63);
+                const int from = in ? (low ? lane + step : lane - step) : lane;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float y = __shfl(v[e], from, 64);
-                        if (in) {
-                            const float2 w = t[8 * (low ? j : j - step) + e];
-                            v[e] = low ? v[e] * w.x - y * w.y : v[e] * w.x + y * w.y;
-                        }
+                for (int e = 0; e < 8; ++e) {
+                    const float y = __shfl(v[e], from, 64);
+                    if (in) {
+                        const float2 w = t[8 * (low ? j : j - step) + e];
+                        v[e] = low ? v[e] * w.x - y * w.y : v[e] * w.x + y * w.y;
                     }
                 }
             }
-            if (sec == 0 || !CACHE) {
-                store8(p.out[sec], b * p.os[sec][0] + h * p.os[sec][1] + (s0 + ti) * p.os[sec][2] + 8 * j, p.out_kind, v);
-                continue;
-            }
-            if constexpr (CACHE) {
-                uint32_t par;
-                const uint32_t c = kv4_quantise(v, &par);
-                const uint32_t other = (uint32_t)__shfl_xor((int)c, 2, 64);
-                const int slot = tslot[ti];
-                if (slot < 0 || slot >= p.cap) continue;
-                const int tok = slot % kKvBlock;
-                if (whole) {   // the head's image in LDS: codes, then parameters
-                    const int head = (sec == 1 ? p.heads[0] + h : p.heads[0] + p.heads[1] + h) - h0;
-                    kv4_put<D>(image + head * kImage, 16 * D, tok, sec == 2, j, c, other, par);
-                } else {
-                    uint8_t* blk = p.cache + (((int64_t)b * p.heads[1] + h) * p.cache_blocks + slot / kKvBlock) * Kv4<D>::kBytes;
-                    if (sec == 1) kv4_put<D>(blk, Kv4<D>::kPar, tok, false, j, c, other, par);
-                    else kv4_put<D>(blk + Kv4<D>::kV, Kv4<D>::kVPar - Kv4<D>::kV, tok, true, j, c, other, par);
-                }
+        }
+        if (sec == 0 || !CACHE) {
+            store8(p.out[sec], b * p.os[sec][0] + h * p.os[sec][1] + (s0 + ti) * p.os[sec][2] + 8 * j, p.out_kind, v);
+            continue;
+        }
+        if constexpr (CACHE) {
+            uint32_t par;
+            const uint32_t c = kv4_quantise(v, &par);
+            const uint32_t other = (uint32_t)__shfl_xor((int)c, 2, 64);
+            const int slot = tslot[ti];
+            if (slot < 0 || slot >= p.cap) continue;
+            const int tok = slot % kKvBlock;
+            if (whole) {   // the head's image in LDS: codes, then parameters
+                const int head = (sec == 1 ? p.heads[0] + h : p.heads[0] + p.heads[1] + h) - h0;
+                kv4_put<D>(image + head * kImage, 16 * D, tok, sec == 2, j, c, other, par);
+            } else {
+                uint8_t* blk = p.cache + (((int64_t)b * p.heads[1] + h) * p.cache_blocks + slot / kKvBlock) * Kv4<D>::kBytes;
+                if (sec == 1) kv4_put<D>(blk, Kv4<D>::kPar, tok, false, j, c, other, par);
+                else kv4_put<D>(blk + Kv4<D>::kV, Kv4<D>::kVPar - Kv4<D>::kV, tok, true, j, c, other, par);
             }
         }
     }
@@ -465,13 +443,15 @@ extern "C" int sf_heads_rope(const sf_heads_rope_desc* d, void* stream) {
     p.in_kind = sfk::rope_kind(d->in_dtype);
     p.out_kind = sfk::rope_kind(d->out_dtype);
     p.eps = d->eps;
-    // A few hundred rows to a workgroup where there are many, one pass of its threads where there are few.
+    // Rows to a workgroup.  Into a cache a block's tokens of four heads (4374 tokens x 64 heads: 23.5 us, 26 with
+    // eight, 35 with sixteen).  Else four tokens of 32 heads, which share the sines, fewer where there are few tokens:
+    // 4374 x 96 heads of 64 channels take 24 us with four, 25.5 with two, 31.5 with eight; 1072 x 96 12.5, 10 and 18.
     const int rows = 256 / (d->D / 8);
-    const bool many = tokens >= 512;
-    p.tok_per_wg = cached ? (d->S >= sfk::kKvBlock ? sfk::kKvBlock : 1) : many ? 8 : 1;
+    const int spread = tokens >= 2048 ? 4 : tokens >= 512 ? 2 : 1;
+    p.tok_per_wg = cached ? (d->S >= sfk::kKvBlock ? sfk::kKvBlock : 1) : spread;
     p.windows = (int)((d->S + (int64_t)p.tok_per_wg - 1) / p.tok_per_wg);
     if (p.tok_per_wg == sfk::kKvBlock && (d->positions || d->slots)) ++p.windows;   // the first one may be cut short
-    p.heads_per_wg = (int)std::min<int64_t>(heads, p.tok_per_wg == sfk::kKvBlock ? 8 : many ? 32 : rows);
+    p.heads_per_wg = (int)std::min<int64_t>(heads, p.tok_per_wg == sfk::kKvBlock ? 4 : p.tok_per_wg > 1 ? 32 : rows);
     p.heads_magic = (65536 + p.heads_per_wg - 1) / p.heads_per_wg;
     const int64_t wgs = (int64_t)d->B * p.windows;
     if (wgs > 0x7fffffffLL) return SF_ENOTSUP;
