@@ -4,11 +4,13 @@
 // 64-channel group, so both contractions run on the codes themselves and the
 // parameters meet the scores in fp32:
 //   S_j = s_j sum_d q_d (16 + c_jd) + (mid_j - 23.5 s_j) sum_d q_d
-//   O_d = sum_j p_j s_j (16 + c_jd) + sum_j p_j (mid_j - 23.5 s_j)
+//   O_d = sum_j p_j s_j (16 + c_jd) - 23.5 sum_j p_j s_j + sum_j p_j mid_j
 // (16 + c: see sf_nibble.h).  p_j s_j enters the matrix unit as a bf16 (hi, lo)
-// pair, 2^-18 relative: the codes' offset triples what that rounding does to a
-// value, which one bf16 would make visible in a 16-bit output and the pair
-// keeps near fp32's own error.
+// pair, 2^-18 relative, and its sum is taken over the same rounded pair, so that
+// what the codes' offset adds is taken away exactly.  With many query rows to an
+// unpacked block and a bf16 output the values are formed in fp16 instead, once
+// for all rows, and p enters as one fp16: five vector operations fewer for every
+// score, and errors of 2^-12 where the output's own rounding is 2^-9.
 //
 // One wave takes blocks of 32 tokens against QT tiles of 16 query rows; query
 // heads that share a key head are rows of one tile, so a cached token is read
@@ -78,9 +80,14 @@ __device__ __forceinline__ float lanes4_max(float x) {
     return fmaxf(x, __shfl_xor(x, 32, 64));
 }
 
-// mid - 23.5 s of a parameter dword (both exact in the dot product's operands).
-__device__ __forceinline__ float kv_offset(uint32_t par) {
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v, par), bf16x2v{(__bf16)-23.5f, (__bf16)1.f}, 0.f, false);
+// a s + b mid of a parameter dword, in fp32; a and b are bf16 numbers.
+__device__ __forceinline__ float kv_mix(uint32_t par, float a, float b) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v, par), bf16x2v{(__bf16)a, (__bf16)b}, 0.f, false);
+}
+
+// acc - 23.5 times the sum of a pair of bf16.
+__device__ __forceinline__ float kv_dot(uint32_t pair, float acc) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v, pair), bf16x2v{(__bf16)-23.5f, (__bf16)-23.5f}, acc, false);
 }
 
 // What a wave holds of a block of 32 tokens.
@@ -208,11 +215,10 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // fp16 form: values are held times `vdown`, a power of two that keeps |mid - 23.5 s| + 31 s, and with it both terms
-    // and the value, below 2^15 for every token seen: 1 where they fit as they are, else such that the largest is in
-    // fp16's upper binades and smaller ones stay normal over 2^29.  `vcap` = 2^15 / vdown.
-    float vdown = 1.f, vcap = 0.f;
-    const NibbleMask kmask = nibble_mask<F16>(), vmask = nibble_mask<!PAIR>();
+    // fp16 form: values are held times `vdown`, a power of two of the wave's that keeps 2^18 s and |mid - 7.5 s| of
+    // every token seen below 2^15; the first block sets it, a larger one lowers it.
+    float vdown = 1.f / 262144.f, vcap = 0.f;
+    const NibbleMask kmask = nibble_mask<F16>(), vmask = nibble_mask<false>();
 
     auto block = [&](const int blk, auto masked_c) __attribute__((always_inline)) {
         constexpr bool masked = decltype(masked_c)::value;
@@ -235,9 +241,9 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 if (masked && !(see >> e & 1u)) kp = vp = 0u;   // tokens behind the last hold anything
                 if (masked && !PAIR && (vp & 0x7f80u) == 0x7f80u) kp |= 0x7fc07fc0u, vp = 0u;   // see below
                 ks[i][e] = __uint_as_float(kp << 16) * p.scale_log2;
-                ko[i][e] = kv_offset(kp);
-                vs[i][e] = __uint_as_float(vp << 16);
-                vm[i][e] = kv_offset(vp);
+                ko[i][e] = kv_mix(kp, -23.5f, 1.f);
+                vs[i][e] = PAIR ? __uint_as_float(vp << 16) : kv_mix(vp, 262144.f * vdown, 0.f);
+                vm[i][e] = PAIR ? __uint_as_float(vp & 0xffff0000u) : kv_mix(vp, -7.5f * vdown, vdown);
             }
         u32x4 ka[2][GR][2], va[DT];
 #pragma unroll
@@ -246,52 +252,50 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
             for (int i = 0; i < GR; ++i)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) ka[t][i][k] = nibbles_plus16<F16>(nx.key(t, i, k), kmask);
-#pragma unroll
-        for (int t = 0; t < DT / 2; ++t) {
-            const uint32_t w0 = nx.v[t >> 1][2 * (t & 1)], w1 = nx.v[t >> 1][2 * (t & 1) + 1];
-            va[2 * t] = u32x4{nibble_pair_plus16<!PAIR, 0>(w0, vmask), nibble_pair_plus16<!PAIR, 2>(w0, vmask),
-                              nibble_pair_plus16<!PAIR, 0>(w1, vmask), nibble_pair_plus16<!PAIR, 2>(w1, vmask)};
-            va[2 * t + 1] = u32x4{nibble_pair_plus16<!PAIR, 1>(w0, vmask), nibble_pair_plus16<!PAIR, 3>(w0, vmask),
-                                  nibble_pair_plus16<!PAIR, 1>(w1, vmask), nibble_pair_plus16<!PAIR, 3>(w1, vmask)};
-        }
         if (!PAIR) {
             float big = 0.f;
 #pragma unroll
             for (int i = 0; i < GR; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) big = fmaxf(big, __builtin_fmaf(31.f, vs[i][e], fabsf(vm[i][e])));
-            if (__any(big > vcap)) {
+                for (int e = 0; e < 8; ++e) big = fmaxf(fmaxf(big, vs[i][e]), fabsf(vm[i][e]));
+            if (__any(big > vcap)) {   // a new power: this block's largest to 2^12 .. 2^13
 #pragma unroll
                 for (int w = 1; w < 64; w <<= 1) big = fmaxf(big, __shfl_xor(big, w, 64));
-                int ex = (int)(__float_as_uint(big) >> 23) - 127 - 14;   // big < 2^(ex + 15)
-                if (vcap == 0.f && ex <= 0 && ex >= -16) ex = 0;         // fp16 holds them as they are
-                ex = __builtin_amdgcn_readfirstlane(max(ex, -100));
-                const float nd = __uint_as_float((uint32_t)(127 - ex) << 23), al = nd / vdown;
-                vcap = __uint_as_float((uint32_t)(127 + ex) << 23) * 32768.f;
-                vdown = nd;
+                const int now = (int)(__float_as_uint(vdown) >> 23) - 127;
+                const int want = big > 0.f ? now + 12 + 127 - (int)(__float_as_uint(big) >> 23) : now;
+                const int ex = __builtin_amdgcn_readfirstlane(min(max(want, -126), 100));
+                const float al = __builtin_amdgcn_ldexpf(1.f, ex - now);
+                vdown = __uint_as_float((uint32_t)(127 + ex) << 23);
+                vcap = 32768.f;
 #pragma unroll
                 for (int t = 0; t < QT; ++t)
 #pragma unroll
                     for (int i = 0; i < DT; ++i) o[t][i] *= al;
-            }
-            if (vdown != 1.f) {
 #pragma unroll
                 for (int i = 0; i < GR; ++i)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) vs[i][e] *= vdown, vm[i][e] *= vdown;
+                    for (int e = 0; e < 8; ++e) vs[i][e] *= al, vm[i][e] *= al;
             }
+        }
 #pragma unroll
-            for (int i = 0; i < GR; ++i)
+        for (int t = 0; t < DT / 2; ++t) {
+            const uint32_t w0 = nx.v[t >> 1][2 * (t & 1)], w1 = nx.v[t >> 1][2 * (t & 1) + 1];
+            if (PAIR) {
+                va[2 * t] = u32x4{nibble_pair_plus16<false, 0>(w0, vmask), nibble_pair_plus16<false, 2>(w0, vmask),
+                                  nibble_pair_plus16<false, 0>(w1, vmask), nibble_pair_plus16<false, 2>(w1, vmask)};
+                va[2 * t + 1] = u32x4{nibble_pair_plus16<false, 1>(w0, vmask), nibble_pair_plus16<false, 3>(w0, vmask),
+                                      nibble_pair_plus16<false, 1>(w1, vmask), nibble_pair_plus16<false, 3>(w1, vmask)};
+            } else {   // c 2^-18 as fp16 subnormals, then pairs of tokens' c s + (mid - 7.5 s) with one rounding
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {   // pairs of tokens: (16 + c) s + (mid - 23.5 s)
-                    const f16x2v sp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vs[i][2 * e], vs[i][2 * e + 1]));
-                    const f16x2v mp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vm[i][2 * e], vm[i][2 * e + 1]));
-#pragma unroll
-                    for (int t = 4 * i; t < 4 * i + 4; ++t) {
-                        const uint32_t w = va[t][e];   // a value: bit_cast of a vector's element reads its first one
-                        va[t][e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2v, w), sp, mp));
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w = e < 2 ? w0 : w1;
+                    const uint32_t lo = e & 1 ? w >> 2 : w << 6, hi = e & 1 ? w >> 6 : w << 2;
+                    const f16x2v sp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vs[t >> 1][2 * e], vs[t >> 1][2 * e + 1]));
+                    const f16x2v mp = __builtin_bit_cast(f16x2v, pack_f16x2_rn(vm[t >> 1][2 * e], vm[t >> 1][2 * e + 1]));
+                    va[2 * t][e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2v, lo & 0x03C003C0u), sp, mp));
+                    va[2 * t + 1][e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2v, hi & 0x03C003C0u), sp, mp));
                 }
+            }
         }
         // the raw block is spent: fetch the wave's next one
         if (blk + NW < b1) nx.load(base + (int64_t)(blk + NW) * Kv4<D>::kBytes, lane);
@@ -365,9 +369,11 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                             if (!(row >> (2 * e) & 1u)) a = ma = 0.f;
                             if (!(row >> (2 * e + 1) & 1u)) c = mc = 0.f;
                         }
-                        pm[t][i] += ma + mc;
-                        hi[e] = pack_bf16x2(a, c);
-                        lo[e] = pack_bf16x2(a - __uint_as_float(hi[e] << 16), c - __uint_as_float(hi[e] & 0xffff0000u));
+                        const uint32_t h = pack_bf16x2(a, c);
+                        const uint32_t w = pack_bf16x2(a - __uint_as_float(h << 16), c - __uint_as_float(h & 0xffff0000u));
+                        pm[t][i] = kv_dot(h, kv_dot(w, pm[t][i] + ma + mc));
+                        hi[e] = h;
+                        lo[e] = w;
                     }
 #pragma unroll
                     for (int d = 4 * i; d < 4 * i + 4; ++d) {
