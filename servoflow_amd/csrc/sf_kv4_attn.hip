@@ -133,7 +133,7 @@ template <bool F16, int D, int QT, bool PAIR, int NW>
 __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     constexpr int GR = D / 64, DT = D / 16;   // 64-channel groups, tiles of 16 channels
     __shared__ float xm[NW][QT * 16], xl[NW][QT * 16], xf[NW][QT * 16], xs[QT * 16];
-    constexpr int kJoin = QT == 5 ? 3 : QT;   // tiles that meet at a time
+    constexpr int kJoin = QT == 5 ? 3 : QT == 4 ? 2 : QT;   // tiles that meet at a time
     __shared__ float xo[NW][kJoin * 16][D + 4], xq[GR][QT * 16];
     __shared__ u32x4 ql[QT > 1 ? QT * GR * 2 : 1][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -531,45 +531,70 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(const KvAttnArgs p)
     }
 }
 
-// Tiles of 16 query rows a workgroup takes, of those the kernel is built for:
-// the fewest passes over the keys first, then the fewest idle rows.
-static int kv_tiles(int D, int rows) {
-    const int tiles = (rows + 15) / 16;
-    const int most = D == 64 ? 5 : 2;
-    const int per = (tiles + (tiles + most - 1) / most - 1) / ((tiles + most - 1) / most);
-    return per <= 2 ? per : most;
-}
-
+// How a call is cut up: tiles of 16 query rows to a workgroup (qt), groups of
+// them (qgroups), key splits.
 struct KvPlan {
     int qt, qgroups, splits;
     int64_t wgs, rows;
 };
 
+static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+static inline bool kv_pair(const sf_attn_kv4_desc* d) { return d->out_dtype != SF_BF16; }
+
+// Up to 16 rows to a key head: one tile, four waves to a workgroup.  Up to 512
+// keys a wave has four blocks at most and a merge costs as much as it saves (8
+// heads x 512 keys of 128 channels: 8.0 us with one split, 7.9 with four);
+// beyond, about two workgroups a CU of at least a block to a wave, and no split
+// over 2048 keys, so that batches of unequal lengths spread (16 x 8 heads,
+// 4096..16384 keys: 61 us with 8 splits, 62 with 4, 137 with 1).
+static int kv_splits_one_tile(const sf_attn_kv4_desc* d, int64_t base) {
+    if (d->Sk <= 512) return 1;
+    const int64_t want = std::max(ceil_div(512, base), ceil_div(d->Sk, 2048));
+    return (int)std::min<int64_t>({want, ceil_div(d->Sk, 128), (int64_t)kKvMaxSplits});
+}
+
+// More rows: a workgroup holds a CU alone, so the time is its rounds times what
+// one takes: per wave and block of 32 keys `step` us times (1.5 + qt) -- the
+// block's unpacking, then each tile -- and 3 + 0.8 qt us around the loop; key
+// splits that fill the card add a merge of 7 us.  Estimated for each qt the
+// kernel is built for, the smallest taken.  Measured against it (64 channels,
+// bf16): 12 x 520 rows x 1537 keys, causal, 12.1 us with qt 2, 14.4 with 3, 18.6
+// with 5 (estimates 12, 15, 21); 32 x 67 x 4374 18.9 with qt 3 and four splits,
+// 19.6 with 5 and eight, 31 with 3 and one (19, 20, 30); 256 x 67 x 4374 42 with
+// qt 5.  The (hi, lo) form takes 0.42 us a step, and qt 5 would spill.  128
+// channels: 2 tiles and four waves are what fits.
 static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
-    KvPlan k;
-    const int R = d->Hq / d->cache.H * d->Sq;
-    k.qt = kv_tiles(d->cache.D, R);
-    k.qgroups = (R + 16 * k.qt - 1) / (16 * k.qt);
+    KvPlan k = {};
+    const int64_t R = (int64_t)(d->Hq / d->cache.H) * d->Sq, heads = (int64_t)d->B * d->cache.H;
     k.rows = (int64_t)d->B * d->Hq * d->Sq;
-    const int64_t base = (int64_t)d->B * d->cache.H * k.qgroups;
-    if (d->num_splits > 0) {
-        k.splits = d->num_splits;
-    } else if (k.qt == 1) {
-        // Four waves to a workgroup.  Up to 512 keys a wave has four blocks at most and a merge costs as much as it
-        // saves (8 heads x 512 keys: 8.0 us with one split, 7.9 with four); beyond, about two workgroups a CU of at
-        // least a block to a wave, and no split over 2048 keys, so that batches of unequal lengths spread (16 x 8
-        // heads, 4096..16384 keys: 61 us with 8 splits, 65 with 4, 132 with 1).
-        const int64_t want = std::max<int64_t>((512 + base - 1) / base, (d->Sk + 2047) / 2048), most = (d->Sk + 127) / 128;
-        k.splits = d->Sk <= 512 ? 1 : (int)std::min<int64_t>({want, most, (int64_t)kKvMaxSplits});
+    if (R <= 16) {
+        k.qt = k.qgroups = 1;
+        k.splits = d->num_splits > 0 ? d->num_splits : kv_splits_one_tile(d, heads);
     } else {
-        // Eight waves to a workgroup and one workgroup a CU.  A split has to save the merge's 7 us at about 1.5 us a
-        // block: 32 heads x 67 rows x 4374 keys 41 -> 19 us with 8 splits, 12 heads x 520 rows x 1537 keys (causal)
-        // 23 us with one split, 30 with four.
-        const int64_t s = std::min<int64_t>(256 / base, kKvMaxSplits), waves = d->cache.D == 64 ? 8 : 4;
-        const int64_t blocks = (d->Sk + kKvBlock * waves - 1) / (kKvBlock * waves);
-        k.splits = s > 1 && blocks * (s - 1) >= 5 * s ? (int)std::min(s, blocks) : 1;
+        const bool wide = d->cache.D == 128;
+        const int most = wide ? 2 : kv_pair(d) ? 4 : 5;
+        const int64_t per_block = kKvBlock * (wide ? 4 : 8);
+        const double step = kv_pair(d) ? 0.42 : 0.3;
+        double best = 0.;
+        for (int qt = 2; qt <= most; ++qt) {
+            const int64_t groups = ceil_div(R, 16 * qt), base = heads * groups;
+            const int64_t fill = std::min<int64_t>(base < 256 ? 256 / base : 1, kKvMaxSplits);
+            for (int64_t s = 1; s <= fill; s += fill > 1 ? fill - 1 : 1) {
+                const int64_t splits = d->num_splits > 0 ? d->num_splits : std::min(s, std::max<int64_t>(1, ceil_div(d->Sk, per_block)));
+                const double us = (double)ceil_div(base * splits, 256) *
+                                      ((double)ceil_div(d->Sk, per_block * splits) * step * (1.5 + qt) + 3. + 0.8 * qt) +
+                                  (splits > 1 ? 7. : 0.);
+                if (k.qt == 0 || us < best) {
+                    best = us;
+                    k.qt = qt;
+                    k.qgroups = (int)groups;
+                    k.splits = (int)splits;
+                }
+            }
+        }
     }
-    k.wgs = base * k.splits;
+    k.wgs = heads * k.qgroups * k.splits;
     return k;
 }
 
@@ -639,12 +664,15 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
         if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT, PAIR, NW>), grid, dim3(64 * NW), 0, s, p);            \
         else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT, PAIR, NW>), grid, dim3(64 * NW), 0, s, p);               \
     } while (0)
-    const bool pair = d->out_dtype != SF_BF16;
+    const bool pair = sfk::kv_pair(d);
     if (d->cache.D == 64) {
         if (k.qt == 1) SF_KV4_LAUNCH(64, 1, true, 4);
         else if (k.qt == 2 && pair) SF_KV4_LAUNCH(64, 2, true, 8);
         else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, false, 8);
-        else if (pair) SF_KV4_LAUNCH(64, 5, true, 8);
+        else if (k.qt == 3 && pair) SF_KV4_LAUNCH(64, 3, true, 8);
+        else if (k.qt == 3) SF_KV4_LAUNCH(64, 3, false, 8);
+        else if (k.qt == 4 && pair) SF_KV4_LAUNCH(64, 4, true, 8);
+        else if (k.qt == 4) SF_KV4_LAUNCH(64, 4, false, 8);
         else SF_KV4_LAUNCH(64, 5, false, 8);
     } else {
         if (k.qt == 1) SF_KV4_LAUNCH(128, 1, true, 4);
