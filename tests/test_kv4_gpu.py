@@ -419,3 +419,26 @@ def test_causal_nan_with_bf16_output(D):
     ref = attend(q[:, :, :30], k[:, :, :30], v[:, :, :30], causal=True)
     assert ((got[:, :, :30].cpu().double() - ref).abs() <= 2.0 ** -9 * 5 + half_step(BF) * ref.abs()).all()
     assert torch.isnan(got[:, :, 30:, :64]).all()
+
+
+@pytest.mark.parametrize("kind", ["plain", "causal", "mask"])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("B,Hq,H,Sq,Sk", [(4, 32, 32, 67, 150), (4, 64, 64, 64, 150), (4, 64, 64, 67, 150), (8, 64, 32, 33, 97)])
+def test_many_heads(B, Hq, H, Sq, Sk, dtype, kind):
+    """Enough heads that a workgroup takes three, four or five tiles of rows, with rows left over in the last."""
+    D = 64
+    c, k, v = _filled(B, H, Sk, D, dtype, 120)
+    q = _randn(123, B, Hq, Sq, D, dtype=dtype)
+    kw = {}
+    if kind == "causal":
+        kw["valid"] = torch.tensor([Sk, 0, 30, Sk - 1][:B] + [Sk] * (B - 4), dtype=torch.int32)
+    if kind == "mask":
+        kw["mask"] = torch.rand(B, Sk, generator=torch.Generator().manual_seed(9)) < 0.5
+        kw["mask"][1] = False
+        kw["mask"][2, :70] = False
+    got = attention_kv4(q.to(DEV), c, is_causal=kind == "causal",
+                        valid_len=kw["valid"].to(DEV) if "valid" in kw else None,
+                        kv_mask=kw["mask"].to(DEV) if "mask" in kw else None)
+    _attn_check(got, q, k, v, dtype, what=kind, causal=kind == "causal", **kw)
+    if kind != "plain":
+        assert (got[1] == 0).all()
