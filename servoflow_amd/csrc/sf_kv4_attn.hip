@@ -127,6 +127,49 @@ __device__ __forceinline__ float kv_raise(float (&x)[8], float mx, float& m) {
     return first ? 1.f : __builtin_amdgcn_exp2f(-up);   // first: nothing to scale
 }
 
+// A query row's operand (channels 64 i + 16 g .. + 15 of the lane's group g) and
+// scale * log2 e times the sum of its channels.
+template <bool F16, int D>
+__device__ __forceinline__ void kv_queries(const KvAttnArgs& p, int b, int hq, int s, int g, u32x4 (&f)[D / 64][2],
+                                           float (&sums)[D / 64]) {
+    const uint16_t* src = p.q + b * p.qs[0] + hq * p.qs[1] + s * p.qs[2];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) f[i][k] = *reinterpret_cast<const u32x4*>(src + 64 * i + 16 * g + 8 * k);
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t v = f[i][k][e];
+                sum += F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v) + (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16))
+                           : __uint_as_float(v << 16) + __uint_as_float(v & 0xffff0000u);
+            }
+        sums[i] = lanes4_sum(sum) * p.scale_log2;
+    }
+}
+
+// A joined row: its output, or its sums for the merge of key splits.
+template <int D, int E>
+__device__ __forceinline__ void kv_finish(const KvAttnArgs& p, int split, int b, int hq, int s, int d0, float (&y)[E],
+                                          float top, float sum) {
+    if (p.splits > 1) {
+        float* dst = p.part + ((int64_t)split * p.rows + ((int64_t)b * p.H * p.G + hq) * p.Sq + s) * (D + 2);
+#pragma unroll
+        for (int e = 0; e < E; ++e) dst[d0 + e] = y[e];
+        if (d0 == 0) dst[D] = top, dst[D + 1] = sum;
+    } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] *= inv;
+        kv_store<E>(p.out, b * p.os[0] + hq * p.os[1] + s * p.os[2] + d0, p.out_kind, y);
+    }
+}
+
+// QT tiles of 16 query rows of a key head to a workgroup.
 // PAIR: p s enters the second product as a bf16 (hi, lo) pair; otherwise p and
 // V as fp16.
 template <bool F16, int D, int QT, bool PAIR, int NW>
@@ -161,43 +204,22 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     if (b0 + wave < b1) nx.load(base + (int64_t)(b0 + wave) * Kv4<D>::kBytes, lane);
 
     // Query fragments (B operands) and row sums: in registers for one tile, else each tile's by one wave into LDS.
+    static_assert(QT <= NW, "a wave for each tile");
     u32x4 qr[GR][2];
     float qs[QT][GR];
-    auto load_q = [&](int t, float (&sums)[GR]) __attribute__((always_inline)) {
-        const int r = min(q0 + 16 * t + col, R - 1);
-        const uint16_t* src = p.q + b * p.qs[0] + (h * p.G + r / p.Sq) * p.qs[1] + r % p.Sq * p.qs[2];
-#pragma unroll
-        for (int i = 0; i < GR; ++i)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) qr[i][k] = *reinterpret_cast<const u32x4*>(src + 64 * i + 16 * g + 8 * k);
-#pragma unroll
-        for (int i = 0; i < GR; ++i) {
-            float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t v = qr[i][k][e];
-                    sum += F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v) + (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16))
-                               : __uint_as_float(v << 16) + __uint_as_float(v & 0xffff0000u);
-                }
-            sums[i] = lanes4_sum(sum) * p.scale_log2;
-        }
-    };
-    if (QT == 1) {
-        load_q(0, qs[0]);
-    } else {
-        static_assert(QT == 1 || QT <= NW, "a wave for each tile");
-        if (wave < QT) {
-            float sums[GR];
-            load_q(wave, sums);
+    if (QT == 1 || wave < QT) {
+        const int t = QT == 1 ? 0 : wave, r = min(q0 + 16 * t + col, R - 1);
+        kv_queries<F16, D>(p, b, h * p.G + r / p.Sq, r % p.Sq, g, qr, qs[0]);
+        if (QT > 1) {
 #pragma unroll
             for (int i = 0; i < GR; ++i) {
-                ql[(wave * GR + i) * 2][lane] = qr[i][0];
-                ql[(wave * GR + i) * 2 + 1][lane] = qr[i][1];
-                if (g == 0) xq[i][16 * wave + col] = sums[i];
+                ql[(t * GR + i) * 2][lane] = qr[i][0];
+                ql[(t * GR + i) * 2 + 1][lane] = qr[i][1];
+                if (g == 0) xq[i][16 * t + col] = qs[0][i];
             }
         }
+    }
+    if (QT > 1) {
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < QT; ++t)
@@ -239,7 +261,8 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
             for (int e = 0; e < 8; ++e) {
                 uint32_t kp = nx.kp[i][e >> 2][e & 3], vp = nx.vp[i][e >> 2][e & 3];
                 if (masked && !(see >> e & 1u)) kp = vp = 0u;   // tokens behind the last hold anything
-                if (masked && !PAIR && (vp & 0x7f80u) == 0x7f80u) kp |= 0x7fc07fc0u, vp = 0u;   // see below
+                // A NaN value reaches the rows that see it through their scores: 0 times NaN would reach the others too.
+                if (masked && !PAIR && (vp & 0x7f80u) == 0x7f80u) kp |= 0x7fc07fc0u, vp = 0u;
                 ks[i][e] = __uint_as_float(kp << 16) * p.scale_log2;
                 ko[i][e] = kv_mix(kp, -23.5f, 1.f);
                 vs[i][e] = PAIR ? __uint_as_float(vp << 16) : kv_mix(vp, 262144.f * vdown, 0.f);
@@ -466,21 +489,231 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
             for (int w = 1; w < NW; ++w)
 #pragma unroll
                 for (int e = 0; e < E; ++e) y[e] += xo[w][16 * j + row][d0 + e];
-            const float sum = xs[16 * (t0 + j) + row];
-            const int hq = h * p.G + r / p.Sq, s = r % p.Sq;
-            if (p.splits > 1) {
-                float* dst = p.part + ((int64_t)split * p.rows + ((int64_t)b * p.H * p.G + hq) * p.Sq + s) * (D + 2);
-#pragma unroll
-                for (int e = 0; e < E; ++e) dst[d0 + e] = y[e];
-                if (d0 == 0) dst[D] = xm[0][16 * (t0 + j) + row], dst[D + 1] = sum;
-            } else {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
-#pragma unroll
-                for (int e = 0; e < E; ++e) y[e] *= inv;
-                kv_store<E>(p.out, b * p.os[0] + hq * p.os[1] + s * p.os[2] + d0, p.out_kind, y);
-            }
+            kv_finish<D, E>(p, split, b, h * p.G + r / p.Sq, r % p.Sq, d0, y, xm[0][16 * (t0 + j) + row], xs[16 * (t0 + j) + row]);
         }
     }
+}
+
+// Up to 16 / NG query rows to a key head: one token's heads, or a few tokens'.
+//
+// One tile of 16 columns would repeat its rows NG times over.  Instead column
+// group j of the tile takes block j of the wave's NG blocks at a time: all NG
+// blocks' codes meet the tile, each with the queries only in its own columns, so
+// the scores of a group's columns are its block's alone, and everything that is
+// done per score -- the parameters, the exponentials, the rounded weights -- is
+// done once for NG blocks.  The column groups are joined at the end like waves.
+// 128 channels and NG = 2: a block's vector instructions go from 542 to about
+// 420, where they took 82% of the time; 16 x 8 key heads x 4 rows over 16384 keys
+// then stream 4.3 TB/s, of the 4.95 that a large copy reaches.
+template <bool F16, int D, int NG>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_token_kernel(const KvAttnArgs p) {
+    constexpr int GR = D / 64, DT = D / 16, NW = 4, RT = 16 / NG;
+    __shared__ float xm[NW * NG][RT], xl[NW * NG][RT], xf[NW * NG][RT], xs[RT], xtop[RT];
+    __shared__ __attribute__((aligned(16))) float xo[NW][16][D + 4];
+    __shared__ u32x4 ql[NG * GR * 2][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, g = lane >> 4, own = col / RT;   // own: the block of the NG that the lane's column takes
+    const int split = blockIdx.x % p.splits, bh = blockIdx.x / p.splits;
+    const int b = bh / p.H, h = bh % p.H;
+    const int R = p.G * p.Sq, row = min(col % RT, R - 1), qh = h * p.G + row / p.Sq, qt = row % p.Sq;
+
+    const int len = p.valid ? min(max(p.valid[b], 0), p.Sk) : p.Sk;
+    const int nblk = (len + kKvBlock - 1) / kKvBlock;   // the last token's row sees them all
+    const int b0 = (int)((int64_t)nblk * split / p.splits), b1 = (int)((int64_t)nblk * (split + 1) / p.splits);
+    const int lim_lo = p.causal ? len - p.Sq + 1 : len, limit = p.causal ? len - p.Sq + 1 + qt : len;
+
+    const uint8_t* base = p.cache + (int64_t)bh * p.cache_blocks * Kv4<D>::kBytes;
+    u32x4 kc[NG][GR], vc[NG][GR], kp[GR][2], vp[GR][2];
+    auto load_keys = [&](int blk) __attribute__((always_inline)) {   // of blocks blk .. blk + NG - 1, the last one repeated
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int i = 0; i < GR; ++i)
+                kc[n][i] = *reinterpret_cast<const u32x4*>(base + (int64_t)min(blk + n, b1 - 1) * Kv4<D>::kBytes + i * 1024 + lane * 16);
+    };
+    auto load_values = [&](int blk) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int i = 0; i < GR; ++i)
+                vc[n][i] = *reinterpret_cast<const u32x4*>(base + (int64_t)min(blk + n, b1 - 1) * Kv4<D>::kBytes + Kv4<D>::kV + i * 1024 + lane * 16);
+    };
+    auto load_pars = [&](u32x4 (&par)[GR][2], int blk, int at) __attribute__((always_inline)) {   // of the own block
+        const uint8_t* mine = base + (int64_t)min(blk + own, b1 - 1) * Kv4<D>::kBytes + at + 16 * g;
+#pragma unroll
+        for (int i = 0; i < GR; ++i)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) par[i][t] = *reinterpret_cast<const u32x4*>(mine + (i * kKvBlock + 16 * t) * 4);
+    };
+    const int first = b0 + NG * wave;
+    if (first < b1) {
+        load_keys(first);
+        load_pars(kp, first, Kv4<D>::kPar);
+        load_pars(vp, first, Kv4<D>::kVPar);
+        load_values(first);
+    }
+
+    u32x4 qf[GR][2];
+    float qs[GR];
+    kv_queries<F16, D>(p, b, qh, qt, g, qf, qs);
+    if (wave < NG) {   // the queries of column group `wave`, zeros in the other columns
+#pragma unroll
+        for (int i = 0; i < GR; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) ql[(wave * GR + i) * 2 + k][lane] = own == wave ? qf[i][k] : u32x4{0, 0, 0, 0};
+    }
+    __syncthreads();
+
+    f32x4 o[DT];   // O^T without the parameters' part pm
+    float m = kKvNoMax, l = 0.f, pm[GR];
+#pragma unroll
+    for (int i = 0; i < GR; ++i) pm[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const NibbleMask kmask = nibble_mask<F16>(), vmask = nibble_mask<false>();
+
+    auto blocks = [&](const int blk, auto masked_c) __attribute__((always_inline)) {
+        constexpr bool masked = decltype(masked_c)::value;
+        const bool next = blk + NG * NW < b1;
+        f32x4 s[2][GR] = {};
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int i = 0; i < GR; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const u32x4 q = ql[(n * GR + i) * 2 + k][lane];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        s[t][i] = mfma_16b<F16>(nibbles_plus16<F16>(D == 64 ? kc[n][0][2 * t + k] : kc[n][t][2 * i + k], kmask), q, s[t][i]);
+                }
+        if (next) load_keys(blk + NG * NW);
+        // scores less the row's maximum, base 2
+        const int key0 = kKvBlock * (blk + own) + 4 * g;
+        uint32_t see = 0xffu;
+        if (masked) {
+            see = 0;
+            if (blk + own < b1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int key = key0 + 16 * (e >> 2) + (e & 3);
+                    if (key < limit && (!p.mask || p.mask[b * p.mask_stride + key])) see |= 1u << e;
+                }
+            }
+        }
+        float x[8];
+        const float neg = m == kKvNoMax ? 0.f : -m;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float u = neg;
+#pragma unroll
+            for (int i = 0; i < GR; ++i) {
+                uint32_t k = kp[i][e >> 2][e & 3];
+                if (masked && !(see >> e & 1u)) k = 0u;   // what the row does not see may hold anything
+                u = __builtin_fmaf(__uint_as_float(k << 16) * p.scale_log2, s[e >> 2][i][e & 3], __builtin_fmaf(kv_mix(k, -23.5f, 1.f), qs[i], u));
+            }
+            x[e] = masked && !(see >> e & 1u) ? -INFINITY : u;
+        }
+        if (next) load_pars(kp, blk + NG * NW, Kv4<D>::kPar);
+        const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        if (__any(mx > (m == kKvNoMax ? -INFINITY : kKvSlack))) {
+            const float al = kv_raise(x, mx, m);
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < GR; ++i) pm[i] *= al;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) o[i] *= al;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[e] = __builtin_amdgcn_exp2f(x[e]);
+            l += x[e];
+        }
+#pragma unroll
+        for (int i = 0; i < GR; ++i) {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t v0 = vp[i][e >> 1][2 * (e & 1)], v1 = vp[i][e >> 1][2 * (e & 1) + 1];
+                if (masked && !(see >> (2 * e) & 1u)) v0 = 0u;
+                if (masked && !(see >> (2 * e + 1) & 1u)) v1 = 0u;
+                const float a = x[2 * e] * __uint_as_float(v0 << 16), c = x[2 * e + 1] * __uint_as_float(v1 << 16);
+                const uint32_t w = pack_bf16x2(a, c);
+                const uint32_t r = pack_bf16x2(a - __uint_as_float(w << 16), c - __uint_as_float(w & 0xffff0000u));
+                pm[i] = kv_dot(w, kv_dot(r, pm[i] + x[2 * e] * __uint_as_float(v0 & 0xffff0000u) + x[2 * e + 1] * __uint_as_float(v1 & 0xffff0000u)));
+                hi[e] = w;
+                lo[e] = r;
+            }
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                const uint32_t keep = own == n ? 0xffffffffu : 0u;
+                const u32x4 ph = hi & keep, pl = lo & keep;   // the weights of block n, zeros in the other columns
+#pragma unroll
+                for (int t = 2 * i; t < 2 * i + 2; ++t) {
+                    const uint32_t w0 = vc[n][t >> 1][2 * (t & 1)], w1 = vc[n][t >> 1][2 * (t & 1) + 1];
+                    const u32x4 va = {nibble_pair_plus16<false, 0>(w0, vmask), nibble_pair_plus16<false, 2>(w0, vmask),
+                                      nibble_pair_plus16<false, 0>(w1, vmask), nibble_pair_plus16<false, 2>(w1, vmask)};
+                    const u32x4 vb = {nibble_pair_plus16<false, 1>(w0, vmask), nibble_pair_plus16<false, 3>(w0, vmask),
+                                      nibble_pair_plus16<false, 1>(w1, vmask), nibble_pair_plus16<false, 3>(w1, vmask)};
+                    o[2 * t] = mfma_16b<false>(va, pl, mfma_16b<false>(va, ph, o[2 * t]));
+                    o[2 * t + 1] = mfma_16b<false>(vb, pl, mfma_16b<false>(vb, ph, o[2 * t + 1]));
+                }
+            }
+        }
+        if (next) {
+            load_pars(vp, blk + NG * NW, Kv4<D>::kVPar);
+            load_values(blk + NG * NW);
+        }
+    };
+    for (int blk = first; blk < b1; blk += NG * NW) {
+        if (p.mask || blk + NG > b1 || kKvBlock * (blk + NG) > lim_lo) blocks(blk, std::true_type{});
+        else blocks(blk, std::false_type{});
+    }
+
+    // Waves and column groups meet.
+    l = lanes4_sum(l);
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+        const float add = lanes4_sum(pm[i]);
+#pragma unroll
+        for (int d = 4 * i; d < 4 * i + 4; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[d][e] += add;
+    }
+    if (g == 0) xm[wave * NG + own][col % RT] = m, xl[wave * NG + own][col % RT] = l;
+    __syncthreads();
+    if (threadIdx.x < RT) {
+        const int i = threadIdx.x;
+        float top = xm[0][i], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < NW * NG; ++w) top = fmaxf(top, xm[w][i]);
+#pragma unroll
+        for (int w = 0; w < NW * NG; ++w) {
+            const float f = __builtin_amdgcn_exp2f(xm[w][i] - top);
+            xf[w][i] = f;
+            sum += f * xl[w][i];
+        }
+        xs[i] = sum;
+        xtop[i] = top;
+    }
+    __syncthreads();
+    const float f = xf[wave * NG + own][col % RT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&xo[wave][col][16 * d + 4 * g]) = o[d] * f;
+    __syncthreads();
+    constexpr int E = RT * D / 256 > 2 ? RT * D / 256 : 2;   // channels a thread finishes
+    const int r = (int)threadIdx.x / (D / E), d0 = E * ((int)threadIdx.x % (D / E));
+    if (r >= RT || r >= R) return;
+    float y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] += xo[w][n * RT + r][d0 + e];
+    kv_finish<D, E>(p, split, b, h * p.G + r / p.Sq, r % p.Sq, d0, y, xtop[r], xs[r]);
 }
 
 // out = sum_splits O 2^(m - M) / sum_splits l 2^(m - M), one wave per row.
@@ -534,7 +767,7 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(const KvAttnArgs p)
 // How a call is cut up: tiles of 16 query rows to a workgroup (qt), groups of
 // them (qgroups), key splits.
 struct KvPlan {
-    int qt, qgroups, splits;
+    int qt, ng, qgroups, splits;
     int64_t wgs, rows;
 };
 
@@ -554,6 +787,17 @@ static int kv_splits_one_tile(const sf_attn_kv4_desc* d, int64_t base) {
     return (int)std::min<int64_t>({want, ceil_div(d->Sk, 128), (int64_t)kKvMaxSplits});
 }
 
+// Column groups of one tile (attn_kv4_token_kernel; 1: attn_kv4_kernel): where
+// there are enough blocks of keys, 16 for each SIMD, that the vector units and
+// the stream bound the call and not its start.  us, with 1, 2 and 4 groups: 8 x
+// 32 heads x 8192 keys of 64 channels 45, 41, 37; 16 x 8 x 16384 of 128, four rows
+// each, 77 and 70 (four groups would spill); 8 x 8 x 4096 17.2 and 16.9; 16 x 8 x
+// 1024 13.0 and 13.4.
+static int kv_column_groups(const sf_attn_kv4_desc* d, int rows, int64_t heads) {
+    if (rows > 8 || heads * ceil_div(d->Sk, kKvBlock) < 16384) return 1;
+    return d->cache.D == 64 && rows <= 4 ? 4 : 2;
+}
+
 // More rows: a workgroup holds a CU alone, so the time is its rounds times what
 // one takes: per wave and block of 32 keys `step` us times (1.5 + qt) -- the
 // block's unpacking, then each tile -- and 3 + 0.8 qt us around the loop; key
@@ -571,6 +815,7 @@ static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
     if (R <= 16) {
         k.qt = k.qgroups = 1;
         k.splits = d->num_splits > 0 ? d->num_splits : kv_splits_one_tile(d, heads);
+        k.ng = kv_column_groups(d, (int)R, heads);
     } else {
         const bool wide = d->cache.D == 128;
         const int most = wide ? 2 : kv_pair(d) ? 4 : 5;
@@ -664,10 +909,23 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
         if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT, PAIR, NW>), grid, dim3(64 * NW), 0, s, p);            \
         else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT, PAIR, NW>), grid, dim3(64 * NW), 0, s, p);               \
     } while (0)
+#define SF_KV4_TOKEN(DD, NG)                                                                                                  \
+    do {                                                                                                                      \
+        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<true, DD, NG>), grid, dim3(256), 0, s, p);                    \
+        else hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<false, DD, NG>), grid, dim3(256), 0, s, p);                       \
+    } while (0)
     const bool pair = sfk::kv_pair(d);
-    if (d->cache.D == 64) {
-        if (k.qt == 1) SF_KV4_LAUNCH(64, 1, true, 4);
-        else if (k.qt == 2 && pair) SF_KV4_LAUNCH(64, 2, true, 8);
+    if (k.qt == 1) {
+        if (d->cache.D == 64) {
+            if (k.ng == 1) SF_KV4_LAUNCH(64, 1, true, 4);
+            else if (k.ng == 2) SF_KV4_TOKEN(64, 2);
+            else SF_KV4_TOKEN(64, 4);
+        } else {
+            if (k.ng == 1) SF_KV4_LAUNCH(128, 1, true, 4);
+            else SF_KV4_TOKEN(128, 2);
+        }
+    } else if (d->cache.D == 64) {
+        if (k.qt == 2 && pair) SF_KV4_LAUNCH(64, 2, true, 8);
         else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, false, 8);
         else if (k.qt == 3 && pair) SF_KV4_LAUNCH(64, 3, true, 8);
         else if (k.qt == 3) SF_KV4_LAUNCH(64, 3, false, 8);
@@ -675,10 +933,10 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
         else if (k.qt == 4) SF_KV4_LAUNCH(64, 4, false, 8);
         else SF_KV4_LAUNCH(64, 5, false, 8);
     } else {
-        if (k.qt == 1) SF_KV4_LAUNCH(128, 1, true, 4);
-        else if (pair) SF_KV4_LAUNCH(128, 2, true, 4);
+        if (pair) SF_KV4_LAUNCH(128, 2, true, 4);
         else SF_KV4_LAUNCH(128, 2, false, 4);
     }
+#undef SF_KV4_TOKEN
 #undef SF_KV4_LAUNCH
     if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
     if (k.splits > 1) {

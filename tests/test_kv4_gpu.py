@@ -442,3 +442,47 @@ def test_many_heads(B, Hq, H, Sq, Sk, dtype, kind):
     _attn_check(got, q, k, v, dtype, what=kind, causal=kind == "causal", **kw)
     if kind != "plain":
         assert (got[1] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["plain", "causal", "ragged", "mask"])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D,Hq,Sq,Sk", [(64, 64, 1, 512), (64, 128, 2, 497), (64, 64, 7, 500), (128, 64, 1, 481), (128, 128, 4, 512)])
+def test_long_streams_of_few_rows(D, Hq, Sq, Sk, dtype, kind):
+    """Blocks of keys enough that the tile's columns take several at a time; blocks left over at the end, splits,
+    masked rows and NaN keys among them.  The reference runs on the device, in 64 bits."""
+    B, H = 16, 64
+    k = _randn(130, 1, H, Sk, D, dtype=dtype).to(DEV).repeat(B, 1, 1, 1) + torch.linspace(-1, 1, B, device=DEV).to(dtype)[:, None, None, None]
+    v = (k * 0.75).flip(2)
+    c = Kv4Cache(B, H, Sk + 9, D, DEV)
+    c.data.fill_(0xff)
+    c.write(k, v)
+    lk, lv = kv4_levels(k), kv4_levels(v)
+    q = _randn(133, B, Hq, Sq, D, dtype=dtype).to(DEV)
+    valid = mask = None
+    if kind in ("causal", "ragged"):
+        valid = (torch.arange(B, device=DEV, dtype=torch.int32) * 41 + 3).clamp_max(Sk)
+        valid[5] = 0
+    if kind == "mask":
+        mask = torch.rand(B, Sk, generator=torch.Generator().manual_seed(9)).to(DEV) < 0.5
+        mask[1] = False
+        mask[:, 40] = False
+        bad = torch.full((B, H, 1, D), float("nan"), dtype=dtype, device=DEV)
+        c.write(bad, bad, torch.full((B, 1), 40, dtype=torch.int32, device=DEV))
+    causal = kind == "causal"
+    sc = 1 / math.sqrt(D)
+    for splits in (0, 3):
+        got = attention_kv4(q, c, keys=Sk, is_causal=causal, valid_len=valid, kv_mask=mask, num_splits=splits)
+        for b in range(B):
+            n = Sk if valid is None else int(valid[b])
+            kk, vv = (t[b, :, :n].repeat_interleave(Hq // H, 0) for t in (lk, lv))
+            x = torch.matmul(q[b].double(), kk.transpose(1, 2).contiguous()) * sc
+            if mask is not None:
+                x[..., ~mask[b, :n]] = -math.inf
+            if causal:
+                x = x.masked_fill(torch.arange(n, device=DEV) > torch.arange(Sq, device=DEV)[:, None] + n - Sq, -math.inf)
+            w = torch.softmax(x, -1)
+            ref = torch.matmul(torch.where(torch.isnan(w), 0.0, w), vv) if n else torch.zeros_like(q[b]).double()
+            dx = 24 * 2.0 ** -24 * sc * float(q.double().abs().sum(-1).max()) * float(lk.abs().max()) * 6
+            rel = 2 * (dx + 2.0 ** -22) + 2.0 ** -16 + (32 + Sk / 32) * 2.0 ** -24 * 16 + (7 * 2.0 ** -12 if Hq // H * Sq > 16 and dtype == BF else 0)
+            tol = rel * float(lv.abs().max()) + half_step(dtype) * ref.abs() + (2.0 ** -25 if dtype == FP else 0)
+            assert ((got[b].double() - ref).abs() <= tol).all(), (splits, b)
