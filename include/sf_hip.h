@@ -599,7 +599,8 @@ int32_t sf_gemm_frag_ss_tiles(const sf_frag_gemm_desc* desc);
  * - zero[n][k / group]) + bias[n]): the weight form below the reference's
  * weight-only int8 (quantization.cu:18-51 ahead of gemm_bias_act,
  * cuda_backend.cu:337-467), which has no 4-bit form.  Codes are 0..15, group
- * 32, 64 or 128 inputs, K a multiple of the group, any N, any M.
+ * 32, 64 or 128 inputs, K a multiple of the group, any N to 2^25, any M to
+ * 2^22, lda to 2^24 (SF_ENOTSUP above).
  *
  * sf_w4_pack lays a checkpoint's codes and scales out once, in the order the
  * matrix operands are read; sf_gemm_w4 reads that.
@@ -636,6 +637,8 @@ typedef struct sf_gemm_w4_desc {
 } sf_gemm_w4_desc;
 /* One launch, no workspace.  Codes and activations meet exactly in fp32
  * accumulators; scale and zero point are applied to each group's sum in fp32.
+ * The sums are of codes + 16: 31 times a group's sum of |A| has to be finite
+ * (an infinity or a NaN in a row of A makes that row of C NaN).
  * C must not overlap A. */
 int sf_gemm_w4(const sf_gemm_w4_desc* desc, void* stream);
 
@@ -685,6 +688,7 @@ size_t sf_kv4_bytes(int32_t B, int32_t H, int32_t capacity, int32_t D);
  * [0, capacity) leaves the cache as it was.  The slots of one batch element
  * have to differ within a call; two tokens at one slot leave a mixture there,
  * and only there.
+ * B * S is below 2^23 (SF_ENOTSUP above; sf_kv4_read likewise).
  * positions, slots: DEVICE [B * S]; positions NULL: token s of each batch
  * element is at s.  A token with a negative position is padding: nothing of it
  * is written. */
@@ -718,7 +722,7 @@ int sf_kv4_read(const sf_kv4_cache* cache, const int32_t* slots, int32_t S, void
  * [B][Hq][Sq][D] through element strides {b, h, s}, channels contiguous,
  * pointers 16-byte aligned, strides non-negative multiples of 8; Hq a multiple
  * of cache.H, query head h reads key head h / (Hq / cache.H).
- * Sk: keys [0, Sk) are read at most (<= cache.capacity).  kv_valid_len: NULL
+ * Sk: keys [0, Sk) are read at most (<= cache.capacity and 2^30).  kv_valid_len: NULL
  * or DEVICE [B]: keys from there on are not seen (clamped to [0, Sk]).
  * kv_mask: NULL or DEVICE bytes, [B] rows of Sk kv_mask_stride apart, nonzero
  * = seen.  is_causal: query s of Sq is the token at valid_len - Sq + s, and
@@ -728,7 +732,7 @@ int sf_kv4_read(const sf_kv4_cache* cache, const int32_t* slots, int32_t S, void
  * no row sees may hold anything.
  * scale 0: 1 / sqrt(D); negative: SF_ENOTSUP.  in_dtype SF_BF16 or SF_F16.
  * The softmax's maximum and sum are fp32; its weights enter the product with V
- * as bf16 (hi, lo) pairs, 2^-17 relative.  With more than 16 query rows to a
+ * as bf16 (hi, lo) pairs, 2^-18 relative.  With more than 16 query rows to a
  * key head and a bf16 output, weights and values enter as fp16, the values
  * under a power of two that keeps them in its range: 5 2^-12 of the largest
  * value seen.  Values are taken up to 2^100 in magnitude.

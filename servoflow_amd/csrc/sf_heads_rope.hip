@@ -115,7 +115,8 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float v[8], uint32_t* par
         *par = 0x7fc07fc0u;
         return 0;
     }
-    const uint32_t mid_bits = f32_to_bf16_bits(0.5f * mx + 0.5f * mn);
+    // fp32's last few numbers would round to an infinity
+    const uint32_t mid_bits = f32_to_bf16_bits(__builtin_amdgcn_fmed3f(0.5f * mx + 0.5f * mn, -0x1.fep127f, 0x1.fep127f));
     const float mid = bf16_bits_to_f32(mid_bits);
     const float a = fmaxf(mx - mid, mid - mn);
     const uint32_t up = min((__float_as_uint(a) + 0xffffu) & 0xffff0000u, 0x7f7f0000u);   // bf16's largest at most
@@ -415,7 +416,7 @@ extern "C" int sf_heads_rope(const sf_heads_rope_desc* d, void* stream) {
     }
     const int64_t tokens = (int64_t)d->B * d->S;
     if (tokens == 0) return SF_OK;
-    if (tokens > 0x7fffffffLL) return SF_ENOTSUP;
+    if (tokens >= 1 << 23) return SF_ENOTSUP;   // a launch counts its threads in 32 bits
     sfk::RopeArgs p = {};
     for (int i = 0; i < 3; ++i) {
         if (!d->heads[i]) continue;
@@ -453,9 +454,7 @@ extern "C" int sf_heads_rope(const sf_heads_rope_desc* d, void* stream) {
     if (p.tok_per_wg == sfk::kKvBlock && (d->positions || d->slots)) ++p.windows;   // the first one may be cut short
     p.heads_per_wg = (int)std::min<int64_t>(heads, p.tok_per_wg == sfk::kKvBlock ? 4 : p.tok_per_wg > 1 ? 32 : rows);
     p.heads_magic = (65536 + p.heads_per_wg - 1) / p.heads_per_wg;
-    const int64_t wgs = (int64_t)d->B * p.windows;
-    if (wgs > 0x7fffffffLL) return SF_ENOTSUP;
-    const dim3 grid((unsigned)wgs, (unsigned)((heads + p.heads_per_wg - 1) / p.heads_per_wg));
+    const dim3 grid((unsigned)(d->B * p.windows), (unsigned)((heads + p.heads_per_wg - 1) / p.heads_per_wg));
     size_t lds = sizeof(float2) * (size_t)p.tok_per_wg * (size_t)(d->rot / 2);
     if (p.tok_per_wg == sfk::kKvBlock) lds += (size_t)p.heads_per_wg * 18 * d->D;
     const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -488,10 +487,9 @@ extern "C" int sf_kv4_read(const sf_kv4_cache* cache, const int32_t* slots, int3
     p.S = S;
     p.cap = cache->capacity;
     p.out_kind = sfk::rope_kind(out_dtype);
-    if ((int64_t)cache->B * S > 0x7fffffffLL || (cache->H + sfk::kReadHeads - 1) / sfk::kReadHeads > 65535) return SF_ENOTSUP;
+    if ((int64_t)cache->B * S >= 1 << 23 || cache->H > 65535) return SF_ENOTSUP;   // as sf_heads_rope
     // with slots the first window may be cut short
     p.windows = (int)((S + (int64_t)sfk::kKvBlock - 1) / sfk::kKvBlock) + (slots ? 1 : 0);
-    if ((int64_t)cache->B * p.windows > 0x7fffffffLL) return SF_ENOTSUP;
     const dim3 grid((unsigned)(cache->B * p.windows), (unsigned)((cache->H + sfk::kReadHeads - 1) / sfk::kReadHeads));
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (cache->D == 64) hipLaunchKernelGGL(sfk::kv4_read_kernel<64>, grid, dim3(256), 0, s, p);

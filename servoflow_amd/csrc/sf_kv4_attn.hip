@@ -850,7 +850,7 @@ static int kv_attn_check(const sf_attn_kv4_desc* d) {
     if (d->cache.D != 64 && d->cache.D != 128) return SF_ENOTSUP;
     if (d->Hq % d->cache.H || d->B != d->cache.B || d->Sk > d->cache.capacity) return SF_EINVAL;
     if (d->num_splits < 0 || d->num_splits > kKvMaxSplits) return SF_EINVAL;
-    if ((int64_t)d->Hq / d->cache.H * d->Sq > 0x7fffff00LL) return SF_ENOTSUP;
+    if (d->Sk > 1 << 30 || (int64_t)d->Hq / d->cache.H * d->Sq > 1 << 30) return SF_ENOTSUP;   // counted in 32 bits
     return SF_OK;
 }
 
@@ -877,7 +877,7 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
         if (d->q_stride[i] < 0 || (d->q_stride[i] & 7) || d->o_stride[i] < 0 || (d->o_stride[i] & 7)) return SF_EINVAL;
     if (d->kv_mask && d->kv_mask_stride < 0) return SF_EINVAL;
     const sfk::KvPlan k = sfk::kv_plan(d);
-    if (k.wgs > 0x7fffffffLL || (k.rows + 3) / 4 > 0x7fffffffLL) return SF_ENOTSUP;
+    if (k.wgs >= 1 << 23 || (k.splits > 1 && k.rows >= 1 << 26)) return SF_ENOTSUP;   // a launch counts its threads in 32 bits
     if (k.splits > 1 && (!workspace || workspace_bytes < sf_attn_kv4_workspace_bytes(d))) return SF_EWORKSPACE;
     if (k.splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 3)) return SF_EINVAL;
     sfk::KvAttnArgs p = {};

@@ -330,7 +330,7 @@ extern "C" int sf_w4_pack(const sf_w4_pack_desc* desc, void* out, void* stream) 
     if (desc->scale_dtype != SF_F16 && desc->scale_dtype != SF_BF16) return SF_ENOTSUP;
     const int64_t words = (int64_t)(sf_w4_bytes(desc->N, desc->K, desc->group) / 4);
     const int64_t blocks = (words + 255) / 256;
-    if (blocks > 0x7fffffffLL) return SF_ENOTSUP;
+    if (blocks >= 1 << 24) return SF_ENOTSUP;   // a launch counts its threads in 32 bits
     hipLaunchKernelGGL(sfk::w4_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream),
                        *desc, static_cast<uint32_t*>(out), (int)(((int64_t)desc->N + 15) / 16), sfk::w4_kb(desc->K),
                        sfk::w4_groups(desc->K, desc->group));
@@ -352,8 +352,8 @@ extern "C" int sf_gemm_w4(const sf_gemm_w4_desc* desc, void* stream) {
     if (desc->c_dtype != SF_F32 && desc->c_dtype != SF_F16 && desc->c_dtype != SF_BF16) return SF_ENOTSUP;
     if (desc->act < SF_ACT_NONE || desc->act > SF_ACT_SILU) return SF_ENOTSUP;
     if (desc->accumulate && desc->c_dtype != SF_F32) return SF_ENOTSUP;
-    if (((int64_t)desc->M + 79) / 80 > 65535) return SF_ENOTSUP;   // the grid's second dimension
-    if (desc->lda > 1 << 24) return SF_ENOTSUP;                     // a workgroup's rows are addressed in 32 bits
+    // the grid's second dimension; a launch counts its threads in 32 bits; a workgroup's rows are addressed in 32 bits
+    if (desc->M > 1 << 22 || desc->N > 1 << 25 || desc->lda > 1 << 24) return SF_ENOTSUP;
     sfk::W4Args p = {};
     p.a = static_cast<const uint16_t*>(desc->A);
     p.lda = desc->lda;

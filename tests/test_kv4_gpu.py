@@ -220,6 +220,17 @@ def test_cache_extreme_values():
         assert ((got[3] - x[0, 0, 3].unflatten(-1, (2, 64))).abs() <= 1e-37).all()
 
 
+def test_cache_of_the_largest_numbers():
+    """Numbers above bf16's largest (3.3895e38): it is their middle, the step an eighth of what is left (1.34e36)."""
+    x = torch.full((1, 1, 3, 64), 3.4028e38)
+    x[0, 0, 1, ::3] = 3.395e38
+    x[0, 0, 2] = -3.4028e38
+    c = Kv4Cache(1, 1, 3, 64, DEV)
+    c.write(x.to(DEV), x.to(DEV))
+    for got in c.read(dtype=F32):
+        assert ((got.cpu().double() - x.double()).abs() <= 0.5 * 1.35e36 / 8).all()
+
+
 def test_rope_into_cache():
     """Normed, rotated keys and plain values at given slots; queries to a tensor."""
     B, S, Hq, H, D = 2, 37, 4, 2, 128

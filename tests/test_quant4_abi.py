@@ -186,6 +186,19 @@ def test_attn_kv4_refusals():
         assert _attn(**kw) == abi.SF_OK, kw
 
 
+def test_sizes_beyond_a_launch_are_refused():
+    for kw in ({"lda": (1 << 24) + 8}, {"N": (1 << 25) + 1, "ldc": 1 << 26}, {"M": (1 << 22) + 1}):
+        assert _gemm(**kw) == abi.SF_ENOTSUP, kw
+    assert _pack(N=1 << 25, K=2048, ldc=1024, lds=64, zeros=None) == abi.SF_ENOTSUP
+    assert _rope(B=1 << 12, S=1 << 11) == abi.SF_ENOTSUP
+    assert _read(S=1 << 22) == abi.SF_ENOTSUP
+    big = (256, 2, 2, (1 << 30) + 1, 64)
+    assert _attn(cache=big, Sk=(1 << 30) + 1) == abi.SF_ENOTSUP
+    assert _attn(Sq=(1 << 28) + 1) == abi.SF_ENOTSUP                  # 4 heads to a key head
+    many = (256, 1 << 22, 2, 100, 64)
+    assert _attn(B=1 << 22, cache=many) == abi.SF_ENOTSUP
+
+
 def test_front_ends_refuse_host_tensors_and_shapes():
     a = torch.zeros(2, 128, dtype=torch.bfloat16)
     codes, scales = torch.zeros(16, 64, dtype=torch.uint8), torch.zeros(16, 1, dtype=torch.float16)
