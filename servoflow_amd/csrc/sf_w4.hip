@@ -43,40 +43,82 @@ __device__ __forceinline__ float w4_scale(uint32_t u, int f16) {
     return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16)) : __uint_as_float(u & 0xffff0000u);
 }
 
-// A wave's operands of one block of 128 columns: codes and parameters of its NT
+// A wave's operands of one block of 128 inputs: codes and parameters of its NT
 // tiles of 16 rows of W.
 template <int NT, int GROUPS>
 struct W4Block {
     u32x4 code[NT], par[NT][GROUPS];
 };
 
-// One workgroup: 16 NT WN columns of C (rows of W) x 16 MB rows.  Its WN x WK
-// waves take NT tiles of columns each and deal the blocks of 128 inputs among
-// WK; the WK sums meet in LDS.  Weights are fetched PF blocks ahead (each byte
-// once, from memory), activations one block ahead (from the caches).
-template <bool F16, int MB, int NT, int WK, int WN, int PF, int GROUP>
-__global__ __launch_bounds__(64 * WK * WN) void gemm_w4_kernel(const W4Args p) {
-    constexpr int kSteps = GROUP / 32, kGroups = 4 / kSteps;   // per block of 128
-    __shared__ f32x4 red[WK > 1 ? WK : 1][WN][WK > 1 ? MB * NT : 1][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wk = wave % WK, wn = wave / WK;
-    const int r = lane & 15, g = lane >> 4;
-    const int nb0 = (blockIdx.x * WN + wn) * NT;
-    const int m0 = blockIdx.y * 16 * MB;
+// Four columns of a row of C, from column n.
+__device__ __forceinline__ void w4_store(const W4Args& p, int m, int n, f32x4 v) {
+    if (m >= p.M || n >= p.N) return;
+    const int64_t at = (int64_t)m * p.ldc + n;
+    const int cols = min(4, p.N - n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < cols) v[i] = apply_act(p.act, v[i] + (p.bias ? p.bias[n + i] : 0.f));
+    if (cols == 4 && p.vec4) {
+        if (p.c_kind == 0) {
+            f32x4* c = reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at);
+            *c = p.accumulate ? *c + v : v;
+        } else {
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.c) + at) =
+                p.c_kind == 1 ? uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}
+                              : uint2{pack_f16x2_rn(v[0], v[1]), pack_f16x2_rn(v[2], v[3])};
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i >= cols) continue;
+        if (p.c_kind == 0) {
+            float* c = static_cast<float*>(p.c) + at + i;
+            *c = p.accumulate ? *c + v[i] : v[i];
+        } else if (p.c_kind == 1) {
+            static_cast<uint16_t*>(p.c)[at + i] = (uint16_t)f32_to_bf16_bits(v[i]);
+        } else {
+            static_cast<_Float16*>(p.c)[at + i] = (_Float16)v[i];
+        }
+    }
+}
 
-    // Activations: lane l reads 16 bytes of row l / 16 (+ 4 i), so an instruction covers four rows' 256 bytes, and the
-    // operand's order is made in LDS, by each wave for itself.  (Read in operand order an instruction takes the same
-    // 64 bytes of 16 rows, which meet in the cache's banks: 67 x 6144 x 2048 took 15.7 us, and 13.4 with rows 16 bytes
-    // longer.)
-    __shared__ __attribute__((aligned(16))) uint16_t xs[WK * WN][16][136];
-    const int xc = 8 * (lane & 15), xr = lane >> 4;
-    const char* abase = reinterpret_cast<const char*>(p.a + (int64_t)m0 * p.lda);
-    uint32_t arow[MB][4];   // bytes: lda is at most 2^24
+// One workgroup: 16 MB rows x 16 NT WN columns.  Its eight waves take NT tiles of
+// columns each and deal the blocks of 128 inputs among 8 / WN; the sums meet in
+// LDS.  A wave brings its activations into LDS itself, straight from memory: with
+// one or two waves to a SIMD that is what keeps a block in flight while another
+// is computed (through registers 67 x 6144 x 2048 took 14 us, and 10.2 so), and
+// pieces of 16 bytes are placed so that neither side meets in a bank.  WN = 2: the
+// waves of two column tiles bring half of each block and read it both, for which
+// they meet at a barrier; the blocks alternate between two places.
+template <bool F16, int MB, int NT, int WN, int GROUP>
+__global__ __launch_bounds__(512) void gemm_w4_kernel(const W4Args p) {
+    constexpr int WK = 8 / WN, kSteps = GROUP / 32, kGroups = 4 / kSteps, kStage = 16 * MB * 256;
+    __shared__ __attribute__((aligned(1024))) char lds[8 * kStage];
+    static_assert(MB * NT * 1024 <= kStage, "the sums take the place of the activations");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int wk = wave / WN, wn = wave % WN;
+    const int nb0 = (blockIdx.x * WN + wn) * NT, m0 = blockIdx.y * 16 * MB, rows = min(16 * MB, p.M - m0);
+    const uint32_t ld = 2u * (uint32_t)p.lda;   // bytes: lda is at most 2^24
+    const __amdgpu_buffer_rsrc_t ars = make_rsrc(p.a + (int64_t)m0 * p.lda, (uint32_t)rows * ld);
+    char* stage = lds + wk * WN * kStage;   // WN of them, in turn
+    // Instruction i brings rows 4 i .. 4 i + 3, 256 bytes each, piece c of row q to place c ^ (q & 15); rows behind M are
+    // behind the buffer's end and come as zeros.
+    auto fetch = [&](int kb, char* to) __attribute__((always_inline)) {
+        const int last = min(16, (p.K - 128 * kb) >> 3) - 1;   // behind K a row's last piece again: its codes' scale is 0
+        uint32_t at[4];
 #pragma unroll
-    for (int b = 0; b < MB; ++b)
+        for (int u = 0; u < 4; ++u) at[u] = (uint32_t)g * ld + 16u * (uint32_t)min(r ^ ((4 * (u + wn * (4 * MB / WN)) & 15) + g), last);
+        uint32_t step = 256u * (uint32_t)kb + (uint32_t)wn * (4 * MB / WN) * 4u * ld;
+        to += wn * (4 * MB / WN) * 1024;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            arow[b][i] = 2u * ((uint32_t)min(16 * b + 4 * i + xr, p.M - 1 - m0) * (uint32_t)p.lda + xc);
+        for (int i = 0; i < 4 * MB / WN; ++i) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ars, (__attribute__((address_space(3))) void*)(to + 1024 * i), 16,
+                                                     at[i & 3] + step, 0, 0, 0);
+            step += 4u * ld;
+        }
+    };
     const uint8_t* wtile[NT];
     const uint32_t* ptile[NT];
 #pragma unroll
@@ -94,26 +136,6 @@ __global__ __launch_bounds__(64 * WK * WN) void gemm_w4_kernel(const W4Args p) {
                 o.par[t][q] = *reinterpret_cast<const u32x4*>(ptile[t] + (int64_t)(kb * kGroups + q) * 16);
         }
     };
-    auto load_x = [&](u32x4 (&x)[MB][4], int kb) __attribute__((always_inline)) {
-        const bool in = 128 * kb + xc < p.K;   // K is a multiple of 32
-#pragma unroll
-        for (int b = 0; b < MB; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (m0 + 16 * b + 4 * i < p.M)   // rows behind the last are other columns of the product, not stored
-                    x[b][i] = in ? *reinterpret_cast<const u32x4*>(abase + 256 * (int64_t)kb + arow[b][i]) : u32x4{0, 0, 0, 0};
-    };
-    auto order_x = [&](u32x4 (&f)[4], const u32x4 (&x)[4]) __attribute__((always_inline)) {
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(&xs[wave][4 * i + xr][xc]) = x[i];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const u32x4*>(&xs[wave][r][32 * j + 8 * g]);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    };
-
     f32x4 acc[NT][MB];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -122,112 +144,74 @@ __global__ __launch_bounds__(64 * WK * WN) void gemm_w4_kernel(const W4Args p) {
     const NibbleMask nmask = nibble_mask<F16>();
     const u32x4 ones = F16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
                            : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-    W4Block<NT, kGroups> st[PF];
-    constexpr bool kAhead = MB <= 2;   // activations a block ahead, where registers allow
-    u32x4 x[MB][4], xahead[kAhead ? MB : 1][4] = {};
-    auto& xn = [&]() -> u32x4(&)[MB][4] {
-        if constexpr (kAhead) return xahead;
-        else return x;
-    }();
+    W4Block<NT, kGroups> cur, nxt;
+    if (wk < p.KB) {
+        load_w(nxt, wk);
+        fetch(wk, stage);
+    }
+    int turn = 0;
+    for (int kb = wk; (WN > 1 ? kb - wk : kb) < p.KB; kb += WK, turn = WN - 1 - turn) {
+        cur = nxt;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (WN > 1) {
+            __syncthreads();
+            if (kb >= p.KB) break;   // the last round of some waves
+        }
+        const char* from = stage + turn * kStage;
+        u32x4 x[MB][4];
 #pragma unroll
-    for (int s = 0; s < PF; ++s)
-        if (wk + s * WK < p.KB) load_w(st[s], wk + s * WK);
-    if (kAhead && wk < p.KB) load_x(xn, wk);
-    for (int kb0 = wk; kb0 < p.KB; kb0 += PF * WK) {
+        for (int b = 0; b < MB; ++b)
 #pragma unroll
-        for (int s = 0; s < PF; ++s) {
-            const int kb = kb0 + s * WK;
-            if (kb >= p.KB) break;
-            if (!kAhead) load_x(xn, kb);
+            for (int j = 0; j < 4; ++j)
+                x[b][j] = *reinterpret_cast<const u32x4*>(from + (16 * b + r) * 256 + 16 * ((4 * j + g) ^ r));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the next block is brought into its place
+        if (kb + WK < p.KB) {
+            load_w(nxt, kb + WK);
+            fetch(kb + WK, stage + (WN - 1 - turn) * kStage);
+        }
 #pragma unroll
-            for (int b = 0; b < MB; ++b) order_x(x[b], xn[b]);
-            if (kAhead && kb + WK < p.KB) load_x(xn, kb + WK);
+        for (int q = 0; q < kGroups; ++q) {
+            f32x4 sx[MB];
 #pragma unroll
-            for (int q = 0; q < kGroups; ++q) {
-                f32x4 sx[MB], pr[NT][MB];
+            for (int b = 0; b < MB; ++b) sx[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int b = 0; b < MB; ++b) {
-                    sx[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = q * kSteps; j < (q + 1) * kSteps; ++j)
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) pr[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-                }
+                for (int b = 0; b < MB; ++b) sx[b] = mfma_16b<F16>(ones, x[b][j], sx[b]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                f32x4 pr[MB];
+#pragma unroll
+                for (int b = 0; b < MB; ++b) pr[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = q * kSteps; j < (q + 1) * kSteps; ++j) {
+                    const u32x4 w = nibbles_plus16<F16>(cur.code[t][j], nmask);
 #pragma unroll
-                    for (int b = 0; b < MB; ++b) sx[b] = mfma_16b<F16>(ones, x[b][j], sx[b]);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const u32x4 w = nibbles_plus16<F16>(st[s].code[t][j], nmask);
-#pragma unroll
-                        for (int b = 0; b < MB; ++b) pr[t][b] = mfma_16b<F16>(w, x[b][j], pr[t][b]);
-                    }
+                    for (int b = 0; b < MB; ++b) pr[b] = mfma_16b<F16>(w, x[b][j], pr[b]);
                 }
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t par = cur.par[t][q][i];
+                    const float sc = w4_scale(par, p.scale_f16), z = 16.f + (float)(par & 0xffu);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t par = st[s].par[t][q][i];
-                        const float sc = w4_scale(par, p.scale_f16);
-                        const float z = -sc * (16.f + (float)(par & 0xffu));
-#pragma unroll
-                        for (int b = 0; b < MB; ++b)
-                            acc[t][b][i] = __builtin_fmaf(z, sx[b][0], __builtin_fmaf(sc, pr[t][b][i], acc[t][b][i]));
-                    }
+                    for (int b = 0; b < MB; ++b)
+                        acc[t][b][i] = __builtin_fmaf(sc, __builtin_fmaf(-z, sx[b][0], pr[b][i]), acc[t][b][i]);
+                }
             }
-            if (kb + PF * WK < p.KB) load_w(st[s], kb + PF * WK);
         }
     }
-    if (WK > 1) {
+    __syncthreads();
+    f32x4* red = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int b = 0; b < MB; ++b) red[wk][wn][t * MB + b][lane] = acc[t][b];
-        __syncthreads();
-    }
-    auto finish = [&](int t, int b, f32x4 v) __attribute__((always_inline)) {
-        const int m = m0 + 16 * b + r, n = 16 * (nb0 + t) + 4 * g;
-        if (m >= p.M || n >= p.N) return;
-        const int64_t at = (int64_t)m * p.ldc + n;
-        const int cols = min(4, p.N - n);
+        for (int b = 0; b < MB; ++b) red[(wave * NT * MB + t * MB + b) * 64 + lane] = acc[t][b];
+    __syncthreads();
+    for (int u = wk; u < NT * MB; u += WK) {
+        f32x4 v = red[(wn * NT * MB + u) * 64 + lane];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < cols) v[i] = apply_act(p.act, v[i] + (p.bias ? p.bias[n + i] : 0.f));
-        if (cols == 4 && p.vec4) {
-            if (p.c_kind == 0) {
-                f32x4* c = reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at);
-                *c = p.accumulate ? *c + v : v;
-            } else {
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.c) + at) =
-                    p.c_kind == 1 ? uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}
-                                  : uint2{pack_f16x2_rn(v[0], v[1]), pack_f16x2_rn(v[2], v[3])};
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (i >= cols) continue;
-            if (p.c_kind == 0) {
-                float* c = static_cast<float*>(p.c) + at + i;
-                *c = p.accumulate ? *c + v[i] : v[i];
-            } else if (p.c_kind == 1) {
-                static_cast<uint16_t*>(p.c)[at + i] = (uint16_t)f32_to_bf16_bits(v[i]);
-            } else {
-                static_cast<_Float16*>(p.c)[at + i] = (_Float16)v[i];
-            }
-        }
-    };
-    if (WK > 1) {
-        for (int u = wk; u < NT * MB; u += WK) {
-            f32x4 v = red[0][wn][u][lane];
-#pragma unroll
-            for (int w = 1; w < WK; ++w) v += red[w][wn][u][lane];
-            finish(u / MB, u % MB, v);
-        }
-    } else {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int b = 0; b < MB; ++b) finish(t, b, acc[t][b]);
+        for (int w = 1; w < WK; ++w) v += red[((w * WN + wn) * NT * MB + u) * 64 + lane];
+        w4_store(p, m0 + 16 * (u % MB) + r, 16 * (nb0 + u / MB) + 4 * g, v);
     }
 }
 
@@ -269,40 +253,41 @@ static inline bool w4_shape_ok(int32_t N, int32_t K, int32_t group) {
 static inline int w4_kb(int K) { return (K + 127) / 128; }
 static inline int w4_groups(int K, int group) { return w4_kb(K) * (128 / group); }
 
-template <bool F16, int MB, int NT, int WK, int WN, int PF, int GROUP>
+template <bool F16, int MB, int NT, int WN, int GROUP>
 static void launch_w4_shape(const W4Args& p, hipStream_t s) {
     const dim3 grid((unsigned)((p.n16 + NT * WN - 1) / (NT * WN)), (unsigned)((p.M + 16 * MB - 1) / (16 * MB)));
-    hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WK, WN, PF, GROUP>), grid, dim3(64 * WK * WN), 0, s, p);
+    hipLaunchKernelGGL((gemm_w4_kernel<F16, MB, NT, WN, GROUP>), grid, dim3(512), 0, s, p);
 }
 
-// Shapes by rows and tiles of 16 columns; us with weights from memory, groups of 128, MB,NT,WK,WN,PF:
-//   up to 16 rows: 16 x 2048 x 8192 8.5 with 1,1,16,1,1 and 12.2 with 1,2,8,1,2; 16 x 8192 x 8192 12.8 with
-//   1,2,16,1,2 and 16.5 with 1,1,16,1,1 (a second tile of columns halves the activations' reads; the first fills
-//   the card with few columns).
-//   up to 32 rows: 32 x 8192 x 8192 16.4 with 2,2,8,1,2 and 25 with 2,1,8,1,2.
-//   beyond, in slabs of 80 rows: 67 x 2048 x 2048 7.3 with 5,1,8,1,2 and 12.3 with 5,2,4,1,2; 67 x 6144 x 2048 14.0
-//   with 5,2,4,1,2 and 24 with 5,1,8,1,2; 268 x 8192 x 8192 107 with 5,4,2,2,2 and 151 with 5,1,4,1,2.
-// Groups of 64 keep twice the parameters, one block ahead; groups of 32 four times, and one tile of columns.
+// The shape whose estimate is the smallest: rounds of 256 workgroups, each 0.5 us
+// and for every block of 128 inputs of a wave 0.2 + 0.25 MB NT - 0.1 MB (WN - 1).
+// Fitted to 63 products of 8..536 rows, 2048..16384 columns and 2048..8192 inputs
+// with the weights from memory, where the choice costs 3% in the mean, and up to a
+// third, over the fastest of 16 shapes.  us, MB,NT,WN:
+//   16 x 2048 x 2048: 3.9 with 1,1,1, 4.9 with 1,2,1; 16 x 8192 x 8192: 11.0 with 1,2,1, 14.6 with 1,1,1;
+//   32 x 8192 x 8192: 14.8 with 2,2,1, 17.7 with 1,2,1; 48 x 6144 x 2048: 8.0 with 3,2,1, 10.1 with 2,2,1;
+//   67 x 6144 x 2048: 10.6 with 5,2,1, 13.1 with 3,2,1; 536 x 8192 x 2048: 46.7 with 5,2,2, 57.2 with 5,2,1.
+// Groups of 32 keep four times the parameters; five tiles of rows do not fit the registers beside them.
 template <bool F16, int GROUP>
 static void launch_w4(const W4Args& p, hipStream_t s) {
-    constexpr int PF = GROUP == 128 ? 2 : 1;
-    const int64_t tiles = (int64_t)p.n16 * ((p.M + 79) / 80);
-    if constexpr (GROUP == 32) {
-        if (p.M <= 16) launch_w4_shape<F16, 1, 1, 16, 1, 1, GROUP>(p, s);
-        else if (p.M <= 32) launch_w4_shape<F16, 2, 1, 8, 1, 1, GROUP>(p, s);
-        else launch_w4_shape<F16, 5, 1, 4, 1, 1, GROUP>(p, s);
-    } else if (p.M <= 16) {
-        if (tiles <= 256) launch_w4_shape<F16, 1, 1, 16, 1, 1, GROUP>(p, s);
-        else launch_w4_shape<F16, 1, 2, 16, 1, PF, GROUP>(p, s);
-    } else if (p.M <= 32) {
-        if (tiles <= 256) launch_w4_shape<F16, 2, 1, 8, 1, PF, GROUP>(p, s);
-        else launch_w4_shape<F16, 2, 2, 8, 1, PF, GROUP>(p, s);
-    } else if (tiles <= 256) {
-        launch_w4_shape<F16, 5, 1, 8, 1, PF, GROUP>(p, s);
-    } else if (tiles < 1024) {
-        launch_w4_shape<F16, 5, 2, 4, 1, PF, GROUP>(p, s);
-    } else {
-        launch_w4_shape<F16, 5, 4, 2, 2, PF, GROUP>(p, s);
+    static const int shapes[6][3] = {{1, 1, 1}, {1, 2, 1}, {2, 2, 1}, {3, 2, 1}, {5, 2, 1}, {5, 2, 2}};
+    int best = 0;
+    double least = 0.;
+    for (int i = 0; i < (GROUP == 32 ? 4 : 6); ++i) {
+        const int mb = shapes[i][0], nt = shapes[i][1], wn = shapes[i][2];
+        const int64_t slabs = ((int64_t)p.M + 16 * mb - 1) / (16 * mb), wgs = slabs * ((p.n16 + nt * wn - 1) / (nt * wn));
+        if (slabs > 65535) continue;   // the grid's second dimension
+        const double us = (double)((wgs + 255) / 256) *
+                          (0.5 + (double)((p.KB * wn + 7) / 8) * (0.2 + 0.25 * mb * nt - 0.1 * mb * (wn - 1)));
+        if (least == 0. || us < least) least = us, best = i;
+    }
+    if (best == 0) launch_w4_shape<F16, 1, 1, 1, GROUP>(p, s);
+    else if (best == 1) launch_w4_shape<F16, 1, 2, 1, GROUP>(p, s);
+    else if (best == 2) launch_w4_shape<F16, 2, 2, 1, GROUP>(p, s);
+    else if (best == 3) launch_w4_shape<F16, 3, 2, 1, GROUP>(p, s);
+    else if constexpr (GROUP != 32) {
+        if (best == 4) launch_w4_shape<F16, 5, 2, 1, GROUP>(p, s);
+        else launch_w4_shape<F16, 5, 2, 2, GROUP>(p, s);
     }
 }
 
@@ -353,7 +338,7 @@ extern "C" int sf_gemm_w4(const sf_gemm_w4_desc* desc, void* stream) {
     if (desc->act < SF_ACT_NONE || desc->act > SF_ACT_SILU) return SF_ENOTSUP;
     if (desc->accumulate && desc->c_dtype != SF_F32) return SF_ENOTSUP;
     // the grid's second dimension; a launch counts its threads in 32 bits; a workgroup's rows are addressed in 32 bits
-    if (desc->M > 1 << 22 || desc->N > 1 << 25 || desc->lda > 1 << 24) return SF_ENOTSUP;
+    if (desc->M > 1 << 21 || desc->N > 1 << 25 || desc->lda > 1 << 24) return SF_ENOTSUP;
     sfk::W4Args p = {};
     p.a = static_cast<const uint16_t*>(desc->A);
     p.lda = desc->lda;

@@ -71,6 +71,19 @@ def test_many_columns(M, N, group):
     _check(kernels.gemm_w4(a.to(DEV), w, out_dtype=F32), a.double() @ ref_w.t(), big, K, F32, what=f"{M} x {N}")
 
 
+@pytest.mark.parametrize("M,N", [(33, 8200), (45, 6100), (67, 6111), (150, 16500)])
+@pytest.mark.parametrize("group,K", [(32, 32), (64, 64), (32, 96), (128, 128), (64, 192), (128, 640), (64, 1088),
+                                     (32, 1184), (128, 2176)])
+def test_tiles_of_rows(M, N, group, K):
+    """Three to five tiles of rows, one or two column tiles to an activation block, fewer blocks than waves, a last
+    block that is not full; rows that are not packed tightly, followed by NaN."""
+    dtype = BF if K % 128 else FP
+    a, w, ref_w, big = _case(M, N, K, group, dtype, True, M + K)
+    wide = torch.full((M, K + 8), float("nan"), dtype=dtype, device=DEV)
+    wide[:, :K] = a.to(DEV)
+    _check(kernels.gemm_w4(wide[:, :K], w, out_dtype=F32), a.double() @ ref_w.t(), big, K, F32, what=f"{M} x {N} x {K}")
+
+
 @pytest.mark.parametrize("M", [1, 67])
 @pytest.mark.parametrize("out_dtype", [F32, BF, FP])
 @pytest.mark.parametrize("act", [abi.SF_ACT_NONE, abi.SF_ACT_GELU_TANH, abi.SF_ACT_SILU])
