@@ -176,7 +176,12 @@ template <bool F16, int D, int QT, bool PAIR, int NW>
 __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     constexpr int GR = D / 64, DT = D / 16;   // 64-channel groups, tiles of 16 channels
     __shared__ float xm[NW][QT * 16], xl[NW][QT * 16], xf[NW][QT * 16], xs[QT * 16];
-    constexpr int kJoin = QT == 5 ? 3 : QT == 4 ? 2 : QT;   // tiles that meet at a time
+    constexpr int kJoin = D == 128 && NW == 8 ? 1 : QT == 5 ? 3 : QT == 4 ? 2 : QT;   // tiles that meet at a time
+    // 128 channels and two tiles leave no registers for the next raw block beside eight waves: it waits in LDS, brought
+    // there straight from memory.  us, against four waves with it in registers: 8 x 32 heads x 67 x 4374 145 and 166,
+    // 2 x 8 x 268 rows x 8192 73 and 96, 2 x 8 x 1024 rows x 2048 causal 31.5 and 34.4.
+    constexpr bool kStaged = D == 128 && QT > 1;
+    __shared__ __attribute__((aligned(16))) uint8_t raw[kStaged ? NW : 1][kStaged ? Kv4<D>::kBytes : 16];
     __shared__ float xo[NW][kJoin * 16][D + 4], xq[GR][QT * 16];
     __shared__ u32x4 ql[QT > 1 ? QT * GR * 2 : 1][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -201,7 +206,26 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 
     const uint8_t* base = p.cache + (int64_t)bh * p.cache_blocks * Kv4<D>::kBytes;
     KvBlock<D> nx;
-    if (b0 + wave < b1) nx.load(base + (int64_t)(b0 + wave) * Kv4<D>::kBytes, lane);
+    auto fetch = [&](int blk) __attribute__((always_inline)) {
+        const uint8_t* from = base + (int64_t)(kStaged ? __builtin_amdgcn_readfirstlane(blk) : blk) * Kv4<D>::kBytes;
+        if constexpr (kStaged) {
+            const __amdgpu_buffer_rsrc_t blocks = make_rsrc(from, Kv4<D>::kBytes);
+            const int w = __builtin_amdgcn_readfirstlane(wave);
+            int at_lane = 16 * lane;
+            asm volatile("" : "+v"(at_lane));   // or 4 * lane is kept in a register, which spills
+#pragma unroll
+            for (int at = 0; at < 32 * D; at += 1024)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(blocks, (__attribute__((address_space(3))) void*)(raw[w] + at), 16,
+                                                         at_lane, at, 0, 0);
+#pragma unroll
+            for (int at = 32 * D; at < 36 * D; at += 256)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(blocks, (__attribute__((address_space(3))) void*)(raw[w] + at), 4,
+                                                         at_lane >> 2, at, 0, 0);
+        } else {
+            nx.load(from, lane);
+        }
+    };
+    if (b0 + wave < b1) fetch(b0 + wave);
 
     // Query fragments (B operands) and row sums: in registers for one tile, else each tile's by one wave into LDS.
     static_assert(QT <= NW, "a wave for each tile");
@@ -245,6 +269,10 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     auto block = [&](const int blk, auto masked_c) __attribute__((always_inline)) {
         constexpr bool masked = decltype(masked_c)::value;
         const int key0 = kKvBlock * blk;
+        if (kStaged) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            nx.load(raw[kStaged ? wave : 0], lane);
+        }
         uint32_t see = 0xffu;   // the lane's 8 tokens, by length and mask
         if (masked) {
             see = 0;
@@ -321,7 +349,8 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
             }
         }
         // the raw block is spent: fetch the wave's next one
-        if (blk + NW < b1) nx.load(base + (int64_t)(blk + NW) * Kv4<D>::kBytes, lane);
+        if (kStaged) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the next one comes into its place
+        if (blk + NW < b1) fetch(blk + NW);
 
         // Raw scores of a tile; the next one's products are issued before this one's exponentials, its operands
         // read before this one's maximum.
@@ -807,7 +836,7 @@ static int kv_column_groups(const sf_attn_kv4_desc* d, int rows, int64_t heads) 
 // with 5 (estimates 12, 15, 21); 32 x 67 x 4374 18.9 with qt 3 and four splits,
 // 19.6 with 5 and eight, 31 with 3 and one (19, 20, 30); 256 x 67 x 4374 42 with
 // qt 5.  The (hi, lo) form takes 0.42 us a step, and qt 5 would spill.  128
-// channels: 2 tiles and four waves are what fits.
+// channels: 2 tiles are what fits.
 static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
     KvPlan k = {};
     const int64_t R = (int64_t)(d->Hq / d->cache.H) * d->Sq, heads = (int64_t)d->B * d->cache.H;
@@ -819,7 +848,7 @@ static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
     } else {
         const bool wide = d->cache.D == 128;
         const int most = wide ? 2 : kv_pair(d) ? 4 : 5;
-        const int64_t per_block = kKvBlock * (wide ? 4 : 8);
+        const int64_t per_block = kKvBlock * 8;   // a block to each wave
         const double step = kv_pair(d) ? 0.42 : 0.3;
         double best = 0.;
         for (int qt = 2; qt <= most; ++qt) {
@@ -933,8 +962,8 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
         else if (k.qt == 4) SF_KV4_LAUNCH(64, 4, false, 8);
         else SF_KV4_LAUNCH(64, 5, false, 8);
     } else {
-        if (pair) SF_KV4_LAUNCH(128, 2, true, 4);
-        else SF_KV4_LAUNCH(128, 2, false, 4);
+        if (pair) SF_KV4_LAUNCH(128, 2, true, 8);
+        else SF_KV4_LAUNCH(128, 2, false, 8);
     }
 #undef SF_KV4_TOKEN
 #undef SF_KV4_LAUNCH
