@@ -497,3 +497,55 @@ def test_long_streams_of_few_rows(D, Hq, Sq, Sk, dtype, kind):
             rel = 2 * (dx + 2.0 ** -22) + 2.0 ** -16 + (32 + Sk / 32) * 2.0 ** -24 * 16 + (7 * 2.0 ** -12 if Hq // H * Sq > 16 and dtype == BF else 0)
             tol = rel * float(lv.abs().max()) + half_step(dtype) * ref.abs() + (2.0 ** -25 if dtype == FP else 0)
             assert ((got[b].double() - ref).abs() <= tol).all(), (splits, b)
+
+
+@pytest.mark.parametrize("kind", ["causal", "mask"])
+@pytest.mark.parametrize("dtype,out_dtype", [(BF, BF), (FP, FP), (BF, F32)])
+@pytest.mark.parametrize("splits", [1, 3, 64])
+def test_many_rows_of_128_channels(splits, dtype, out_dtype, kind):
+    """Several blocks to a wave, splits with nothing to read, lengths of zero and below the rows' number."""
+    B, Hq, H, Sq, Sk, D = 4, 6, 2, 19, 1100, 128
+    c, k, v = _filled(B, H, Sk, D, dtype, 140, cap=1111)
+    q = _randn(143, B, Hq, Sq, D, dtype=dtype)
+    kw = {"valid": torch.tensor([1100, 0, 7, 513], dtype=torch.int32)}
+    if kind == "mask":
+        kw["mask"] = torch.rand(B, Sk, generator=torch.Generator().manual_seed(5)) < 0.4
+        kw["mask"][0, 64:900] = False
+    got = attention_kv4(q.to(DEV), c, keys=Sk, is_causal=kind == "causal", valid_len=kw["valid"].to(DEV), num_splits=splits,
+                        kv_mask=kw["mask"].to(DEV) if "mask" in kw else None, out_dtype=out_dtype)
+    _attn_check(got, q, k, v, out_dtype, what=kind, causal=kind == "causal", **kw)
+    assert (got[1] == 0).all()
+
+
+@pytest.mark.parametrize("Sq", [1, 40])
+def test_no_keys_and_in_place(Sq):
+    B, Hq, H, Sk, D = 2, 8, 2, 90, 64
+    c, k, v = _filled(B, H, Sk, D, BF, 150)
+    q = _randn(153, B, Hq, Sq, D, dtype=BF).to(DEV)
+    assert (attention_kv4(q, c, keys=0) == 0).all()
+    assert (attention_kv4(q, c, keys=0, is_causal=True, num_splits=2) == 0).all()
+    assert attention_kv4(q[:, :, :0], c).shape == (B, Hq, 0, D)
+    ref = attention_kv4(q, c)
+    for splits in (0, 3):   # the output in the queries' place
+        x = q.clone()
+        attention_kv4(x, c, out=x, num_splits=splits)
+        assert ((x.double() - ref.double()).abs() <= 2 * half_step(BF) * ref.double().abs() + 2.0 ** -9 * float(v.abs().max())).all()
+        assert splits or torch.equal(x, ref)
+
+
+def test_two_tokens_at_one_slot():
+    """They leave a mixture there; what lies beside is as written."""
+    B, H, S, D = 1, 3, 40, 64
+    c = Kv4Cache(B, H, 64, D, DEV)
+    old = _randn(160, B, H, 64, D, dtype=BF)
+    c.write(old.to(DEV), old.to(DEV))
+    new = _randn(161, B, H, S, D, dtype=BF)
+    slots = torch.arange(S, dtype=torch.int32)[None].clone()
+    slots[0, 7] = 20
+    c.write(new.to(DEV), new.to(DEV), slots.to(DEV))
+    want = old.clone()
+    want[:, :, :S] = new
+    want[:, :, 7] = old[:, :, 7]
+    keep = torch.arange(64) != 20
+    for got in c.read(dtype=F32):
+        assert torch.equal(got.cpu()[:, :, keep], _levels(want).float()[:, :, keep])
