@@ -745,52 +745,54 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     kv_finish<D, E>(p, split, b, h * p.G + r / p.Sq, r % p.Sq, d0, y, xtop[r], xs[r]);
 }
 
-// out = sum_splits O 2^(m - M) / sum_splits l 2^(m - M), one wave per row.
+// out = sum_splits O 2^(m - M) / sum_splits l 2^(m - M), a workgroup for each row
+// whose four waves deal the splits: all of a row's loads are in flight at once
+// (with one wave to a row, eight splits at a time, 32 rows of 20 splits took 3.6
+// us).
 template <int D>
 __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(const KvAttnArgs p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= p.rows) return;
+    constexpr int E = D / 64, kEach = kKvMaxSplits / 4;
+    __shared__ float part[4][D];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = blockIdx.x;
     const float* src = p.part + row * (D + 2);
     const int64_t step = p.rows * (D + 2);
-    float m = kKvNoMax, l = 0.f;
+    float m = kKvNoMax, l = 0.f, v[kEach][E];
     if (lane < p.splits) m = src[lane * step + D], l = src[lane * step + D + 1];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+        if (wave + 4 * j < p.splits)
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[j][e] = src[(wave + 4 * j) * step + 64 * e + lane];
     float mm = m;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
-    const float w = lane < p.splits ? __builtin_amdgcn_exp2f(m - mm) : 0.f;
+    const float w = __builtin_amdgcn_exp2f(m - mm);   // l is 0 behind the last split
     float sum = l * w;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    constexpr int E = D / 64;
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int s0 = 0; s0 < p.splits; s0 += 8) {   // eight splits' loads in flight
-        float v[8][E];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[j][e] = s0 + j < p.splits ? src[(s0 + j) * step + 64 * e + lane] : 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float ws = __shfl(w, s0 + j, 64);   // 0 behind the last split
+    for (int j = 0; j < kEach; ++j)
+        if (wave + 4 * j < p.splits) {
+            const float ws = __shfl(w, wave + 4 * j, 64);
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] += ws * v[j][e];
         }
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[wave][64 * e + lane] = acc[e];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= D) return;
+    const float y = (part[0][d] + part[1][d] + part[2][d] + part[3][d]) * (sum == 0.f ? 0.f : 1.f / sum);
     const int s = (int)(row % p.Sq);
     const int64_t bh = row / p.Sq, Hq = (int64_t)p.H * p.G;
-    const int64_t at = bh / Hq * p.os[0] + bh % Hq * p.os[1] + s * p.os[2];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float y = acc[e] * inv;
-        const int64_t i = at + 64 * e + lane;
-        if (p.out_kind == 0) static_cast<float*>(p.out)[i] = y;
-        else if (p.out_kind == 1) static_cast<uint16_t*>(p.out)[i] = (uint16_t)f32_to_bf16_bits(y);
-        else static_cast<_Float16*>(p.out)[i] = (_Float16)y;
-    }
+    const int64_t i = bh / Hq * p.os[0] + bh % Hq * p.os[1] + s * p.os[2] + d;
+    if (p.out_kind == 0) static_cast<float*>(p.out)[i] = y;
+    else if (p.out_kind == 1) static_cast<uint16_t*>(p.out)[i] = (uint16_t)f32_to_bf16_bits(y);
+    else static_cast<_Float16*>(p.out)[i] = (_Float16)y;
 }
 
 // How a call is cut up: tiles of 16 query rows to a workgroup (qt), groups of
@@ -906,7 +908,7 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
         if (d->q_stride[i] < 0 || (d->q_stride[i] & 7) || d->o_stride[i] < 0 || (d->o_stride[i] & 7)) return SF_EINVAL;
     if (d->kv_mask && d->kv_mask_stride < 0) return SF_EINVAL;
     const sfk::KvPlan k = sfk::kv_plan(d);
-    if (k.wgs >= 1 << 23 || (k.splits > 1 && k.rows >= 1 << 26)) return SF_ENOTSUP;   // a launch counts its threads in 32 bits
+    if (k.wgs >= 1 << 23 || (k.splits > 1 && k.rows >= 1 << 24)) return SF_ENOTSUP;   // a launch counts its threads in 32 bits
     if (k.splits > 1 && (!workspace || workspace_bytes < sf_attn_kv4_workspace_bytes(d))) return SF_EWORKSPACE;
     if (k.splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 3)) return SF_EINVAL;
     sfk::KvAttnArgs p = {};
@@ -969,7 +971,7 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
 #undef SF_KV4_LAUNCH
     if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
     if (k.splits > 1) {
-        const dim3 mg((unsigned)((k.rows + 3) / 4));
+        const dim3 mg((unsigned)k.rows);
         if (d->cache.D == 64) hipLaunchKernelGGL(sfk::attn_kv4_merge_kernel<64>, mg, dim3(256), 0, s, p);
         else hipLaunchKernelGGL(sfk::attn_kv4_merge_kernel<128>, mg, dim3(256), 0, s, p);
         if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
