@@ -807,11 +807,12 @@ static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline bool kv_pair(const sf_attn_kv4_desc* d) { return d->out_dtype != SF_BF16; }
 
 // Up to 16 rows to a key head: one tile, four waves to a workgroup.  Up to 512
-// keys a wave has four blocks at most and a merge costs as much as it saves (8
-// heads x 512 keys of 128 channels: 8.0 us with one split, 7.9 with four);
-// beyond, about two workgroups a CU of at least a block to a wave, and no split
-// over 2048 keys, so that batches of unequal lengths spread (16 x 8 heads,
-// 4096..16384 keys: 61 us with 8 splits, 62 with 4, 137 with 1).
+// keys a wave has four blocks at most and a merge costs what it saves (us with
+// one split and four, 512 keys: 8 heads of 128 channels 8.0 and 7.4, 16 x 8 heads
+// 8.6 and 9.6, 8 x 8 of 64 5.8 and 6.7; 700 keys, 8 heads: 10.6 and 8.9); beyond,
+// about two workgroups a CU of at least a block to a wave, and no split over 2048
+// keys, so that batches of unequal lengths spread (16 x 8 heads, 4096..16384
+// keys: 59 us with 8 splits, 58 with 4, 148 with 1).
 static int kv_splits_one_tile(const sf_attn_kv4_desc* d, int64_t base) {
     if (d->Sk <= 512) return 1;
     const int64_t want = std::max(ceil_div(512, base), ceil_div(d->Sk, 2048));
