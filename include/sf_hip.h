@@ -732,12 +732,11 @@ int sf_kv4_read(const sf_kv4_cache* cache, const int32_t* slots, int32_t S, void
  * no row sees may hold anything.
  * scale 0: 1 / sqrt(D); negative: SF_ENOTSUP.  in_dtype SF_BF16 or SF_F16.
  * The softmax's maximum and sum are fp32; its weights enter the product with V
- * as bf16 (hi, lo) pairs, 2^-18 relative, and the fp32 sums are of codes + 16:
- * an fp32 output is off by 1.4e-6 of its norm at 20 keys and 1e-5 at 8192, where
- * the mean of many values is small beside them.  With more than 16 query rows to
- * a key head and a bf16 output, weights and values enter as fp16, the values
- * under a power of two that keeps them in its range: 5 2^-12 of the largest
- * value seen.  Values are taken up to 2^100 in magnitude.  out may be Q itself
+ * as bf16 (hi, lo) pairs, 2^-18 relative, and for an fp32 output as three bf16
+ * terms, which leaves it within 1e-6 of its norm up to 16384 keys (as sums over
+ * fp32 values).  With more than 16 query rows to a key head and a bf16 output,
+ * weights and values enter as fp16, the values under a power of two that keeps
+ * them in its range: 5 2^-12 of the largest value seen.  Values are taken up to 2^100 in magnitude.  out may be Q itself
  * (same strides and type); otherwise they must not overlap.
  * num_splits: 0 chooses; n > 0 forces n key splits (at most 64). */
 typedef struct sf_attn_kv4_desc {

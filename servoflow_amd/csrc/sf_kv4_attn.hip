@@ -38,6 +38,19 @@ constexpr int kKvMaxSplits = 64;
 constexpr float kKvSlack = 8.f;       // log2
 constexpr float kKvNoMax = -1.5e38f;  // the maximum of a row that has seen nothing
 
+// How p and V meet.  kKvHalf (bf16 outputs of many rows): both in fp16.  kKvPair
+// (other 16-bit outputs): p s as a bf16 (hi, lo) pair with the codes, whose offset
+// the pairs' sums take away at the end.  kKvExact (fp32 outputs): three terms
+// instead of two, and the offset, which is many times a mean of values and would
+// leave its own rounding, is taken away inside the products: -23.5 times the
+// queries' sums under the scores, a product with -23.5 beside each block's.  Of
+// the output's norm that is off by 1.3e-7 (20 keys) to 7e-7 (8192), as the same
+// sums over fp32 values are, where the pair is off by 1.4e-6 to 1e-5; it costs
+// 16 x 8 heads x 16384 keys x 4 rows 78 us instead of 70, 4 x 32 x 4374 x 67 rows
+// 47 instead of 39, and 4 x 8 x 4096 x 268 rows of 128 channels, which spill, 114
+// instead of 87.
+enum { kKvHalf, kKvPair, kKvExact };
+
 struct KvAttnArgs {
     const uint16_t* q;
     const uint8_t* cache;
@@ -90,6 +103,9 @@ __device__ __forceinline__ float kv_dot(uint32_t pair, float acc) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v, pair), bf16x2v{(__bf16)-23.5f, (__bf16)-23.5f}, acc, false);
 }
 
+// A matrix operand of -23.5.
+__device__ __forceinline__ u32x4 kv_offset() { return u32x4{0xC1BCC1BCu, 0xC1BCC1BCu, 0xC1BCC1BCu, 0xC1BCC1BCu}; }
+
 // What a wave holds of a block of 32 tokens.
 template <int D>
 struct KvBlock {
@@ -128,7 +144,7 @@ __device__ __forceinline__ float kv_raise(float (&x)[8], float mx, float& m) {
 }
 
 // A query row's operand (channels 64 i + 16 g .. + 15 of the lane's group g) and
-// scale * log2 e times the sum of its channels.
+// the sums of its channels.
 template <bool F16, int D>
 __device__ __forceinline__ void kv_queries(const KvAttnArgs& p, int b, int hq, int s, int g, u32x4 (&f)[D / 64][2],
                                            float (&sums)[D / 64]) {
@@ -148,7 +164,7 @@ __device__ __forceinline__ void kv_queries(const KvAttnArgs& p, int b, int hq, i
                 sum += F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v) + (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16))
                            : __uint_as_float(v << 16) + __uint_as_float(v & 0xffff0000u);
             }
-        sums[i] = lanes4_sum(sum) * p.scale_log2;
+        sums[i] = lanes4_sum(sum);
     }
 }
 
@@ -170,11 +186,10 @@ __device__ __forceinline__ void kv_finish(const KvAttnArgs& p, int split, int b,
 }
 
 // QT tiles of 16 query rows of a key head to a workgroup.
-// PAIR: p s enters the second product as a bf16 (hi, lo) pair; otherwise p and
-// V as fp16.
-template <bool F16, int D, int QT, bool PAIR, int NW>
+template <bool F16, int D, int QT, int FORM, int NW>
 __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     constexpr int GR = D / 64, DT = D / 16;   // 64-channel groups, tiles of 16 channels
+    constexpr bool PAIR = FORM != kKvHalf, EXACT = FORM == kKvExact;
     __shared__ float xm[NW][QT * 16], xl[NW][QT * 16], xf[NW][QT * 16], xs[QT * 16];
     constexpr int kJoin = D == 128 && NW == 8 ? 1 : QT == 5 ? 3 : QT == 4 ? 2 : QT;   // tiles that meet at a time
     // 128 channels and two tiles leave no registers for the next raw block beside eight waves: it waits in LDS, brought
@@ -230,7 +245,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     // Query fragments (B operands) and row sums: in registers for one tile, else each tile's by one wave into LDS.
     static_assert(QT <= NW, "a wave for each tile");
     u32x4 qr[GR][2];
-    float qs[QT][GR];
+    float qs[QT][GR], off[QT][GR];   // scale * log2 e times a row's sum; what the codes' offset adds to its scores
     if (QT == 1 || wave < QT) {
         const int t = QT == 1 ? 0 : wave, r = min(q0 + 16 * t + col, R - 1);
         kv_queries<F16, D>(p, b, h * p.G + r / p.Sq, r % p.Sq, g, qr, qs[0]);
@@ -250,6 +265,13 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 #pragma unroll
             for (int i = 0; i < GR; ++i) qs[t][i] = xq[i][16 * t + col];
     }
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int i = 0; i < GR; ++i) {
+            off[t][i] = EXACT ? -23.5f * qs[t][i] : 0.f;
+            qs[t][i] *= p.scale_log2;
+        }
 
     f32x4 o[QT][DT];   // O^T; PAIR: without the parameters' part pm
     float m[QT], l[QT], pm[QT][PAIR ? GR : 1];
@@ -292,7 +314,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 // A NaN value reaches the rows that see it through their scores: 0 times NaN would reach the others too.
                 if (masked && !PAIR && (vp & 0x7f80u) == 0x7f80u) kp |= 0x7fc07fc0u, vp = 0u;
                 ks[i][e] = __uint_as_float(kp << 16) * p.scale_log2;
-                ko[i][e] = kv_mix(kp, -23.5f, 1.f);
+                ko[i][e] = EXACT ? __uint_as_float(kp & 0xffff0000u) : kv_mix(kp, -23.5f, 1.f);
                 vs[i][e] = PAIR ? __uint_as_float(vp << 16) : kv_mix(vp, 262144.f * vdown, 0.f);
                 vm[i][e] = PAIR ? __uint_as_float(vp & 0xffff0000u) : kv_mix(vp, -7.5f * vdown, vdown);
             }
@@ -362,15 +384,15 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) qf[i][k] = QT == 1 ? qr[i][k] : ql[(t * GR + i) * 2 + k][lane];
         };
-        auto scores = [&]() __attribute__((always_inline)) {
+        auto scores = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < GR; ++i)
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
-                    s[kt][i] = mfma_16b<F16>(ka[kt][i][1], qf[i][1], mfma_16b<F16>(ka[kt][i][0], qf[i][0], f32x4{0.f, 0.f, 0.f, 0.f}));
+                    s[kt][i] = mfma_16b<F16>(ka[kt][i][1], qf[i][1], mfma_16b<F16>(ka[kt][i][0], qf[i][0], f32x4{off[t][i], off[t][i], off[t][i], off[t][i]}));
         };
         operands(0);
-        scores();
+        scores(0);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             if (t + 1 < QT) operands(t + 1);
@@ -404,7 +426,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 #pragma unroll
                 for (int i = 0; i < DT; ++i) o[t][i] *= al;
             }
-            if (t + 1 < QT) scores();
+            if (t + 1 < QT) scores(t + 1);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(x[e]);
             if (PAIR) {
@@ -412,7 +434,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 for (int e = 0; e < 8; ++e) l[t] += x[e];
 #pragma unroll
                 for (int i = 0; i < GR; ++i) {
-                    u32x4 hi, lo;
+                    u32x4 hi, lo, rest;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float a = x[2 * e] * vs[i][2 * e], c = x[2 * e + 1] * vs[i][2 * e + 1];
@@ -422,15 +444,21 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                             if (!(row >> (2 * e + 1) & 1u)) c = mc = 0.f;
                         }
                         const uint32_t h = pack_bf16x2(a, c);
-                        const uint32_t w = pack_bf16x2(a - __uint_as_float(h << 16), c - __uint_as_float(h & 0xffff0000u));
-                        pm[t][i] = kv_dot(h, kv_dot(w, pm[t][i] + ma + mc));
+                        a -= __uint_as_float(h << 16), c -= __uint_as_float(h & 0xffff0000u);
+                        const uint32_t w = pack_bf16x2(a, c);
+                        pm[t][i] = EXACT ? pm[t][i] + ma + mc : kv_dot(h, kv_dot(w, pm[t][i] + ma + mc));
                         hi[e] = h;
                         lo[e] = w;
+                        if (EXACT) rest[e] = pack_bf16x2(a - __uint_as_float(w << 16), c - __uint_as_float(w & 0xffff0000u));
                     }
 #pragma unroll
                     for (int d = 4 * i; d < 4 * i + 4; ++d) {
-                        o[t][d] = mfma_16b<false>(va[d], hi, o[t][d]);
-                        o[t][d] = mfma_16b<false>(va[d], lo, o[t][d]);
+                        if (EXACT) o[t][d] = mfma_16b<false>(kv_offset(), hi, o[t][d]);
+                        o[t][d] = mfma_16b<false>(va[d], lo, mfma_16b<false>(va[d], hi, o[t][d]));
+                        if (EXACT) {   // the small terms where the sum is small again
+                            o[t][d] = mfma_16b<false>(va[d], rest, mfma_16b<false>(kv_offset(), lo, o[t][d]));
+                            o[t][d] = mfma_16b<false>(kv_offset(), rest, o[t][d]);
+                        }
                     }
                 }
             } else {   // the sum is taken over the rounded p, as the product is
@@ -534,7 +562,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 // 128 channels and NG = 2: a block's vector instructions go from 542 to about
 // 420, where they took 82% of the time; 16 x 8 key heads x 4 rows over 16384 keys
 // then stream 4.3 TB/s, of the 4.95 that a large copy reaches.
-template <bool F16, int D, int NG>
+template <bool F16, int D, int NG, bool EXACT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_token_kernel(const KvAttnArgs p) {
     constexpr int GR = D / 64, DT = D / 16, NW = 4, RT = 16 / NG;
     __shared__ float xm[NW * NG][RT], xl[NW * NG][RT], xf[NW * NG][RT], xs[RT], xtop[RT];
@@ -585,6 +613,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     u32x4 qf[GR][2];
     float qs[GR];
     kv_queries<F16, D>(p, b, qh, qt, g, qf, qs);
+    float off[GR];
+#pragma unroll
+    for (int i = 0; i < GR; ++i) off[i] = EXACT ? -23.5f * qs[i] : 0.f, qs[i] *= p.scale_log2;
     if (wave < NG) {   // the queries of column group `wave`, zeros in the other columns
 #pragma unroll
         for (int i = 0; i < GR; ++i)
@@ -604,7 +635,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     auto blocks = [&](const int blk, auto masked_c) __attribute__((always_inline)) {
         constexpr bool masked = decltype(masked_c)::value;
         const bool next = blk + NG * NW < b1;
-        f32x4 s[2][GR] = {};
+        f32x4 s[2][GR];
+#pragma unroll
+        for (int i = 0; i < GR; ++i) s[0][i] = s[1][i] = f32x4{off[i], off[i], off[i], off[i]};
 #pragma unroll
         for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -639,7 +672,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
             for (int i = 0; i < GR; ++i) {
                 uint32_t k = kp[i][e >> 2][e & 3];
                 if (masked && !(see >> e & 1u)) k = 0u;   // what the row does not see may hold anything
-                u = __builtin_fmaf(__uint_as_float(k << 16) * p.scale_log2, s[e >> 2][i][e & 3], __builtin_fmaf(kv_mix(k, -23.5f, 1.f), qs[i], u));
+                u = __builtin_fmaf(__uint_as_float(k << 16) * p.scale_log2, s[e >> 2][i][e & 3], __builtin_fmaf(EXACT ? __uint_as_float(k & 0xffff0000u) : kv_mix(k, -23.5f, 1.f), qs[i], u));
             }
             x[e] = masked && !(see >> e & 1u) ? -INFINITY : u;
         }
@@ -660,19 +693,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
         }
 #pragma unroll
         for (int i = 0; i < GR; ++i) {
-            u32x4 hi, lo;
+            u32x4 hi, lo, rest;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 uint32_t v0 = vp[i][e >> 1][2 * (e & 1)], v1 = vp[i][e >> 1][2 * (e & 1) + 1];
                 if (masked && !(see >> (2 * e) & 1u)) v0 = 0u;
                 if (masked && !(see >> (2 * e + 1) & 1u)) v1 = 0u;
-                const float a = x[2 * e] * __uint_as_float(v0 << 16), c = x[2 * e + 1] * __uint_as_float(v1 << 16);
+                float a = x[2 * e] * __uint_as_float(v0 << 16), c = x[2 * e + 1] * __uint_as_float(v1 << 16);
                 const uint32_t w = pack_bf16x2(a, c);
-                const uint32_t r = pack_bf16x2(a - __uint_as_float(w << 16), c - __uint_as_float(w & 0xffff0000u));
-                pm[i] = kv_dot(w, kv_dot(r, pm[i] + x[2 * e] * __uint_as_float(v0 & 0xffff0000u) + x[2 * e + 1] * __uint_as_float(v1 & 0xffff0000u)));
+                a -= __uint_as_float(w << 16), c -= __uint_as_float(w & 0xffff0000u);
+                const uint32_t r = pack_bf16x2(a, c);
+                pm[i] += x[2 * e] * __uint_as_float(v0 & 0xffff0000u) + x[2 * e + 1] * __uint_as_float(v1 & 0xffff0000u);
+                if (!EXACT) pm[i] = kv_dot(w, kv_dot(r, pm[i]));
                 hi[e] = w;
                 lo[e] = r;
+                if (EXACT) rest[e] = pack_bf16x2(a - __uint_as_float(r << 16), c - __uint_as_float(r & 0xffff0000u));
             }
+#pragma unroll
+            for (int d = 4 * i; d < 4 * i + 4; ++d)
+                if (EXACT) o[d] = mfma_16b<false>(kv_offset(), hi, o[d]);
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
                 const uint32_t keep = own == n ? 0xffffffffu : 0u;
@@ -686,8 +725,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
                                       nibble_pair_plus16<false, 1>(w1, vmask), nibble_pair_plus16<false, 3>(w1, vmask)};
                     o[2 * t] = mfma_16b<false>(va, pl, mfma_16b<false>(va, ph, o[2 * t]));
                     o[2 * t + 1] = mfma_16b<false>(vb, pl, mfma_16b<false>(vb, ph, o[2 * t + 1]));
+                    if (EXACT) {
+                        o[2 * t] = mfma_16b<false>(va, rest & keep, o[2 * t]);
+                        o[2 * t + 1] = mfma_16b<false>(vb, rest & keep, o[2 * t + 1]);
+                    }
                 }
             }
+#pragma unroll
+            for (int d = 4 * i; d < 4 * i + 4; ++d)   // the small terms where the sum is small again
+                if (EXACT) o[d] = mfma_16b<false>(kv_offset(), rest, mfma_16b<false>(kv_offset(), lo, o[d]));
         }
         if (next) {
             load_pars(vp, blk + NG * NW, Kv4<D>::kVPar);
@@ -804,7 +850,9 @@ struct KvPlan {
 
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-static inline bool kv_pair(const sf_attn_kv4_desc* d) { return d->out_dtype != SF_BF16; }
+static inline int kv_form(const sf_attn_kv4_desc* d) {   // with more than one tile of rows
+    return d->out_dtype == SF_F32 ? kKvExact : d->out_dtype == SF_F16 ? kKvPair : kKvHalf;
+}
 
 // Up to 16 rows to a key head: one tile, four waves to a workgroup.  Up to 512
 // keys a wave has four blocks at most and a merge costs what it saves (us with
@@ -838,8 +886,8 @@ static int kv_column_groups(const sf_attn_kv4_desc* d, int rows, int64_t heads) 
 // bf16): 12 x 520 rows x 1537 keys, causal, 12.1 us with qt 2, 14.4 with 3, 18.6
 // with 5 (estimates 12, 15, 21); 32 x 67 x 4374 18.9 with qt 3 and four splits,
 // 19.6 with 5 and eight, 31 with 3 and one (19, 20, 30); 256 x 67 x 4374 42 with
-// qt 5.  The (hi, lo) form takes 0.42 us a step, and qt 5 would spill.  128
-// channels: 2 tiles are what fits.
+// qt 5.  The (hi, lo) form takes 0.42 us a step, and qt 5 would spill,
+// with three terms qt 4.  128 channels: 2 tiles are what fits.
 static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
     KvPlan k = {};
     const int64_t R = (int64_t)(d->Hq / d->cache.H) * d->Sq, heads = (int64_t)d->B * d->cache.H;
@@ -850,9 +898,9 @@ static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
         k.ng = kv_column_groups(d, (int)R, heads);
     } else {
         const bool wide = d->cache.D == 128;
-        const int most = wide ? 2 : kv_pair(d) ? 4 : 5;
+        const int form = kv_form(d), most = wide ? 2 : form == kKvExact ? 3 : form == kKvPair ? 4 : 5;
         const int64_t per_block = kKvBlock * 8;   // a block to each wave
-        const double step = kv_pair(d) ? 0.42 : 0.3;
+        const double step = form == kKvHalf ? 0.3 : 0.42;
         double best = 0.;
         for (int qt = 2; qt <= most; ++qt) {
             const int64_t groups = ceil_div(R, 16 * qt), base = heads * groups;
@@ -936,37 +984,51 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)k.wgs);
     const bool f16 = d->in_dtype == SF_F16;
-#define SF_KV4_LAUNCH(DD, QT, PAIR, NW)                                                                                       \
+#define SF_KV4_LAUNCH(DD, QT, FORM, NW)                                                                                       \
     do {                                                                                                                      \
-        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT, PAIR, NW>), grid, dim3(64 * NW), 0, s, p);            \
-        else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT, PAIR, NW>), grid, dim3(64 * NW), 0, s, p);               \
+        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT, FORM, NW>), grid, dim3(64 * NW), 0, s, p);            \
+        else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT, FORM, NW>), grid, dim3(64 * NW), 0, s, p);               \
     } while (0)
-#define SF_KV4_TOKEN(DD, NG)                                                                                                  \
+#define SF_KV4_TOKEN(DD, NG, EXACT)                                                                                           \
     do {                                                                                                                      \
-        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<true, DD, NG>), grid, dim3(256), 0, s, p);                    \
-        else hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<false, DD, NG>), grid, dim3(256), 0, s, p);                       \
+        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<true, DD, NG, EXACT>), grid, dim3(256), 0, s, p);             \
+        else hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<false, DD, NG, EXACT>), grid, dim3(256), 0, s, p);                \
     } while (0)
-    const bool pair = sfk::kv_pair(d);
-    if (k.qt == 1) {
+    const int form = sfk::kv_form(d);
+    if (k.qt == 1 && form == sfk::kKvExact) {
         if (d->cache.D == 64) {
-            if (k.ng == 1) SF_KV4_LAUNCH(64, 1, true, 4);
-            else if (k.ng == 2) SF_KV4_TOKEN(64, 2);
-            else SF_KV4_TOKEN(64, 4);
+            if (k.ng == 1) SF_KV4_LAUNCH(64, 1, sfk::kKvExact, 4);
+            else if (k.ng == 2) SF_KV4_TOKEN(64, 2, true);
+            else SF_KV4_TOKEN(64, 4, true);
         } else {
-            if (k.ng == 1) SF_KV4_LAUNCH(128, 1, true, 4);
-            else SF_KV4_TOKEN(128, 2);
+            if (k.ng == 1) SF_KV4_LAUNCH(128, 1, sfk::kKvExact, 4);
+            else SF_KV4_TOKEN(128, 2, true);
         }
-    } else if (d->cache.D == 64) {
-        if (k.qt == 2 && pair) SF_KV4_LAUNCH(64, 2, true, 8);
-        else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, false, 8);
-        else if (k.qt == 3 && pair) SF_KV4_LAUNCH(64, 3, true, 8);
-        else if (k.qt == 3) SF_KV4_LAUNCH(64, 3, false, 8);
-        else if (k.qt == 4 && pair) SF_KV4_LAUNCH(64, 4, true, 8);
-        else if (k.qt == 4) SF_KV4_LAUNCH(64, 4, false, 8);
-        else SF_KV4_LAUNCH(64, 5, false, 8);
+    } else if (k.qt == 1) {
+        if (d->cache.D == 64) {
+            if (k.ng == 1) SF_KV4_LAUNCH(64, 1, sfk::kKvPair, 4);
+            else if (k.ng == 2) SF_KV4_TOKEN(64, 2, false);
+            else SF_KV4_TOKEN(64, 4, false);
+        } else {
+            if (k.ng == 1) SF_KV4_LAUNCH(128, 1, sfk::kKvPair, 4);
+            else SF_KV4_TOKEN(128, 2, false);
+        }
+    } else if (d->cache.D == 128) {
+        if (form == sfk::kKvExact) SF_KV4_LAUNCH(128, 2, sfk::kKvExact, 8);
+        else if (form == sfk::kKvPair) SF_KV4_LAUNCH(128, 2, sfk::kKvPair, 8);
+        else SF_KV4_LAUNCH(128, 2, sfk::kKvHalf, 8);
+    } else if (form == sfk::kKvExact) {
+        if (k.qt == 2) SF_KV4_LAUNCH(64, 2, sfk::kKvExact, 8);
+        else SF_KV4_LAUNCH(64, 3, sfk::kKvExact, 8);
+    } else if (form == sfk::kKvPair) {
+        if (k.qt == 2) SF_KV4_LAUNCH(64, 2, sfk::kKvPair, 8);
+        else if (k.qt == 3) SF_KV4_LAUNCH(64, 3, sfk::kKvPair, 8);
+        else SF_KV4_LAUNCH(64, 4, sfk::kKvPair, 8);
     } else {
-        if (pair) SF_KV4_LAUNCH(128, 2, true, 8);
-        else SF_KV4_LAUNCH(128, 2, false, 8);
+        if (k.qt == 2) SF_KV4_LAUNCH(64, 2, sfk::kKvHalf, 8);
+        else if (k.qt == 3) SF_KV4_LAUNCH(64, 3, sfk::kKvHalf, 8);
+        else if (k.qt == 4) SF_KV4_LAUNCH(64, 4, sfk::kKvHalf, 8);
+        else SF_KV4_LAUNCH(64, 5, sfk::kKvHalf, 8);
     }
 #undef SF_KV4_TOKEN
 #undef SF_KV4_LAUNCH

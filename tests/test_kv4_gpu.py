@@ -549,3 +549,23 @@ def test_two_tokens_at_one_slot():
     keep = torch.arange(64) != 20
     for got in c.read(dtype=F32):
         assert torch.equal(got.cpu()[:, :, keep], _levels(want).float()[:, :, keep])
+
+
+@pytest.mark.parametrize("B,Hq,H,Sq,Sk,D", [(2, 8, 2, 1, 300, 128), (1, 2, 1, 40, 5000, 64), (1, 4, 2, 20, 5000, 128),
+                                            (4, 32, 32, 1, 4096, 64), (2, 64, 64, 6, 4096, 128), (1, 8, 8, 16, 8192, 128)])
+def test_fp32_outputs_are_near(B, Hq, H, Sq, Sk, D):
+    """Within 1e-6 of the output's norm, over values whose mean is small beside them.  The reference runs on the
+    device, in 64 bits."""
+    k, v = _randn(170, B, H, Sk, D, dtype=BF).to(DEV), _randn(171, B, H, Sk, D, dtype=BF).to(DEV)
+    c = Kv4Cache(B, H, Sk, D, DEV)
+    c.write(k, v)
+    q = _randn(172, B, Hq, Sq, D, dtype=BF).to(DEV)
+    got = attention_kv4(q, c, out_dtype=F32)
+    off = norm = 0.0
+    for b in range(B):
+        kk, vv = (kv4_levels(t[b]).repeat_interleave(Hq // H, 0) for t in (k, v))
+        w = torch.softmax(torch.matmul(q[b].double(), kk.transpose(1, 2).contiguous()) / math.sqrt(D), -1)
+        ref = torch.matmul(w, vv)
+        off += float((got[b].double() - ref).square().sum())
+        norm += float(ref.square().sum())
+    assert math.sqrt(off / norm) <= 1e-6
