@@ -600,7 +600,7 @@ int32_t sf_gemm_frag_ss_tiles(const sf_frag_gemm_desc* desc);
  * weight-only int8 (quantization.cu:18-51 ahead of gemm_bias_act,
  * cuda_backend.cu:337-467), which has no 4-bit form.  Codes are 0..15, group
  * 32, 64 or 128 inputs, K a multiple of the group, any N to 2^25, any M to
- * 2^21, lda to 2^24 (SF_ENOTSUP above).
+ * 2^21, lda to 2^23 (SF_ENOTSUP above).
  *
  * sf_w4_pack lays a checkpoint's codes and scales out once, in the order the
  * matrix operands are read; sf_gemm_w4 reads that.

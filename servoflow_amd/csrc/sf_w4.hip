@@ -100,7 +100,7 @@ __global__ __launch_bounds__(512) void gemm_w4_kernel(const W4Args p) {
     const int r = lane & 15, g = lane >> 4;
     const int wk = wave / WN, wn = wave % WN;
     const int nb0 = (blockIdx.x * WN + wn) * NT, m0 = blockIdx.y * 16 * MB, rows = min(16 * MB, p.M - m0);
-    const uint32_t ld = 2u * (uint32_t)p.lda;   // bytes: lda is at most 2^24
+    const uint32_t ld = 2u * (uint32_t)p.lda;   // bytes: lda is at most 2^23
     const __amdgpu_buffer_rsrc_t ars = make_rsrc(p.a + (int64_t)m0 * p.lda, (uint32_t)rows * ld);
     char* stage = lds + wk * WN * kStage;   // WN of them, in turn
     // Instruction i brings rows 4 i .. 4 i + 3, 256 bytes each, piece c of row q to place c ^ (q & 15); rows behind M are
@@ -338,7 +338,7 @@ extern "C" int sf_gemm_w4(const sf_gemm_w4_desc* desc, void* stream) {
     if (desc->act < SF_ACT_NONE || desc->act > SF_ACT_SILU) return SF_ENOTSUP;
     if (desc->accumulate && desc->c_dtype != SF_F32) return SF_ENOTSUP;
     // the grid's second dimension; a launch counts its threads in 32 bits; a workgroup's rows are addressed in 32 bits
-    if (desc->M > 1 << 21 || desc->N > 1 << 25 || desc->lda > 1 << 24) return SF_ENOTSUP;
+    if (desc->M > 1 << 21 || desc->N > 1 << 25 || desc->lda > 1 << 23) return SF_ENOTSUP;
     sfk::W4Args p = {};
     p.a = static_cast<const uint16_t*>(desc->A);
     p.lda = desc->lda;

@@ -187,7 +187,7 @@ def test_attn_kv4_refusals():
 
 
 def test_sizes_beyond_a_launch_are_refused():
-    for kw in ({"lda": (1 << 24) + 8}, {"N": (1 << 25) + 1, "ldc": 1 << 26}, {"M": (1 << 21) + 1}):
+    for kw in ({"lda": (1 << 23) + 8}, {"N": (1 << 25) + 1, "ldc": 1 << 26}, {"M": (1 << 21) + 1}):
         assert _gemm(**kw) == abi.SF_ENOTSUP, kw
     assert _pack(N=1 << 25, K=2048, ldc=1024, lds=64, zeros=None) == abi.SF_ENOTSUP
     assert _rope(B=1 << 12, S=1 << 11) == abi.SF_ENOTSUP

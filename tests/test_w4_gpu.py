@@ -113,6 +113,17 @@ def test_accumulate_and_strides():
     assert torch.equal(c[:, 0], was[:, 0]) and torch.equal(c[:, 1 + N:], was[:, 1 + N:])
 
 
+@pytest.mark.parametrize("N", [48, 6150])
+def test_rows_far_apart(N):
+    """The widest row stride: a workgroup's rows span 1.3 GB."""
+    M, K, ld = 83, 320, 1 << 23
+    a, w, ref_w, big = _case(M, N, K, 64, BF, True, 7)
+    wide = torch.empty(M, ld, dtype=BF, device=DEV)
+    wide[:, K:K + 64] = float("nan")
+    wide[:, :K] = a.to(DEV)
+    _check(kernels.gemm_w4(wide[:, :K], w, out_dtype=F32), a.double() @ ref_w.t(), big, K, F32)
+
+
 def test_rows_are_independent_of_a_bad_one():
     a, w, ref_w, big = _case(20, 32, 128, 32, BF, True)
     a[7, 5], a[18, 3] = float("nan"), float("inf")
