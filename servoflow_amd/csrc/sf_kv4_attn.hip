@@ -7,7 +7,8 @@
 //   O_d = sum_j p_j s_j (16 + c_jd) - 23.5 sum_j p_j s_j + sum_j p_j mid_j
 // (16 + c: see sf_nibble.h).  p_j s_j enters the matrix unit as a bf16 (hi, lo)
 // pair, 2^-18 relative, and its sum is taken over the same rounded pair, so that
-// what the codes' offset adds is taken away exactly.  With many query rows to an
+// what the codes' offset adds is taken away exactly; for fp32 outputs it enters as
+// three terms.  With many query rows to an
 // unpacked block and a bf16 output the values are formed in fp16 instead, once
 // for all rows, and p enters as one fp16: five vector operations fewer for every
 // score, and errors of 2^-12 where the output's own rounding is 2^-9.
