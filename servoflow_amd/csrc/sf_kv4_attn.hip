@@ -104,6 +104,13 @@ __device__ __forceinline__ float kv_dot(uint32_t pair, float acc) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v, pair), bf16x2v{(__bf16)-23.5f, (__bf16)-23.5f}, acc, false);
 }
 
+// The exponent, offset by 127 as in fp32, of the larger of 2^18 s and |mid| of a parameter dword (0: a NaN, or nothing
+// above the subnormals).
+__device__ __forceinline__ uint32_t kv_size(uint32_t par) {
+    const uint32_t s = par >> 7 & 0xffu, mid = par >> 23 & 0xffu;
+    return s == 0xffu ? 0u : max(s ? s + 18u : 0u, mid);
+}
+
 // A matrix operand of -23.5.
 __device__ __forceinline__ u32x4 kv_offset() { return u32x4{0xC1BCC1BCu, 0xC1BCC1BCu, 0xC1BCC1BCu, 0xC1BCC1BCu}; }
 
@@ -333,11 +340,17 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) big = fmaxf(fmaxf(big, vs[i][e]), fabsf(vm[i][e]));
             if (__any(big > vcap)) {   // a new power: this block's largest to 2^12 .. 2^13
+                // From the parameters themselves: times the old power they may have passed fp32's range.
+                uint32_t top = 0;
 #pragma unroll
-                for (int w = 1; w < 64; w <<= 1) big = fmaxf(big, __shfl_xor(big, w, 64));
+                for (int i = 0; i < GR; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (!masked || (see >> e & 1u)) top = max(top, kv_size(nx.vp[i][e >> 2][e & 3]));
+#pragma unroll
+                for (int w = 16; w < 64; w <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, w, 64));   // a group's 16 lanes hold the same
                 const int now = (int)(__float_as_uint(vdown) >> 23) - 127;
-                const int want = big > 0.f ? now + 12 + 127 - (int)(__float_as_uint(big) >> 23) : now;
-                const int ex = __builtin_amdgcn_readfirstlane(min(max(want, -126), 100));
+                const int ex = __builtin_amdgcn_readfirstlane(min(max(127 + 12 - (int)top, -126), 100));
                 const float al = __builtin_amdgcn_ldexpf(1.f, ex - now);
                 vdown = __uint_as_float((uint32_t)(127 + ex) << 23);
                 vcap = 32768.f;
@@ -348,7 +361,12 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 #pragma unroll
                 for (int i = 0; i < GR; ++i)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) vs[i][e] *= al, vm[i][e] *= al;
+                    for (int e = 0; e < 8; ++e) {
+                        uint32_t vp = nx.vp[i][e >> 2][e & 3];
+                        if (masked && (!(see >> e & 1u) || (vp & 0x7f80u) == 0x7f80u)) vp = 0u;
+                        vs[i][e] = kv_mix(vp, 262144.f * vdown, 0.f);
+                        vm[i][e] = kv_mix(vp, -7.5f * vdown, vdown);
+                    }
             }
         }
 #pragma unroll

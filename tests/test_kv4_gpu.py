@@ -569,3 +569,36 @@ def test_fp32_outputs_are_near(B, Hq, H, Sq, Sk, D):
         off += float((got[b].double() - ref).square().sum())
         norm += float(ref.square().sum())
     assert math.sqrt(off / norm) <= 1e-6
+
+
+def _near_the_largest(got, q, lk, lv, what="", causal=False, **kw):
+    """A bf16 output of many rows: 7 2^-12 of the largest value that a row sees, and its own rounding.
+
+    To the first order: p, its sum taken over the rounded p, and the value rounds by 2^-11 each, as does mid - 7.5 s
+    (at most the largest value; s itself is exact), which comes to 5.2 2^-12 where they add up worst; values far
+    below the largest, and weights, stand on fp16's last step, 0.5 and 1 2^-12 more (4096 keys of a wave)."""
+    ref = attend(q, lk, lv, causal=causal, **kw)
+    G, Sq, Sk = q.shape[1] // lk.shape[1], q.shape[2], lk.shape[2]
+    top = lv.abs().amax(-1).repeat_interleave(G, 1)[:, :, None].expand(-1, -1, Sq, -1)
+    if causal:
+        seen = torch.arange(Sk) <= torch.arange(Sq)[:, None] + Sk - Sq
+        top = torch.where(seen, top, 0.0)
+    tol = 7 * 2.0 ** -12 * top.amax(-1, keepdim=True) + half_step(BF) * ref.abs()
+    err = (got.cpu().double() - ref).abs()
+    assert torch.isfinite(got).all(), what
+    assert (err <= tol).all(), f"{what}: {float((err / tol.clamp_min(1e-300)).max())} of the tolerance"
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("first,then", [(-60, 60), (-100, 30), (-100, 100), (-126, 0), (60, -60)])
+def test_values_that_grow_along_the_keys(D, first, then):
+    """Every wave's first block of keys holds values by a factor 2^(then - first) away from its later ones'."""
+    H, Sk = 2, 600
+    k, v = _randn(180, 1, H, Sk, D, dtype=BF), _randn(181, 1, H, Sk, D)
+    v[:, :, :256] *= 2.0 ** first
+    v[:, :, 256:] *= 2.0 ** then
+    c = Kv4Cache(1, H, Sk, D, DEV)
+    c.write(k.to(DEV), v.to(BF).to(DEV))
+    q = _randn(182, 1, H, 40, D, dtype=BF)
+    got = attention_kv4(q.to(DEV), c, num_splits=1)
+    _near_the_largest(got, q, kv4_levels(k), kv4_levels(v.to(BF)))
