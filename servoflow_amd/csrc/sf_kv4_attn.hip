@@ -312,6 +312,9 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 if (key < len && (!p.mask || p.mask[b * p.mask_stride + key])) see |= 1u << e;
             }
         }
+        // Masked, fp16 values: the lane's tokens of a NaN group of values, 8 bits a group of channels.  They are taken as
+        // zeros, as 0 times NaN would reach the rows that do not see them; the others' sums are marked tile by tile.
+        uint32_t nan = 0;
         float ks[GR][8], ko[GR][8], vs[GR][8], vm[GR][8];
 #pragma unroll
         for (int i = 0; i < GR; ++i)
@@ -319,8 +322,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
             for (int e = 0; e < 8; ++e) {
                 uint32_t kp = nx.kp[i][e >> 2][e & 3], vp = nx.vp[i][e >> 2][e & 3];
                 if (masked && !(see >> e & 1u)) kp = vp = 0u;   // tokens behind the last hold anything
-                // A NaN value reaches the rows that see it through their scores: 0 times NaN would reach the others too.
-                if (masked && !PAIR && (vp & 0x7f80u) == 0x7f80u) kp |= 0x7fc07fc0u, vp = 0u;
+                if (masked && !PAIR && (vp & 0x7f80u) == 0x7f80u) nan |= 1u << (8 * i + e), vp = 0u;
                 ks[i][e] = __uint_as_float(kp << 16) * p.scale_log2;
                 ko[i][e] = EXACT ? __uint_as_float(kp & 0xffff0000u) : kv_mix(kp, -23.5f, 1.f);
                 vs[i][e] = PAIR ? __uint_as_float(vp << 16) : kv_mix(vp, 262144.f * vdown, 0.f);
@@ -446,6 +448,18 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 for (int i = 0; i < DT; ++i) o[t][i] *= al;
             }
             if (t + 1 < QT) scores(t + 1);
+            if (masked && !PAIR && __any(nan != 0)) {
+#pragma unroll
+                for (int i = 0; i < GR; ++i) {
+                    uint32_t mark = nan >> (8 * i) & row ? 0x7fc00000u : 0u;
+                    mark |= (uint32_t)__shfl_xor((int)mark, 16, 64);
+                    mark |= (uint32_t)__shfl_xor((int)mark, 32, 64);
+#pragma unroll
+                    for (int d = 4 * i; d < 4 * i + 4; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[t][d][e] = __uint_as_float(__float_as_uint(o[t][d][e]) | mark);
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(x[e]);
             if (PAIR) {

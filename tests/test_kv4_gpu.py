@@ -602,3 +602,33 @@ def test_values_that_grow_along_the_keys(D, first, then):
     q = _randn(182, 1, H, 40, D, dtype=BF)
     got = attention_kv4(q.to(DEV), c, num_splits=1)
     _near_the_largest(got, q, kv4_levels(k), kv4_levels(v.to(BF)))
+
+
+@pytest.mark.parametrize("kind", ["causal", "mask", "plain"])
+@pytest.mark.parametrize("bad", [5, 100])
+@pytest.mark.parametrize("out_dtype", [BF, FP, F32])
+def test_bad_values_stay_in_their_channels(kind, bad, out_dtype):
+    """An infinity among the values of a token: its 64 channels are NaN in the rows that see it, the others right."""
+    H, Sk, D = 2, 75, 128
+    _, k, v = _filled(1, H, Sk, D, BF, 183)
+    c, _, _ = _filled(1, H, Sk, D, BF, 183)
+    one = _randn(184, 1, H, 1, D, dtype=BF)
+    spoilt = one.clone()
+    spoilt[0, 0, 0, bad] = float("inf")
+    c.write(one.to(DEV), spoilt.to(DEV), torch.tensor([[30]], dtype=torch.int32, device=DEV))
+    k[:, :, 30:31] = v[:, :, 30:31] = kv4_levels(one)
+    q = _randn(185, 1, H, Sk, D, dtype=BF)
+    mask = None
+    if kind == "mask":
+        mask = torch.ones(1, Sk, dtype=torch.bool)
+        mask[0, 3] = False
+    got = attention_kv4(q.to(DEV), c, is_causal=kind == "causal", kv_mask=None if mask is None else mask.to(DEV),
+                        out_dtype=out_dtype)
+    sees = torch.arange(Sk) >= (30 if kind == "causal" else 0)
+    part = slice(0, 64) if bad < 64 else slice(64, 128)
+    assert torch.isnan(got[0, 0, sees, part]).all()
+    got = got.cpu()
+    # what is NaN for certain is given the right value, so that all the rest is compared
+    ref = attend(q, k, v, causal=kind == "causal", mask=mask)
+    got[0, 0, sees, part] = ref[0, 0, sees, part].to(got.dtype)
+    _attn_check(got, q, k, v, out_dtype, causal=kind == "causal", mask=mask)
