@@ -39,7 +39,13 @@ constexpr int kKvMaxSplits = 64;
 constexpr float kKvSlack = 8.f;       // log2
 constexpr float kKvNoMax = -1.5e38f;  // the maximum of a row that has seen nothing
 
-// How p and V meet.  kKvHalf (bf16 outputs of many rows): both in fp16.  kKvPair
+// How p and V meet.  kKvHalf (bf16 outputs of many rows that see the same tokens):
+// both in fp16.  Not for causal rows: what later rows alone see would set the power
+// under which an earlier row's values are rounded, and a NaN among it, as V, would
+// reach rows whose weight for it is 0.  (us with the pair, and with fp16 when the
+// blocks that some rows see a part of are taken in steps of values of like size: 64
+// channels, 8 heads of 4 x 256 rows over 2048 keys, twice, 18.5 and 17.5, of 4 x 4096
+// over 4096 193 and 168; 128 channels, the first of these 30.5 and 34.8.)  kKvPair
 // (other 16-bit outputs): p s as a bf16 (hi, lo) pair with the codes, whose offset
 // the pairs' sums take away at the end.  kKvExact (fp32 outputs): three terms
 // instead of two, and the offset, which is many times a mean of values and would
@@ -218,7 +224,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     const int len = p.valid ? min(max(p.valid[b], 0), p.Sk) : p.Sk;
     // Query s sees keys below len - Sq + s + 1 (causal) or len; the smallest and largest limit of the group's rows.
     int lim_lo = len, lim_hi = len;
-    if (p.causal) {
+    if (PAIR && p.causal) {
         const int q1 = min(q0 + 16 * QT, R) - 1;
         const bool one = q0 / p.Sq == q1 / p.Sq;
         lim_lo = len - p.Sq + 1 + (one ? q0 % p.Sq : 0);
@@ -312,9 +318,6 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 if (key < len && (!p.mask || p.mask[b * p.mask_stride + key])) see |= 1u << e;
             }
         }
-        // Masked, fp16 values: the lane's tokens of a NaN group of values, 8 bits a group of channels.  They are taken as
-        // zeros, as 0 times NaN would reach the rows that do not see them; the others' sums are marked tile by tile.
-        uint32_t nan = 0;
         float ks[GR][8], ko[GR][8], vs[GR][8], vm[GR][8];
 #pragma unroll
         for (int i = 0; i < GR; ++i)
@@ -322,7 +325,6 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
             for (int e = 0; e < 8; ++e) {
                 uint32_t kp = nx.kp[i][e >> 2][e & 3], vp = nx.vp[i][e >> 2][e & 3];
                 if (masked && !(see >> e & 1u)) kp = vp = 0u;   // tokens behind the last hold anything
-                if (masked && !PAIR && (vp & 0x7f80u) == 0x7f80u) nan |= 1u << (8 * i + e), vp = 0u;
                 ks[i][e] = __uint_as_float(kp << 16) * p.scale_log2;
                 ko[i][e] = EXACT ? __uint_as_float(kp & 0xffff0000u) : kv_mix(kp, -23.5f, 1.f);
                 vs[i][e] = PAIR ? __uint_as_float(vp << 16) : kv_mix(vp, 262144.f * vdown, 0.f);
@@ -365,7 +367,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         uint32_t vp = nx.vp[i][e >> 2][e & 3];
-                        if (masked && (!(see >> e & 1u) || (vp & 0x7f80u) == 0x7f80u)) vp = 0u;
+                        if (masked && !(see >> e & 1u)) vp = 0u;
                         vs[i][e] = kv_mix(vp, 262144.f * vdown, 0.f);
                         vm[i][e] = kv_mix(vp, -7.5f * vdown, vdown);
                     }
@@ -431,7 +433,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 }
             uint32_t row = see;
             if (masked) {
-                const int limit = p.causal ? len - p.Sq + 1 + min(q0 + 16 * t + col, R - 1) % p.Sq : len;
+                const int limit = PAIR && p.causal ? len - p.Sq + 1 + min(q0 + 16 * t + col, R - 1) % p.Sq : len;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) >= limit) row &= ~(1u << e);
@@ -448,18 +450,6 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 for (int i = 0; i < DT; ++i) o[t][i] *= al;
             }
             if (t + 1 < QT) scores(t + 1);
-            if (masked && !PAIR && __any(nan != 0)) {
-#pragma unroll
-                for (int i = 0; i < GR; ++i) {
-                    uint32_t mark = nan >> (8 * i) & row ? 0x7fc00000u : 0u;
-                    mark |= (uint32_t)__shfl_xor((int)mark, 16, 64);
-                    mark |= (uint32_t)__shfl_xor((int)mark, 32, 64);
-#pragma unroll
-                    for (int d = 4 * i; d < 4 * i + 4; ++d)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[t][d][e] = __uint_as_float(__float_as_uint(o[t][d][e]) | mark);
-                }
-            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(x[e]);
             if (PAIR) {
@@ -884,7 +874,7 @@ struct KvPlan {
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 static inline int kv_form(const sf_attn_kv4_desc* d) {   // with more than one tile of rows
-    return d->out_dtype == SF_F32 ? kKvExact : d->out_dtype == SF_F16 ? kKvPair : kKvHalf;
+    return d->out_dtype == SF_F32 ? kKvExact : d->out_dtype == SF_F16 || d->is_causal ? kKvPair : kKvHalf;
 }
 
 // Up to 16 rows to a key head: one tile, four waves to a workgroup.  Up to 512

@@ -632,3 +632,24 @@ def test_bad_values_stay_in_their_channels(kind, bad, out_dtype):
     ref = attend(q, k, v, causal=kind == "causal", mask=mask)
     got[0, 0, sees, part] = ref[0, 0, sees, part].to(got.dtype)
     _attn_check(got, q, k, v, out_dtype, causal=kind == "causal", mask=mask)
+
+
+@pytest.mark.parametrize("D,Hq,H,Sq", [(64, 2, 1, 96), (64, 2, 2, 96), (128, 2, 1, 96), (128, 1, 1, 33), (64, 8, 1, 20)])
+@pytest.mark.parametrize("up", [8, 16, 20, 60, -20])
+def test_rows_do_not_feel_later_values(D, Hq, H, Sq, up):
+    """Causal rows with a bf16 output: tokens 2^up as large behind a row leave its accuracy as it is."""
+    Sk = 128
+    k, v = _randn(186, 1, H, Sk, D, dtype=BF), _randn(187, 1, H, Sk, D)
+    for at in (Sk - Sq + 7, Sk - Sq + 15, Sk - 5):   # several in one block, one in the last
+        v[:, :, at] *= 2.0 ** up
+    v = v.to(BF)
+    v[:, :, Sk - 3] = 0
+    c = Kv4Cache(1, H, Sk, D, DEV)
+    c.write(k.to(DEV), v.to(DEV))
+    q = _randn(188, 1, Hq, Sq, D, dtype=BF)
+    lk, lv = kv4_levels(k), kv4_levels(v)
+    _near_the_largest(attention_kv4(q.to(DEV), c, is_causal=True), q, lk, lv, causal=True)
+    mask = torch.rand(1, Sk, generator=torch.Generator().manual_seed(6)) < 0.8
+    mask[0, 0] = True
+    _near_the_largest(attention_kv4(q.to(DEV), c, is_causal=True, kv_mask=mask.to(DEV), num_splits=2), q, lk,
+                      torch.where(mask[:, None, :, None], lv, 0.0), causal=True, mask=mask)
