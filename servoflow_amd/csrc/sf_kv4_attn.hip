@@ -37,12 +37,15 @@ namespace sfk {
 
 constexpr int kKvMaxSplits = 64;
 constexpr float kKvSlack = 8.f;       // log2
+constexpr int kKvHalfKeys = 4096;     // of a wave, with weights in fp16
 constexpr float kKvNoMax = -1.5e38f;  // the maximum of a row that has seen nothing
 
 // How p and V meet.  kKvHalf (bf16 outputs of many rows that see the same tokens):
 // both in fp16.  Not for causal rows: what later rows alone see would set the power
 // under which an earlier row's values are rounded, and a NaN among it, as V, would
-// reach rows whose weight for it is 0.  (us with the pair, and with fp16 when the
+// reach rows whose weight for it is 0.  Nor for more than 4096 keys of a wave: a
+// weight below 2^-14 of the wave's largest is held to 2^-25 only, one below 2^-25 not
+// at all, which N keys make N 2^-24 of the largest value (2^-12 for 4096).  (us with the pair, and with fp16 when the
 // blocks that some rows see a part of are taken in steps of values of like size: 64
 // channels, 8 heads of 4 x 256 rows over 2048 keys, twice, 18.5 and 17.5, of 4 x 4096
 // over 4096 193 and 168; 128 channels, the first of these 30.5 and 34.8.)  kKvPair
@@ -867,7 +870,7 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(const KvAttnArgs p)
 // How a call is cut up: tiles of 16 query rows to a workgroup (qt), groups of
 // them (qgroups), key splits.
 struct KvPlan {
-    int qt, ng, qgroups, splits;
+    int qt, ng, qgroups, splits, form;
     int64_t wgs, rows;
 };
 
@@ -911,35 +914,44 @@ static int kv_column_groups(const sf_attn_kv4_desc* d, int rows, int64_t heads) 
 // 19.6 with 5 and eight, 31 with 3 and one (19, 20, 30); 256 x 67 x 4374 42 with
 // qt 5.  The (hi, lo) form takes 0.42 us a step, and qt 5 would spill,
 // with three terms qt 4.  128 channels: 2 tiles are what fits.
+static void kv_tiles(const sf_attn_kv4_desc* d, int64_t R, int64_t heads, KvPlan& k) {
+    const bool wide = d->cache.D == 128;
+    const int most = wide ? 2 : k.form == kKvExact ? 3 : k.form == kKvPair ? 4 : 5;
+    const int64_t per_block = kKvBlock * 8;   // a block to each wave
+    const double step = k.form == kKvHalf ? 0.3 : 0.42;
+    double best = 0.;
+    for (int qt = 2; qt <= most; ++qt) {
+        const int64_t groups = ceil_div(R, 16 * qt), base = heads * groups;
+        const int64_t fill = std::min<int64_t>(base < 256 ? 256 / base : 1, kKvMaxSplits);
+        for (int64_t s = 1; s <= fill; s += fill > 1 ? fill - 1 : 1) {
+            const int64_t splits = d->num_splits > 0 ? d->num_splits : std::min(s, std::max<int64_t>(1, ceil_div(d->Sk, per_block)));
+            const double us = (double)ceil_div(base * splits, 256) *
+                                  ((double)ceil_div(d->Sk, per_block * splits) * step * (1.5 + qt) + 3. + 0.8 * qt) +
+                              (splits > 1 ? 7. : 0.);
+            if (best == 0. || us < best) {
+                best = us;
+                k.qt = qt;
+                k.qgroups = (int)groups;
+                k.splits = (int)splits;
+            }
+        }
+    }
+}
+
 static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
     KvPlan k = {};
     const int64_t R = (int64_t)(d->Hq / d->cache.H) * d->Sq, heads = (int64_t)d->B * d->cache.H;
     k.rows = (int64_t)d->B * d->Hq * d->Sq;
+    k.form = kv_form(d);
     if (R <= 16) {
         k.qt = k.qgroups = 1;
         k.splits = d->num_splits > 0 ? d->num_splits : kv_splits_one_tile(d, heads);
         k.ng = kv_column_groups(d, (int)R, heads);
     } else {
-        const bool wide = d->cache.D == 128;
-        const int form = kv_form(d), most = wide ? 2 : form == kKvExact ? 3 : form == kKvPair ? 4 : 5;
-        const int64_t per_block = kKvBlock * 8;   // a block to each wave
-        const double step = form == kKvHalf ? 0.3 : 0.42;
-        double best = 0.;
-        for (int qt = 2; qt <= most; ++qt) {
-            const int64_t groups = ceil_div(R, 16 * qt), base = heads * groups;
-            const int64_t fill = std::min<int64_t>(base < 256 ? 256 / base : 1, kKvMaxSplits);
-            for (int64_t s = 1; s <= fill; s += fill > 1 ? fill - 1 : 1) {
-                const int64_t splits = d->num_splits > 0 ? d->num_splits : std::min(s, std::max<int64_t>(1, ceil_div(d->Sk, per_block)));
-                const double us = (double)ceil_div(base * splits, 256) *
-                                      ((double)ceil_div(d->Sk, per_block * splits) * step * (1.5 + qt) + 3. + 0.8 * qt) +
-                                  (splits > 1 ? 7. : 0.);
-                if (k.qt == 0 || us < best) {
-                    best = us;
-                    k.qt = qt;
-                    k.qgroups = (int)groups;
-                    k.splits = (int)splits;
-                }
-            }
+        kv_tiles(d, R, heads, k);
+        if (k.form == kKvHalf && ceil_div(d->Sk, 8 * k.splits) > kKvHalfKeys) {
+            k.form = kKvPair;
+            kv_tiles(d, R, heads, k);
         }
     }
     k.wgs = heads * k.qgroups * k.splits;
@@ -1017,7 +1029,7 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
         if (f16) hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<true, DD, NG, EXACT>), grid, dim3(256), 0, s, p);             \
         else hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<false, DD, NG, EXACT>), grid, dim3(256), 0, s, p);                \
     } while (0)
-    const int form = sfk::kv_form(d);
+    const int form = k.form;
     if (k.qt == 1 && form == sfk::kKvExact) {
         if (d->cache.D == 64) {
             if (k.ng == 1) SF_KV4_LAUNCH(64, 1, sfk::kKvExact, 4);

@@ -653,3 +653,24 @@ def test_rows_do_not_feel_later_values(D, Hq, H, Sq, up):
     mask[0, 0] = True
     _near_the_largest(attention_kv4(q.to(DEV), c, is_causal=True, kv_mask=mask.to(DEV), num_splits=2), q, lk,
                       torch.where(mask[:, None, :, None], lv, 0.0), causal=True, mask=mask)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_strong_key_before_a_million(D):
+    """A million keys of 2^-25.2 of the first one's weight each, 1/38 of it together: no wave may round its own away.
+    Keys and values are constants, which the cache holds exactly."""
+    Sk, R = 1 << 20, 20
+    c = Kv4Cache(1, 1, Sk, D, DEV)
+    k = torch.zeros(1, 1, Sk, D, dtype=BF, device=DEV)
+    v = torch.ones(1, 1, Sk, D, dtype=BF, device=DEV)
+    k[:, :, 0] = 2.1875 * 8 / math.sqrt(D)
+    v[:, :, 0] = -1 / 32
+    c.write(k, v)
+    q = torch.ones(1, 1, R, D, dtype=BF, device=DEV)
+    x = float(k[0, 0, 0].double().sum()) / math.sqrt(D)
+    assert 2.0 ** -25.5 < math.exp(-x) < 2.0 ** -25.05
+    w = (Sk - 1) * math.exp(-x)
+    ref = (w - 1 / 32) / (w + 1)
+    for splits in (0, 1, 3):
+        got = attention_kv4(q, c, num_splits=splits).double()
+        assert ((got - ref).abs() <= 7 * 2.0 ** -12 + half_step(BF) * abs(ref)).all(), splits
