@@ -734,7 +734,7 @@ int sf_kv4_read(const sf_kv4_cache* cache, const int32_t* slots, int32_t S, void
  * The softmax's maximum and sum are fp32; its weights enter the product with V
  * as bf16 (hi, lo) pairs, 2^-18 relative, and for an fp32 output as three bf16
  * terms, which leaves it within 1e-6 of its norm up to 16384 keys (as sums over
- * fp32 values).  Without is_causal, with more than 16 query rows to a key head, at
+ * fp32 values).  Unless exact_pv is set, without is_causal, with more than 16 query rows to a key head, at
  * most 2^15 keys to a split and a bf16 output, weights and values enter as fp16,
  * the values under a power of two that keeps them in its range: 7 2^-12 of the
  * largest value that the row sees, beside the output's own rounding (6e-4 of the
@@ -748,6 +748,7 @@ typedef struct sf_attn_kv4_desc {
     int32_t in_dtype, out_dtype;
     int32_t is_causal;
     int32_t num_splits;
+    int32_t exact_pv;      /* weights as bf16 pairs, values as cached, for bf16 outputs of many rows too */
     const int32_t* kv_valid_len;
     const uint8_t* kv_mask;
     int64_t kv_mask_stride;

@@ -217,7 +217,7 @@ class AttnKv4Desc(ctypes.Structure):
     _fields_ = [("B", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Sq", ctypes.c_int32), ("Sk", ctypes.c_int32),
                 ("scale", ctypes.c_float),
                 ("in_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
-                ("is_causal", ctypes.c_int32), ("num_splits", ctypes.c_int32),
+                ("is_causal", ctypes.c_int32), ("num_splits", ctypes.c_int32), ("exact_pv", ctypes.c_int32),
                 ("kv_valid_len", ctypes.c_void_p), ("kv_mask", ctypes.c_void_p), ("kv_mask_stride", ctypes.c_int64),
                 ("q_stride", ctypes.c_int64 * 3), ("o_stride", ctypes.c_int64 * 3),
                 ("cache", Kv4CacheDesc)]

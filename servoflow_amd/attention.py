@@ -144,18 +144,20 @@ class Kv4Cache:
 
 
 # sf_attn_kv4_desc in one pack.
-_KV4_DESC = struct.Struct("@4if4i4x2Pq3q3qP4i")
+_KV4_DESC = struct.Struct("@4if5i2Pq3q3qP4i")
 assert _KV4_DESC.size == ctypes.sizeof(abi.AttnKv4Desc)
 
 
 def attention_kv4(q, cache, out=None, scale=0.0, is_causal=False, valid_len=None, kv_mask=None, keys=None,
-                  num_splits=0, out_dtype=None, workspace=None):
+                  num_splits=0, out_dtype=None, workspace=None, exact_pv=False):
     """softmax(q K^T scale) V over a Kv4Cache: q [B, Hq, Sq, D] bf16 or fp16
     (any strides with a contiguous last axis), Hq a multiple of the cache's H.
     keys: how many slots are read at most (the capacity); valid_len: device
     int32 [B] lengths; kv_mask: device bool [B, keys] (True = attend);
-    is_causal: query s is the token at valid_len - Sq + s.  Runs on torch's
-    current stream; a row that sees nothing is zeros."""
+    is_causal: query s is the token at valid_len - Sq + s.  exact_pv: weights
+    as bf16 (hi, lo) pairs also where a bf16 output of many rows takes weights
+    and values in fp16 (6e-4 of the output's norm; sf_attn_kv4_desc).  Runs on
+    torch's current stream; a row that sees nothing is zeros."""
     dev, shape = cache.data.device, q.shape
     if len(shape) != 4 or shape[0] != cache.B or shape[3] != cache.D or shape[1] % cache.H:
         raise ValueError(f"q{tuple(shape)} over a cache of B {cache.B}, H {cache.H}, D {cache.D}")
@@ -180,7 +182,7 @@ def attention_kv4(q, cache, out=None, scale=0.0, is_causal=False, valid_len=None
             raise ValueError(f"kv_mask must be a device bool/uint8 tensor [{B}, {Sk}] with contiguous rows")
         mask_ptr, mask_st = kv_mask.data_ptr(), kv_mask.stride(0) if B > 1 else 0
     raw = _KV4_DESC.pack(B, Hq, Sq, Sk, scale, _DT[q.dtype], _DT[out.dtype], 1 if is_causal else 0, int(num_splits),
-                         valid_ptr, mask_ptr, mask_st, *kernels.strides_bhs(q), *kernels.strides_bhs(out),
+                         1 if exact_pv else 0, valid_ptr, mask_ptr, mask_st, *kernels.strides_bhs(q), *kernels.strides_bhs(out),
                          *cache.fields())
     d = ctypes.byref(abi.AttnKv4Desc.from_buffer_copy(raw))
     ws, n = None, 0

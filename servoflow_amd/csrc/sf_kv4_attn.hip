@@ -877,7 +877,7 @@ struct KvPlan {
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 static inline int kv_form(const sf_attn_kv4_desc* d) {   // with more than one tile of rows
-    return d->out_dtype == SF_F32 ? kKvExact : d->out_dtype == SF_F16 || d->is_causal ? kKvPair : kKvHalf;
+    return d->out_dtype == SF_F32 ? kKvExact : d->out_dtype == SF_F16 || d->is_causal || d->exact_pv ? kKvPair : kKvHalf;
 }
 
 // Up to 16 rows to a key head: one tile, four waves to a workgroup.  Up to 512

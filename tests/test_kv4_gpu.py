@@ -674,3 +674,22 @@ def test_one_strong_key_before_a_million(D):
     for splits in (0, 1, 3):
         got = attention_kv4(q, c, num_splits=splits).double()
         assert ((got - ref).abs() <= 7 * 2.0 ** -12 + half_step(BF) * abs(ref)).all(), splits
+
+
+@pytest.mark.parametrize("D,Sk", [(64, 400), (64, 4374), (128, 2000)])
+def test_exact_pv(D, Sk):
+    """exact_pv: a bf16 output of many rows is the fp32 output rounded, but for sums that lie 2^-14 of the output's
+    norm or less from a border between two numbers (the pair is off by about 2^-16 of it; fp16 weights by 2^-11)."""
+    B, H, Sq = 2, 4, 67
+    c, _, _ = _filled(B, H, Sk, D, BF, 190)
+    q = _randn(193, B, H, Sq, D, dtype=BF).to(DEV)
+    fine = attention_kv4(q, c, out_dtype=F32)
+    got = attention_kv4(q, c, exact_pv=True)
+    rms = float(fine.double().square().mean().sqrt())
+    # a sum moves by at most 2^-14 rms: it may then round to a neighbour, and not further
+    lo, hi = (fine + 2.0 ** -14 * rms).to(BF), (fine - 2.0 ** -14 * rms).to(BF)
+    assert (torch.minimum(lo, hi) <= got).all() and (got <= torch.maximum(lo, hi)).all()
+    for dt in (FP, F32):   # nothing changes where there is no fp16 form
+        assert torch.equal(attention_kv4(q, c, out_dtype=dt), attention_kv4(q, c, out_dtype=dt, exact_pv=True))
+    one = q[:, :, :1]
+    assert torch.equal(attention_kv4(one, c), attention_kv4(one, c, exact_pv=True))
