@@ -106,10 +106,17 @@ __global__ __launch_bounds__(512) void gemm_w4_kernel(const W4Args p) {
     // Instruction i brings rows 4 i .. 4 i + 3, 256 bytes each, piece c of row q to place c ^ (q & 15); rows behind M are
     // behind the buffer's end and come as zeros.
     auto fetch = [&](int kb, char* to) __attribute__((always_inline)) {
-        const int last = min(16, (p.K - 128 * kb) >> 3) - 1;   // behind K a row's last piece again: its codes' scale is 0
+        // A last block that is not full: one of its groups again in the places of the missing ones, whose scale is 0 (0
+        // times a finite sum, as the group's own is).
+        const int have = GROUP < 128 ? min(16, (p.K - 128 * kb) >> 3) : 16;
         uint32_t at[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) at[u] = (uint32_t)g * ld + 16u * (uint32_t)min(r ^ ((4 * (u + wn * (4 * MB / WN)) & 15) + g), last);
+        for (int u = 0; u < 4; ++u) {
+            int c = r ^ ((4 * (u + wn * (4 * MB / WN)) & 15) + g);
+            if (GROUP == 64) c &= have - 1;                               // 8 or 16 of them
+            if (GROUP == 32) c = c < have ? c : have == 12 ? c & 11 : c & (have - 1);
+            at[u] = (uint32_t)g * ld + 16u * (uint32_t)c;
+        }
         uint32_t step = 256u * (uint32_t)kb + (uint32_t)wn * (4 * MB / WN) * 4u * ld;
         to += wn * (4 * MB / WN) * 1024;
 #pragma unroll

@@ -163,3 +163,16 @@ def test_strided_checkpoint():
 def test_empty_rows():
     _, w, _, _ = _case(1, 16, 128, 128, BF, False)
     assert kernels.gemm_w4(torch.empty(0, 128, dtype=BF, device=DEV), w).shape == (0, 16)
+
+
+@pytest.mark.parametrize("M,N", [(3, 48), (20, 4113), (67, 6111), (90, 8200)])
+@pytest.mark.parametrize("group,K", [(32, 32), (32, 160), (64, 64)])
+def test_largest_sums_in_a_last_block_that_is_not_full(M, N, group, K):
+    """31 times a group's sum of |A| is just finite (2^127.96): nothing of it may be added up more than once."""
+    codes, scales, z, w = w4_random(N, K, group, BF, True, 11)
+    a = torch.zeros(M, K, dtype=BF)
+    a[:, K - 1] = 2.0 ** 123
+    ref = a.double() @ w.t()
+    packed = kernels.w4_pack(w4_bytes(codes).to(DEV), scales.to(DEV), z.to(DEV), group=group)
+    big = a.double() @ ((47 + z.double().repeat_interleave(group, 1)) * scales.double().repeat_interleave(group, 1)).t()
+    _check(kernels.gemm_w4(a.to(DEV), packed, out_dtype=F32), ref, big, K, F32)
