@@ -741,7 +741,10 @@ int sf_kv4_read(const sf_kv4_cache* cache, const int32_t* slots, int32_t S, void
  * output's norm, where that rounding is 1.7e-3).  Values are taken up to 2^100 in
  * magnitude.  out may be Q itself
  * (same strides and type); otherwise they must not overlap.
- * num_splits: 0 chooses; n > 0 forces n key splits (at most 64). */
+ * num_splits: 0 chooses; n > 0 forces n key splits (at most 64; with more than
+ * one of them B * Hq * Sq is below 2^24).  B * cache.H times the splits and the
+ * groups of 16 or more query rows of a key head is below 2^23 (SF_ENOTSUP above
+ * either). */
 typedef struct sf_attn_kv4_desc {
     int32_t B, Hq, Sq, Sk;
     float scale;

@@ -37,6 +37,7 @@ namespace sfk {
 
 constexpr int kKvMaxSplits = 64;
 constexpr float kKvSlack = 8.f;       // log2
+constexpr int64_t kKvMergeRows = 1 << 24;   // the merge's workgroups: a launch counts its threads in 32 bits
 constexpr int kKvHalfKeys = 4096;     // of a wave, with weights in fp16
 constexpr float kKvNoMax = -1.5e38f;  // the maximum of a row that has seen nothing
 
@@ -888,7 +889,7 @@ static inline int kv_form(const sf_attn_kv4_desc* d) {   // with more than one t
 // keys, so that batches of unequal lengths spread (16 x 8 heads, 4096..16384
 // keys: 59 us with 8 splits, 58 with 4, 148 with 1).
 static int kv_splits_one_tile(const sf_attn_kv4_desc* d, int64_t base) {
-    if (d->Sk <= 512) return 1;
+    if (d->Sk <= 512 || (int64_t)d->B * d->Hq * d->Sq >= kKvMergeRows) return 1;
     const int64_t want = std::max(ceil_div(512, base), ceil_div(d->Sk, 2048));
     return (int)std::min<int64_t>({want, ceil_div(d->Sk, 128), (int64_t)kKvMaxSplits});
 }
@@ -992,7 +993,7 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
         if (d->q_stride[i] < 0 || (d->q_stride[i] & 7) || d->o_stride[i] < 0 || (d->o_stride[i] & 7)) return SF_EINVAL;
     if (d->kv_mask && d->kv_mask_stride < 0) return SF_EINVAL;
     const sfk::KvPlan k = sfk::kv_plan(d);
-    if (k.wgs >= 1 << 23 || (k.splits > 1 && k.rows >= 1 << 24)) return SF_ENOTSUP;   // a launch counts its threads in 32 bits
+    if (k.wgs >= 1 << 23 || (k.splits > 1 && k.rows >= sfk::kKvMergeRows)) return SF_ENOTSUP;   // threads in 32 bits
     if (k.splits > 1 && (!workspace || workspace_bytes < sf_attn_kv4_workspace_bytes(d))) return SF_EWORKSPACE;
     if (k.splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 3)) return SF_EINVAL;
     sfk::KvAttnArgs p = {};

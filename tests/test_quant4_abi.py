@@ -216,3 +216,13 @@ def test_front_ends_refuse_host_tensors_and_shapes():
               torch.zeros(1, 2, 1, 64)):
         with pytest.raises(ValueError):
             attention_kv4(q, c)
+
+
+def test_no_key_splits_that_the_merge_cannot_take():
+    """The choice of splits knows the merge's limit of rows (it refused what it had chosen itself)."""
+    L = abi.lib()
+    for D in (64, 128):
+        d = _attn_desc(B=1 << 16, Hq=256, Sk=4096, cache=(256, 1 << 16, 16, 4096, D))
+        assert L.sf_attn_kv4_workspace_bytes(ctypes.byref(d)) == 0
+    d = _attn_desc(B=1 << 14, Hq=64, Sk=4096, cache=(256, 1 << 14, 16, 4096, 64))   # few enough rows
+    assert L.sf_attn_kv4_workspace_bytes(ctypes.byref(d)) == 2 * (1 << 20) * 66 * 4
