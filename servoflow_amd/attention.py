@@ -192,8 +192,8 @@ def attention_kv4(q, cache, out=None, scale=0.0, is_causal=False, valid_len=None
             workspace = torch.empty(n, dtype=torch.uint8, device=dev)   # needs no init
             ws = workspace.data_ptr()
     else:
-        if workspace.device != dev:
-            raise ValueError(f"workspace must be on {dev}")
+        if workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {dev}")
         ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     kernels.call_on(dev, "sf_attn_kv4", abi.lib().sf_attn_kv4, d, q.data_ptr(), out.data_ptr(), ws, n)
     return out

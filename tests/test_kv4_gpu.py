@@ -693,3 +693,19 @@ def test_exact_pv(D, Sk):
         assert torch.equal(attention_kv4(q, c, out_dtype=dt), attention_kv4(q, c, out_dtype=dt, exact_pv=True))
     one = q[:, :, :1]
     assert torch.equal(attention_kv4(one, c), attention_kv4(one, c, exact_pv=True))
+
+
+def test_a_workspace_is_one_piece():
+    """A view that names a place more than once has fewer bytes behind its pointer than elements."""
+    c, k, v = _filled(1, 2, 300, 64, BF, 210)
+    q = _randn(213, 1, 4, 1, 64, dtype=BF).to(DEV)
+    n = 3 * 4 * 66   # floats: three splits of four rows
+    with pytest.raises(ValueError):
+        attention_kv4(q, c, num_splits=3, workspace=torch.zeros(1, dtype=F32, device=DEV).expand(n))
+    with pytest.raises(ValueError):
+        attention_kv4(q, c, num_splits=3, workspace=torch.zeros(2 * n, dtype=F32, device=DEV)[::2])
+    with pytest.raises(RuntimeError):
+        attention_kv4(q, c, num_splits=3, workspace=torch.zeros(n - 1, dtype=F32, device=DEV))
+    room = torch.full((n + 8,), 7.0, dtype=F32, device=DEV)
+    _attn_check(attention_kv4(q, c, num_splits=3, workspace=room[4:-4], out_dtype=F32), q.cpu(), k, v, F32)
+    assert (room[:4] == 7).all() and (room[-4:] == 7).all()
