@@ -709,3 +709,109 @@ def test_a_workspace_is_one_piece():
     room = torch.full((n + 8,), 7.0, dtype=F32, device=DEV)
     _attn_check(attention_kv4(q, c, num_splits=3, workspace=room[4:-4], out_dtype=F32), q.cpu(), k, v, F32)
     assert (room[:4] == 7).all() and (room[-4:] == 7).all()
+
+
+@pytest.mark.parametrize("D,H,Hq,Sq,Sk,kind", [(64, 8, 8, 67, 404, "plain"), (64, 32, 32, 67, 4374, "plain"), (64, 4, 8, 130, 1537, "causal"),
+                                               (64, 8, 8, 67, 4374, "mask"), (128, 8, 8, 67, 4374, "plain"), (128, 4, 16, 33, 2000, "causal"),
+                                               (128, 2, 8, 268, 3000, "mask"), (128, 4, 16, 1, 16384, "plain"), (64, 4, 4, 4, 8192, "mask")])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_outputs_of_16_bits_in_the_norm(D, H, Hq, Sq, Sk, kind, dtype):
+    """The 2-norm of the error over the output's.  Rounding the output adds at most half_step / sqrt(3) of it (an error
+    spread evenly over its step).  The pair adds below 2^-15.  fp16 weights and values add, for values with a mean of
+    zero, three errors that are independent from key to key: of p and of V, 2^-11 / sqrt(3) each, and of mid - 7.5 s,
+    the same of a number about 2.5 times the values' own size: at most 2.9 2^-11 / sqrt(3).  The reference runs on the
+    device, in 64 bits."""
+    B = 2
+    c = Kv4Cache(B, H, Sk, D, DEV)
+    k, v = (_randn(s, B, H, Sk, D, dtype=dtype).to(DEV) for s in (194, 195))
+    c.write(k, v)
+    q = _randn(196, B, Hq, Sq, D, dtype=dtype).to(DEV)
+    mask = torch.rand(B, Sk, generator=torch.Generator().manual_seed(8)).to(DEV) < 0.7 if kind == "mask" else None
+    got = attention_kv4(q, c, is_causal=kind == "causal", kv_mask=mask)
+    off = norm = 0.0
+    for b in range(B):
+        kk, vv = (kv4_levels(t[b]).repeat_interleave(Hq // H, 0) for t in (k, v))
+        x = torch.matmul(q[b].double(), kk.transpose(1, 2).contiguous()) / math.sqrt(D)
+        if mask is not None:
+            x[..., ~mask[b]] = -math.inf
+        if kind == "causal":
+            x = x.masked_fill(torch.arange(Sk, device=DEV) > torch.arange(Sq, device=DEV)[:, None] + Sk - Sq, -math.inf)
+        ref = torch.matmul(torch.softmax(x, -1), vv)
+        off += float((got[b].double() - ref).square().sum())
+        norm += float(ref.square().sum())
+    half = dtype == BF and Hq // H * Sq > 16
+    own = 2.9 * 2.0 ** -11 / math.sqrt(3) if half else 2.0 ** -15
+    assert math.sqrt(off / norm) <= math.hypot(half_step(dtype) / math.sqrt(3), own)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,Sq,out_dtype", [(2, 2, F32), (2, 2, BF), (2, 2, FP), (2, 33, F32), (2, 33, FP), (64, 1, F32), (64, 1, FP)])
+def test_large_values_of_unseen_weight(D, Hq, Sq, out_dtype):
+    """Tokens whose values are 2^20 larger and whose weights are below 2^-45 of the rest: what a row is off by goes by
+    the products of both, not by the values.  Many heads take several blocks of keys in one tile."""
+    B, H, Sk = (8, 64, 1024) if Hq == 64 else (1, 2, 200)
+    base = _randn(198, 1, 1, 1, D)
+    k, v = _randn(199, 1, H, Sk, D, dtype=BF), _randn(200, 1, H, Sk, D, dtype=BF)
+    # against rows near base a score of -44 (2^-63)
+    far = (base * (-44.0 * math.sqrt(D) / float(base.square().sum()))).to(BF).expand(1, H, 1, D)
+    k[:, :, ::9] = far
+    v[:, :, ::9] *= 2.0 ** 20
+    q = (base + _randn(201, 1, Hq, Sq, D) / 16).to(BF)
+    c = Kv4Cache(B, H, Sk, D, DEV)
+    c.write(*(t.expand(B, -1, -1, -1).contiguous().to(DEV) for t in (k, v)))
+    got = attention_kv4(q.expand(B, -1, -1, -1).contiguous().to(DEV), c, out_dtype=out_dtype)
+    lk, lv = kv4_levels(k), kv4_levels(v)
+    x = torch.matmul(q.double(), lk.repeat_interleave(Hq // H, 1).transpose(2, 3)) / math.sqrt(D)
+    p = torch.softmax(x, -1)
+    assert float(p[..., ::9].max()) < 2.0 ** -45
+    vv = lv.repeat_interleave(Hq // H, 1)
+    ref, size = torch.matmul(p, vv), torch.matmul(p, vv.unflatten(-1, (-1, 64)).abs().amax(-1, keepdim=True).expand(*vv.shape[:-1], -1, 64).flatten(-2))
+    # of the sum of p |v| (the largest of the 64 channels): the tolerance of _attn_check, its parts as there
+    dx = 24 * 2.0 ** -24 / math.sqrt(D) * float(q.double().abs().sum(-1).max()) * float(lk.abs().max()) * 6
+    rel = 2 * (dx + 2.0 ** -22) + 2.0 ** -16 + (32 + Sk / 32) * 2.0 ** -24 * 16
+    tol = rel * size + half_step(out_dtype) * ref.abs() + (2.0 ** -25 if out_dtype == FP else 0)
+    for b in range(B):
+        assert ((got[b].cpu().double() - ref[0]).abs() <= tol[0]).all(), b
+
+
+@pytest.mark.parametrize("kind", ["plain", "causal", "ragged", "mask"])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D,Hq,Sq,Sk", [(64, 64, 1, 512), (64, 128, 2, 497), (64, 64, 7, 500), (128, 64, 1, 481), (128, 128, 4, 512)])
+def test_long_streams_of_few_rows_to_fp32(D, Hq, Sq, Sk, dtype, kind):
+    """The three-term form of several blocks of keys in one tile, as test_long_streams_of_few_rows has the pair's."""
+    B, H = 16, 64
+    k = _randn(202, 1, H, Sk, D, dtype=dtype).to(DEV).repeat(B, 1, 1, 1) + torch.linspace(-1, 1, B, device=DEV).to(dtype)[:, None, None, None]
+    v = (k * 0.75).flip(2)
+    c = Kv4Cache(B, H, Sk + 9, D, DEV)
+    c.data.fill_(0xff)
+    c.write(k, v)
+    lk, lv = kv4_levels(k), kv4_levels(v)
+    q = _randn(203, B, Hq, Sq, D, dtype=dtype).to(DEV)
+    valid = mask = None
+    if kind in ("causal", "ragged"):
+        valid = (torch.arange(B, device=DEV, dtype=torch.int32) * 41 + 3).clamp_max(Sk)
+        valid[5] = 0
+    if kind == "mask":
+        mask = torch.rand(B, Sk, generator=torch.Generator().manual_seed(9)).to(DEV) < 0.5
+        mask[1] = False
+        mask[:, 40] = False
+        bad = torch.full((B, H, 1, D), float("nan"), dtype=dtype, device=DEV)
+        c.write(bad, bad, torch.full((B, 1), 40, dtype=torch.int32, device=DEV))
+    sc = 1 / math.sqrt(D)
+    for splits in (0, 3):
+        got = attention_kv4(q, c, keys=Sk, is_causal=kind == "causal", valid_len=valid, kv_mask=mask, num_splits=splits,
+                            out_dtype=F32)
+        for b in range(B):
+            n = Sk if valid is None else int(valid[b])
+            kk, vv = (t[b, :, :n].repeat_interleave(Hq // H, 0) for t in (lk, lv))
+            x = torch.matmul(q[b].double(), kk.transpose(1, 2).contiguous()) * sc
+            if mask is not None:
+                x[..., ~mask[b, :n]] = -math.inf
+                vv = torch.where(mask[b, :n, None], vv, 0.0)
+            if kind == "causal":
+                x = x.masked_fill(torch.arange(n, device=DEV) > torch.arange(Sq, device=DEV)[:, None] + n - Sq, -math.inf)
+            w = torch.softmax(x, -1)
+            ref = torch.matmul(torch.where(torch.isnan(w), 0.0, w), vv) if n else torch.zeros_like(q[b]).double()
+            dx = 24 * 2.0 ** -24 * sc * float(q.double().abs().sum(-1).max()) * float(lk.abs().max()) * 6
+            rel = 2 * (dx + 2.0 ** -22) + 2.0 ** -16 + (32 + Sk / 32) * 2.0 ** -24 * 16
+            assert ((got[b].double() - ref).abs() <= rel * float(lv.abs().max())).all(), (splits, b)
