@@ -226,3 +226,15 @@ def test_no_key_splits_that_the_merge_cannot_take():
         assert L.sf_attn_kv4_workspace_bytes(ctypes.byref(d)) == 0
     d = _attn_desc(B=1 << 14, Hq=64, Sk=4096, cache=(256, 1 << 14, 16, 4096, 64))   # few enough rows
     assert L.sf_attn_kv4_workspace_bytes(ctypes.byref(d)) == 2 * (1 << 20) * 66 * 4
+
+
+def test_nan_is_honoured_where_it_is_promised():
+    """The 4-bit operators' sources are not compiled under the assumption that no NaN is met."""
+    make = shutil.which("make")
+    if make is None:
+        pytest.skip("no make")
+    out = subprocess.run([make, "-n", "-B", "-C", os.path.join(ROOT, "servoflow_amd"), "lib/libsf_hip_kernels.so"],
+                         check=True, capture_output=True, text=True).stdout
+    for name in ("sf_heads_rope", "sf_kv4_attn", "sf_w4"):
+        flags = next(line for line in out.splitlines() if f"-c csrc/{name}.hip" in line).split()
+        assert flags.index("-fhonor-nans") > flags.index("-fno-honor-nans"), name
