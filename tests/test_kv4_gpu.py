@@ -815,3 +815,20 @@ def test_long_streams_of_few_rows_to_fp32(D, Hq, Sq, Sk, dtype, kind):
             dx = 24 * 2.0 ** -24 * sc * float(q.double().abs().sum(-1).max()) * float(lk.abs().max()) * 6
             rel = 2 * (dx + 2.0 ** -22) + 2.0 ** -16 + (32 + Sk / 32) * 2.0 ** -24 * 16
             assert ((got[b].double() - ref).abs() <= rel * float(lv.abs().max())).all(), (splits, b)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq", [1, 3, 40])
+@pytest.mark.parametrize("out_dtype,causal", [(BF, False), (BF, True), (FP, False), (F32, False), (F32, True)])
+def test_a_bad_query_stays_alone(D, Sq, out_dtype, causal):
+    """An infinity and a NaN in two query rows: those are NaN, the tiles' other rows are right."""
+    Hq, H, Sk = 4, 1, 333
+    c, k, v = _filled(1, H, Sk, D, BF, 220)
+    q = _randn(223, 1, Hq, Sq, D, dtype=BF)
+    bad = q.clone()
+    bad[0, 1, Sq - 1, 3], bad[0, 2, 0, D - 1] = float("inf"), float("nan")
+    got = attention_kv4(bad.to(DEV), c, is_causal=causal, out_dtype=out_dtype)
+    assert torch.isnan(got[0, 1, Sq - 1]).all() and torch.isnan(got[0, 2, 0]).all()
+    ref = attend(q, k, v, causal=causal)
+    got[0, 1, Sq - 1], got[0, 2, 0] = (ref[0, h, s].to(DEV, got.dtype) for h, s in ((1, Sq - 1), (2, 0)))
+    _attn_check(got, q, k, v, out_dtype, causal=causal)
