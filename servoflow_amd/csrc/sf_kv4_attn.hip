@@ -8,17 +8,18 @@
 // (16 + c: see sf_nibble.h).  p_j s_j enters the matrix unit as a bf16 (hi, lo)
 // pair, 2^-18 relative, and its sum is taken over the same rounded pair, so that
 // what the codes' offset adds is taken away exactly; for fp32 outputs it enters as
-// three terms.  With many query rows to an
-// unpacked block and a bf16 output the values are formed in fp16 instead, once
-// for all rows, and p enters as one fp16: five vector operations fewer for every
-// score, and errors of 2^-12 where the output's own rounding is 2^-9.
+// three terms.  With many query rows that see the same tokens and a bf16 output the
+// values are formed in fp16 instead, once for all rows, and p enters as one fp16:
+// five vector operations fewer for every score, and roundings of 2^-11 where the
+// output's own is 2^-8 (6e-4 of its norm beside 1.7e-3); exact_pv keeps the pair.
 //
 // One wave takes blocks of 32 tokens against QT tiles of 16 query rows; query
 // heads that share a key head are rows of one tile, so a cached token is read
 // and unpacked once for all of them.  S^T = K Q^T puts a row's scores in the
 // lanes that the second product wants them in as P^T (the cache's value order,
-// sf_kv4.h): nothing passes through LDS inside the loop.  The running maximum
-// moves only when a score exceeds it by 2^8: p stays below 2^8, far inside
+// sf_kv4.h): no score passes through LDS.  What does, inside the loop, are the
+// queries of more than one tile, read back as operands, and with them the raw
+// blocks of 128 channels.  The running maximum moves only when a score exceeds it by 2^8: p stays below 2^8, far inside
 // bf16 and fp32, and the common block has neither a cross-lane maximum nor a
 // rescale.
 #include <hip/hip_runtime.h>
@@ -58,7 +59,7 @@ constexpr float kKvNoMax = -1.5e38f;  // the maximum of a row that has seen noth
 // the output's norm that is off by 1.3e-7 (20 keys) to 7e-7 (8192), as the same
 // sums over fp32 values are, where the pair is off by 1.4e-6 to 1e-5; it costs
 // 16 x 8 heads x 16384 keys x 4 rows 78 us instead of 70, 4 x 32 x 4374 x 67 rows
-// 47 instead of 39, and 4 x 8 x 4096 x 268 rows of 128 channels, which spill, 114
+// 48 instead of 40, and 4 x 8 x 4096 x 268 rows of 128 channels, which spill, 110
 // instead of 87.
 enum { kKvHalf, kKvPair, kKvExact };
 
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     constexpr int kJoin = D == 128 && NW == 8 ? 1 : QT == 5 ? 3 : QT == 4 ? 2 : QT;   // tiles that meet at a time
     // 128 channels and two tiles leave no registers for the next raw block beside eight waves: it waits in LDS, brought
     // there straight from memory.  us, against four waves with it in registers: 8 x 32 heads x 67 x 4374 145 and 166,
-    // 2 x 8 x 268 rows x 8192 73 and 96, 2 x 8 x 1024 rows x 2048 causal 31.5 and 34.4.
+    // 2 x 8 x 268 rows x 8192 73 and 96 (129 and 70 since the fp16 form knows no causal rows and does not spill).
     constexpr bool kStaged = D == 128 && QT > 1;
     __shared__ __attribute__((aligned(16))) uint8_t raw[kStaged ? NW : 1][kStaged ? Kv4<D>::kBytes : 16];
     __shared__ float xo[NW][kJoin * 16][D + 4], xq[GR][QT * 16];
@@ -910,11 +911,12 @@ static int kv_column_groups(const sf_attn_kv4_desc* d, int rows, int64_t heads) 
 // block's unpacking, then each tile -- and 3 + 0.8 qt us around the loop; key
 // splits that fill the card add a merge of 7 us.  Estimated for each qt the
 // kernel is built for, the smallest taken.  Measured against it (64 channels,
-// bf16): 12 x 520 rows x 1537 keys, causal, 12.1 us with qt 2, 14.4 with 3, 18.6
-// with 5 (estimates 12, 15, 21); 32 x 67 x 4374 18.9 with qt 3 and four splits,
-// 19.6 with 5 and eight, 31 with 3 and one (19, 20, 30); 256 x 67 x 4374 42 with
-// qt 5.  The (hi, lo) form takes 0.42 us a step, and qt 5 would spill,
-// with three terms qt 4.  128 channels: 2 tiles are what fits.
+// bf16): 32 x 67 rows x 4374 keys 20.1 us with qt 3 and four splits, 21.1 with 5 and
+// eight, 32 with 3 and one (estimates 19, 20, 30); 256 x 67 x 4374 42 with qt 5, 64
+// with 3; 256 x 67 x 67 9.8 with qt 5, 13.8 with 3.  The (hi, lo) form takes 0.42 us
+// a step, and qt 5 would spill, with three terms qt 4: causal, 12 x 520 rows x 1537
+// keys 16.2 with qt 2, 19.4 with 3, 23 with 4; 16 x 1024 x 2048 26.7 with 4, 35 with
+// 2.  128 channels: 2 tiles are what fits.
 static void kv_tiles(const sf_attn_kv4_desc* d, int64_t R, int64_t heads, KvPlan& k) {
     const bool wide = d->cache.D == 128;
     const int most = wide ? 2 : k.form == kKvExact ? 3 : k.form == kKvPair ? 4 : 5;
