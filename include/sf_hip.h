@@ -739,8 +739,8 @@ int sf_kv4_read(const sf_kv4_cache* cache, const int32_t* slots, int32_t S, void
  * as bf16 (hi, lo) pairs, 2^-18 relative, and for an fp32 output as three bf16
  * terms, which leaves it within 1e-6 of its norm up to 16384 keys (as sums over
  * fp32 values).  Unless exact_pv is set, a bf16 output of more than 16 query rows
- * to a key head that all see the same tokens (no is_causal), with at most 2^15 keys
- * to a split, takes weights and values as fp16, the values under a power of two
+ * to a key head that all see the same tokens (no is_causal, or Sq 1), with at most
+ * 2^15 keys to a split, takes weights and values as fp16, the values under a power of two
  * that keeps them in its range: 7 2^-12 of the largest value that the row sees,
  * beside the output's own rounding (6e-4 of the output's norm, where that rounding
  * is 1.7e-3; rows whose largest value is below 2^-100 lose bits).

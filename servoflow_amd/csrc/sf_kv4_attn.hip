@@ -19,9 +19,9 @@
 // lanes that the second product wants them in as P^T (the cache's value order,
 // sf_kv4.h): no score passes through LDS.  What does, inside the loop, are the
 // queries of more than one tile, read back as operands, and with them the raw
-// blocks of 128 channels.  The running maximum moves only when a score exceeds it by 2^8: p stays below 2^8, far inside
-// bf16 and fp32, and the common block has neither a cross-lane maximum nor a
-// rescale.
+// blocks of 128 channels.  The running maximum moves only when a score exceeds it
+// by 2^8: p stays below 2^8, far inside bf16 and fp32, and the common block has
+// neither a cross-lane maximum nor a rescale.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -46,21 +46,21 @@ constexpr float kKvNoMax = -1.5e38f;  // the maximum of a row that has seen noth
 // both in fp16.  Not for causal rows: what later rows alone see would set the power
 // under which an earlier row's values are rounded, and a NaN among it, as V, would
 // reach rows whose weight for it is 0.  Nor for more than 4096 keys of a wave: a
-// weight below 2^-14 of the wave's largest is held to 2^-25 only, one below 2^-25 not
-// at all, which N keys make N 2^-24 of the largest value (2^-12 for 4096).  (us with the pair, and with fp16 when the
-// blocks that some rows see a part of are taken in steps of values of like size: 64
-// channels, 8 heads of 4 x 256 rows over 2048 keys, twice, 18.5 and 17.5, of 4 x 4096
-// over 4096 193 and 168; 128 channels, the first of these 30.5 and 34.8.)  kKvPair
-// (other 16-bit outputs): p s as a bf16 (hi, lo) pair with the codes, whose offset
-// the pairs' sums take away at the end.  kKvExact (fp32 outputs): three terms
-// instead of two, and the offset, which is many times a mean of values and would
-// leave its own rounding, is taken away inside the products: -23.5 times the
-// queries' sums under the scores, a product with -23.5 beside each block's.  Of
-// the output's norm that is off by 1.3e-7 (20 keys) to 7e-7 (8192), as the same
-// sums over fp32 values are, where the pair is off by 1.4e-6 to 1e-5; it costs
-// 16 x 8 heads x 16384 keys x 4 rows 78 us instead of 70, 4 x 32 x 4374 x 67 rows
-// 48 instead of 40, and 4 x 8 x 4096 x 268 rows of 128 channels, which spill, 110
-// instead of 87.
+// weight below 2^-14 of the wave's largest is held to 2^-25 only, one below 2^-25
+// not at all, which N keys make N 2^-24 of the largest value (2^-12 for 4096).
+// (Causal, us with the pair, and with fp16 when the blocks that some rows see a part
+// of are taken in steps of values of like size: 64 channels, 8 heads of 4 x 256 rows
+// over 2048 keys, twice, 18.5 and 17.5, of 4 x 4096 over 4096 193 and 168; 128
+// channels, the first of these 30.5 and 34.8.)  kKvPair (other 16-bit outputs): p s
+// as a bf16 (hi, lo) pair with the codes, whose offset the pairs' sums take away at
+// the end.  kKvExact (fp32 outputs): three terms instead of two, and the offset,
+// which is many times a mean of values and would leave its own rounding, is taken
+// away inside the products: -23.5 times the queries' sums under the scores, a
+// product with -23.5 beside each block's.  Of the output's norm that is off by
+// 1.3e-7 (20 keys) to 7e-7 (8192), as the same sums over fp32 values are, where the
+// pair is off by 1.4e-6 to 1e-5; it costs 16 x 8 heads x 16384 keys x 4 rows 78 us
+// instead of 70, 4 x 32 x 4374 x 67 rows 48 instead of 40, and 4 x 8 x 4096 x 268
+// rows of 128 channels, which spill, 110 instead of 87.
 enum { kKvHalf, kKvPair, kKvExact };
 
 struct KvAttnArgs {
@@ -870,7 +870,7 @@ __global__ __launch_bounds__(256) void attn_kv4_merge_kernel(const KvAttnArgs p)
 }
 
 // How a call is cut up: tiles of 16 query rows to a workgroup (qt), groups of
-// them (qgroups), key splits.
+// them (qgroups), key splits; and how p and V meet.
 struct KvPlan {
     int qt, ng, qgroups, splits, form;
     int64_t wgs, rows;
@@ -879,7 +879,8 @@ struct KvPlan {
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 static inline int kv_form(const sf_attn_kv4_desc* d) {   // with more than one tile of rows
-    return d->out_dtype == SF_F32 ? kKvExact : d->out_dtype == SF_F16 || d->is_causal || d->exact_pv ? kKvPair : kKvHalf;
+    const bool apart = d->is_causal && d->Sq > 1;   // rows that see different tokens
+    return d->out_dtype == SF_F32 ? kKvExact : d->out_dtype == SF_F16 || apart || d->exact_pv ? kKvPair : kKvHalf;
 }
 
 // Up to 16 rows to a key head: one tile, four waves to a workgroup.  Up to 512

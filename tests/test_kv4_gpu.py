@@ -832,3 +832,15 @@ def test_a_bad_query_stays_alone(D, Sq, out_dtype, causal):
     ref = attend(q, k, v, causal=causal)
     got[0, 1, Sq - 1], got[0, 2, 0] = (ref[0, h, s].to(DEV, got.dtype) for h, s in ((1, Sq - 1), (2, 0)))
     _attn_check(got, q, k, v, out_dtype, causal=causal)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_causal_token_is_as_one_that_is_not(D):
+    """One token's many heads see the same keys, causal or not: the same form, bit for bit."""
+    B, Hq, H, Sk = 2, 64, 2, 700
+    c, k, v = _filled(B, H, Sk, D, BF, 230)
+    q = _randn(233, B, Hq, 1, D, dtype=BF)
+    valid = torch.tensor([700, 331], dtype=torch.int32)
+    got = [attention_kv4(q.to(DEV), c, is_causal=causal, valid_len=valid.to(DEV)) for causal in (True, False)]
+    assert torch.equal(*got)
+    _attn_check(got[0], q, k, v, BF, valid=valid, causal=True)
