@@ -255,7 +255,7 @@ def _act(name, x):
 
 def _plain_i8(s, c):
     a = s["a"].float()
-    scale = a.abs().amax(1, keepdim=True) / 127
+    scale = a.abs().amax(1, keepdim=True) / torch.full((), 127.0, device=a.device)   # (by a number: times its reciprocal)
     code = torch.round(a.double() / torch.where(scale > 0, scale, 1.0).double())   # next to a border: 64 bits
     y = torch.matmul(code, s["w"].double().t()).float()                            # whole numbers beyond 2^24
     y = y * scale * s["scale"]
@@ -420,7 +420,7 @@ def _levels64(x):
 def _exact_i8(case, seed):
     t = _i8_inputs(case, seed)
     a = t["a"].double()
-    step = (a.abs().max(1).values.float() / 127).double()
+    step = torch.div(a.abs().max(1).values.float(), torch.full((a.shape[0],), 127.0, device=DEV)).double()
     q = a / step.clamp_min(1e-300)[:, None]
     lo = torch.floor(q)
     up = (q - lo > 0.5) | ((q - lo == 0.5) & (lo % 2 != 0))
