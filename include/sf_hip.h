@@ -771,6 +771,130 @@ size_t sf_attn_kv4_workspace_bytes(const sf_attn_kv4_desc* desc);
 int sf_attn_kv4(const sf_attn_kv4_desc* desc, const void* q, void* out, void* workspace, size_t workspace_bytes,
                 void* stream);
 
+/* ---------------------------------------------------------------------------
+ * A step that verifies a tree of drafted tokens over the 4-bit cache: the
+ * tree's tables, attention of its nodes, the path that sampled tokens confirm,
+ * and the cache with that path alone.
+ *
+ * Node 0 is the root, the last token already decided; parents[j] < j is node j's
+ * parent, and any other value (node 0's too) counts as none: such a node has no
+ * ancestors and is on no path.  `each` 0: one tree [T] for all batch elements;
+ * otherwise a tree for each of them ([B][T]).  T to SF_TREE_MAX_NODES
+ * (SF_ENOTSUP above).  All arrays are device memory.
+ * ------------------------------------------------------------------------- */
+#define SF_TREE_MAX_NODES 1024
+
+/* masks [trees][T][ceil(T / 32)]: bit i of node j's row (word i / 32) is set
+ * where i is j or an ancestor of j; the bits behind T are zero.  depth [trees][T]: a
+ * node's number of ancestors (its position is the root's and that). */
+int sf_tree_build(const int32_t* parents, int32_t trees, int32_t T, uint32_t* masks, int32_t* depth, void* stream);
+
+typedef struct sf_draft_tree {
+    const uint32_t* masks;   /* sf_tree_build's */
+    int32_t T, each;
+} sf_draft_tree;
+
+/* sf_attn_kv4 for a tree: its T nodes are the last T of a sequence's cached
+ * tokens (node i in slot valid_len - T + i; kv_valid_len NULL: Sk), the Sq <= T
+ * queries the last Sq nodes.  A query sees every token before the nodes, itself
+ * and its ancestors (of those, what kv_mask leaves).  Nodes before a sequence's
+ * first token (valid_len < T) see nothing: zeros.  is_causal: SF_EINVAL.
+ * Everything else as sf_attn_kv4, without the form in fp16. */
+size_t sf_attn_kv4_tree_workspace_bytes(const sf_attn_kv4_desc* desc, const sf_draft_tree* tree);
+int sf_attn_kv4_tree(const sf_attn_kv4_desc* desc, const sf_draft_tree* tree, const void* q, void* out, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* The path of drafted tokens that sampled ones confirm.  drafted [B][T]: the
+ * nodes' tokens; sampled [B][T]: the token sampled behind each node.  From the
+ * root on, the child whose drafted token is the node's sampled one follows, the
+ * first such child by index, until there is none.  nodes, tokens [B][T]: the path
+ * and the tokens sampled along it (one more than the drafted tokens confirmed), -1
+ * behind the end; count [B]: the path's length, 1 at least.  Tokens sampled one by one
+ * from the model give the same sequence.  drafted[b][0] is not read. */
+int sf_tree_accept(const int32_t* parents, int32_t each, const int32_t* drafted, const int32_t* sampled, int32_t B,
+                   int32_t T, int32_t* nodes, int32_t* count, int32_t* tokens, void* stream);
+
+/* Keeps a path's tokens: for every batch element the cached token of slot first[b] +
+ * nodes[b][i] moves to slot first[b] + i, as if all were read before any is
+ * written.  nodes [B][n] (n to SF_TREE_MAX_NODES); a negative node, and one whose
+ * slot or place is outside [0, capacity), is left out. */
+int sf_kv4_keep(const sf_kv4_cache* cache, const int32_t* nodes, int32_t n, const int32_t* first, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * One token from each row of logits, with given uniform numbers.
+ *
+ * With m the row's largest logit a token's weight is exp((l - m) / temperature),
+ * held to 2^-44 of the largest.  In falling order of logits, ties by index: the
+ * first top_k tokens (0 or less: all); of these the fewest whose weights reach
+ * top_p of their sum (1 or more: all; one at least); of these the ones of at
+ * least min_p times the largest weight (0: all).  The token is the first whose
+ * running weight exceeds u times the sum of what is left, logprob the logarithm of
+ * its share of that sum.  temperature 0 or less: the first in order, the lowest
+ * index of the largest logits.
+ * A logit of -infinity is never taken; logits of +infinity share all the weight.
+ * A row with a NaN, or without a logit above -infinity, gives token -1 and a NaN.
+ * Sums are of whole numbers: a row's token depends on the row and its parameters
+ * alone.  One launch, no workspace.
+ * ------------------------------------------------------------------------- */
+#define SF_SAMPLE_MAX_VOCAB (1 << 20)
+typedef struct sf_sample_desc {
+    int32_t rows, V;
+    const void* logits;          /* [rows][ld], SF_F32, SF_BF16 or SF_F16, any alignment of the type */
+    int64_t ld;
+    int32_t dtype;
+    const float* u;              /* DEVICE [rows], in [0, 1) */
+    const float* temperature;    /* DEVICE [rows], or NULL: temperature_all; the others likewise */
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    float temperature_all;
+    int32_t top_k_all;
+    float top_p_all, min_p_all;
+    int32_t* token;              /* [rows] */
+    float* logprob;              /* [rows] or NULL */
+} sf_sample_desc;
+int sf_sample(const sf_sample_desc* desc, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Projections in 8-bit integers: activations with a scale for each row (token),
+ * weights with one for each output channel.
+ *
+ * C[m][n] = act(a_scale[m] w_scale[n] sum_k a[m][k] w[n][k] + bias[n]), the sum exact
+ * in 32 bits.  The reference's int8 is weight-only (quantization.cu:18-51); sf_gemm
+ * with SF_I8 weights is that, and sf_gemm_i8 takes the same codes and scales.
+ * K a multiple of 16 to 2^16, M to 2^22, N to 2^25, lda and ldw to 2^22; rows of A, W and
+ * codes 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+
+/* Rows of fp32, bf16 or fp16 (ldx in elements, rows 16-byte aligned) to codes
+ * [rows][ldc] (8-byte aligned rows) and scale [rows]: scale = max |x| / 127, code = x / scale to
+ * the nearest, ties to even, exactly.  A row of zeros has scale 0 and codes 0;
+ * one with an infinity or a NaN has that scale, codes 0, and NaN products. */
+int sf_quant_i8(const void* x, int64_t ldx, int32_t dtype, int32_t rows, int32_t cols, int8_t* codes, int64_t ldc,
+                float* scale, void* stream);
+
+typedef struct sf_gemm_i8_desc {
+    int32_t M, N, K;
+    const void* A;           /* [M][lda]: SF_I8 codes, or SF_F32, SF_BF16, SF_F16 rows to be quantised as sf_quant_i8 does */
+    int64_t lda;
+    int32_t a_dtype;
+    const float* a_scale;    /* [M], with SF_I8 codes */
+    const int8_t* W;         /* [N][ldw] */
+    int64_t ldw;
+    const float* w_scale;    /* [N] */
+    const float* bias;       /* [N] or NULL */
+    int32_t act;             /* sf_act */
+    void* C;                 /* [M][ldc] */
+    int64_t ldc;
+    int32_t c_dtype;         /* SF_F32, SF_BF16 or SF_F16 */
+    int32_t accumulate;      /* SF_F32 only: C += act(...) */
+} sf_gemm_i8_desc;
+/* Bytes of device workspace (the codes and scales of rows to be quantised, 0 for SF_I8 rows),
+ * 16-byte aligned, no initialisation; calls that may run concurrently need separate ones. */
+size_t sf_gemm_i8_workspace_bytes(const sf_gemm_i8_desc* desc);
+/* C must not overlap A. */
+int sf_gemm_i8(const sf_gemm_i8_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Static text for a status code. */
 const char* sf_strerror(int status);
 

@@ -223,6 +223,39 @@ class AttnKv4Desc(ctypes.Structure):
                 ("cache", Kv4CacheDesc)]
 
 
+SF_TREE_MAX_NODES = 1024
+
+
+class DraftTreeDesc(ctypes.Structure):
+    """Mirror of `sf_draft_tree`."""
+
+    _fields_ = [("masks", ctypes.c_void_p), ("T", ctypes.c_int32), ("each", ctypes.c_int32)]
+
+
+SF_SAMPLE_MAX_VOCAB = 1 << 20
+
+
+class SampleDesc(ctypes.Structure):
+    """Mirror of `sf_sample_desc`."""
+
+    _fields_ = [("rows", ctypes.c_int32), ("V", ctypes.c_int32), ("logits", ctypes.c_void_p), ("ld", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("u", ctypes.c_void_p), ("temperature", ctypes.c_void_p),
+                ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p),
+                ("temperature_all", ctypes.c_float), ("top_k_all", ctypes.c_int32), ("top_p_all", ctypes.c_float),
+                ("min_p_all", ctypes.c_float), ("token", ctypes.c_void_p), ("logprob", ctypes.c_void_p)]
+
+
+class GemmI8Desc(ctypes.Structure):
+    """Mirror of `sf_gemm_i8_desc`."""
+
+    _fields_ = [("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32),
+                ("A", ctypes.c_void_p), ("lda", ctypes.c_int64), ("a_dtype", ctypes.c_int32), ("a_scale", ctypes.c_void_p),
+                ("W", ctypes.c_void_p), ("ldw", ctypes.c_int64), ("w_scale", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("act", ctypes.c_int32),
+                ("C", ctypes.c_void_p), ("ldc", ctypes.c_int64), ("c_dtype", ctypes.c_int32),
+                ("accumulate", ctypes.c_int32)]
+
+
 class SfError(RuntimeError):
     def __init__(self, status: int, what: str):
         super().__init__(f"{what}: {strerror(status)} (status {status})")
@@ -316,6 +349,25 @@ def lib() -> ctypes.CDLL:
     L.sf_attn_kv4_workspace_bytes.restype = ctypes.c_size_t
     L.sf_attn_kv4.argtypes = [ctypes.POINTER(AttnKv4Desc), vp, vp, vp, ctypes.c_size_t, vp]
     L.sf_attn_kv4.restype = ctypes.c_int
+    T = ctypes.POINTER(DraftTreeDesc)
+    L.sf_tree_build.argtypes = [vp, i32, i32, vp, vp, vp]
+    L.sf_tree_build.restype = ctypes.c_int
+    L.sf_attn_kv4_tree_workspace_bytes.argtypes = [ctypes.POINTER(AttnKv4Desc), T]
+    L.sf_attn_kv4_tree_workspace_bytes.restype = ctypes.c_size_t
+    L.sf_attn_kv4_tree.argtypes = [ctypes.POINTER(AttnKv4Desc), T, vp, vp, vp, ctypes.c_size_t, vp]
+    L.sf_attn_kv4_tree.restype = ctypes.c_int
+    L.sf_tree_accept.argtypes = [vp, i32, vp, vp, i32, i32, vp, vp, vp, vp]
+    L.sf_tree_accept.restype = ctypes.c_int
+    L.sf_kv4_keep.argtypes = [ctypes.POINTER(Kv4CacheDesc), vp, i32, vp, vp]
+    L.sf_kv4_keep.restype = ctypes.c_int
+    L.sf_sample.argtypes = [ctypes.POINTER(SampleDesc), vp]
+    L.sf_sample.restype = ctypes.c_int
+    L.sf_quant_i8.argtypes = [vp, i64, i32, i32, i32, vp, i64, vp, vp]
+    L.sf_quant_i8.restype = ctypes.c_int
+    L.sf_gemm_i8_workspace_bytes.argtypes = [ctypes.POINTER(GemmI8Desc)]
+    L.sf_gemm_i8_workspace_bytes.restype = ctypes.c_size_t
+    L.sf_gemm_i8.argtypes = [ctypes.POINTER(GemmI8Desc), vp, ctypes.c_size_t, vp]
+    L.sf_gemm_i8.restype = ctypes.c_int
     L.sf_strerror.argtypes = [ctypes.c_int]
     L.sf_strerror.restype = ctypes.c_char_p
     _lib = L

@@ -1,5 +1,6 @@
-"""Torch-tensor front ends for `sf_attn_fwd` and for the 4-bit key / value
-cache with `sf_attn_kv4` (tests and bench plumbing).
+"""Torch-tensor front ends for `sf_attn_fwd`, for the 4-bit key / value cache
+with `sf_attn_kv4`, and for trees of drafted tokens over it (tests and bench
+plumbing).
 
 torch supplies device memory and the current HIP stream; the arithmetic runs
 in libsf_hip_kernels.so.  Mirrors IBackend::attention
@@ -10,6 +11,7 @@ semantics as documented on `sf_attn_desc`.
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 import struct
 
 import torch
@@ -142,6 +144,68 @@ class Kv4Cache:
                         S, k.data_ptr(), st, v.data_ptr(), st, _DT[dtype])
         return k, v
 
+    def keep(self, nodes, first):
+        """Of the tokens from slot first[b] on (int32 [B]) keeps those that
+        nodes (int32 [B, n], accept_tree's) names, in its order: the one at
+        first[b] + nodes[b, i] moves to first[b] + i.  Negative nodes, and slots
+        outside [0, capacity), are left out."""
+        dev = self.data.device
+        nodes_ptr = _ints(nodes, "nodes", (self.B, nodes.shape[-1]), dev)
+        kernels.call_on(dev, "sf_kv4_keep", abi.lib().sf_kv4_keep, ctypes.byref(abi.Kv4CacheDesc(*self.fields())), nodes_ptr,
+                        nodes.shape[-1], _ints(first, "first", (self.B,), dev))
+
+
+def _ints(t, name, shape, device):
+    """The pointer of a contiguous device int32 tensor of `shape`."""
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{name}{tuple(t.shape)} {t.dtype}: contiguous int32 {tuple(shape)} on {device}, a device, expected")
+    return t.data_ptr()
+
+
+@dataclasses.dataclass(frozen=True)
+class DraftTree:
+    """A tree of T drafted tokens, or one for each of B batch elements (draft_tree)."""
+
+    parents: torch.Tensor   # int32 [1 or B, T]
+    masks: torch.Tensor     # int32 [1 or B, T, ceil(T / 32)]: a node's ancestors and itself, a bit each
+    depth: torch.Tensor     # int32 [1 or B, T]: a node's number of ancestors
+
+
+def draft_tree(parents):
+    """The tables of trees of drafted tokens.  parents: device int32 [T] or [1,
+    T] (one tree for all batch elements) or [B, T]; node 0 is the root, the last
+    token already decided, and a node's parent comes before it (-1, or any other
+    value, for none).  A node's position is the root's plus its depth."""
+    if parents.dim() == 1:
+        parents = parents[None]
+    if parents.dim() != 2:
+        raise ValueError(f"parents{tuple(parents.shape)}: [T] or [B, T] expected")
+    dev, (n, T) = parents.device, parents.shape
+    ptr = _ints(parents, "parents", (n, T), dev)
+    masks = torch.empty(n, T, (T + 31) // 32, dtype=torch.int32, device=dev)
+    depth = torch.empty(n, T, dtype=torch.int32, device=dev)
+    kernels.call_on(dev, "sf_tree_build", abi.lib().sf_tree_build, ptr, n, T, masks.data_ptr(), depth.data_ptr())
+    return DraftTree(parents, masks, depth)
+
+
+def accept_tree(tree, drafted, sampled):
+    """The path of drafted tokens that sampled ones confirm: (nodes [B, T], count
+    [B], tokens [B, T]), int32.  drafted, sampled: int32 [B, T], the nodes'
+    tokens and the token sampled behind each.  From the root on the first child
+    whose drafted token is the node's sampled one follows; nodes and the tokens
+    sampled along them, -1 behind the end."""
+    dev, T = tree.parents.device, tree.parents.shape[1]
+    B = drafted.shape[0]
+    if tree.parents.shape[0] not in (1, B):
+        raise ValueError(f"{tree.parents.shape[0]} trees for {B} batch elements")
+    d_ptr, s_ptr = _ints(drafted, "drafted", (B, T), dev), _ints(sampled, "sampled", (B, T), dev)
+    nodes, tokens = (torch.empty(B, T, dtype=torch.int32, device=dev) for _ in range(2))
+    count = torch.empty(B, dtype=torch.int32, device=dev)
+    kernels.call_on(dev, "sf_tree_accept", abi.lib().sf_tree_accept, tree.parents.data_ptr(),
+                    1 if tree.parents.shape[0] > 1 else 0, d_ptr, s_ptr, B, T, nodes.data_ptr(), count.data_ptr(),
+                    tokens.data_ptr())
+    return nodes, count, tokens
+
 
 # sf_attn_kv4_desc in one pack.
 _KV4_DESC = struct.Struct("@4if5i2Pq3q3qP4i")
@@ -149,15 +213,18 @@ assert _KV4_DESC.size == ctypes.sizeof(abi.AttnKv4Desc)
 
 
 def attention_kv4(q, cache, out=None, scale=0.0, is_causal=False, valid_len=None, kv_mask=None, keys=None,
-                  num_splits=0, out_dtype=None, workspace=None, exact_pv=False):
+                  num_splits=0, out_dtype=None, workspace=None, exact_pv=False, tree=None):
     """softmax(q K^T scale) V over a Kv4Cache: q [B, Hq, Sq, D] bf16 or fp16
     (any strides with a contiguous last axis), Hq a multiple of the cache's H.
     keys: how many slots are read at most (the capacity); valid_len: device
     int32 [B] lengths; kv_mask: device bool [B, keys] (True = attend);
     is_causal: query s is the token at valid_len - Sq + s.  exact_pv: weights
     as bf16 (hi, lo) pairs also where a bf16 output of many rows takes weights
-    and values in fp16 (6e-4 of the output's norm; sf_attn_kv4_desc).  Runs on
-    torch's current stream; a row that sees nothing is zeros."""
+    and values in fp16 (6e-4 of the output's norm; sf_attn_kv4_desc).  tree
+    (draft_tree): the last T cached tokens of each sequence are the tree's nodes,
+    the queries the last Sq of them, and each sees what lies before the nodes,
+    its ancestors and itself.  Runs on torch's current stream; a row that sees
+    nothing is zeros."""
     dev, shape = cache.data.device, q.shape
     if len(shape) != 4 or shape[0] != cache.B or shape[3] != cache.D or shape[1] % cache.H:
         raise ValueError(f"q{tuple(shape)} over a cache of B {cache.B}, H {cache.H}, D {cache.D}")
@@ -184,10 +251,18 @@ def attention_kv4(q, cache, out=None, scale=0.0, is_causal=False, valid_len=None
     raw = _KV4_DESC.pack(B, Hq, Sq, Sk, scale, _DT[q.dtype], _DT[out.dtype], 1 if is_causal else 0, int(num_splits),
                          1 if exact_pv else 0, valid_ptr, mask_ptr, mask_st, *kernels.strides_bhs(q), *kernels.strides_bhs(out),
                          *cache.fields())
-    d = ctypes.byref(abi.AttnKv4Desc.from_buffer_copy(raw))
+    args = (ctypes.byref(abi.AttnKv4Desc.from_buffer_copy(raw)),)
+    what, fn, need = "sf_attn_kv4", abi.lib().sf_attn_kv4, abi.lib().sf_attn_kv4_workspace_bytes
+    if tree is not None:
+        n, T = tree.parents.shape
+        if tree.masks.device != dev or n not in (1, B) or Sq > T or is_causal:
+            raise ValueError(f"{n} trees of {T} on {tree.masks.device} for {B} x {Sq} queries on {dev}"
+                             + (", not causal ones" if is_causal else ""))
+        args += (ctypes.byref(abi.DraftTreeDesc(tree.masks.data_ptr(), T, 1 if n > 1 else 0)),)
+        what, fn, need = "sf_attn_kv4_tree", abi.lib().sf_attn_kv4_tree, abi.lib().sf_attn_kv4_tree_workspace_bytes
     ws, n = None, 0
     if workspace is None:
-        n = abi.lib().sf_attn_kv4_workspace_bytes(d)
+        n = need(*args)
         if n:
             workspace = torch.empty(n, dtype=torch.uint8, device=dev)   # needs no init
             ws = workspace.data_ptr()
@@ -195,5 +270,5 @@ def attention_kv4(q, cache, out=None, scale=0.0, is_causal=False, valid_len=None
         if workspace.device != dev or not workspace.is_contiguous():
             raise ValueError(f"workspace must be a contiguous tensor on {dev}")
         ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    kernels.call_on(dev, "sf_attn_kv4", abi.lib().sf_attn_kv4, d, q.data_ptr(), out.data_ptr(), ws, n)
+    kernels.call_on(dev, what, fn, *args, q.data_ptr(), out.data_ptr(), ws, n)
     return out

@@ -75,7 +75,26 @@ struct KvAttnArgs {
     int64_t rows;
     int B, H, G, Sq, Sk, splits, qgroups, causal, out_kind;
     float scale_log2;
+    const uint32_t* tree;   // [B or 1][T][words]: bit i of a node's row is set where it sees node i
+    int64_t tree_stride;    // words between batch elements, 0 for one tree
+    int T, tree_words;
 };
+
+// A tree: the T nodes are the last T tokens, all before them are seen by every row.  Which of
+// the 32 tokens from key0 on the row of node `node` sees, the nodes' first token at key `at`:
+// two words of its ancestors, shifted (about one block in T / 32 + 1 asks).
+__device__ __forceinline__ uint32_t kv_tree_bits(const KvAttnArgs& p, int b, int node, int key0, int at) {
+    const uint32_t* row = p.tree + b * p.tree_stride + (int64_t)node * p.tree_words;
+    const int r = key0 - at, w = r >> 5;   // rounded down
+    const uint32_t lo = w < 0 ? ~0u : w < p.tree_words ? row[w] : 0u;
+    const uint32_t hi = w + 1 < 0 ? ~0u : w + 1 < p.tree_words ? row[w + 1] : 0u;
+    return (uint32_t)(((uint64_t)hi << 32 | lo) >> (r & 31));
+}
+
+// A lane's 8 tokens of a block's 32 bits: 4 g .. + 3 and 16 + 4 g .. + 3.
+__device__ __forceinline__ uint32_t kv_lane_bits(uint32_t bits, int g) {
+    return (bits >> (4 * g) & 15u) | (bits >> (16 + 4 * g) & 15u) << 4;
+}
 
 // N consecutive channels to out: kind 0 fp32, 1 bf16, 2 fp16 (stores of 2 N and 4 N bytes, N even).
 template <int N>
@@ -205,10 +224,11 @@ __device__ __forceinline__ void kv_finish(const KvAttnArgs& p, int split, int b,
 }
 
 // QT tiles of 16 query rows of a key head to a workgroup.
-template <bool F16, int D, int QT, int FORM, int NW>
+template <bool F16, int D, int QT, int FORM, int NW, bool TREE = false>
 __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
     constexpr int GR = D / 64, DT = D / 16;   // 64-channel groups, tiles of 16 channels
     constexpr bool PAIR = FORM != kKvHalf, EXACT = FORM == kKvExact;
+    static_assert(PAIR || !TREE, "rows of a tree see different tokens");
     __shared__ float xm[NW][QT * 16], xl[NW][QT * 16], xf[NW][QT * 16], xs[QT * 16];
     constexpr int kJoin = D == 128 && NW == 8 ? 1 : QT == 5 ? 3 : QT == 4 ? 2 : QT;   // tiles that meet at a time
     // 128 channels and two tiles leave no registers for the next raw block beside eight waves: it waits in LDS, brought
@@ -228,8 +248,8 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 
     const int len = p.valid ? min(max(p.valid[b], 0), p.Sk) : p.Sk;
     // Query s sees keys below len - Sq + s + 1 (causal) or len; the smallest and largest limit of the group's rows.
-    int lim_lo = len, lim_hi = len;
-    if (PAIR && p.causal) {
+    int lim_lo = TREE ? len - p.T : len, lim_hi = len;
+    if (PAIR && !TREE && p.causal) {
         const int q1 = min(q0 + 16 * QT, R) - 1;
         const bool one = q0 / p.Sq == q1 / p.Sq;
         lim_lo = len - p.Sq + 1 + (one ? q0 % p.Sq : 0);
@@ -322,6 +342,12 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                 const int key = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
                 if (key < len && (!p.mask || p.mask[b * p.mask_stride + key])) see |= 1u << e;
             }
+        }
+        uint32_t mine[TREE && masked ? QT : 1];   // the lane's tokens, by each tile's rows
+        if constexpr (TREE && masked) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+                mine[t] = kv_lane_bits(kv_tree_bits(p, b, p.T - p.Sq + min(q0 + 16 * t + col, R - 1) % p.Sq, key0, len - p.T), g);
         }
         float ks[GR][8], ko[GR][8], vs[GR][8], vm[GR][8];
 #pragma unroll
@@ -437,7 +463,12 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
                     x[4 * kt + e] = u;
                 }
             uint32_t row = see;
-            if (masked) {
+            if constexpr (TREE && masked) {
+                row &= mine[t];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!(row >> e & 1u)) x[e] = -INFINITY;
+            } else if (masked) {
                 const int limit = PAIR && p.causal ? len - p.Sq + 1 + min(q0 + 16 * t + col, R - 1) % p.Sq : len;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -590,7 +621,7 @@ __global__ __launch_bounds__(64 * NW) void attn_kv4_kernel(const KvAttnArgs p) {
 // 128 channels and NG = 2: a block's vector instructions go from 542 to about
 // 420, where they took 82% of the time; 16 x 8 key heads x 4 rows over 16384 keys
 // then stream 4.3 TB/s, of the 4.95 that a large copy reaches.
-template <bool F16, int D, int NG, bool EXACT>
+template <bool F16, int D, int NG, bool EXACT, bool TREE = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_token_kernel(const KvAttnArgs p) {
     constexpr int GR = D / 64, DT = D / 16, NW = 4, RT = 16 / NG;
     __shared__ float xm[NW * NG][RT], xl[NW * NG][RT], xf[NW * NG][RT], xs[RT], xtop[RT];
@@ -605,7 +636,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     const int len = p.valid ? min(max(p.valid[b], 0), p.Sk) : p.Sk;
     const int nblk = (len + kKvBlock - 1) / kKvBlock;   // the last token's row sees them all
     const int b0 = (int)((int64_t)nblk * split / p.splits), b1 = (int)((int64_t)nblk * (split + 1) / p.splits);
-    const int lim_lo = p.causal ? len - p.Sq + 1 : len, limit = p.causal ? len - p.Sq + 1 + qt : len;
+    const int lim_lo = TREE ? len - p.T : p.causal ? len - p.Sq + 1 : len;
+    const int limit = !TREE && p.causal ? len - p.Sq + 1 + qt : len;
 
     const uint8_t* base = p.cache + (int64_t)bh * p.cache_blocks * Kv4<D>::kBytes;
     u32x4 kc[NG][GR], vc[NG][GR], kp[GR][2], vp[GR][2];
@@ -689,6 +721,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
                     const int key = key0 + 16 * (e >> 2) + (e & 3);
                     if (key < limit && (!p.mask || p.mask[b * p.mask_stride + key])) see |= 1u << e;
                 }
+                if (TREE) see &= kv_lane_bits(kv_tree_bits(p, b, p.T - p.Sq + qt, kKvBlock * (blk + own), len - p.T), g);
             }
         }
         float x[8];
@@ -878,8 +911,8 @@ struct KvPlan {
 
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-static inline int kv_form(const sf_attn_kv4_desc* d) {   // with more than one tile of rows
-    const bool apart = d->is_causal && d->Sq > 1;   // rows that see different tokens
+static inline int kv_form(const sf_attn_kv4_desc* d, bool tree) {   // with more than one tile of rows
+    const bool apart = tree || (d->is_causal && d->Sq > 1);   // rows that see different tokens
     return d->out_dtype == SF_F32 ? kKvExact : d->out_dtype == SF_F16 || apart || d->exact_pv ? kKvPair : kKvHalf;
 }
 
@@ -942,11 +975,11 @@ static void kv_tiles(const sf_attn_kv4_desc* d, int64_t R, int64_t heads, KvPlan
     }
 }
 
-static KvPlan kv_plan(const sf_attn_kv4_desc* d) {
+static KvPlan kv_plan(const sf_attn_kv4_desc* d, bool tree) {
     KvPlan k = {};
     const int64_t R = (int64_t)(d->Hq / d->cache.H) * d->Sq, heads = (int64_t)d->B * d->cache.H;
     k.rows = (int64_t)d->B * d->Hq * d->Sq;
-    k.form = kv_form(d);
+    k.form = kv_form(d, tree);
     if (R <= 16) {
         k.qt = k.qgroups = 1;
         k.splits = d->num_splits > 0 ? d->num_splits : kv_splits_one_tile(d, heads);
@@ -973,18 +1006,64 @@ static int kv_attn_check(const sf_attn_kv4_desc* d) {
     return SF_OK;
 }
 
-}  // namespace sfk
-
-extern "C" size_t sf_attn_kv4_workspace_bytes(const sf_attn_kv4_desc* d) {
-    if (sfk::kv_attn_check(d) != SF_OK || !d->B || !d->Hq || !d->Sq) return 0;
-    const sfk::KvPlan k = sfk::kv_plan(d);
+static size_t kv_workspace(const sf_attn_kv4_desc* d, bool tree) {
+    const KvPlan k = kv_plan(d, tree);
     return k.splits > 1 ? (size_t)k.splits * (size_t)k.rows * (d->cache.D + 2) * sizeof(float) : 0;
 }
 
-extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, void* workspace, size_t workspace_bytes,
-                           void* stream) {
-    const int st = sfk::kv_attn_check(d);
-    if (st != SF_OK) return st;
+static int kv_tree_check(const sf_attn_kv4_desc* d, const sf_draft_tree* tree) {
+    if (!tree || d->is_causal || tree->T <= 0 || d->Sq > tree->T) return SF_EINVAL;
+    if (tree->T > SF_TREE_MAX_NODES) return SF_ENOTSUP;
+    return SF_OK;
+}
+
+template <bool F16, bool TREE>
+static void kv_launch(const KvAttnArgs& p, const KvPlan& k, int D, hipStream_t s) {
+    const dim3 grid((unsigned)k.wgs);
+#define SF_KV4_LAUNCH(DD, QT, FORM, NW) \
+    hipLaunchKernelGGL((attn_kv4_kernel<F16, DD, QT, FORM, NW, TREE>), grid, dim3(64 * NW), 0, s, p)
+#define SF_KV4_TOKEN(DD, NG, EXACT) hipLaunchKernelGGL((attn_kv4_token_kernel<F16, DD, NG, EXACT, TREE>), grid, dim3(256), 0, s, p)
+    const int form = k.form;
+    if (k.qt == 1 && form == kKvExact) {
+        if (D == 64) {
+            if (k.ng == 1) SF_KV4_LAUNCH(64, 1, kKvExact, 4);
+            else if (k.ng == 2) SF_KV4_TOKEN(64, 2, true);
+            else SF_KV4_TOKEN(64, 4, true);
+        } else {
+            if (k.ng == 1) SF_KV4_LAUNCH(128, 1, kKvExact, 4);
+            else SF_KV4_TOKEN(128, 2, true);
+        }
+    } else if (k.qt == 1) {
+        if (D == 64) {
+            if (k.ng == 1) SF_KV4_LAUNCH(64, 1, kKvPair, 4);
+            else if (k.ng == 2) SF_KV4_TOKEN(64, 2, false);
+            else SF_KV4_TOKEN(64, 4, false);
+        } else {
+            if (k.ng == 1) SF_KV4_LAUNCH(128, 1, kKvPair, 4);
+            else SF_KV4_TOKEN(128, 2, false);
+        }
+    } else if (form == kKvExact) {
+        if (D == 128) SF_KV4_LAUNCH(128, 2, kKvExact, 8);
+        else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, kKvExact, 8);
+        else SF_KV4_LAUNCH(64, 3, kKvExact, 8);
+    } else if (form == kKvPair) {
+        if (D == 128) SF_KV4_LAUNCH(128, 2, kKvPair, 8);
+        else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, kKvPair, 8);
+        else if (k.qt == 3) SF_KV4_LAUNCH(64, 3, kKvPair, 8);
+        else SF_KV4_LAUNCH(64, 4, kKvPair, 8);
+    } else if constexpr (!TREE) {
+        if (D == 128) SF_KV4_LAUNCH(128, 2, kKvHalf, 8);
+        else if (k.qt == 2) SF_KV4_LAUNCH(64, 2, kKvHalf, 8);
+        else if (k.qt == 3) SF_KV4_LAUNCH(64, 3, kKvHalf, 8);
+        else if (k.qt == 4) SF_KV4_LAUNCH(64, 4, kKvHalf, 8);
+        else SF_KV4_LAUNCH(64, 5, kKvHalf, 8);
+    }
+#undef SF_KV4_TOKEN
+#undef SF_KV4_LAUNCH
+}
+
+static int kv_attn(const sf_attn_kv4_desc* d, const sf_draft_tree* tree, const void* q, void* out, void* workspace,
+                   size_t workspace_bytes, void* stream) {
     if (!d->B || !d->Hq || !d->Sq) return SF_OK;
     if (d->in_dtype != SF_BF16 && d->in_dtype != SF_F16) return SF_ENOTSUP;
     if (d->out_dtype != SF_BF16 && d->out_dtype != SF_F16 && d->out_dtype != SF_F32) return SF_ENOTSUP;
@@ -995,11 +1074,11 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
     for (int i = 0; i < 3; ++i)
         if (d->q_stride[i] < 0 || (d->q_stride[i] & 7) || d->o_stride[i] < 0 || (d->o_stride[i] & 7)) return SF_EINVAL;
     if (d->kv_mask && d->kv_mask_stride < 0) return SF_EINVAL;
-    const sfk::KvPlan k = sfk::kv_plan(d);
-    if (k.wgs >= 1 << 23 || (k.splits > 1 && k.rows >= sfk::kKvMergeRows)) return SF_ENOTSUP;   // threads in 32 bits
-    if (k.splits > 1 && (!workspace || workspace_bytes < sf_attn_kv4_workspace_bytes(d))) return SF_EWORKSPACE;
+    const KvPlan k = kv_plan(d, tree != nullptr);
+    if (k.wgs >= 1 << 23 || (k.splits > 1 && k.rows >= kKvMergeRows)) return SF_ENOTSUP;   // threads in 32 bits
+    if (k.splits > 1 && (!workspace || workspace_bytes < kv_workspace(d, tree != nullptr))) return SF_EWORKSPACE;
     if (k.splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 3)) return SF_EINVAL;
-    sfk::KvAttnArgs p = {};
+    KvAttnArgs p = {};
     p.q = static_cast<const uint16_t*>(q);
     p.cache = static_cast<const uint8_t*>(d->cache.data);
     p.out = out;
@@ -1007,7 +1086,7 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
     p.valid = d->kv_valid_len;
     p.mask = d->kv_mask;
     p.mask_stride = d->kv_mask_stride;
-    p.cache_blocks = sfk::kv4_blocks(d->cache.capacity);
+    p.cache_blocks = kv4_blocks(d->cache.capacity);
     for (int i = 0; i < 3; ++i) p.qs[i] = d->q_stride[i], p.os[i] = d->o_stride[i];
     p.rows = k.rows;
     p.B = d->B;
@@ -1020,63 +1099,54 @@ extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, 
     p.causal = d->is_causal != 0;
     p.out_kind = d->out_dtype == SF_BF16 ? 1 : (d->out_dtype == SF_F16 ? 2 : 0);
     p.scale_log2 = (d->scale == 0.f ? 1.f / sqrtf((float)d->cache.D) : d->scale) * 1.4426950408889634f;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)k.wgs);
-    const bool f16 = d->in_dtype == SF_F16;
-#define SF_KV4_LAUNCH(DD, QT, FORM, NW)                                                                                       \
-    do {                                                                                                                      \
-        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_kernel<true, DD, QT, FORM, NW>), grid, dim3(64 * NW), 0, s, p);            \
-        else hipLaunchKernelGGL((sfk::attn_kv4_kernel<false, DD, QT, FORM, NW>), grid, dim3(64 * NW), 0, s, p);               \
-    } while (0)
-#define SF_KV4_TOKEN(DD, NG, EXACT)                                                                                           \
-    do {                                                                                                                      \
-        if (f16) hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<true, DD, NG, EXACT>), grid, dim3(256), 0, s, p);             \
-        else hipLaunchKernelGGL((sfk::attn_kv4_token_kernel<false, DD, NG, EXACT>), grid, dim3(256), 0, s, p);                \
-    } while (0)
-    const int form = k.form;
-    if (k.qt == 1 && form == sfk::kKvExact) {
-        if (d->cache.D == 64) {
-            if (k.ng == 1) SF_KV4_LAUNCH(64, 1, sfk::kKvExact, 4);
-            else if (k.ng == 2) SF_KV4_TOKEN(64, 2, true);
-            else SF_KV4_TOKEN(64, 4, true);
-        } else {
-            if (k.ng == 1) SF_KV4_LAUNCH(128, 1, sfk::kKvExact, 4);
-            else SF_KV4_TOKEN(128, 2, true);
-        }
-    } else if (k.qt == 1) {
-        if (d->cache.D == 64) {
-            if (k.ng == 1) SF_KV4_LAUNCH(64, 1, sfk::kKvPair, 4);
-            else if (k.ng == 2) SF_KV4_TOKEN(64, 2, false);
-            else SF_KV4_TOKEN(64, 4, false);
-        } else {
-            if (k.ng == 1) SF_KV4_LAUNCH(128, 1, sfk::kKvPair, 4);
-            else SF_KV4_TOKEN(128, 2, false);
-        }
-    } else if (d->cache.D == 128) {
-        if (form == sfk::kKvExact) SF_KV4_LAUNCH(128, 2, sfk::kKvExact, 8);
-        else if (form == sfk::kKvPair) SF_KV4_LAUNCH(128, 2, sfk::kKvPair, 8);
-        else SF_KV4_LAUNCH(128, 2, sfk::kKvHalf, 8);
-    } else if (form == sfk::kKvExact) {
-        if (k.qt == 2) SF_KV4_LAUNCH(64, 2, sfk::kKvExact, 8);
-        else SF_KV4_LAUNCH(64, 3, sfk::kKvExact, 8);
-    } else if (form == sfk::kKvPair) {
-        if (k.qt == 2) SF_KV4_LAUNCH(64, 2, sfk::kKvPair, 8);
-        else if (k.qt == 3) SF_KV4_LAUNCH(64, 3, sfk::kKvPair, 8);
-        else SF_KV4_LAUNCH(64, 4, sfk::kKvPair, 8);
-    } else {
-        if (k.qt == 2) SF_KV4_LAUNCH(64, 2, sfk::kKvHalf, 8);
-        else if (k.qt == 3) SF_KV4_LAUNCH(64, 3, sfk::kKvHalf, 8);
-        else if (k.qt == 4) SF_KV4_LAUNCH(64, 4, sfk::kKvHalf, 8);
-        else SF_KV4_LAUNCH(64, 5, sfk::kKvHalf, 8);
+    if (tree) {
+        p.tree = tree->masks;
+        p.T = tree->T;
+        p.tree_words = (tree->T + 31) / 32;
+        p.tree_stride = tree->each ? (int64_t)p.T * p.tree_words : 0;
     }
-#undef SF_KV4_TOKEN
-#undef SF_KV4_LAUNCH
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool f16 = d->in_dtype == SF_F16;
+    if (tree) {
+        if (f16) kv_launch<true, true>(p, k, d->cache.D, s);
+        else kv_launch<false, true>(p, k, d->cache.D, s);
+    } else {
+        if (f16) kv_launch<true, false>(p, k, d->cache.D, s);
+        else kv_launch<false, false>(p, k, d->cache.D, s);
+    }
     if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
     if (k.splits > 1) {
         const dim3 mg((unsigned)k.rows);
-        if (d->cache.D == 64) hipLaunchKernelGGL(sfk::attn_kv4_merge_kernel<64>, mg, dim3(256), 0, s, p);
-        else hipLaunchKernelGGL(sfk::attn_kv4_merge_kernel<128>, mg, dim3(256), 0, s, p);
+        if (d->cache.D == 64) hipLaunchKernelGGL(attn_kv4_merge_kernel<64>, mg, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL(attn_kv4_merge_kernel<128>, mg, dim3(256), 0, s, p);
         if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
     }
     return SF_OK;
+}
+
+}  // namespace sfk
+
+extern "C" size_t sf_attn_kv4_workspace_bytes(const sf_attn_kv4_desc* d) {
+    if (sfk::kv_attn_check(d) != SF_OK || !d->B || !d->Hq || !d->Sq) return 0;
+    return sfk::kv_workspace(d, false);
+}
+
+extern "C" int sf_attn_kv4(const sf_attn_kv4_desc* d, const void* q, void* out, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+    const int st = sfk::kv_attn_check(d);
+    return st != SF_OK ? st : sfk::kv_attn(d, nullptr, q, out, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t sf_attn_kv4_tree_workspace_bytes(const sf_attn_kv4_desc* d, const sf_draft_tree* tree) {
+    if (sfk::kv_attn_check(d) != SF_OK || sfk::kv_tree_check(d, tree) != SF_OK || !d->B || !d->Hq || !d->Sq) return 0;
+    return sfk::kv_workspace(d, true);
+}
+
+extern "C" int sf_attn_kv4_tree(const sf_attn_kv4_desc* d, const sf_draft_tree* tree, const void* q, void* out,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+    int st = sfk::kv_attn_check(d);
+    if (st == SF_OK) st = sfk::kv_tree_check(d, tree);
+    if (st != SF_OK) return st;
+    if (!tree->masks || (reinterpret_cast<uintptr_t>(tree->masks) & 3)) return SF_EINVAL;
+    return sfk::kv_attn(d, tree, q, out, workspace, workspace_bytes, stream);
 }

@@ -1,7 +1,7 @@
 """Torch-tensor front ends for sf_gemm, sf_rmsnorm, sf_add_rmsnorm,
-sf_dequant_int8, sf_gemm_w4 and sf_heads_rope (test and bench plumbing: torch
-supplies device memory and the stream; the arithmetic runs in
-libsf_hip_kernels.so)."""
+sf_dequant_int8, sf_gemm_w4, sf_heads_rope, sf_gemm_i8 and sf_sample (test and
+bench plumbing: torch supplies device memory and the stream; the arithmetic runs
+in libsf_hip_kernels.so)."""
 from __future__ import annotations
 
 import ctypes
@@ -471,3 +471,96 @@ def heads_rope(p, S, heads, D, gammas=(None, None), positions=None, inv_freq=Non
                 (Hq * S * D, S * D, D, Hk * S * D, S * D, D, Hv * S * D, S * D, D),
                 D, gammas, positions, inv_freq, interleaved, eps, cache, slots)
     return q, k, v
+
+
+# sf_gemm_i8_desc and sf_sample_desc in one pack each.
+_I8_DESC = struct.Struct("@3iPqiPPqPPiPq2i")
+assert _I8_DESC.size == ctypes.sizeof(abi.GemmI8Desc)
+_SAMPLE_DESC = struct.Struct("@2iPqi5Pfi2f2P")
+assert _SAMPLE_DESC.size == ctypes.sizeof(abi.SampleDesc)
+
+
+def quant_i8(x):
+    """Rows x [M, K] (fp32, bf16 or fp16; K a multiple of 16) as 8-bit codes:
+    (codes int8 [M, K], scale fp32 [M]), scale = max |x| / 127, code = x / scale
+    to the nearest, ties to even."""
+    _check(x, "x", _FLOATS, None, 2)
+    M, K = x.shape
+    codes = torch.empty(M, K, dtype=torch.int8, device=x.device)
+    scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    call_on(x.device, "sf_quant_i8", abi.lib().sf_quant_i8, x.data_ptr(), x.stride(0) if M > 1 else K, _DT[x.dtype], M, K,
+            codes.data_ptr(), K, scale.data_ptr())
+    return codes, scale
+
+
+def gemm_i8(a, w, w_scale, a_scale=None, bias=None, act=abi.SF_ACT_NONE, out=None, out_dtype=None, accumulate=False,
+            workspace=None):
+    """out[M, N] = act(a w^T + bias) in 8-bit integers: w int8 [N, K] with a
+    scale for each row (w_scale, fp32 [N]); a either codes and their scales
+    (quant_i8), or fp32, bf16 or fp16 rows, quantised first (workspace: where,
+    allocated unless given).  out_dtype a's unless given, bf16 for codes.
+    accumulate adds into an fp32 `out`."""
+    _check(w, "w", (torch.int8,), None, 2)
+    dev, (N, K) = w.device, w.shape
+    codes = a.dtype is torch.int8
+    _check(a, "a", (torch.int8,) if codes else _FLOATS, dev, 2)
+    M = a.shape[0]
+    if a.shape[1] != K:
+        raise ValueError(f"a{tuple(a.shape)} against weights [{N}, {K}]")
+    if codes != (a_scale is not None):
+        raise ValueError("a_scale goes with int8 codes, and only with them")
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate adds into out: give one")
+        out = torch.empty(M, N, dtype=out_dtype or (torch.bfloat16 if codes else a.dtype), device=dev)
+    else:
+        _check(out, "out", _FLOATS, dev, 2)
+        if out.shape != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError(f"out{tuple(out.shape)} {out.dtype}: [{M}, {N}] of {out_dtype or out.dtype} expected")
+    if w_scale is None:
+        raise ValueError("w_scale: a scale for each row of w")
+    raw = _I8_DESC.pack(M, N, K, a.data_ptr(), a.stride(0) if M > 1 else K, _DT[a.dtype],
+                        _vector(a_scale, "a_scale", torch.float32, M, dev), w.data_ptr(), w.stride(0) if N > 1 else K,
+                        _vector(w_scale, "w_scale", torch.float32, N, dev), _vector(bias, "bias", torch.float32, N, dev), act,
+                        out.data_ptr(), out.stride(0) if M > 1 else N, _DT[out.dtype], 1 if accumulate else 0)
+    d = ctypes.byref(abi.GemmI8Desc.from_buffer_copy(raw))
+    ws, n = None, 0
+    if workspace is not None:
+        if workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+        ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif not codes:
+        n = abi.lib().sf_gemm_i8_workspace_bytes(d)
+        workspace = torch.empty(n, dtype=torch.uint8, device=dev)   # needs no init
+        ws = workspace.data_ptr()
+    call_on(dev, "sf_gemm_i8", abi.lib().sf_gemm_i8, d, ws, n)
+    return out
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """A token from each row of logits [rows, V] (fp32, bf16 or fp16) by the
+    uniform numbers u (fp32 [rows], in [0, 1)): (tokens int32 [rows], logprobs
+    fp32 [rows]).  In falling order of logits, ties by index: the first top_k
+    (0: all), of these the fewest that reach top_p of their weight, of these the
+    ones of at least min_p times the largest; the token is the first whose
+    running weight exceeds u times what is left, the logprob that of its share.
+    temperature 0: the largest logit.  Each parameter is a number or, for a
+    value a row, a tensor (top_k int32, the others fp32); None is its default.  -1
+    and NaN for a row with a NaN or with nothing above -infinity."""
+    _check(logits, "logits", _FLOATS, None, 2)
+    dev, (rows, V) = logits.device, logits.shape
+    ptr, val = [], []
+    for name, t, none, dtype in (("temperature", temperature, 1.0, torch.float32), ("top_k", top_k, 0, torch.int32),
+                                 ("top_p", top_p, 1.0, torch.float32), ("min_p", min_p, 0.0, torch.float32)):
+        each = isinstance(t, torch.Tensor)
+        ptr.append(_vector(t, name, dtype, rows, dev) if each else 0)
+        val.append(none if each or t is None else t)
+    if u is None:
+        raise ValueError("u: a uniform number for each row")
+    token = torch.empty(rows, dtype=torch.int32, device=dev)
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    raw = _SAMPLE_DESC.pack(rows, V, logits.data_ptr(), logits.stride(0) if rows > 1 else V, _DT[logits.dtype],
+                            _vector(u, "u", torch.float32, rows, dev), *ptr, val[0], val[1], val[2], val[3],
+                            token.data_ptr(), logprob.data_ptr())
+    call_on(dev, "sf_sample", abi.lib().sf_sample, ctypes.byref(abi.SampleDesc.from_buffer_copy(raw)))
+    return token, logprob

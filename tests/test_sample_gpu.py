@@ -1,0 +1,173 @@
+"""sf_sample against its definition in 64 bits.
+
+Tokens are equal: weights are held to 2^-44 of the largest, and no case here puts
+u within that (times the vocabulary) of a border but where the sums are exact on
+both sides (equal logits).  A logprob is rounded to 32 bits once, from a value off by
+2^-40 at most."""
+import math
+
+import pytest
+import torch
+
+from servoflow_amd import kernels
+
+from _drafts import sample as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _logits(B, V, seed, dtype=F32, std=2.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, V, generator=g) * std
+    x.scatter_add_(1, torch.randint(0, V, (B, 9), generator=g), 3 * torch.rand(B, 9, generator=g) + 4)
+    return x.to(dtype)
+
+
+def _u(B, seed):
+    return torch.rand(B, generator=torch.Generator().manual_seed(seed + 99))
+
+
+def _check(x, u, t=1.0, k=0, p=1.0, mp=0.0, what=""):
+    """Every parameter a number or a list of one a row."""
+    B = x.shape[0]
+    dev = lambda v, dt: torch.tensor(v, dtype=dt, device=DEV) if isinstance(v, list) else v   # noqa: E731
+    tok, lp = kernels.sample(x if x.is_cuda else x.to(DEV), u.to(DEV), dev(t, F32), dev(k, torch.int32), dev(p, F32), dev(mp, F32))
+    x = x.cpu()
+    for b in range(B):
+        at = lambda v: float(torch.tensor(v[b] if isinstance(v, list) else v, dtype=F32))   # noqa: E731
+        want, ref = plain(x[b], float(u[b]), at(t), int(k[b] if isinstance(k, list) else k), at(p), at(mp))
+        assert int(tok[b]) == want, (what, b, int(tok[b]), want)
+        got = float(lp[b])
+        if math.isnan(ref):
+            assert math.isnan(got)
+        else:
+            assert abs(got - ref) <= 2.0 ** -24 * abs(ref) + 2.0 ** -40, (what, b, got, ref)
+    return tok
+
+
+RULES = [{}, {"t": 0.7}, {"k": 50}, {"p": 0.9}, {"mp": 0.05}, {"t": 1.3, "k": 40, "p": 0.8, "mp": 0.02}, {"k": 1}, {"t": 0.0},
+         {"p": 0.999, "t": 2.0}, {"k": 3000, "p": 0.95}]
+
+
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 63, 64, 65, 1000, 2047, 2049, 5001, 32000])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_rules(V, dtype):
+    B = 3
+    for i, r in enumerate(RULES):
+        _check(_logits(B, V, V + i, dtype), _u(B, V + i), what=str(r), **r)
+
+
+@pytest.mark.parametrize("V,dtype", [(131072, BF), (131073, FP), (200001, F32), (1 << 20, BF)])
+def test_large_vocabularies(V, dtype):
+    for i, r in enumerate(RULES):
+        _check(_logits(2, V, i, dtype), _u(2, i), what=str(r), **r)
+
+
+def test_parameters_a_row():
+    B = 12
+    x, u = _logits(B, 4000, 5, BF), _u(B, 5)
+    _check(x, u, t=[0.0, 1.0, 0.5, 2.0, -1.0, 1e-30, 1e30, math.inf, 1.0, 1.0, 1.0, 1.0],
+           k=[0, 1, 5, 4000, 9, 0, 0, 0, -3, 2 ** 31 - 1, 4001, 7], p=[0.5, 1.0, 0.3, 0.99, 0.2, 1.0, 1.0, 1.0, 0.0, -1.0, 1.5, 0.6],
+           mp=[0.0, 0.0, 0.1, 0.0, 0.5, 0.0, 0.0, 0.0, 0.0, 0.2, 1.0, 2.0])
+
+
+def test_views_and_alignment():
+    for dtype in (BF, F32):
+        wide = _logits(5, 3011, 8, dtype).to(DEV)
+        for at, V in ((0, 3000), (1, 3000), (3, 2999), (7, 3), (9, 1)):
+            x = wide[:, at:at + V]
+            _check(x, _u(5, at), k=30, what=f"{at} {V}")
+    one = _logits(1, 500, 3, BF).to(DEV)
+    _check(one[:, 1:], _u(1, 3))
+
+
+@pytest.mark.parametrize("V", [3, 1000, 5000, 131072])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_equal_logits(V, dtype):
+    """Ties go by index: token n of V is the one whose range of 1 / V holds u; sums are exact."""
+    x = torch.full((6, V), -1.25, dtype=dtype)
+    u = torch.tensor([0.0, 0.24, 0.5, 0.77, 0.9999, 1 - 2.0 ** -24])
+    _check(x, u)
+    _check(x, u, k=max(1, V // 3))
+    _check(x, u, p=0.5)
+    _check(x, u, t=0.0)
+    x[:, V // 2] = 0.5   # one above, its own weight
+    _check(x, u, t=0.5)
+    _check(x, u, p=[0.1, 0.3, 0.61, 0.72, 0.9, 0.95])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("V,std", [(131072, 0.01), (131072, 0.3), (60000, 1e-4), (60000, 1e-6)])
+def test_flat_rows(V, dtype, std):
+    """Thousands of tokens in one bucket: parts of its keys, down to one value."""
+    B = 4
+    x = torch.randn(B, V, generator=torch.Generator().manual_seed(3)) * std + 1.0
+    x = x.to(dtype)
+    u = _u(B, 7)
+    for r in ({}, {"p": 0.4}, {"k": V // 2}, {"k": V // 3, "p": 0.37}, {"k": 5000, "p": 0.9, "mp": 0.5}, {"t": 30.0}):
+        _check(x, u, what=f"{r}", **r)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_masked_and_special_logits(dtype):
+    V = 3000
+    low = torch.finfo(dtype).min
+    x = _logits(9, V, 4, dtype)
+    x[0] = -math.inf                       # nothing
+    x[1, 5:] = -math.inf
+    x[2, torch.arange(V) != 1234] = -math.inf
+    x[3, 17] = math.nan
+    x[4, [40, 2000]] = math.inf            # the two share all the weight
+    x[5, 100:] = low                       # masks of the type's lowest value
+    x[6] = low                             # every token masked so: all the same
+    x[7, ::2] = -math.inf
+    x[8, :] = torch.where(torch.arange(V) % 3 == 0, 0.0, -0.0)   # equal
+    for r in ({}, {"k": 10}, {"p": 0.7}, {"mp": 0.3}, {"t": 0.0}, {"t": 5.0, "k": 2000, "p": 0.9}):
+        tok = _check(x, torch.tensor([0.3, 0.9, 0.5, 0.5, 0.75, 0.99, 0.3334, 0.6, 0.5]), what=str(r), **r)
+        assert tok[0] == -1 and tok[3] == -1
+
+
+def test_u_at_its_ends():
+    x = _logits(6, 777, 9)
+    u = torch.tensor([0.0, 1 - 2.0 ** -24, 2.0 ** -149, 0.5, 2.0 ** -24, 0.0])
+    _check(x, u)
+    a, _ = kernels.sample(x[:3].to(DEV), torch.tensor([1.0, -1.0, math.nan], device=DEV), top_k=20)
+    b, _ = kernels.sample(x[:3].to(DEV), torch.tensor([1 - 2.0 ** -24, 0.0, 0.0], device=DEV), top_k=20)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("r", [{"t": 0.9}, {"k": 7}, {"p": 0.8}])
+def test_frequencies(r):
+    """u on a grid of N gives every token N times its share, but for one at each end."""
+    N, V = 4096, 300
+    row = _logits(1, V, 2, F32)
+    u = (torch.arange(N) + 0.5) / N
+    dev = {"t": "temperature", "k": "top_k", "p": "top_p"}
+    tok, lp = kernels.sample(row.expand(N, V).contiguous().to(DEV), u.to(DEV), **{dev[a]: b for a, b in r.items()})
+    share = torch.zeros(V, dtype=torch.float64)
+    share[tok.cpu().long()] = torch.exp(lp.cpu().double())
+    assert 1 - V / N < float(share.sum()) <= 1 + 1e-6   # a token that no u of the grid meets has less than 1 / N, V of them V / N
+    got = torch.bincount(tok.cpu().long(), minlength=V).double()
+    assert ((got - N * share).abs() <= 1.001).all()
+
+
+def test_runs_are_equal():
+    x, u = _logits(64, 50001, 6, BF).to(DEV), _u(64, 6).to(DEV)
+    first = kernels.sample(x, u, temperature=1.5, top_p=0.97)
+    for _ in range(5):
+        again = kernels.sample(x, u, temperature=1.5, top_p=0.97)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    alone = torch.cat([kernels.sample(x[i:i + 1], u[i:i + 1], temperature=1.5, top_p=0.97)[0] for i in range(64)])
+    assert torch.equal(first[0], alone)
+
+
+def test_no_rows_and_refusals():
+    x, u = torch.zeros(2, 10, device=DEV), torch.zeros(2, device=DEV)
+    tok, lp = kernels.sample(x[:0], u[:0])
+    assert tok.shape == lp.shape == (0,)
+    for kw in ({"u": u[:1]}, {"u": None}, {"temperature": u[:1]}, {"top_k": u}, {"top_p": u.double()}, {"logits": x.double()},
+               {"logits": x.t()}, {"logits": x[0]}):
+        with pytest.raises(ValueError):
+            kernels.sample(**{"logits": x, "u": u, **kw})
