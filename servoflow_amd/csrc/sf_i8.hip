@@ -5,12 +5,11 @@
 // a = x / s_m to the nearest, ties to even, exactly -- the quotient by a
 // reciprocal, then put right by the sign of what is left of x.
 //
-// A workgroup of eight waves takes 64 MI x 128 NI outputs, 2 x 4 waves of MI x NI
-// tiles of v_mfma_i32_32x32x32_i8.  128 inputs of both operands at a time go
-// straight from memory into LDS, rows of 128 bytes whose pieces of 16 are placed by the
-// row (piece c of row r at c ^ (r / 2 & 7)), so that the 16 rows that a read of 16 bytes
-// takes at a time lie in different banks.  The next 128 inputs are on their way while
-// these are multiplied.
+// Many rows: a workgroup multiplies tiles of v_mfma_i32_32x32x32_i8 from LDS, 128
+// inputs of both operands at a time, which come straight from memory.  A row's 128 bytes
+// lie there in pieces of 16, piece c of row r at c ^ (r / 2 & 7): the 16 rows that a
+// read of 16 bytes takes at a time then lie in different banks.  Few rows: see
+// gemm_i8_rows_kernel.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -126,16 +125,33 @@ struct I8Args {
     int mt, nt;   // tiles
 };
 
+// Scales and bias of four columns from n on (0 behind the last).
+struct I8Columns {
+    f32x4 scale, bias;
+};
+__device__ __forceinline__ I8Columns i8_columns(const I8Args& p, int n) {
+    I8Columns c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool in = n + i < p.N;
+        c.scale[i] = in ? p.w_scale[n + i] : 0.f;
+        c.bias[i] = in && p.bias ? p.bias[n + i] : 0.f;
+    }
+    return c;
+}
+
 // Four columns of a row of C, from column n.
-__device__ __forceinline__ void i8_store(const I8Args& p, int m, int n, i32x4 acc) {
+__device__ __forceinline__ void i8_store(const I8Args& p, int m, int n, i32x4 acc, float s, const I8Columns& c4) {
     if (m >= p.M || n >= p.N) return;
-    const float s = p.a_scale[m];
     const int64_t at = (int64_t)m * p.ldc + n;
     const int cols = min(4, p.N - n);
     float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        v[i] = i < cols ? apply_act(p.act, (float)acc[i] * s * p.w_scale[n + i] + (p.bias ? p.bias[n + i] : 0.f)) : 0.f;
+    for (int i = 0; i < 4; ++i) v[i] = (float)acc[i] * s * c4.scale[i] + c4.bias[i];
+    if (p.act) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = apply_act(p.act, v[i]);
+    }
     if (cols == 4 && p.vec4) {
         if (p.c_kind == 0) {
             f32x4* c = reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at);
@@ -173,31 +189,63 @@ __device__ __forceinline__ void i8_tile(const I8Args& p, int& tm, int& tn) {
     tn = 4 * band + in % wide;
 }
 
-template <int MI, int NI>
-__global__ __launch_bounds__(512) void gemm_i8_kernel(const I8Args p) {
-    constexpr int BM = 64 * MI, BN = 128 * NI, kStage = (BM + BN) * 128;
-    __shared__ __attribute__((aligned(1024))) int8_t lds[2 * kStage];
+// WM x WN waves of MI x NI tiles each.  128 inputs of both operands are a stage, whole lines of memory (with stages of 64
+// inputs, two to a line, the loads alone took 217 us of 4096 x 8192 x 8192, so 166); STAGES of them in a ring.  A quarter's
+// operands are read under the products of the one before it, those of the next stage's first under the last one's,
+// behind the one barrier of a stage.
+template <int MI, int NI, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(const I8Args p) {
+    constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, NW = WM * WN, kStage = (BM + BN) * 128;
+    constexpr int kLoads = (BM + BN) / 8 / NW;   // instructions of a wave, 8 rows each
+    static_assert(BM % 8 == 0 && kLoads * 8 * NW == BM + BN, "whole instructions");
+    // One array: beside a second one the compiler waits for every load into LDS before each read from it.
+    __shared__ __attribute__((aligned(1024))) int8_t lds[STAGES * kStage + 4 * (BM + 2 * BN)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave >> 2, wn = wave & 3, col = lane & 31, g = lane >> 5;
+    const int wm = wave / WN, wn = wave % WN, col = lane & 31, g = lane >> 5;
     int tm, tn;
     i8_tile(p, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int rows = min(BM, p.M - m0), cols = min(BN, p.N - n0);
+    // Scales and bias wait in LDS: read from memory tile by tile at the end they cost 25 us of a 256 x 256 tile.
+    float* w_scale = reinterpret_cast<float*>(lds + STAGES * kStage);
+    float* bias = w_scale + BN;
+    float* a_scale = bias + BN;
+    static_assert(BM <= 64 * NW && BN <= 64 * NW, "a thread for each");
+    if ((int)threadIdx.x < BM) a_scale[threadIdx.x] = (int)threadIdx.x < rows ? p.a_scale[m0 + threadIdx.x] : 0.f;
+    if ((int)threadIdx.x < BN) {
+        const bool in = (int)threadIdx.x < cols;
+        w_scale[threadIdx.x] = in ? p.w_scale[n0 + threadIdx.x] : 0.f;
+        bias[threadIdx.x] = in && p.bias ? p.bias[n0 + threadIdx.x] : 0.f;
+    }
     const __amdgpu_buffer_rsrc_t ars = make_rsrc(p.a + (int64_t)m0 * p.lda, (uint32_t)((rows - 1) * (int)p.lda + p.K));
     const __amdgpu_buffer_rsrc_t wrs = make_rsrc(p.w + (int64_t)n0 * p.ldw, (uint32_t)((cols - 1) * (int)p.ldw + p.K));
-    // An instruction brings 8 rows of 128 bytes: lane l the place l & 7 of row l >> 3.
-    const int row = lane >> 3, place = lane & 7;
-    auto fetch = [&](int k0, int8_t* to) __attribute__((always_inline)) {
+    // Lane l brings the place l & 7 of row l >> 3: of row r the inputs 16 (place ^ (r / 2 & 7)).  Rows behind the last, and
+    // inputs behind K, are behind the buffer's end and come as zeros.
+    uint32_t at[kLoads];
+    int k_lane[2];   // of rows 0 .. 7 and 8 .. 15 of 16
 #pragma unroll
-        for (int i = 0; i < (BM + BN) / 64; ++i) {
-            const int r8 = 8 * (8 * i + wave);   // of the stage; BM is a multiple of 64
-            const bool is_a = i < BM / 64;
-            const int r = (is_a ? r8 : r8 - BM) + row;
-            const int k = k0 + 16 * (place ^ (r >> 1 & 7));
-            const int limit = is_a ? rows : cols;
-            const uint32_t at = r < limit && k < p.K ? (uint32_t)r * (uint32_t)(is_a ? p.lda : p.ldw) + (uint32_t)k : 0x80000000u;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(is_a ? ars : wrs, (__attribute__((address_space(3))) void*)(to + 128 * r8), 16,
-                                                     at, 0, 0, 0);
+    for (int i = 0; i < 2; ++i) k_lane[i] = 16 * ((lane & 7) ^ (4 * i + (lane >> 4)));
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int piece = i * NW + wave;
+        const bool is_a = piece < BM / 8;
+        const int r = 8 * (is_a ? piece : piece - BM / 8) + (lane >> 3);
+        at[i] = r < (is_a ? rows : cols) ? (uint32_t)r * (uint32_t)(is_a ? p.lda : p.ldw) + (uint32_t)k_lane[piece & 1] : 0x80000000u;
+    }
+    auto fetch = [&](int s, int8_t* to) __attribute__((always_inline)) {
+        const int k0 = 128 * s;
+        auto load = [&](int i, uint32_t off) __attribute__((always_inline)) {
+            const int piece = i * NW + wave;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(piece < BM / 8 ? ars : wrs,
+                                                     (__attribute__((address_space(3))) void*)(to + 1024 * piece), 16, off, 0, 0, 0);
+        };
+        if (k0 + 128 <= p.K) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) load(i, at[i] + (uint32_t)k0);   // behind the end stays there: k0 is below 2^17
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                load(i, k0 + k_lane[(i * NW + wave) & 1] < p.K ? at[i] + (uint32_t)k0 : 0x80000000u);
         }
     };
     i32x16 acc[NI][MI];
@@ -207,52 +255,204 @@ __global__ __launch_bounds__(512) void gemm_i8_kernel(const I8Args p) {
         for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[j][i][e] = 0;
-    fetch(0, lds);
+    i32x4 x[2][MI], w[2][NI];
+    // Quarter kk of a stage: lane (col, g) holds piece 2 kk + g of its row.
+    auto operands = [&](const int8_t* from, int kk) __attribute__((always_inline)) {
+        auto read = [&](int r0) __attribute__((always_inline)) {
+            const int r = r0 + col;
+            return *reinterpret_cast<const i32x4*>(from + 128 * r + 16 * ((2 * kk + g) ^ (r >> 1 & 7)));
+        };
+#pragma unroll
+        for (int j = 0; j < NI; ++j) w[kk & 1][j] = read(BM + 32 * (NI * wn + j));
+#pragma unroll
+        for (int i = 0; i < MI; ++i) x[kk & 1][i] = read(32 * (MI * wm + i));
+    };
+    auto multiply = [&](int kk) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[kk & 1][j], x[kk & 1][i], acc[j][i], 0, 0, 0);
+    };
+    // What the wave has read is in registers and its loads of the stage that follows are in LDS; so it is of every wave behind
+    // the barrier.
+    auto meet = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
     const int steps = (p.K + 127) / 128;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) fetch(i, lds + i * kStage);   // behind K: zeros
+    meet();
+    int here = 0, last = (STAGES - 1) * kStage;   // the stage that is multiplied, and the place of the one before it
+    operands(lds, 0);
     for (int s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        const int8_t* from = lds + (s & 1) * kStage;
-        if (s + 1 < steps) fetch(128 * (s + 1), lds + (1 - (s & 1)) * kStage);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            i32x4 x[MI], w[NI];
-#pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                const int r = 32 * (MI * wm + i) + col;
-                x[i] = *reinterpret_cast<const i32x4*>(from + 128 * r + 16 * ((2 * kk + g) ^ (r >> 1 & 7)));
-            }
-#pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                const int r = 32 * (NI * wn + j) + col;
-                w[j] = *reinterpret_cast<const i32x4*>(from + 128 * (BM + r) + 16 * ((2 * kk + g) ^ (r >> 1 & 7)));
-            }
-#pragma unroll
-            for (int j = 0; j < NI; ++j)
-#pragma unroll
-                for (int i = 0; i < MI; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[j], x[i], acc[j][i], 0, 0, 0);
-        }
+        fetch(s + STAGES - 1, lds + last);   // every wave has read what is there
+        operands(lds + here, 1);
+        multiply(0);
+        operands(lds + here, 2);
+        multiply(1);
+        operands(lds + here, 3);
+        multiply(2);
+        meet();
+        last = here;
+        here = here == (STAGES - 1) * kStage ? 0 : here + kStage;
+        operands(lds + here, 0);   // behind the last stage: not used
+        multiply(3);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing comes into LDS behind the end
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MI; ++i) {
+        const int m = 32 * (MI * wm + i) + col;
+        const float sm = a_scale[m];
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                i8_store(p, m0 + 32 * (MI * wm + i) + col, n0 + 32 * (NI * wn + j) + 8 * q + 4 * g,
-                         i32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]});
+            for (int q = 0; q < 4; ++q) {
+                const int n = 32 * (NI * wn + j) + 8 * q + 4 * g;
+                const I8Columns c = {*reinterpret_cast<const f32x4*>(w_scale + n), *reinterpret_cast<const f32x4*>(bias + n)};
+                i8_store(p, m0 + m, n0 + n, i32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]},
+                         sm, c);
+            }
+    }
 }
 
-template <int MI, int NI>
+// Few rows: MB tiles of 16 rows against NT tiles of 16 columns to a workgroup, whose eight waves deal the inputs, 128 at a
+// time, and join in LDS.  Both operands go straight into registers, DEPTH blocks of inputs ahead; the weights are read once.
+template <int MB, int NT, int DEPTH>
+__global__ __launch_bounds__(512) void gemm_i8_rows_kernel(const I8Args p) {
+    constexpr int NW = 8;
+    __shared__ i32x4 sums[NW][MB * NT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int n0 = 16 * NT * blockIdx.x, m0 = 16 * MB * blockIdx.y;
+    const int rows = min(16 * MB, p.M - m0), cols = min(16 * NT, p.N - n0);
+    const __amdgpu_buffer_rsrc_t ars = make_rsrc(p.a + (int64_t)m0 * p.lda, (uint32_t)((rows - 1) * (int)p.lda + p.K));
+    const __amdgpu_buffer_rsrc_t wrs = make_rsrc(p.w + (int64_t)n0 * p.ldw, (uint32_t)((cols - 1) * (int)p.ldw + p.K));
+    uint32_t wat[NT], xat[MB];   // rows behind the last repeat it; they are not stored
+#pragma unroll
+    for (int t = 0; t < NT; ++t) wat[t] = (uint32_t)min(16 * t + r, cols - 1) * (uint32_t)p.ldw;
+#pragma unroll
+    for (int b = 0; b < MB; ++b) xat[b] = (uint32_t)min(16 * b + r, rows - 1) * (uint32_t)p.lda;
+    constexpr int kUnits = (NT * MB + NW - 1) / NW;   // tiles that a wave joins and stores
+    float sm[kUnits];
+    I8Columns cn[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        const int u = wave + i * NW, m = m0 + 16 * (u % MB) + r;
+        if (u >= NT * MB) break;
+        sm[i] = m < p.M ? p.a_scale[m] : 0.f;
+        cn[i] = i8_columns(p, n0 + 16 * (u / MB) + 4 * g);
+    }
+    i32x4 acc[NT][MB];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[t][b] = i32x4{0, 0, 0, 0};
+    i32x4 w[DEPTH][NT][2], x[DEPTH][MB][2];
+    auto load = [&](int d, int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t k = 128u * kb + 64u * j + 16u * g;
+            const bool in = (int)k < p.K;   // behind K: zeros
+#pragma unroll
+            for (int t = 0; t < NT; ++t) w[d][t][j] = __builtin_bit_cast(i32x4, buffer_load16(wrs, in ? wat[t] + k : 0x80000000u));
+#pragma unroll
+            for (int b = 0; b < MB; ++b) x[d][b][j] = __builtin_bit_cast(i32x4, buffer_load16(ars, in ? xat[b] + k : 0x80000000u));
+        }
+    };
+    const int blocks = (p.K + 127) / 128;
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (wave + d * NW < blocks) load(d, wave + d * NW);
+    for (int kb = wave; kb < blocks; kb += DEPTH * NW) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (kb + d * NW >= blocks) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) acc[t][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d][t][j], x[d][b][j], acc[t][b], 0, 0, 0);
+            if (kb + (d + DEPTH) * NW < blocks) load(d, kb + (d + DEPTH) * NW);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) sums[wave][t * MB + b][lane] = acc[t][b];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        const int u = wave + i * NW;
+        if (u >= NT * MB) break;
+        i32x4 v = sums[0][u][lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v += sums[w][u][lane];
+        i8_store(p, m0 + 16 * (u % MB) + r, n0 + 16 * (u / MB) + 4 * g, v, sm[i], cn[i]);
+    }
+}
+
+template <int MI, int NI, int WM, int WN, int STAGES>
 static void launch_i8(I8Args p, hipStream_t s) {
-    p.mt = (p.M + 64 * MI - 1) / (64 * MI);
-    p.nt = (p.N + 128 * NI - 1) / (128 * NI);
-    hipLaunchKernelGGL((gemm_i8_kernel<MI, NI>), dim3((unsigned)(p.mt * p.nt)), dim3(512), 0, s, p);
+    p.mt = (p.M + 32 * MI * WM - 1) / (32 * MI * WM);
+    p.nt = (p.N + 32 * NI * WN - 1) / (32 * NI * WN);
+    hipLaunchKernelGGL((gemm_i8_kernel<MI, NI, WM, WN, STAGES>), dim3((unsigned)(p.mt * p.nt)), dim3(64 * WM * WN), 0, s, p);
+}
+
+template <int MB, int NT, int DEPTH>
+static void launch_i8_rows(const I8Args& p, hipStream_t s) {
+    const dim3 grid((unsigned)((p.N + 16 * NT - 1) / (16 * NT)), (unsigned)((p.M + 16 * MB - 1) / (16 * MB)));
+    hipLaunchKernelGGL((gemm_i8_rows_kernel<MB, NT, DEPTH>), grid, dim3(512), 0, s, p);
+}
+
+// The shape whose estimate is the smallest.  A CU takes its share of the workgroups, `resident` at a time; such a round
+// of k of them takes `each` us and for every step max(alone, shared k): a workgroup's own chain, or what the CU fetches
+// and multiplies.  A step is 128 inputs of a tile, 1024 of the forms for few rows (a block for each wave).  Fitted to
+// 270 products of 1..4374 rows, 256..8192 columns and 512..8192 inputs, where the choice costs 0.7% in the mean, and up to
+// 14%, over the fastest of 16 shapes.  us:
+//   1 x 8192 x 8192 14.0 with 16 x 16, 16.5 with 32 x 32 (weights from memory); 67 x 8192 x 8192 21.6 with 64 x 64,
+//   25.3 with 64 x 128, 29.5 with 80 x 32; 1072 x 256 x 8192 18.8 with 64 x 64 and four stages, 33.8 with two; 268 x 8192
+//   x 8192 35.3 with 128 x 128 and 16 waves, 37.0 with 8; 4374 x 2048 x 2048 29.5 with 192 x 256, 36.5 with 128 x 128;
+//   4374 x 8192 x 8192 290 with 192 x 256 (three full rounds of workgroups), 346 with 256 x 256.
+struct I8Shape {
+    int bm, bn, step, resident;
+    double start, alone, shared, each;
+};
+constexpr I8Shape kI8Shapes[] = {
+    {16, 16, 1024, 4, 2.25, 0.94, 0.88, 0.0},  {16, 32, 1024, 4, 2.03, 1.47, 1.26, 0.0},  {32, 32, 1024, 4, 2.19, 1.83, 1.83, 0.0},
+    {64, 64, 128, 2, 1.38, 0.235, 0.19, 2.65}, {64, 128, 128, 1, 0.99, 0.307, 0.0, 3.1},  {128, 128, 128, 2, 0.0, 0.62, 0.54, 4.5},
+    {128, 128, 128, 1, 0.0, 0.41, 0.0, 4.9},   {128, 256, 128, 1, 0.0, 0.71, 0.0, 7.6},   {192, 256, 128, 1, 0.0, 1.05, 0.0, 9.0},
+};
+
+static int i8_shape(const I8Args& p) {
+    int best = -1;
+    double least = 0.;
+    for (int i = 0; i < (int)(sizeof(kI8Shapes) / sizeof(kI8Shapes[0])); ++i) {
+        const I8Shape& f = kI8Shapes[i];
+        const int64_t slabs = (p.M + f.bm - 1) / f.bm, wgs = slabs * ((p.N + f.bn - 1) / f.bn);
+        if (f.step == 1024 && slabs > 65535) continue;   // the grid's second dimension
+        const int64_t n = (wgs + 255) / 256, steps = (p.K + f.step - 1) / f.step;
+        auto round = [&](int64_t k) { return k ? f.each + (double)steps * std::max(f.alone, f.shared * (double)k) : 0.; };
+        const double us = f.start + (double)(n / f.resident) * round(f.resident) + round(n % f.resident);
+        if (best < 0 || us < least) least = us, best = i;
+    }
+    return best;
 }
 
 static void launch_gemm_i8(const I8Args& p, hipStream_t s) {
-    if (p.M <= 64) launch_i8<1, 1>(p, s);
-    else launch_i8<4, 2>(p, s);
+    switch (i8_shape(p)) {
+    case 0: return launch_i8_rows<1, 1, 4>(p, s);
+    case 1: return launch_i8_rows<1, 2, 3>(p, s);
+    case 2: return launch_i8_rows<2, 2, 3>(p, s);
+    case 3: return launch_i8<1, 1, 2, 2, 4>(p, s);
+    case 4: return launch_i8<1, 1, 2, 4, 4>(p, s);
+    case 5: return launch_i8<2, 1, 2, 4, 2>(p, s);
+    case 6: return launch_i8<1, 1, 4, 4, 4>(p, s);
+    case 7: return launch_i8<2, 2, 2, 4, 3>(p, s);
+    default: return launch_i8<3, 2, 2, 4, 2>(p, s);
+    }
 }
 
 static int quant_i8(const void* a, int64_t lda, int dtype, int M, int K, int8_t* codes, int64_t ldc, float* scale, hipStream_t s) {
@@ -297,7 +497,7 @@ extern "C" int sf_gemm_i8(const sf_gemm_i8_desc* d, void* workspace, size_t work
     if (!sfk::i8_float(d->c_dtype) || d->act < SF_ACT_NONE || d->act > SF_ACT_SILU) return SF_ENOTSUP;
     if (d->accumulate && d->c_dtype != SF_F32) return SF_ENOTSUP;
     if (d->M > sfk::kI8MaxRows || d->N > 1 << 25 || d->K > sfk::kI8MaxInputs || d->lda > sfk::kI8MaxStride ||
-        d->ldw > sfk::kI8MaxStride || ((int64_t)(d->M + 63) / 64) * ((d->N + 127) / 128) >= 1 << 22)
+        d->ldw > sfk::kI8MaxStride || ((int64_t)(d->M + 63) / 64) * ((d->N + 63) / 64) >= 1 << 22)
         return SF_ENOTSUP;
     if (d->M == 0) return SF_OK;
     if (!d->A || !d->W || !d->w_scale || !d->C || (codes && !d->a_scale)) return SF_EINVAL;
