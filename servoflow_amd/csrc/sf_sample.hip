@@ -10,12 +10,20 @@
 //
 // Every filter keeps a prefix of the tokens in falling order, so all that is ever
 // asked of that order is the first position whose running count or running weight
-// passes a number.  Nothing is sorted for it: the row is spread over 2048 buckets
-// of (l - m) / temperature, 1 / 44.5 octave each, with count and weight of each; the bucket
-// that holds the position is found from their running sums, and only its
-// tokens (with those above it where they are few) are put in order, in LDS.  A
-// bucket of more than 2048 tokens is halved by keys, 2048 parts at a time, until one
-// value is left, of which the tokens go by index.
+// passes a number.  Nothing is sorted for it.
+//
+// 16-bit logits have few values: a row is counted by value, 65536 counts of 16 bits in
+// LDS, in one pass that needs no maximum; the values that occur are put together in
+// order, each gets its weight once, and the position is a value and a number among its
+// equals, whose index one more pass over the row finds in registers.
+//
+// 32-bit logits, and rows in which that fails (a value that occurs more than 65535
+// times), are spread over 2048 buckets of (l - m) /
+// temperature, 1 / 44.5 octave each, with count and weight of each; the bucket that
+// holds the position is found from their running sums, and only its tokens (with
+// those above it where they are few) are put in order, in LDS.  A bucket of more than
+// 2048 tokens is cut by keys, 2048 parts at a time, until one value is left, of which
+// the tokens go by index.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -59,7 +67,6 @@ struct SampleShared {
             uint32_t count[kBuckets];
         } part;
     };
-    double exp2[1 << kExpBits];
     uint64_t wave64[kSampleWaves];
     uint32_t wave32[kSampleWaves];
     // what one thread found
@@ -68,6 +75,11 @@ struct SampleShared {
     uint32_t lo, hi;
     int token;
 };
+
+// 2^43 2^(j / 128).
+__device__ __forceinline__ void sample_table(double* table) {
+    if (threadIdx.x < 1 << kExpBits) table[threadIdx.x] = kUnit * exp2((double)threadIdx.x / (1 << kExpBits));
+}
 
 // fp32 -> whole numbers in the same order, and back; -0 counts as 0.
 __device__ __forceinline__ uint32_t sample_key(float l) {
@@ -89,7 +101,13 @@ struct SampleRow {
         const uint16_t h = reinterpret_cast<const uint16_t*>(base)[i];
         return KIND == 1 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
     }
-    // f(logit, index) for every element, each thread its own: whole pieces of 16 bytes, and singly what lies before the
+    // f(logit, index) for every element, each thread its own: one by one, for what is rare.
+    template <class F>
+    __device__ __forceinline__ void each_slowly(F f) const {
+#pragma unroll 1
+        for (int i = threadIdx.x; i < V; i += kSampleThreads) f(one(i), i);
+    }
+    // The same, whole pieces of 16 bytes, and singly what lies before the
     // first and behind the last.
     template <class F>
     __device__ __forceinline__ void each(F f) const {
@@ -98,13 +116,21 @@ struct SampleRow {
         const int head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / size);
         const int pieces = (V - head) / E, tail = head + pieces * E;
         const u32x4* from = reinterpret_cast<const u32x4*>(base + head * size);
-        for (int c0 = t; c0 < pieces; c0 += 4 * kSampleThreads) {
-            u32x4 v[4];
+        constexpr int kAtOnce = 2;   // (four: code that no cache of instructions holds)
+        u32x4 next[kAtOnce];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (c0 + j * kSampleThreads < pieces) v[j] = from[c0 + j * kSampleThreads];
+        for (int j = 0; j < kAtOnce; ++j)
+            if (t + j * kSampleThreads < pieces) next[j] = from[t + j * kSampleThreads];
+        for (int c0 = t; c0 < pieces; c0 += kAtOnce * kSampleThreads) {
+            u32x4 v[kAtOnce];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < kAtOnce; ++j) {
+                v[j] = next[j];
+                const int c = c0 + (kAtOnce + j) * kSampleThreads;
+                if (c < pieces) next[j] = from[c];
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
                 const int c = c0 + j * kSampleThreads;
                 if (c >= pieces) break;
 #pragma unroll
@@ -140,34 +166,67 @@ struct SampleScale {
         const int n = (int)(uint32_t)__double_as_longlong(z);
         const double r = (fmax(y, -128. * 64.) - (z - magic)) * (M_LN2 / 128.);
         const double p = 1. + r * (1. + r * (0.5 + r * (1. / 6. + r * (1. / 24.))));
-        const double w = ldexp(p * table[n & 127], (n >> kExpBits) + 43);
+        const double w = ldexp(p * table[n & 127], n >> kExpBits);
         return (uint64_t)__double_as_longlong(w + 4503599627370496.) & 0xfffffffffffffull;   // + 2^52: rounded
     }
 };
 
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
-    const uint32_t lo = __shfl_up((uint32_t)v, d, 64), hi = __shfl_up((uint32_t)(v >> 32), d, 64);
-    return (uint64_t)hi << 32 | lo;
+// Running sums over a wave's lanes (16 lanes: over each row), vector instructions alone.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_or_0(uint64_t x) {
+    return (uint64_t)dpp_or_0<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | dpp_or_0<CTRL, ROWS>((uint32_t)x);
+}
+template <class T>
+__device__ __forceinline__ T running16(T x) {
+    x += dpp_or_0<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8
+    x += dpp_or_0<0x112, 0xf>(x);
+    x += dpp_or_0<0x114, 0xf>(x);
+    x += dpp_or_0<0x118, 0xf>(x);
+    return x;
+}
+template <class T>
+__device__ __forceinline__ T running64(T x) {
+    x = running16(x);
+    x += dpp_or_0<0x142, 0xa>(x);   // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+    x += dpp_or_0<0x143, 0xc>(x);
+    return x;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ uint64_t lane_of(uint64_t x, int lane) {
+    return (uint64_t)lane_of((uint32_t)(x >> 32), lane) << 32 | lane_of((uint32_t)x, lane);
+}
+// What the waves before `wave` put into sums, and all of them.
+template <class T>
+__device__ __forceinline__ T before_wave(const T* sums, int wave, T& all) {
+    const T own = sums[threadIdx.x & (kSampleWaves - 1)], run = running16(own);
+    all = lane_of(run, kSampleWaves - 1);
+    return lane_of(run, wave) - lane_of(own, wave);
+}
+
+// A barrier for what is in LDS: loads from memory stay under way.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 // Running sums over 2048 counts and weights (either may be null), two to a thread.
 __device__ __forceinline__ void sample_running(SampleShared& s, uint32_t* count, uint64_t* mass) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    uint32_t c0 = 0, c = 0;
-    uint64_t m0 = 0, m = 0;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    uint32_t c0 = 0, c = 0, all_c;
+    uint64_t m0 = 0, m = 0, all_m;
     if (count) c0 = count[2 * t], c = c0 + count[2 * t + 1];
     if (mass) m0 = mass[2 * t], m = m0 + mass[2 * t + 1];
-    uint32_t ci = c;
-    uint64_t mi = m;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t a = __shfl_up(ci, d, 64);
-        const uint64_t b = shfl_up64(mi, d);
-        if (lane >= d) ci += a, mi += b;
-    }
+    uint32_t ci = running64(c);
+    uint64_t mi = running64(m);
     if (lane == 63) s.wave32[wave] = ci, s.wave64[wave] = mi;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) ci += s.wave32[w], mi += s.wave64[w];
+    ci += before_wave(s.wave32, wave, all_c);
+    mi += before_wave(s.wave64, wave, all_m);
     if (count) count[2 * t] = ci - c + c0, count[2 * t + 1] = ci;
     if (mass) mass[2 * t] = mi - m + m0, mass[2 * t + 1] = mi;
     __syncthreads();
@@ -209,13 +268,101 @@ struct SampleHit {
     int index;   // -1: not known, by rank
 };
 
+// The first of n equal tokens of weight w, behind (c0, m0), that answers q; the last one does.
+__device__ __forceinline__ uint32_t sample_among_equals(const SampleQuery& q, uint32_t n, uint32_t c0, uint64_t m0, uint64_t w) {
+    uint32_t below = 0, r = n;
+    while (r - below > 1) {
+        const uint32_t mid = below + (r - below) / 2;
+        if (q.at(c0 + mid, m0 + mid * w)) r = mid;
+        else below = mid;
+    }
+    return r;
+}
+
+// The parameters of a row.
+struct SampleRule {
+    float temperature, top_p;
+    int k;
+    SampleScale sc;
+    double y_min;   // min-p: exponents from here on
+    __device__ __forceinline__ void read(const SampleArgs& p, int64_t row) {
+        temperature = p.temperature ? p.temperature[row] : p.temperature1;
+        k = p.top_k ? p.top_k[row] : p.top_k1;
+        top_p = p.top_p ? p.top_p[row] : p.top_p1;
+        const float min_p = p.min_p ? p.min_p[row] : p.min_p1;
+        if (!(temperature > 0.f)) temperature = 1.f, k = 1;   // the first in order
+        y_min = min_p > 0.f ? 128. * log2((double)min_p) : -INFINITY;
+        sc.octaves = 128. * M_LOG2E / (double)temperature;
+        sc.per_bucket = fminf((float)(sc.octaves * (kBuckets / (128. * kOctaves))), 3e38f);
+    }
+    // The three questions that a row's token takes: what top-k keeps, what top-p and min-p keep of that (`above`: the tokens
+    // that min-p leaves), and where u falls.  ask(query, last) answers.
+    template <class Ask>
+    __device__ __forceinline__ SampleHit token(uint32_t all, uint64_t all_mass, uint32_t above, float u, uint64_t& kept, Ask ask) const {
+        const uint32_t first_k = k <= 0 ? all : min((uint32_t)k, all), most = max(1u, min(first_k, above));
+        const bool with_p = top_p < 1.f;
+        SampleHit hit = {};
+        kept = all_mass;
+#pragma unroll 1
+        for (int step = 0; step < 3; ++step) {
+            SampleQuery q = {0xffffffffu, INFINITY, false};
+            if (step == 0) {
+                if (!with_p || first_k >= all) continue;
+                q.count = first_k;
+            } else if (step == 1) {
+                if (!with_p && most >= all) continue;
+                q.count = most;
+                if (with_p) q.mass = (double)top_p * (double)kept;
+            } else {
+                const double total = (double)kept;
+                q.mass = fmin(fmax((double)u, 0.) * total, total * (1. - 0x1p-53));
+                q.strict = true;
+            }
+            hit = ask(q, step == 2);
+            if (step < 2) kept = hit.mass;
+        }
+        return hit;
+    }
+    __device__ __forceinline__ float logprob(float l, uint64_t kept) const {
+        return (float)((l == sc.m ? 0. : ((double)l - (double)sc.m) / (double)temperature) - log((double)kept * (1. / kUnit)));
+    }
+};
+
+// The index of the rank-th token of a key: counts of ranges of 512 indexes, then the range that holds it.
 template <int KIND>
-__global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs p) {
-    __shared__ SampleShared s;
+__device__ __forceinline__ int sample_nth(SampleShared& s, const SampleRow<KIND>& x, uint32_t key, uint32_t rank) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int64_t row = blockIdx.x;
-    SampleRow<KIND> x = {static_cast<const char*>(p.logits) + row * p.ld * (KIND == 0 ? 4 : 2), p.V};
-    if (t < 1 << kExpBits) s.exp2[t] = exp2((double)t / (1 << kExpBits));
+    for (int i = t; i < kBuckets; i += kSampleThreads) s.cursor[i] = 0;
+    __syncthreads();
+    x.each([&](float l, int i) {
+        if (sample_key(l) == key) atomicAdd(&s.cursor[i >> 9], 1u);
+    });
+    __syncthreads();
+    sample_running(s, s.cursor, nullptr);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int i = 2 * t + j;
+        const uint32_t b = i ? s.cursor[i - 1] : 0u;
+        if (s.cursor[i] >= rank && b < rank) s.found = i, s.found_before = b;
+    }
+    __syncthreads();
+    const int i = 512 * (int)s.found + t;
+    const bool is = t < 512 && i < x.V && sample_key(x.one(i)) == key;
+    const uint64_t set = __ballot(is);
+    if (lane == 0) s.wave32[wave] = __popcll(set);
+    __syncthreads();
+    uint32_t place = s.found_before + __popcll(set & ((1ull << lane) - 1ull)) + 1;
+    for (int w = 0; w < wave; ++w) place += s.wave32[w];
+    if (is && place == rank) s.token = i;
+    __syncthreads();
+    return s.token;
+}
+
+// A row by buckets of its logits; rule's sc.m is not set yet.
+template <int KIND>
+__device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleShared& s, const double* table, const SampleRow<KIND>& x,
+                                                  SampleRule& rule, int64_t row) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     for (int i = t; i < kBuckets; i += kSampleThreads) s.mass[i] = 0, s.count[i] = 0;
     float m = -INFINITY;
     bool bad = false;
@@ -224,7 +371,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
     if (lane == 0) s.wave32[wave] = __float_as_uint(m);
     const bool none = __syncthreads_or(bad);
-    for (int w = 0; w < kSampleWaves; ++w) m = fmaxf(m, __uint_as_float(s.wave32[w]));
+    m = __uint_as_float(s.wave32[lane & (kSampleWaves - 1)]);
+#pragma unroll
+    for (int d = kSampleWaves / 2; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
     if (none || m == -INFINITY) {   // a NaN, or nothing to take
         if (t == 0) {
             p.token[row] = -1;
@@ -232,15 +381,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         }
         return;
     }
-    float temperature = p.temperature ? p.temperature[row] : p.temperature1;
-    int k = p.top_k ? p.top_k[row] : p.top_k1;
-    const float top_p = p.top_p ? p.top_p[row] : p.top_p1, min_p = p.min_p ? p.min_p[row] : p.min_p1;
-    if (!(temperature > 0.f)) temperature = 1.f, k = 1;   // the first in order
-    SampleScale sc;
+    SampleScale& sc = rule.sc;
     sc.m = m;
-    sc.octaves = 128. * M_LOG2E / (double)temperature;
-    sc.per_bucket = fminf((float)(sc.octaves * (kBuckets / (128. * kOctaves))), 3e38f);
-    const double y_min = min_p > 0.f ? 128. * log2((double)min_p) : -INFINITY;
     __syncthreads();
 
     // Buckets, and how many tokens min-p leaves.
@@ -249,20 +391,19 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         const int b = sc.bucket(l);
         if (b >= kBuckets) return;
         const double y = sc.exponent(l);
-        above += y >= y_min;
+        above += y >= rule.y_min;
         atomicAdd(&s.count[b], 1u);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), (unsigned long long)sc.weight(y, s.exp2));
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), (unsigned long long)sc.weight(y, table));
     });
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) above += __shfl_xor(above, d, 64);
     if (lane == 0) s.wave32[wave] = above;
     __syncthreads();
-    above = 0;
-    for (int w = 0; w < kSampleWaves; ++w) above += s.wave32[w];
+    above = s.wave32[lane & (kSampleWaves - 1)];
+#pragma unroll
+    for (int d = kSampleWaves / 2; d >= 1; d >>= 1) above += __shfl_xor(above, d, 64);
     __syncthreads();
     sample_running(s, s.count, s.mass);
-    const uint32_t all = s.count[kBuckets - 1];
-    const uint64_t all_mass = s.mass[kBuckets - 1];
 
     int list_lo = 0, list_hi = -1;   // buckets whose tokens are in the list, in order
     auto before_count = [&](int b) { return b ? s.count[b - 1] : 0u; };
@@ -288,7 +429,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         }
         __syncthreads();
         for (int i = t; i < kSampleList; i += kSampleThreads)
-            s.list.run[i] = (uint32_t)i < n ? sc.weight(sc.exponent(sample_value(~(uint32_t)(s.list.sorted[i] >> 32))), s.exp2) : 0ull;
+            s.list.run[i] = (uint32_t)i < n ? sc.weight(sc.exponent(sample_value(~(uint32_t)(s.list.sorted[i] >> 32))), table) : 0ull;
         __syncthreads();
         sample_running(s, nullptr, s.list.run);
         list_lo = lo;
@@ -301,10 +442,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         uint32_t c0 = s.found_before, n = s.found_count - c0;
         uint64_t m0 = s.found_mass_before;
         __syncthreads();
-        if (b < list_lo || b > list_hi) {
-            if (!last && s.count[b] <= kSampleList) collect(0, b);
-            else if (n <= kSampleList) collect(b, b);
-        }
+        if ((b < list_lo || b > list_hi) && n <= kSampleList) collect(!last && s.count[b] <= kSampleList ? 0 : b, b);
         if (b >= list_lo && b <= list_hi) {
             const uint32_t start = before_count(list_lo), len = s.count[list_hi] - start;
             const uint64_t mass0 = before_mass(list_lo);
@@ -329,7 +467,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
             if (t == 0) s.lo = 0xffffffffu, s.hi = 0;
             __syncthreads();
             uint32_t lo1 = 0xffffffffu, hi1 = 0;
-            x.each([&](float l, int) {
+            x.each_slowly([&](float l, int) {
                 const uint32_t key = sample_key(l);
                 if (key >= lo && key <= hi && sc.bucket(l) == b) lo1 = min(lo1, key), hi1 = max(hi1, key);
             });
@@ -341,12 +479,12 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
             while ((hi - lo) >> shift >= (uint32_t)kBuckets) ++shift;
             for (int i = t; i < kBuckets; i += kSampleThreads) s.part.mass[i] = 0, s.part.count[i] = 0;
             __syncthreads();
-            x.each([&](float l, int) {
+            x.each_slowly([&](float l, int) {
                 const uint32_t key = sample_key(l);
                 if (key < lo || key > hi || sc.bucket(l) != b) return;
                 const uint32_t i = (hi - key) >> shift;
                 atomicAdd(&s.part.count[i], 1u);
-                atomicAdd(reinterpret_cast<unsigned long long*>(&s.part.mass[i]), (unsigned long long)sc.weight(sc.exponent(l), s.exp2));
+                atomicAdd(reinterpret_cast<unsigned long long*>(&s.part.mass[i]), (unsigned long long)sc.weight(sc.exponent(l), table));
             });
             __syncthreads();
             sample_running(s, s.part.count, s.part.mass);
@@ -359,60 +497,389 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
             hi -= i << shift;
             lo = hi - lo > width ? hi - width : lo;
         }
-        const uint64_t w = sc.weight(sc.exponent(sample_value(lo)), s.exp2);
-        uint32_t below = 0, r = n;   // n equals: the first that answers, in (below, r]
-        while (r - below > 1) {
-            const uint32_t mid = below + (r - below) / 2;
-            if (q.at(c0 + mid, m0 + mid * w)) r = mid;
-            else below = mid;
-        }
+        const uint64_t w = sc.weight(sc.exponent(sample_value(lo)), table);
+        const uint32_t r = sample_among_equals(q, n, c0, m0, w);
         return SampleHit{m0 + r * w, lo, r, -1};
     };
 
-    // What top-k keeps, of that what top-p and min-p keep.
-    const uint32_t first_k = k <= 0 ? all : min((uint32_t)k, all);
-    const bool with_p = top_p < 1.f;
-    const SampleQuery any = {0xffffffffu, INFINITY, false};
-    uint64_t kept = all_mass;
-    if (with_p && first_k < all) kept = ask(SampleQuery{first_k, any.mass, false}, false).mass;
-    const uint32_t most = max(1u, min(first_k, above));
-    if (with_p || most < all) kept = ask(SampleQuery{most, with_p ? (double)top_p * (double)kept : any.mass, false}, false).mass;
-    const double total = (double)kept;
-    const double u = fmax((double)p.u[row], 0.);
-    const SampleHit hit = ask(SampleQuery{any.count, fmin(u * total, total * (1. - 0x1p-53)), true}, true);
-    int index = hit.index;
-    if (index < 0) {   // the hit.rank-th of its equals: ranges of 512 indexes, then the one that holds it
-        for (int i = t; i < kBuckets; i += kSampleThreads) s.cursor[i] = 0;
-        __syncthreads();
-        x.each([&](float l, int i) {
-            if (sample_key(l) == hit.key) atomicAdd(&s.cursor[i >> 9], 1u);
-        });
-        __syncthreads();
-        sample_running(s, s.cursor, nullptr);
+    uint64_t kept;
+    const SampleHit hit = rule.token(s.count[kBuckets - 1], s.mass[kBuckets - 1], above, p.u[row], kept, ask);
+    const int index = hit.index >= 0 ? hit.index : sample_nth(s, x, hit.key, hit.rank);
+    if (t == 0) {
+        p.token[row] = index;
+        if (p.logprob) p.logprob[row] = rule.logprob(sample_value(hit.key), kept);
+    }
+}
+
+__global__ __launch_bounds__(kSampleThreads) void sample_f32_kernel(const SampleArgs p) {
+    __shared__ SampleShared s;
+    __shared__ double table[1 << kExpBits];
+    const int64_t row = blockIdx.x;
+    sample_table(table);
+    SampleRule rule;
+    rule.read(p, row);
+    sample_by_buckets<0>(p, s, table, SampleRow<0>{static_cast<const char*>(p.logits) + row * p.ld * 4, p.V}, rule, row);
+}
+
+// --------------------------------------------------------------- by value
+
+constexpr int kHeld = 16;             // pieces of 16 bytes that a thread keeps: 131072 tokens of a row
+constexpr int kOverflow = -2;         // a token that is still to be found
+constexpr uint32_t kMaxTies = 1024;   // equals that are told apart in a list
+constexpr uint32_t kValueList = 6656;   // values beside the counts
+
+struct SampleValues {
+    uint32_t bins[1 << 15];        // two counts each: falling keys 2 i and 2 i + 1
+    uint32_t beside[kValueList];   // the values that occur, key << 16 | count; more than that take the counts' place, if they fit
+    uint64_t wave64[kSampleWaves];
+    uint32_t wave32[kSampleWaves], tokens[kSampleWaves], steps[128];
+    uint32_t found, found_count;
+    uint64_t found_mass;
+    uint32_t above, key, rank, equals, ties, nan, fail, least, none;
+    uint64_t mass;
+    int token;
+};
+
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// Falling keys of two 16-bit floats: whole numbers in falling order (-0 behind 0).
+__device__ __forceinline__ uint32_t sample_falling(uint32_t w) {
+    const uint32_t minus = __builtin_bit_cast(uint32_t, __builtin_bit_cast(s16x2, w) >> 15);
+    return w ^ (~minus & 0x7fff7fffu);
+}
+
+template <int KIND>   // 1 bf16, 2 fp16
+__global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleArgs p) {
+    __shared__ union {
+        SampleShared nth;
+        SampleValues values;
+    } shared;
+    __shared__ double table[1 << kExpBits];
+    constexpr uint32_t kInf = KIND == 1 ? 0x7fu : 0x3ffu, kNegInf = 0xffffu - kInf;   // falling keys of the infinities
+    constexpr uint32_t kLeast = kNegInf - 1;                                          // of the lowest number
+    SampleValues& s = shared.values;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int64_t row = blockIdx.x;
+    const SampleRow<KIND> x = {static_cast<const char*>(p.logits) + row * p.ld * 2, p.V};
+    const int head = min(p.V, (int)((16 - (reinterpret_cast<uintptr_t>(x.base) & 15)) & 15) / 2);
+    const int pieces = (p.V - head) / 8, tail = head + pieces * 8;
+    const u32x4* from = reinterpret_cast<const u32x4*>(x.base + head * 2);
+    u32x4 held[kHeld];
+    const bool in_head = t < head, in_tail = t < p.V - tail;
+    const uint32_t first = in_head ? reinterpret_cast<const uint16_t*>(x.base)[t] : 0u;
+    const uint32_t last = in_tail ? reinterpret_cast<const uint16_t*>(x.base)[tail + t] : 0u;
+    SampleRule rule;
+    rule.read(p, row);
+    // keys: the key in the low half (what is above it does not matter)
+    auto count1 = [&](uint32_t keys) __attribute__((always_inline)) {
+        atomicAdd(reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(s.bins) + (keys << 1 & 0x1fffcu)), 1u << (keys << 4 & 16u));
+    };
+    // A row's masked logits, -infinity or the lowest number, are counted apart: all in one place they would be added one by
+    // one, and pass 16 bits.
+    uint32_t least = 0, none = 0;
+    bool nan = false;
+    auto count_any = [&](uint32_t key) __attribute__((always_inline)) {
+        if (key < kLeast) count1(key);
+        least += key == kLeast;
+        none += key == kNegInf;
+        nan = nan || key > kNegInf;
+    };
+    auto count8 = [&](const u32x4& v) __attribute__((always_inline)) {
+        uint32_t k[4];
+        u16x2 most = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int i = 2 * t + j;
-            const uint32_t b = i ? s.cursor[i - 1] : 0u;
-            if (s.cursor[i] >= hit.rank && b < hit.rank) s.found = i, s.found_before = b;
+        for (int e = 0; e < 4; ++e) {
+            k[e] = sample_falling(v[e]);
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, k[e]));
+        }
+        if (__any(most[0] >= kLeast || most[1] >= kLeast)) {
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t x01 = e & 2 ? k[1] : k[0], x23 = e & 2 ? k[3] : k[2];
+                count_any((e & 4 ? x23 : x01) >> (16 * (e & 1)) & 0xffffu);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                count1(k[e]);
+                count1(k[e] >> 16);
+            }
+        }
+    };
+    auto clear = [&]() __attribute__((always_inline)) {
+        sample_table(table);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) reinterpret_cast<u32x4*>(s.bins)[t + i * kSampleThreads] = u32x4{0, 0, 0, 0};
+        lds_barrier();
+    };
+    if (pieces > kHeld / 2 * kSampleThreads) {   // all loads at once, the last piece again behind it: each is waited for by itself
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) held[j] = from[min(t + j * kSampleThreads, pieces - 1)];
+        clear();
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (t + j * kSampleThreads < pieces) count8(held[j]);
+        for (int c = t + kHeld * kSampleThreads; c < pieces; c += kSampleThreads) count8(from[c]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kHeld / 2; ++j) {
+            if (j * kSampleThreads >= pieces) break;   // (at once, not piece by piece)
+            if (t + j * kSampleThreads < pieces) held[j] = from[t + j * kSampleThreads];
+        }
+        clear();
+#pragma unroll
+        for (int j = 0; j < kHeld / 2; ++j) {
+            if (j * kSampleThreads >= pieces) break;
+            if (t + j * kSampleThreads < pieces) count8(held[j]);
+        }
+    }
+    if (in_head) count_any(sample_falling(first) & 0xffffu);
+    if (in_tail) count_any(sample_falling(last) & 0xffffu);
+    __syncthreads();
+    bool fail = false;
+    if (t == 0) {   // -0, the first of its count, counts as 0, the second of the one before
+        const uint32_t minus = s.bins[0x4000] & 0xffffu;
+        s.bins[0x4000] &= 0xffff0000u;
+        fail = (s.bins[0x3fff] >> 16) + minus > 0xffffu;
+        s.bins[0x3fff] += minus << 16;
+        s.above = s.ties = s.nan = s.fail = s.least = s.none = 0;
+    }
+    __syncthreads();
+
+    // The values that occur, in order: 128 times 256 counts of two values, which the waves deal.  (Most hold nothing: a
+    // row's values are a few thousand, side by side.)
+    uint32_t tokens = least + none;
+    if (__any(tokens != 0)) {
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) least += __shfl_xor(least, d, 64), none += __shfl_xor(none, d, 64);
+        if (lane == 0) atomicAdd(&s.least, least), atomicAdd(&s.none, none);
+    }
+    auto occur = [](const u32x4& v) __attribute__((always_inline)) {
+        uint32_t k = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k += ((v[e] & 0xffffu) ? 1u : 0u) + (v[e] >> 16 ? 1u : 0u);
+        return k;
+    };
+    const u32x4* counts = reinterpret_cast<const u32x4*>(s.bins) + 64 * wave + lane;
+    auto key_of = [&](int i) __attribute__((always_inline)) { return 8u * (64 * (16 * i + wave) + lane); };
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        u32x4 v = counts[1024 * i];
+        uint32_t mine = 0;
+        if (__any((v[0] | v[1] | v[2] | v[3]) != 0)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                tokens += (v[e] & 0xffffu) + (v[e] >> 16);
+                nan = nan || ((v[e] & 0xffffu) && key_of(i) + 2 * e < kInf) || (v[e] >> 16 && key_of(i) + 2 * e + 1 < kInf);
+            }
+            mine = lane_of(running64(occur(v)), 63);
+        }
+        if (lane == 0) s.steps[16 * i + wave] = mine;
+    }
+    tokens = running64(tokens);
+    if (lane == 63) s.tokens[wave] = tokens;
+    if (nan) s.nan = 1;
+    if (fail) s.fail = 1;
+    __syncthreads();
+    before_wave(s.tokens, wave, tokens);
+    const uint32_t own0 = s.steps[lane], own1 = s.steps[64 + lane];
+    const uint32_t to0 = running64(own0), to1 = running64(own1) + lane_of(to0, 63), n = lane_of(to1, 63);
+    const uint32_t lowest = s.least;   // tokens of the lowest number: behind all that are in the list
+    if (s.fail || tokens != (uint32_t)p.V) {   // a count that passed 16 bits: the sum of all is too small
+        if (t == 0) p.token[row] = kOverflow;
+        return;
+    }
+    if (s.nan || n + lowest == 0) {
+        if (t == 0) {
+            p.token[row] = -1;
+            if (p.logprob) p.logprob[row] = NAN;
+        }
+        return;
+    }
+    uint32_t* list = s.beside;
+    auto put = [&](const u32x4& v, int i) __attribute__((always_inline)) {
+        const uint32_t k = occur(v), run = running64(k), key = key_of(i);
+        const int step = 16 * i + wave;
+        uint32_t place = (step < 64 ? lane_of(to0 - own0, step) : lane_of(to1 - own1, step - 64)) + run - k;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (v[e] & 0xffffu) list[place++] = (key + 2 * e) << 16 | (v[e] & 0xffffu);
+            if (v[e] >> 16) list[place++] = (key + 2 * e + 1) << 16 | v[e] >> 16;
+        }
+    };
+    const bool listed = n <= sizeof(s.bins) / sizeof(s.bins[0]);
+    if (n <= kValueList) {
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            const u32x4 v = counts[1024 * i];
+            if (__any((v[0] | v[1] | v[2] | v[3]) != 0)) put(v, i);
+        }
+    } else if (listed) {   // in the counts' place, once they are in registers
+        list = s.bins;
+        u32x4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = counts[1024 * i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) put(v[i], i);
+    }
+    __syncthreads();
+    // Value i of them, or of all keys.
+    const uint32_t values = listed ? n : 65536u;
+    auto entry = [&](uint32_t i) __attribute__((always_inline)) {
+        return listed ? list[i] : i << 16 | (s.bins[i >> 1] >> (16 * (i & 1)) & 0xffffu);
+    };
+
+    // Weights: each thread some consecutive values, `each` of them.
+    auto value = [](uint32_t key) __attribute__((always_inline)) {
+        const uint32_t h = key & 0x8000u ? key : key ^ 0x7fffu;
+        return KIND == 1 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+    };
+    SampleScale& sc = rule.sc;
+    uint32_t top = kLeast;   // the largest value's key
+    if (listed) {
+        if (n) top = list[0] >> 16;
+    } else {
+        const uint64_t has0 = __ballot(own0 != 0), has1 = __ballot(own1 != 0);
+        const int step = has0 ? __builtin_ctzll(has0) : 64 + __builtin_ctzll(has1);
+        const u32x4 v = reinterpret_cast<const u32x4*>(s.bins)[64 * step + lane];
+        uint32_t at = 8;
+#pragma unroll
+        for (int e = 3; e >= 0; --e) at = v[e] & 0xffffu ? 2 * e : v[e] >> 16 ? 2 * e + 1 : at;
+        const int first_lane = __builtin_ctzll(__ballot(at < 8));
+        top = 8u * (64 * step + first_lane) + lane_of(at, first_lane);
+    }
+    sc.m = value(top);
+    const uint32_t each = (values + kSampleThreads - 1) / kSampleThreads;   // 64 at most
+    uint32_t c = 0, above = 0;
+    uint64_t w = 0;
+    for (uint32_t i = t * each; i < min(values, (t + 1) * each); ++i) {
+        const uint32_t e = entry(i);
+        if (!(e & 0xffffu)) continue;
+        const float l = value(e >> 16);
+        const double y = sc.exponent(l);
+        c += e & 0xffffu;
+        above += y >= rule.y_min ? e & 0xffffu : 0u;
+        if (sc.bucket(l) < kBuckets) w += (e & 0xffffu) * sc.weight(y, table);
+    }
+    if (rule.y_min > -INFINITY) {
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) above += __shfl_xor(above, d, 64);
+        if (lane == 0) atomicAdd(&s.above, above);
+    } else if (t == 0) {
+        s.above = 0xffffffffu;
+    }
+    uint32_t c1 = running64(c), all;
+    uint64_t w1 = running64(w), all_mass;
+    if (lane == 63) s.wave32[wave] = c1, s.wave64[wave] = w1;
+    __syncthreads();
+    c1 += before_wave(s.wave32, wave, all);
+    w1 += before_wave(s.wave64, wave, all_mass);
+    const uint32_t c0 = c1 - c, listed_count = all;
+    const uint64_t w0 = w1 - w, listed_mass = all_mass;
+    const float lowest_value = value(kLeast);
+    const uint64_t lowest_weight = lowest && sc.bucket(lowest_value) < kBuckets ? sc.weight(sc.exponent(lowest_value), table) : 0ull;
+    all += lowest;
+    all_mass += lowest * lowest_weight;
+    uint32_t min_p_leaves = s.above;
+    if (sc.exponent(lowest_value) >= rule.y_min && min_p_leaves != 0xffffffffu) min_p_leaves += lowest;
+
+    uint32_t equals = 0;
+    auto ask = [&](const SampleQuery& q, bool) -> SampleHit {
+        if (!q.at(listed_count, listed_mass) || listed_count == 0) {   // among the lowest
+            const uint32_t r = sample_among_equals(q, lowest, listed_count, listed_mass, lowest_weight);
+            equals = lowest;
+            return SampleHit{listed_mass + r * lowest_weight, kLeast, r, -1};
+        }
+        if (c && q.at(c1, w1) && (c0 == 0 || !q.at(c0, w0))) s.found = t, s.found_count = c0, s.found_mass = w0;
+        __syncthreads();
+        if (wave == 0) {   // that thread's values, one a lane
+            const uint32_t i = s.found * each + lane;
+            const bool in = (uint32_t)lane < each && i < values;
+            const uint32_t e = in ? entry(i) : 0u, mult = e & 0xffffu;
+            const float l = value(e >> 16);
+            const uint64_t one = in && sc.bucket(l) < kBuckets ? sc.weight(sc.exponent(l), table) : 0ull;
+            uint32_t cs = running64(mult);
+            uint64_t ws = running64(mult * one);
+            cs += s.found_count;
+            ws += s.found_mass;
+            const uint32_t cb = cs - mult;
+            const uint64_t wb = ws - mult * one;
+            if (mult && q.at(cs, ws) && (cb == 0 || !q.at(cb, wb))) {
+                s.rank = sample_among_equals(q, mult, cb, wb, one);
+                s.mass = wb + s.rank * one;
+                s.key = e >> 16;
+                s.equals = mult;
+            }
         }
         __syncthreads();
-        const int i = 512 * (int)s.found + t;
-        const bool is = t < 512 && i < p.V && sample_key(x.one(i)) == hit.key;
-        const uint64_t set = __ballot(is);
-        if (lane == 0) s.wave32[wave] = __popcll(set);
+        equals = s.equals;
+        return SampleHit{s.mass, s.key, s.rank, -1};
+    };
+    uint64_t kept;
+    const SampleHit hit = rule.token(all, all_mass, min_p_leaves, p.u[row], kept, ask);
+    __syncthreads();   // the list of values is spent
+    int index;
+    if (equals <= kMaxTies) {
+        const uint32_t bits = hit.key & 0x8000u ? hit.key : hit.key ^ 0x7fffu;
+        const uint32_t want = bits | bits << 16, care = bits ? 0xffffffffu : 0x7fff7fffu;   // 0 is -0 too
+        auto found = [&](int i) __attribute__((always_inline)) { s.bins[atomicAdd(&s.ties, 1u)] = (uint32_t)i; };
+        auto look8 = [&](const u32x4& v, int i0) __attribute__((always_inline)) {
+            uint32_t d[4];
+            u16x2 least = {0xffff, 0xffff};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                d[e] = (v[e] ^ want) & care;
+                least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2, d[e]));
+            }
+            if (least[0] && least[1]) return;
+            uint32_t hits = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hits |= (d[e] & 0xffffu ? 0u : 1u << 2 * e) | (d[e] >> 16 ? 0u : 2u << 2 * e);
+            for (; hits; hits &= hits - 1) found(i0 + __builtin_ctz(hits));
+        };
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            if (j * kSampleThreads >= pieces) break;
+            if (t + j * kSampleThreads < pieces) look8(held[j], head + 8 * (t + j * kSampleThreads));
+        }
+        for (int i = t + kHeld * kSampleThreads; i < pieces; i += kSampleThreads) look8(from[i], head + 8 * i);
+        if (in_head && !((first ^ want) & care & 0xffffu)) found(t);
+        if (in_tail && !((last ^ want) & care & 0xffffu)) found(tail + t);
         __syncthreads();
-        uint32_t place = s.found_before + __popcll(set & ((1ull << lane) - 1ull)) + 1;
-        for (int w = 0; w < wave; ++w) place += s.wave32[w];
-        if (is && place == hit.rank) s.token = i;
+        if ((uint32_t)t < equals) {
+            const uint32_t i = s.bins[t];
+            uint32_t place = 1, j = 0;
+            for (; j + 4 <= equals; j += 4) {
+                const u32x4 e = *reinterpret_cast<const u32x4*>(s.bins + j);
+                place += (e[0] < i) + (e[1] < i) + (e[2] < i) + (e[3] < i);
+            }
+            for (; j < equals; ++j) place += s.bins[j] < i;
+            if (place == hit.rank) s.token = (int)i;
+        }
         __syncthreads();
         index = s.token;
+    } else {
+        index = sample_nth(shared.nth, x, sample_key(value(hit.key)), hit.rank);
     }
     if (t == 0) {
         p.token[row] = index;
-        const float l = sample_value(hit.key);
-        if (p.logprob)
-            p.logprob[row] = (float)((l == m ? 0. : ((double)l - (double)m) / (double)temperature) - log(total * (1. / kUnit)));
+        if (p.logprob) p.logprob[row] = rule.logprob(value(hit.key), kept);
     }
+}
+
+// Rows of more than 65535 tokens in which a count of 16 bits was too small.
+template <int KIND>
+__global__ __launch_bounds__(kSampleThreads) void sample_overflow_kernel(const SampleArgs p) {
+    __shared__ SampleShared s;
+    __shared__ double table[1 << kExpBits];
+    const int64_t row = blockIdx.x;
+    if (p.token[row] != kOverflow) return;
+    sample_table(table);
+    SampleRule rule;
+    rule.read(p, row);
+    sample_by_buckets<KIND>(p, s, table, SampleRow<KIND>{static_cast<const char*>(p.logits) + row * p.ld * 2, p.V}, rule, row);
 }
 
 }  // namespace sfk
@@ -431,8 +898,13 @@ extern "C" int sf_sample(const sf_sample_desc* d, void* stream) {
                                d->temperature_all, d->top_p_all, d->min_p_all, d->top_k_all, d->V, d->token, d->logprob};
     const dim3 grid((unsigned)d->rows), block(sfk::kSampleThreads);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (d->dtype == SF_F32) hipLaunchKernelGGL(sfk::sample_kernel<0>, grid, block, 0, s, p);
-    else if (d->dtype == SF_BF16) hipLaunchKernelGGL(sfk::sample_kernel<1>, grid, block, 0, s, p);
-    else hipLaunchKernelGGL(sfk::sample_kernel<2>, grid, block, 0, s, p);
+    if (d->dtype == SF_F32) hipLaunchKernelGGL(sfk::sample_f32_kernel, grid, block, 0, s, p);
+    else if (d->dtype == SF_BF16) hipLaunchKernelGGL(sfk::sample_16_kernel<1>, grid, block, 0, s, p);
+    else hipLaunchKernelGGL(sfk::sample_16_kernel<2>, grid, block, 0, s, p);
+    if (d->dtype != SF_F32 && d->V > 65535) {
+        if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
+        if (d->dtype == SF_BF16) hipLaunchKernelGGL(sfk::sample_overflow_kernel<1>, grid, block, 0, s, p);
+        else hipLaunchKernelGGL(sfk::sample_overflow_kernel<2>, grid, block, 0, s, p);
+    }
     return hipGetLastError() == hipSuccess ? SF_OK : SF_ELAUNCH;
 }

@@ -171,3 +171,38 @@ def test_no_rows_and_refusals():
                {"logits": x.t()}, {"logits": x[0]}):
         with pytest.raises(ValueError):
             kernels.sample(**{"logits": x, "u": u, **kw})
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("V", [70000, 131072, 300001])
+def test_many_equal_16_bit_logits(V, dtype):
+    """More than 65535 tokens of one value: a mask's, the row's largest, zeros of both signs, or all of them; and many values."""
+    g = torch.Generator().manual_seed(V)
+    x = (torch.randn(8, V, generator=g) * 2).to(dtype)
+    x[0, torch.rand(V, generator=g) < 0.99] = -math.inf
+    x[1, torch.rand(V, generator=g) < 0.99] = torch.finfo(dtype).min
+    x[2, torch.rand(V, generator=g) < 0.97] = -3.0
+    x[3] = 0.0
+    x[3, ::2] = -0.0
+    x[4, torch.rand(V, generator=g) < 0.97] = 9.0
+    x[5] = torch.randint(-32768, 32767, (V,), generator=g, dtype=torch.int16).view(dtype)   # any 16 bits
+    x[5][torch.isnan(x[5])] = 1.0
+    x[5][torch.isinf(x[5])] = 2.0
+    x[6] = math.nan
+    x[7, :65536] = -1.5
+    u = torch.tensor([0.1, 0.999, 0.7, 0.3, 0.6, 0.5, 0.2, 0.97])
+    for r in ({}, {"t": 3.0}, {"k": 1000}, {"p": 0.9}, {"t": 1e4, "p": 0.6}, {"k": 60000, "p": 0.99, "mp": 1e-3}, {"t": 0.0}):
+        _check(x, u, what=str(r), **r)
+
+
+def test_only_lowest_numbers_are_left():
+    """A row masked by the lowest number but for -infinity: its tokens share the weight."""
+    for dtype in (BF, FP, F32):
+        low = torch.finfo(dtype).min
+        x = torch.full((3, 5000), -math.inf, dtype=dtype)
+        x[0, 100:2000] = low
+        x[1, 4999] = low
+        x[2, ::3] = low
+        x[2, 17] = low / 2
+        for r in ({}, {"p": 0.5}, {"k": 7}, {"mp": 0.5}, {"t": math.inf}):
+            _check(x, torch.tensor([0.77, 0.5, 0.3]), what=str(r), **r)
