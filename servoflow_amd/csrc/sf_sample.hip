@@ -36,6 +36,7 @@ namespace sfk {
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
 constexpr int kBuckets = 2 * kSampleThreads;        // two to a thread
 constexpr int kSampleList = 2 * kSampleThreads;     // tokens put in order at a time, two to a thread
+constexpr uint32_t kListFromTop = 512;              // so many at most of all buckets above one, too
 constexpr int kExpBits = 7;
 constexpr float kOctaves = 46.f;                    // 2^-46 and below: no weight
 constexpr double kUnit = 8796093022208.;            // 2^43
@@ -161,13 +162,17 @@ struct SampleScale {
         return l == m ? 0. : ((double)l - (double)m) * octaves;
     }
     __device__ __forceinline__ uint64_t weight(double y, const double* table) const {
-        const double magic = 6755399441055744.;   // 1.5 2^52: the nearest whole number in the low bits
-        const double z = fmax(y, -128. * 64.) + magic;
-        const int n = (int)(uint32_t)__double_as_longlong(z);
-        const double r = (fmax(y, -128. * 64.) - (z - magic)) * (M_LN2 / 128.);
-        const double p = 1. + r * (1. + r * (0.5 + r * (1. / 6. + r * (1. / 24.))));
-        const double w = ldexp(p * table[n & 127], n >> kExpBits);
-        return (uint64_t)__double_as_longlong(w + 4503599627370496.) & 0xfffffffffffffull;   // + 2^52: rounded
+        return weight_in_play(fmax(y, -128. * (kOctaves + 1.)), table);
+    }
+    // y not below -128 (kOctaves + 1): a bucket's.
+    __device__ __forceinline__ uint64_t weight_in_play(double y, const double* table) const {
+        constexpr double c = M_LN2 / 128., magic = 6755399441055744.;   // 1.5 2^52: the nearest whole number in the low bits
+        const double z = y + magic, r = y - (z - magic);
+        const uint32_t n = (uint32_t)__double_as_longlong(z);
+        const double e = 1. + r * (c + r * (c * c / 2. + r * (c * c * c / 6. + r * (c * c * c * c / 24.))));
+        const uint64_t w = (uint64_t)__double_as_longlong(e * table[n & 127u]);   // to be times 2^(n / 128), rounded down
+        const double scaled = __longlong_as_double((long long)((uint64_t)((uint32_t)(w >> 32) + ((n & ~127u) << 13)) << 32 | (uint32_t)w));
+        return (uint64_t)__double_as_longlong(scaled + 4503599627370496.) & 0xfffffffffffffull;   // + 2^52: rounded
     }
 };
 
@@ -295,11 +300,11 @@ struct SampleRule {
         sc.octaves = 128. * M_LOG2E / (double)temperature;
         sc.per_bucket = fminf((float)(sc.octaves * (kBuckets / (128. * kOctaves))), 3e38f);
     }
-    // The three questions that a row's token takes: what top-k keeps, what top-p and min-p keep of that (`above`: the tokens
-    // that min-p leaves), and where u falls.  ask(query, last) answers.
+    // The three questions that a row's token takes: what top-k keeps, what top-p keeps of that, and where u falls.  What
+    // min-p leaves is a beginning of the order too: `above`, its weight.  ask(query, last) answers.
     template <class Ask>
-    __device__ __forceinline__ SampleHit token(uint32_t all, uint64_t all_mass, uint32_t above, float u, uint64_t& kept, Ask ask) const {
-        const uint32_t first_k = k <= 0 ? all : min((uint32_t)k, all), most = max(1u, min(first_k, above));
+    __device__ __forceinline__ SampleHit token(uint32_t all, uint64_t all_mass, uint64_t above, float u, uint64_t& kept, Ask ask) const {
+        const uint32_t first_k = k <= 0 ? all : min((uint32_t)k, all);
         const bool with_p = top_p < 1.f;
         SampleHit hit = {};
         kept = all_mass;
@@ -310,10 +315,11 @@ struct SampleRule {
                 if (!with_p || first_k >= all) continue;
                 q.count = first_k;
             } else if (step == 1) {
-                if (!with_p && most >= all) continue;
-                q.count = most;
+                if (!with_p && first_k >= all) continue;
+                q.count = first_k;
                 if (with_p) q.mass = (double)top_p * (double)kept;
             } else {
+                kept = min(kept, max(above, (uint64_t)kUnit));   // one at least
                 const double total = (double)kept;
                 q.mass = fmin(fmax((double)u, 0.) * total, total * (1. - 0x1p-53));
                 q.strict = true;
@@ -385,48 +391,61 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
     sc.m = m;
     __syncthreads();
 
-    // Buckets, and how many tokens min-p leaves.
-    uint32_t above = 0;
+    // Buckets, and the weight that min-p leaves.  Counts are for top-k alone, and for lists of few tokens; without them a
+    // bucket's weight tells how many it holds at most.
+    const bool counted = rule.k > 0, with_min_p = rule.y_min > -INFINITY;
+    uint64_t above = 0;
     x.each([&](float l, int) {
         const int b = sc.bucket(l);
         if (b >= kBuckets) return;
         const double y = sc.exponent(l);
-        above += y >= rule.y_min;
-        atomicAdd(&s.count[b], 1u);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), (unsigned long long)sc.weight(y, table));
+        const uint64_t w = sc.weight_in_play(y, table);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), (unsigned long long)w);
+        if (counted) atomicAdd(&s.count[b], 1u);
+        if (with_min_p) above += y >= rule.y_min ? w : 0ull;
     });
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) above += __shfl_xor(above, d, 64);
-    if (lane == 0) s.wave32[wave] = above;
-    __syncthreads();
-    above = s.wave32[lane & (kSampleWaves - 1)];
-#pragma unroll
-    for (int d = kSampleWaves / 2; d >= 1; d >>= 1) above += __shfl_xor(above, d, 64);
+    if (with_min_p) {
+        above = running64(above);
+        if (lane == 63) s.wave64[wave] = above;
+        __syncthreads();
+        before_wave(s.wave64, __builtin_amdgcn_readfirstlane(wave), above);
+    } else {
+        above = ~0ull;
+    }
     __syncthreads();
     sample_running(s, s.count, s.mass);
 
     int list_lo = 0, list_hi = -1;   // buckets whose tokens are in the list, in order
-    auto before_count = [&](int b) { return b ? s.count[b - 1] : 0u; };
+    auto before_count = [&](int b) { return b ? s.count[b - 1] : 0u; };   // 0 where nothing is counted
     auto before_mass = [&](int b) { return b ? s.mass[b - 1] : 0ull; };
 
+    // Tokens of the buckets lo .. hi; how many there are (more than kSampleList: no list).
     auto collect = [&](int lo, int hi) {
-        for (int i = t; i < kBuckets; i += kSampleThreads) s.cursor[i] = 0;
+        uint32_t* place = s.cursor;   // of a token, as it was found
+        for (int i = t; i < kSampleList; i += kSampleThreads) place[i] = 0;
+        if (t == 0) s.lo = 0;
         __syncthreads();
-        const uint32_t start = before_count(lo), n = s.count[hi] - start;
         x.each([&](float l, int i) {
             const int b = sc.bucket(l);
             if (b < lo || b > hi) return;
-            s.list.raw[before_count(b) - start + atomicAdd(&s.cursor[b], 1u)] = (uint64_t)~sample_key(l) << 32 | (uint32_t)i;
+            const uint32_t at = atomicAdd(&s.lo, 1u);
+            if (at < kSampleList) s.list.raw[at] = (uint64_t)~sample_key(l) << 32 | (uint32_t)i;
         });
         __syncthreads();
-        for (uint32_t i = t; i < n; i += kSampleThreads) {   // its place among its bucket's
-            const uint64_t e = s.list.raw[i];
-            const int b = sc.bucket(sample_value(~(uint32_t)(e >> 32)));
-            const uint32_t from = before_count(b) - start, to = s.count[b] - start;
-            uint32_t place = from;
-            for (uint32_t j = from; j < to; ++j) place += s.list.raw[j] < e;
-            s.list.sorted[place] = e;
+        const uint32_t n = s.lo;
+        if (n > kSampleList) return n;
+        // A token's place is the number of those before it; several threads share it where they are few.
+        const uint32_t parts = max(1u, kSampleThreads / n), each = (n + parts - 1) / parts;
+        for (uint32_t i = t; i < n * parts; i += kSampleThreads) {
+            const uint32_t at = i % n, from = i / n * each, to = min(n, from + each);
+            const uint64_t e = s.list.raw[at];
+            uint32_t less = 0;
+#pragma unroll 8
+            for (uint32_t j = from; j < to; ++j) less += s.list.raw[j] < e;
+            if (less) atomicAdd(&place[at], less);
         }
+        __syncthreads();
+        for (uint32_t i = t; i < n; i += kSampleThreads) s.list.sorted[place[i]] = s.list.raw[i];
         __syncthreads();
         for (int i = t; i < kSampleList; i += kSampleThreads)
             s.list.run[i] = (uint32_t)i < n ? sc.weight(sc.exponent(sample_value(~(uint32_t)(s.list.sorted[i] >> 32))), table) : 0ull;
@@ -434,17 +453,29 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
         sample_running(s, nullptr, s.list.run);
         list_lo = lo;
         list_hi = hi;
+        return n;
     };
 
+    uint32_t len = 0;   // of the list
     auto ask = [&](const SampleQuery& q, bool last) -> SampleHit {
         sample_find(s, s.count, s.mass, 0u, 0ull, q);
         const int b = (int)s.found;
-        uint32_t c0 = s.found_before, n = s.found_count - c0;
+        uint32_t c0 = s.found_before, n = 0;
         uint64_t m0 = s.found_mass_before;
+        if (!counted) {   // at most
+            const double least = kUnit * exp2(-(double)(b + 1) * (kOctaves / kBuckets)) * (1. - 0x1p-14) - 1.;
+            const double most = least > 0. ? (double)(s.mass[b] - m0) / least : 1e9;
+            n = most < 1e9 ? (uint32_t)most : 1000000000u;
+        } else {
+            n = s.found_count - c0;
+        }
         __syncthreads();
-        if ((b < list_lo || b > list_hi) && n <= kSampleList) collect(!last && s.count[b] <= kSampleList ? 0 : b, b);
+        if (b < list_lo || b > list_hi) {
+            list_hi = -1, list_lo = 0;
+            if (n <= kSampleList) len = collect(!last && counted && s.count[b] <= kListFromTop ? 0 : b, b);
+        }
         if (b >= list_lo && b <= list_hi) {
-            const uint32_t start = before_count(list_lo), len = s.count[list_hi] - start;
+            const uint32_t start = before_count(list_lo);
             const uint64_t mass0 = before_mass(list_lo);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -461,7 +492,6 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
             return hit;
         }
         // More tokens than the list takes: parts of the bucket's keys, from the largest down.
-        list_hi = -1, list_lo = 0;
         uint32_t lo = 0, hi = 0xffffffffu;
         while (true) {
             if (t == 0) s.lo = 0xffffffffu, s.hi = 0;
@@ -474,7 +504,7 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
             if (lo1 <= hi1) atomicMin(&s.lo, lo1), atomicMax(&s.hi, hi1);
             __syncthreads();
             lo = s.lo, hi = s.hi;
-            if (lo == hi) break;
+            if (lo == hi) break;   // (of a bucket of one value and no counts the most it can hold is what it holds)
             int shift = 0;
             while ((hi - lo) >> shift >= (uint32_t)kBuckets) ++shift;
             for (int i = t; i < kBuckets; i += kSampleThreads) s.part.mass[i] = 0, s.part.count[i] = 0;
@@ -503,7 +533,8 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
     };
 
     uint64_t kept;
-    const SampleHit hit = rule.token(s.count[kBuckets - 1], s.mass[kBuckets - 1], above, p.u[row], kept, ask);
+    const uint32_t all = counted ? s.count[kBuckets - 1] : 0xffffffffu;
+    const SampleHit hit = rule.token(all, s.mass[kBuckets - 1], above, p.u[row], kept, ask);
     const int index = hit.index >= 0 ? hit.index : sample_nth(s, x, hit.key, hit.rank);
     if (t == 0) {
         p.token[row] = index;
@@ -533,10 +564,12 @@ struct SampleValues {
     uint32_t beside[kValueList];   // the values that occur, key << 16 | count; more than that take the counts' place, if they fit
     uint64_t wave64[kSampleWaves];
     uint32_t wave32[kSampleWaves], tokens[kSampleWaves], steps[128];
-    uint32_t found, found_count;
-    uint64_t found_mass;
-    uint32_t above, key, rank, equals, ties, nan, fail, least, none;
-    uint64_t mass;
+    struct Hit {
+        uint64_t mass;
+        uint32_t key, rank, equals;
+    } hits[3];
+    uint64_t above;
+    uint32_t ties, nan, fail, least, none;
     int token;
 };
 
@@ -663,7 +696,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     };
     const u32x4* counts = reinterpret_cast<const u32x4*>(s.bins) + 64 * wave + lane;
     auto key_of = [&](int i) __attribute__((always_inline)) { return 8u * (64 * (16 * i + wave) + lane); };
-#pragma unroll 1
+#pragma unroll 4
     for (int i = 0; i < 8; ++i) {
         u32x4 v = counts[1024 * i];
         uint32_t mine = 0;
@@ -752,23 +785,24 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     }
     sc.m = value(top);
     const uint32_t each = (values + kSampleThreads - 1) / kSampleThreads;   // 64 at most
-    uint32_t c = 0, above = 0;
-    uint64_t w = 0;
+    uint32_t c = 0;
+    uint64_t w = 0, above = 0;
     for (uint32_t i = t * each; i < min(values, (t + 1) * each); ++i) {
         const uint32_t e = entry(i);
         if (!(e & 0xffffu)) continue;
         const float l = value(e >> 16);
         const double y = sc.exponent(l);
         c += e & 0xffffu;
-        above += y >= rule.y_min ? e & 0xffffu : 0u;
-        if (sc.bucket(l) < kBuckets) w += (e & 0xffffu) * sc.weight(y, table);
+        if (sc.bucket(l) < kBuckets) {
+            const uint64_t one = (e & 0xffffu) * sc.weight_in_play(y, table);
+            w += one;
+            above += y >= rule.y_min ? one : 0ull;
+        }
     }
-    if (rule.y_min > -INFINITY) {
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) above += __shfl_xor(above, d, 64);
-        if (lane == 0) atomicAdd(&s.above, above);
-    } else if (t == 0) {
-        s.above = 0xffffffffu;
+    const bool with_min_p = rule.y_min > -INFINITY;
+    if (with_min_p) {
+        above = running64(above);
+        if (lane == 63) atomicAdd(reinterpret_cast<unsigned long long*>(&s.above), (unsigned long long)above);
     }
     uint32_t c1 = running64(c), all;
     uint64_t w1 = running64(w), all_mass;
@@ -782,43 +816,40 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     const uint64_t lowest_weight = lowest && sc.bucket(lowest_value) < kBuckets ? sc.weight(sc.exponent(lowest_value), table) : 0ull;
     all += lowest;
     all_mass += lowest * lowest_weight;
-    uint32_t min_p_leaves = s.above;
-    if (sc.exponent(lowest_value) >= rule.y_min && min_p_leaves != 0xffffffffu) min_p_leaves += lowest;
-
+    above = with_min_p ? s.above + (sc.exponent(lowest_value) >= rule.y_min ? lowest * lowest_weight : 0ull) : ~0ull;
     uint32_t equals = 0;
+    int asked = 0;
     auto ask = [&](const SampleQuery& q, bool) -> SampleHit {
         if (!q.at(listed_count, listed_mass) || listed_count == 0) {   // among the lowest
             const uint32_t r = sample_among_equals(q, lowest, listed_count, listed_mass, lowest_weight);
             equals = lowest;
             return SampleHit{listed_mass + r * lowest_weight, kLeast, r, -1};
         }
-        if (c && q.at(c1, w1) && (c0 == 0 || !q.at(c0, w0))) s.found = t, s.found_count = c0, s.found_mass = w0;
-        __syncthreads();
-        if (wave == 0) {   // that thread's values, one a lane
-            const uint32_t i = s.found * each + lane;
+        const uint64_t owner = __ballot(c && q.at(c1, w1) && (c0 == 0 || !q.at(c0, w0)));
+        SampleValues::Hit& found = s.hits[asked++];   // a place for each question: a slow wave may still read the last one's
+        if (owner) {   // this wave's: that thread's values, one a lane
+            const int who = __builtin_ctzll(owner);
+            const uint32_t i = (64 * wave + who) * each + lane;
             const bool in = (uint32_t)lane < each && i < values;
             const uint32_t e = in ? entry(i) : 0u, mult = e & 0xffffu;
             const float l = value(e >> 16);
-            const uint64_t one = in && sc.bucket(l) < kBuckets ? sc.weight(sc.exponent(l), table) : 0ull;
-            uint32_t cs = running64(mult);
-            uint64_t ws = running64(mult * one);
-            cs += s.found_count;
-            ws += s.found_mass;
-            const uint32_t cb = cs - mult;
-            const uint64_t wb = ws - mult * one;
+            const uint64_t one = in && sc.bucket(l) < kBuckets ? sc.weight_in_play(sc.exponent(l), table) : 0ull;
+            const uint32_t cs = running64(mult) + lane_of(c0, who), cb = cs - mult;
+            const uint64_t ws = running64(mult * one) + lane_of(w0, who), wb = ws - mult * one;
             if (mult && q.at(cs, ws) && (cb == 0 || !q.at(cb, wb))) {
-                s.rank = sample_among_equals(q, mult, cb, wb, one);
-                s.mass = wb + s.rank * one;
-                s.key = e >> 16;
-                s.equals = mult;
+                const uint32_t r = sample_among_equals(q, mult, cb, wb, one);
+                found.mass = wb + r * one;
+                found.key = e >> 16;
+                found.rank = r;
+                found.equals = mult;
             }
         }
         __syncthreads();
-        equals = s.equals;
-        return SampleHit{s.mass, s.key, s.rank, -1};
+        equals = found.equals;
+        return SampleHit{found.mass, found.key, found.rank, -1};
     };
     uint64_t kept;
-    const SampleHit hit = rule.token(all, all_mass, min_p_leaves, p.u[row], kept, ask);
+    const SampleHit hit = rule.token(all, all_mass, above, p.u[row], kept, ask);
     __syncthreads();   // the list of values is spent
     int index;
     if (equals <= kMaxTies) {
