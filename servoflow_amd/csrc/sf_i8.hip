@@ -56,6 +56,27 @@ __device__ __forceinline__ void i8_load8(const void* row, int k, float (&x)[8]) 
     }
 }
 
+// A row's step from its largest |x|, and the same for i8_code where the step's half or reciprocal is no normal number.
+struct I8Step {
+    float s, step, inv, up;
+    bool plain;   // no: codes 0 (a row of zeros; an infinity or a NaN, whose step makes the products NaN)
+    __device__ __forceinline__ explicit I8Step(float big) {
+        s = big / 127.f;
+        plain = s > 0.f && s < INFINITY;
+        up = s < 0x1p-60f ? 0x1p100f : 1.f;
+        step = s * up;
+        inv = 1.f / step;
+    }
+    __device__ __forceinline__ uint2 codes(const float (&y)[8]) const {
+        uint32_t u[2] = {0u, 0u};
+        if (plain) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e >> 2] |= ((uint32_t)i8_code(y[e] * up, step, inv) & 0xffu) << (8 * (e & 3));
+        }
+        return uint2{u[0], u[1]};
+    }
+};
+
 // One workgroup a row.  Up to 8192 inputs stay in registers between the maximum and the codes.
 template <int KIND>
 __global__ __launch_bounds__(256) void quant_i8_kernel(const void* a, int64_t lda, int K, int8_t* codes, int64_t ldc, float* scale) {
@@ -86,20 +107,10 @@ __global__ __launch_bounds__(256) void quant_i8_kernel(const void* a, int64_t ld
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = big;
     bad = __syncthreads_or(bad);
     big = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    const float s = bad ? NAN : big / 127.f;   // an infinity: an infinite step, whose products are NaN
-    const bool plain = s > 0.f && s < INFINITY;
-    const float up = s < 0x1p-60f ? 0x1p100f : 1.f;   // steps whose half or reciprocal is no normal number
-    const float step = s * up, inv = 1.f / step;
-    if (threadIdx.x == 0) scale[m] = s;
+    const I8Step st(bad ? NAN : big);
+    if (threadIdx.x == 0) scale[m] = st.s;
     int8_t* dst = codes + m * ldc;
-    auto store = [&](int k, const float (&y)[8]) {
-        uint32_t u[2] = {0u, 0u};
-        if (plain) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) u[e >> 2] |= ((uint32_t)i8_code(y[e] * up, step, inv) & 0xffu) << (8 * (e & 3));
-        }
-        *reinterpret_cast<uint2*>(dst + k) = uint2{u[0], u[1]};
-    };
+    auto store = [&](int k, const float (&y)[8]) { *reinterpret_cast<uint2*>(dst + k) = st.codes(y); };
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const int k = 8 * (int)threadIdx.x + 2048 * i;
@@ -123,6 +134,8 @@ struct I8Args {
     int M, N, K;
     int act, c_kind, accumulate, vec4;
     int mt, nt;   // tiles
+    const void* x;   // rows to be quantised by the workgroup that multiplies them
+    int64_t ldx;
 };
 
 // Scales and bias of four columns from n on (0 behind the last).
@@ -319,7 +332,10 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(const I8Args p) {
 
 // Few rows: MB tiles of 16 rows against NT tiles of 16 columns to a workgroup, whose eight waves deal the inputs, 128 at a
 // time, and join in LDS.  Both operands go straight into registers, DEPTH blocks of inputs ahead; the weights are read once.
-template <int MB, int NT, int DEPTH>
+// KIND: of rows that the workgroup quantises itself (as i8_load8; MB 1), -1 for codes.  Up to kFusedCodes inputs in all:
+// every workgroup does it for itself, while its weights are on their way, and a launch is saved.
+constexpr int kFusedCodes = 8192;
+template <int MB, int NT, int DEPTH, int KIND = -1>
 __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(const I8Args p) {
     constexpr int NW = 8;
     __shared__ i32x4 sums[NW][MB * NT][64];
@@ -327,13 +343,16 @@ __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(const I8Args p) {
     const int r = lane & 15, g = lane >> 4;
     const int n0 = 16 * NT * blockIdx.x, m0 = 16 * MB * blockIdx.y;
     const int rows = min(16 * MB, p.M - m0), cols = min(16 * NT, p.N - n0);
-    const __amdgpu_buffer_rsrc_t ars = make_rsrc(p.a + (int64_t)m0 * p.lda, (uint32_t)((rows - 1) * (int)p.lda + p.K));
+    constexpr bool kFused = KIND >= 0;
+    __shared__ __attribute__((aligned(16))) int8_t held[kFused ? kFusedCodes + 16 * 16 + 128 : 16];   // rows 16 bytes further apart than K
+    __shared__ uint32_t biggest[16];
+    const __amdgpu_buffer_rsrc_t ars = make_rsrc(p.a + (int64_t)m0 * p.lda, kFused ? 0u : (uint32_t)((rows - 1) * (int)p.lda + p.K));
     const __amdgpu_buffer_rsrc_t wrs = make_rsrc(p.w + (int64_t)n0 * p.ldw, (uint32_t)((cols - 1) * (int)p.ldw + p.K));
     uint32_t wat[NT], xat[MB];   // rows behind the last repeat it; they are not stored
 #pragma unroll
     for (int t = 0; t < NT; ++t) wat[t] = (uint32_t)min(16 * t + r, cols - 1) * (uint32_t)p.ldw;
 #pragma unroll
-    for (int b = 0; b < MB; ++b) xat[b] = (uint32_t)min(16 * b + r, rows - 1) * (uint32_t)p.lda;
+    for (int b = 0; b < MB; ++b) xat[b] = (uint32_t)min(16 * b + r, rows - 1) * (uint32_t)(kFused ? p.K + 16 : p.lda);
     constexpr int kUnits = (NT * MB + NW - 1) / NW;   // tiles that a wave joins and stores
     float sm[kUnits];
     I8Columns cn[kUnits];
@@ -341,7 +360,7 @@ __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(const I8Args p) {
     for (int i = 0; i < kUnits; ++i) {
         const int u = wave + i * NW, m = m0 + 16 * (u % MB) + r;
         if (u >= NT * MB) break;
-        sm[i] = m < p.M ? p.a_scale[m] : 0.f;
+        sm[i] = !kFused && m < p.M ? p.a_scale[m] : 0.f;
         cn[i] = i8_columns(p, n0 + 16 * (u / MB) + 4 * g);
     }
     i32x4 acc[NT][MB];
@@ -358,17 +377,55 @@ __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(const I8Args p) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) w[d][t][j] = __builtin_bit_cast(i32x4, buffer_load16(wrs, in ? wat[t] + k : 0x80000000u));
 #pragma unroll
-            for (int b = 0; b < MB; ++b) x[d][b][j] = __builtin_bit_cast(i32x4, buffer_load16(ars, in ? xat[b] + k : 0x80000000u));
+            for (int b = 0; b < MB && !kFused; ++b) x[d][b][j] = __builtin_bit_cast(i32x4, buffer_load16(ars, in ? xat[b] + k : 0x80000000u));
         }
     };
     const int blocks = (p.K + 127) / 128;
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d)
         if (wave + d * NW < blocks) load(d, wave + d * NW);
+    if constexpr (kFused) {
+        constexpr int kChunks = kFusedCodes / 8 / 512;   // of 8 inputs, of a thread
+        const int per_row = p.K / 8, all = p.M * per_row;
+        float y[kChunks][8];
+        int at[kChunks];
+        if (threadIdx.x < 16) biggest[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            const int c = (int)threadIdx.x + 512 * i, row = c / per_row;
+            at[i] = c < all ? row : -1;
+            if (c >= all) continue;
+            i8_load8<KIND>(static_cast<const char*>(p.x) + row * p.ldx * (KIND == 0 ? 4 : 2), 8 * (c % per_row), y[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            if (at[i] < 0) continue;
+            uint32_t big = 0;   // as whole numbers: an infinity is above all numbers, and a NaN above that
+#pragma unroll
+            for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(y[i][e]) & 0x7fffffffu);
+            atomicMax(&biggest[at[i]], big);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            if (at[i] < 0) continue;
+            const int c = (int)threadIdx.x + 512 * i;
+            *reinterpret_cast<uint2*>(held + at[i] * (p.K + 16) + 8 * (c % per_row)) = I8Step(__uint_as_float(biggest[at[i]])).codes(y[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) sm[i] = I8Step(__uint_as_float(biggest[r])).s;   // rows behind the last: 0, not stored
+        __syncthreads();
+    }
     for (int kb = wave; kb < blocks; kb += DEPTH * NW) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
             if (kb + d * NW >= blocks) break;
+            if constexpr (kFused) {   // behind K anything, against weights of 0
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    x[d][0][j] = *reinterpret_cast<const i32x4*>(held + xat[0] + 128 * (kb + d * NW) + 64 * j + 16 * g);
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -441,6 +498,20 @@ static int i8_shape(const I8Args& p) {
     return best;
 }
 
+// Few inputs are quantised where they are multiplied.  us in a graph, so and in two launches: 1 x 2048 x 2048 6.4 and 8.5,
+// 1 x 8192 x 8192 17.7 and 22.3, 5 x 2051 x 1152 6.5 and 8.5; of more inputs every workgroup's own quantising counts: 8 x 2048
+// x 2048 10.0 and 9.0, 8 x 8192 x 2048 15.3 and 11.0.
+static inline bool i8_fused(const sf_gemm_i8_desc* d) {
+    return d->a_dtype != SF_I8 && d->M <= 16 && (int64_t)d->M * d->K <= kFusedCodes;
+}
+template <int KIND>
+static void launch_i8_fused(const I8Args& p, hipStream_t s) {
+    const bool narrow = p.N <= 16 * 512;   // as many workgroups as two to a CU, or wider ones
+    const dim3 grid((unsigned)(narrow ? (p.N + 15) / 16 : (p.N + 31) / 32));
+    if (narrow) hipLaunchKernelGGL((gemm_i8_rows_kernel<1, 1, 4, KIND>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((gemm_i8_rows_kernel<1, 2, 3, KIND>), grid, dim3(512), 0, s, p);
+}
+
 static void launch_gemm_i8(const I8Args& p, hipStream_t s) {
     switch (i8_shape(p)) {
     case 0: return launch_i8_rows<1, 1, 4>(p, s);
@@ -486,7 +557,7 @@ extern "C" int sf_quant_i8(const void* x, int64_t ldx, int32_t dtype, int32_t ro
 }
 
 extern "C" size_t sf_gemm_i8_workspace_bytes(const sf_gemm_i8_desc* d) {
-    if (!d || d->M <= 0 || d->K <= 0 || d->a_dtype == SF_I8) return 0;
+    if (!d || d->M <= 0 || d->K <= 0 || d->a_dtype == SF_I8 || sfk::i8_fused(d)) return 0;
     return sfk::i8_scales_at(d) + (size_t)d->M * sizeof(float);
 }
 
@@ -511,7 +582,11 @@ extern "C" int sf_gemm_i8(const sf_gemm_i8_desc* d, void* workspace, size_t work
     p.a = static_cast<const int8_t*>(d->A);
     p.lda = d->lda;
     p.a_scale = d->a_scale;
-    if (!codes) {
+    const bool fused = sfk::i8_fused(d);
+    if (fused) {
+        p.x = d->A;
+        p.ldx = d->lda;
+    } else if (!codes) {
         if (!workspace || workspace_bytes < sf_gemm_i8_workspace_bytes(d)) return SF_EWORKSPACE;
         if (!sfk::aligned(workspace, 16)) return SF_EINVAL;
         int8_t* held = static_cast<int8_t*>(workspace);
@@ -535,6 +610,9 @@ extern "C" int sf_gemm_i8(const sf_gemm_i8_desc* d, void* workspace, size_t work
     p.c_kind = d->c_dtype == SF_BF16 ? 1 : (d->c_dtype == SF_F16 ? 2 : 0);
     p.accumulate = d->accumulate != 0;
     p.vec4 = d->ldc % 4 == 0 && sfk::aligned(d->C, p.c_kind == 0 ? 16 : 8);
-    sfk::launch_gemm_i8(p, s);
+    if (!fused) sfk::launch_gemm_i8(p, s);
+    else if (d->a_dtype == SF_F32) sfk::launch_i8_fused<0>(p, s);
+    else if (d->a_dtype == SF_BF16) sfk::launch_i8_fused<1>(p, s);
+    else sfk::launch_i8_fused<2>(p, s);
     return hipGetLastError() == hipSuccess ? SF_OK : SF_ELAUNCH;
 }

@@ -531,8 +531,9 @@ def gemm_i8(a, w, w_scale, a_scale=None, bias=None, act=abi.SF_ACT_NONE, out=Non
         ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif not codes:
         n = abi.lib().sf_gemm_i8_workspace_bytes(d)
-        workspace = torch.empty(n, dtype=torch.uint8, device=dev)   # needs no init
-        ws = workspace.data_ptr()
+        if n:
+            workspace = torch.empty(n, dtype=torch.uint8, device=dev)   # needs no init
+            ws = workspace.data_ptr()
     call_on(dev, "sf_gemm_i8", abi.lib().sf_gemm_i8, d, ws, n)
     return out
 

@@ -132,10 +132,13 @@ def test_int8_refusals():
         assert _gemm(**kw)[0] == abi.SF_ENOTSUP, kw
     assert _gemm(M=0)[0] == abi.SF_OK
     assert _gemm()[1] == 0
-    need = 4 * 256 + 4 * 4
-    assert _gemm(a_dtype=abi.SF_BF16) == (abi.SF_EWORKSPACE, need)
-    assert _gemm(a_dtype=abi.SF_BF16, ws=256, n=need - 1)[0] == abi.SF_EWORKSPACE
-    assert _gemm(a_dtype=abi.SF_BF16, ws=264, n=need)[0] == abi.SF_EINVAL
+    need = 100 * 256 + 100 * 4
+    assert _gemm(a_dtype=abi.SF_BF16, M=100) == (abi.SF_EWORKSPACE, need)
+    assert _gemm(a_dtype=abi.SF_BF16, M=100, ws=256, n=need - 1)[0] == abi.SF_EWORKSPACE
+    assert _gemm(a_dtype=abi.SF_BF16, M=100, ws=264, n=need)[0] == abi.SF_EINVAL
+    for M, K, want in ((16, 512, 0), (1, 1 << 13, 0), (16, 528, 16 * 528 + 64), (17, 16, 17 * 16 + 68), (1, 8208, 8208 + 4)):
+        d = abi.GemmI8Desc(M=M, N=8, K=K, a_dtype=abi.SF_F16)   # few inputs are quantised where they are multiplied
+        assert abi.lib().sf_gemm_i8_workspace_bytes(ctypes.byref(d)) == want
 
 
 def test_front_ends_refuse_host_tensors_and_shapes():

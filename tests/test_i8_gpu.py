@@ -136,6 +136,28 @@ def test_floats_and_activations(dtype, act):
         _check(out, codes, s, w, t, bias, act)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("M,K", [(1, 16), (1, 48), (1, 4096), (1, 8192), (1, 8208), (2, 4096), (3, 2064), (5, 1152), (8, 1024), (13, 624),
+                                 (16, 512), (16, 528), (16, 16), (17, 480)])
+def test_few_rows_quantised_on_the_way(M, K, dtype):
+    """One launch or two, at the border between them; strided rows, zeros, and rows that are no numbers."""
+    for N in (5, 16, 100, 8200):
+        wide = torch.randn(M, K + 32, generator=_gen(M + K)).to(dtype)
+        wide[M // 2] = 0 if M > 1 else wide[M // 2]
+        x = wide[:, 16:16 + K]
+        w, t = _codes(K, N, K), _scales(3, N) * 0.01
+        out = kernels.gemm_i8(wide.to(DEV)[:, 16:16 + K], w.to(DEV), t.to(DEV), out_dtype=F32)
+        codes, s = quant(x.contiguous())
+        _check(out, codes, s, w, t, what=f"N {N}")
+    x = x.clone()
+    x[0, K // 2] = math.inf
+    x[M - 1, 0] = math.nan
+    out = kernels.gemm_i8(x.contiguous().to(DEV), w.to(DEV), t.to(DEV))
+    assert torch.isnan(out[0]).all() and torch.isnan(out[M - 1]).all()
+    if M > 2:
+        _check(kernels.gemm_i8(x[1:-1].contiguous().to(DEV), w.to(DEV), t.to(DEV), out_dtype=F32), codes[1:-1], s[1:-1], w, t)
+
+
 @pytest.mark.parametrize("M", [4, 90, 300])
 def test_strides_accumulate_and_neighbours(M):
     """Views of wider rows, fp32 sums in place, and nothing written beside them."""
@@ -210,7 +232,7 @@ def test_no_rows_and_refusals():
         with pytest.raises(ValueError):
             kernels.gemm_i8(*args, **kw)
     with pytest.raises(abi.SfError):
-        kernels.gemm_i8(x, w, t, workspace=torch.empty(8, dtype=torch.uint8, device=DEV))
+        kernels.gemm_i8(torch.zeros(40, 32, device=DEV), w, t, workspace=torch.empty(8, dtype=torch.uint8, device=DEV))
     with pytest.raises(abi.SfError):
         kernels.gemm_i8(x, w, t, out=torch.zeros(2, 8, dtype=BF, device=DEV), accumulate=True)
     with pytest.raises(abi.SfError):
