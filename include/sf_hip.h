@@ -834,7 +834,7 @@ int sf_kv4_keep(const sf_kv4_cache* cache, const int32_t* nodes, int32_t n, cons
  * A logit of -infinity is never taken; logits of +infinity share all the weight.
  * A row with a NaN, or without a logit above -infinity, gives token -1 and a NaN.
  * Sums are of whole numbers: a row's token depends on the row and its parameters
- * alone.  One launch, no workspace.
+ * alone.
  * ------------------------------------------------------------------------- */
 #define SF_SAMPLE_MAX_VOCAB (1 << 20)
 typedef struct sf_sample_desc {
@@ -853,7 +853,10 @@ typedef struct sf_sample_desc {
     int32_t* token;              /* [rows] */
     float* logprob;              /* [rows] or NULL */
 } sf_sample_desc;
-int sf_sample(const sf_sample_desc* desc, void* stream);
+/* Bytes of device workspace (the sums of few long rows, which several workgroups share), 0 where none is needed;
+ * 8-byte aligned, no initialisation; calls that may run concurrently need separate ones. */
+size_t sf_sample_workspace_bytes(const sf_sample_desc* desc);
+int sf_sample(const sf_sample_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Projections in 8-bit integers: activations with a scale for each row (token),

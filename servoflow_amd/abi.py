@@ -360,7 +360,9 @@ def lib() -> ctypes.CDLL:
     L.sf_tree_accept.restype = ctypes.c_int
     L.sf_kv4_keep.argtypes = [ctypes.POINTER(Kv4CacheDesc), vp, i32, vp, vp]
     L.sf_kv4_keep.restype = ctypes.c_int
-    L.sf_sample.argtypes = [ctypes.POINTER(SampleDesc), vp]
+    L.sf_sample_workspace_bytes.argtypes = [ctypes.POINTER(SampleDesc)]
+    L.sf_sample_workspace_bytes.restype = ctypes.c_size_t
+    L.sf_sample.argtypes = [ctypes.POINTER(SampleDesc), vp, ctypes.c_size_t, vp]
     L.sf_sample.restype = ctypes.c_int
     L.sf_quant_i8.argtypes = [vp, i64, i32, i32, i32, vp, i64, vp, vp]
     L.sf_quant_i8.restype = ctypes.c_int

@@ -24,6 +24,17 @@
 // those above it where they are few) are put in order, in LDS.  A bucket of more than
 // 2048 tokens is cut by keys, 2048 parts at a time, until one value is left, of which
 // the tokens go by index.
+//
+// A workgroup takes a row alone in both.  Few long rows of 32 bits are cut into parts
+// first: their largest logits, then their buckets added up in memory, two launches
+// that the whole card shares, before the one that chooses.
+//
+// What bounds them (us): 256 rows of 131072 bf16 logits take 40, 18 of them until the
+// row is counted (the rows come at 3.7 TB/s, and the counts, one LDS addition for every
+// logit, go 8.8 clocks for 64), then a chain of a row's own: the values put in order 4,
+// their weights 2, each question 1, the pass for the index 2.  A CU reads 45 GB/s: 50001
+// fp32 logits take 6.6 a pass.  Straight code costs, run once by every row: a row of
+// 1000 logits took 33 with all loops unrolled, and 14 now.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -51,25 +62,36 @@ struct SampleArgs {
     int V;
     int32_t* token;
     float* logprob;
+    char* parts;   // of a row cut into parts: SampleParts
+    int n_parts;
 };
 
-struct SampleShared {
+constexpr int kMaxParts = 64;
+struct SampleParts {
+    uint64_t mass[kBuckets];
+    uint32_t count[kBuckets];
+    uint64_t above;
+    float largest[kMaxParts];   // a NaN where there is one
+};
+
+struct SampleSums {
     uint64_t mass[kBuckets];     // running, once summed
     uint32_t count[kBuckets];
-    uint32_t cursor[kBuckets];   // tokens of a bucket that are in the list; counts of index ranges
-    union {
-        struct {
-            uint64_t raw[kSampleList];      // ~key << 32 | index: falling order of keys, rising of indexes
-            uint64_t sorted[kSampleList];
-            uint64_t run[kSampleList];      // running weight, from the list's first
-        } list;
-        struct {
-            uint64_t mass[kBuckets];
-            uint32_t count[kBuckets];
-        } part;
-    };
     uint64_t wave64[kSampleWaves];
     uint32_t wave32[kSampleWaves];
+};
+
+struct SampleShared : SampleSums {
+    uint32_t cursor[kBuckets];   // a part's tokens; counts of index ranges
+    struct {
+        uint64_t mass[kBuckets];
+        uint32_t count[kBuckets];
+    } part;                      // the list by parts of its buckets, or a bucket by keys
+    struct {
+        uint64_t token[kSampleList];   // ~key << 32 | index: falling order of keys, rising of indexes
+        uint64_t weight[kSampleList];
+        uint32_t part[kSampleList];
+    } list;
     // what one thread found
     uint32_t found, found_count, found_before;
     uint64_t found_mass, found_mass_before, found_entry;
@@ -108,41 +130,49 @@ struct SampleRow {
 #pragma unroll 1
         for (int i = threadIdx.x; i < V; i += kSampleThreads) f(one(i), i);
     }
-    // The same, whole pieces of 16 bytes, and singly what lies before the
-    // first and behind the last.
-    template <class F>
+    // The same in whole pieces of 16 bytes, AT_ONCE of them under way beside as many that are looked at, and singly what lies
+    // before the first and behind the last.  (Many at once keep a row's loads from waiting for each other; what does much
+    // with each logit takes few, or no cache of instructions holds it.)
+    template <int AT_ONCE, class F>
     __device__ __forceinline__ void each(F f) const {
+        pieces_of<AT_ONCE>([&](const u32x4* v, int c0, int head, int pieces) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const int c = c0 + j * kSampleThreads;
+                if (c >= pieces) break;
+#pragma unroll
+                for (int e = 0; e < E; ++e) f(element(v[j], e), head + c * E + e);
+            }
+        }, f);
+    }
+
+private:
+    static __device__ __forceinline__ float element(const u32x4& v, int e) {
+        if (KIND == 0) return __uint_as_float(v[e & 3]);
+        if (KIND == 1) return __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)(v[e >> 1] >> (16 * (e & 1))));
+    }
+    template <int AT_ONCE, class Pieces, class F>
+    __device__ __forceinline__ void pieces_of(Pieces take, F f) const {
         const int t = threadIdx.x;
         const int size = KIND == 0 ? 4 : 2;
         const int head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / size);
         const int pieces = (V - head) / E, tail = head + pieces * E;
         const u32x4* from = reinterpret_cast<const u32x4*>(base + head * size);
-        constexpr int kAtOnce = 2;   // (four: code that no cache of instructions holds)
-        u32x4 next[kAtOnce];
+        u32x4 next[AT_ONCE];
 #pragma unroll
-        for (int j = 0; j < kAtOnce; ++j)
+        for (int j = 0; j < AT_ONCE; ++j)
             if (t + j * kSampleThreads < pieces) next[j] = from[t + j * kSampleThreads];
-        for (int c0 = t; c0 < pieces; c0 += kAtOnce * kSampleThreads) {
-            u32x4 v[kAtOnce];
+#pragma unroll 1
+        for (int c0 = t; c0 < pieces; c0 += AT_ONCE * kSampleThreads) {
+            u32x4 v[AT_ONCE];
 #pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) {
+            for (int j = 0; j < AT_ONCE; ++j) {
                 v[j] = next[j];
-                const int c = c0 + (kAtOnce + j) * kSampleThreads;
+                const int c = c0 + (AT_ONCE + j) * kSampleThreads;
                 if (c < pieces) next[j] = from[c];
             }
-#pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) {
-                const int c = c0 + j * kSampleThreads;
-                if (c >= pieces) break;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    float l;
-                    if (KIND == 0) l = __uint_as_float(v[j][e & 3]);
-                    else if (KIND == 1) l = __uint_as_float(e & 1 ? v[j][e >> 1] & 0xffff0000u : v[j][e >> 1] << 16);
-                    else l = (float)__builtin_bit_cast(_Float16, (uint16_t)(v[j][e >> 1] >> (16 * (e & 1))));
-                    f(l, head + c * E + e);
-                }
-            }
+            take(v, c0, head, pieces);
         }
         if (t < head) f(one(t), t);
         if (t < V - tail) f(one(tail + t), tail + t);
@@ -157,6 +187,13 @@ struct SampleScale {
     __device__ __forceinline__ int bucket(float l) const {   // kBuckets and more: no weight
         const float b = -below(l) * per_bucket;
         return b < (float)kBuckets ? (int)b : kBuckets;
+    }
+    // Bounds of the logits of buckets lo .. hi, 2^-18 of them and of m wider than the roundings of `bucket` ask for.
+    __device__ __forceinline__ void range(int lo, int hi, float& from, float& to) const {
+        const double step = 1. / (double)per_bucket, slack = fabs((double)m) * 0x1p-18;
+        from = per_bucket > 0.f ? (float)((double)m - (double)(hi + 1) * step * (1. + 0x1p-18) - slack) : -INFINITY;
+        to = per_bucket > 0.f && lo > 0 ? (float)((double)m - (double)lo * step * (1. - 0x1p-18) + slack) : INFINITY;
+        if (fabsf(m) == INFINITY) from = m;
     }
     __device__ __forceinline__ double exponent(float l) const {   // of two, times 128
         return l == m ? 0. : ((double)l - (double)m) * octaves;
@@ -220,7 +257,7 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // Running sums over 2048 counts and weights (either may be null), two to a thread.
-__device__ __forceinline__ void sample_running(SampleShared& s, uint32_t* count, uint64_t* mass) {
+__device__ __forceinline__ void sample_running(SampleSums& s, uint32_t* count, uint64_t* mass) {
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     uint32_t c0 = 0, c = 0, all_c;
     uint64_t m0 = 0, m = 0, all_m;
@@ -340,7 +377,7 @@ __device__ __forceinline__ int sample_nth(SampleShared& s, const SampleRow<KIND>
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     for (int i = t; i < kBuckets; i += kSampleThreads) s.cursor[i] = 0;
     __syncthreads();
-    x.each([&](float l, int i) {
+    x.template each<2>([&](float l, int i) {
         if (sample_key(l) == key) atomicAdd(&s.cursor[i >> 9], 1u);
     });
     __syncthreads();
@@ -364,15 +401,13 @@ __device__ __forceinline__ int sample_nth(SampleShared& s, const SampleRow<KIND>
     return s.token;
 }
 
-// A row by buckets of its logits; rule's sc.m is not set yet.
+// The largest of a workgroup's logits, a NaN if there is one.
 template <int KIND>
-__device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleShared& s, const double* table, const SampleRow<KIND>& x,
-                                                  SampleRule& rule, int64_t row) {
+__device__ __forceinline__ float sample_largest(SampleSums& s, const SampleRow<KIND>& x) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    for (int i = t; i < kBuckets; i += kSampleThreads) s.mass[i] = 0, s.count[i] = 0;
     float m = -INFINITY;
     bool bad = false;
-    x.each([&](float l, int) { m = fmaxf(m, l), bad = bad || l != l; });
+    x.template each<4>([&](float l, int) { m = fmaxf(m, l), bad = bad || l != l; });
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
     if (lane == 0) s.wave32[wave] = __float_as_uint(m);
@@ -380,22 +415,20 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
     m = __uint_as_float(s.wave32[lane & (kSampleWaves - 1)]);
 #pragma unroll
     for (int d = kSampleWaves / 2; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    if (none || m == -INFINITY) {   // a NaN, or nothing to take
-        if (t == 0) {
-            p.token[row] = -1;
-            if (p.logprob) p.logprob[row] = NAN;
-        }
-        return;
-    }
-    SampleScale& sc = rule.sc;
-    sc.m = m;
-    __syncthreads();
+    return none ? NAN : m;
+}
 
-    // Buckets, and the weight that min-p leaves.  Counts are for top-k alone, and for lists of few tokens; without them a
-    // bucket's weight tells how many it holds at most.
+// Adds a workgroup's logits to the buckets; the weight that min-p leaves of them.  Counts are for top-k alone, and for
+// lists of few tokens; without them a bucket's weight tells how many it holds at most.
+template <int KIND>
+__device__ __forceinline__ uint64_t sample_fill(SampleSums& s, const double* table, const SampleRow<KIND>& x, const SampleRule& rule) {
+    const SampleScale& sc = rule.sc;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const bool counted = rule.k > 0, with_min_p = rule.y_min > -INFINITY;
     uint64_t above = 0;
-    x.each([&](float l, int) {
+    for (int i = t; i < kBuckets; i += kSampleThreads) s.mass[i] = 0, s.count[i] = 0;
+    __syncthreads();
+    x.template each<2>([&](float l, int) {
         const int b = sc.bucket(l);
         if (b >= kBuckets) return;
         const double y = sc.exponent(l);
@@ -408,49 +441,56 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
         above = running64(above);
         if (lane == 63) s.wave64[wave] = above;
         __syncthreads();
-        before_wave(s.wave64, __builtin_amdgcn_readfirstlane(wave), above);
-    } else {
-        above = ~0ull;
+        before_wave(s.wave64, wave, above);
     }
     __syncthreads();
+    return above;
+}
+
+// A row's token from its buckets (rule.sc.m set; above: as sample_fill's).
+template <int KIND>
+__device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleShared& s, const double* table, const SampleRow<KIND>& x,
+                                                  const SampleRule& rule, uint64_t above, int64_t row) {
+    const int t = threadIdx.x;
+    const SampleScale& sc = rule.sc;
+    const bool counted = rule.k > 0;
+    if (!(rule.y_min > -INFINITY)) above = ~0ull;
     sample_running(s, s.count, s.mass);
 
     int list_lo = 0, list_hi = -1;   // buckets whose tokens are in the list, in order
     auto before_count = [&](int b) { return b ? s.count[b - 1] : 0u; };   // 0 where nothing is counted
     auto before_mass = [&](int b) { return b ? s.mass[b - 1] : 0ull; };
 
-    // Tokens of the buckets lo .. hi; how many there are (more than kSampleList: no list).
+    // Tokens of the buckets lo .. hi, and their sums by 2048 parts of these; how many there are (more than kSampleList: no
+    // list).
     auto collect = [&](int lo, int hi) {
-        uint32_t* place = s.cursor;   // of a token, as it was found
-        for (int i = t; i < kSampleList; i += kSampleThreads) place[i] = 0;
+        for (int i = t; i < kBuckets; i += kSampleThreads) s.part.mass[i] = 0, s.part.count[i] = 0;
         if (t == 0) s.lo = 0;
+        float from, to;   // the buckets' logits lie between them
+        sc.range(lo, hi, from, to);
+        const float finer = (float)kBuckets / (float)(hi - lo + 1);
         __syncthreads();
-        x.each([&](float l, int i) {
-            const int b = sc.bucket(l);
-            if (b < lo || b > hi) return;
+        x.template each<2>([&](float l, int i) {
+            if (!(l >= from && l <= to)) return;
             const uint32_t at = atomicAdd(&s.lo, 1u);
-            if (at < kSampleList) s.list.raw[at] = (uint64_t)~sample_key(l) << 32 | (uint32_t)i;
+            if (at < kSampleList) s.list.token[at] = (uint64_t)~sample_key(l) << 32 | (uint32_t)i;
         });
         __syncthreads();
-        const uint32_t n = s.lo;
+        const uint32_t n = s.lo;   // a few of the buckets beside them among them: they belong to no part
         if (n > kSampleList) return n;
-        // A token's place is the number of those before it; several threads share it where they are few.
-        const uint32_t parts = max(1u, kSampleThreads / n), each = (n + parts - 1) / parts;
-        for (uint32_t i = t; i < n * parts; i += kSampleThreads) {
-            const uint32_t at = i % n, from = i / n * each, to = min(n, from + each);
-            const uint64_t e = s.list.raw[at];
-            uint32_t less = 0;
-#pragma unroll 8
-            for (uint32_t j = from; j < to; ++j) less += s.list.raw[j] < e;
-            if (less) atomicAdd(&place[at], less);
+        for (uint32_t i = t; i < n; i += kSampleThreads) {
+            const float l = sample_value(~(uint32_t)(s.list.token[i] >> 32));
+            const int b = sc.bucket(l);
+            const uint64_t w = b >= lo && b <= hi ? sc.weight_in_play(sc.exponent(l), table) : 0ull;
+            const uint32_t part = b >= lo && b <= hi ? min((int)((-sc.below(l) * sc.per_bucket - (float)lo) * finer), kBuckets - 1) : kBuckets;
+            s.list.weight[i] = w;
+            s.list.part[i] = part;
+            if (part == kBuckets) continue;
+            atomicAdd(&s.part.count[part], 1u);
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.part.mass[part]), (unsigned long long)w);
         }
         __syncthreads();
-        for (uint32_t i = t; i < n; i += kSampleThreads) s.list.sorted[place[i]] = s.list.raw[i];
-        __syncthreads();
-        for (int i = t; i < kSampleList; i += kSampleThreads)
-            s.list.run[i] = (uint32_t)i < n ? sc.weight(sc.exponent(sample_value(~(uint32_t)(s.list.sorted[i] >> 32))), table) : 0ull;
-        __syncthreads();
-        sample_running(s, nullptr, s.list.run);
+        sample_running(s, s.part.count, s.part.mass);
         list_lo = lo;
         list_hi = hi;
         return n;
@@ -463,7 +503,7 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
         uint32_t c0 = s.found_before, n = 0;
         uint64_t m0 = s.found_mass_before;
         if (!counted) {   // at most
-            const double least = kUnit * exp2(-(double)(b + 1) * (kOctaves / kBuckets)) * (1. - 0x1p-14) - 1.;
+            const double least = (double)sc.weight_in_play(-128. * (double)(b + 1) * (kOctaves / kBuckets), table) * (1. - 0x1p-14) - 1.;
             const double most = least > 0. ? (double)(s.mass[b] - m0) / least : 1e9;
             n = most < 1e9 ? (uint32_t)most : 1000000000u;
         } else {
@@ -475,15 +515,23 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
             if (n <= kSampleList) len = collect(!last && counted && s.count[b] <= kListFromTop ? 0 : b, b);
         }
         if (b >= list_lo && b <= list_hi) {
-            const uint32_t start = before_count(list_lo);
-            const uint64_t mass0 = before_mass(list_lo);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t i = 2 * t + j;
-                if (i < len && q.at(start + i + 1, mass0 + s.list.run[i]) &&
-                    (i == 0 || !q.at(start + i, mass0 + s.list.run[i - 1]))) {
-                    s.found_entry = s.list.sorted[i];
-                    s.found_mass = mass0 + s.list.run[i];
+            if (t == 0) s.hi = 0;
+            sample_find(s, s.part.count, s.part.mass, before_count(list_lo), before_mass(list_lo), q);
+            const uint32_t part = s.found, start = s.found_before;
+            const uint64_t mass0 = s.found_mass_before;
+            for (uint32_t i = t; i < len; i += kSampleThreads)
+                if (s.list.part[i] == part) s.cursor[atomicAdd(&s.hi, 1u)] = i;
+            __syncthreads();
+            const uint32_t few = s.hi;   // in order: each looks at every other
+            for (uint32_t i = t; i < few; i += kSampleThreads) {
+                const uint64_t e = s.list.token[s.cursor[i]], w = s.list.weight[s.cursor[i]];
+                uint32_t c = start;
+                uint64_t m = mass0;
+                for (uint32_t j = 0; j < few; ++j)
+                    if (s.list.token[s.cursor[j]] < e) ++c, m += s.list.weight[s.cursor[j]];
+                if (q.at(c + 1, m + w) && (c == start || !q.at(c, m))) {
+                    s.found_entry = e;
+                    s.found_mass = m + w;
                 }
             }
             __syncthreads();
@@ -542,14 +590,104 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
     }
 }
 
+// A row that has no token: a NaN, or nothing to take.
+__device__ __forceinline__ bool sample_none(const SampleArgs& p, float m, int64_t row) {
+    const bool none = !(m > -INFINITY);
+    if (none && threadIdx.x == 0) {
+        p.token[row] = -1;
+        if (p.logprob) p.logprob[row] = NAN;
+    }
+    return none;
+}
+
+template <int KIND>
+__device__ __forceinline__ void sample_row(const SampleArgs& p, SampleShared& s, double* table, int64_t row) {
+    const SampleRow<KIND> x = {static_cast<const char*>(p.logits) + row * p.ld * (KIND == 0 ? 4 : 2), p.V};
+    SampleRule rule;
+    rule.read(p, row);
+    sample_table(table);
+    rule.sc.m = sample_largest(s, x);
+    if (sample_none(p, rule.sc.m, row)) return;
+    const uint64_t above = sample_fill(s, table, x, rule);
+    sample_by_buckets(p, s, table, x, rule, above, row);
+}
+
 __global__ __launch_bounds__(kSampleThreads) void sample_f32_kernel(const SampleArgs p) {
     __shared__ SampleShared s;
     __shared__ double table[1 << kExpBits];
-    const int64_t row = blockIdx.x;
-    sample_table(table);
+    sample_row<0>(p, s, table, blockIdx.x);
+}
+
+// ------------------------------------------------------------------ in parts
+
+// Part `part` of a row: whole 4096 bytes of it, but for the first and the last.
+__device__ __forceinline__ SampleRow<0> sample_part(const SampleArgs& p, int64_t row, int part) {
+    const int each = ((p.V + p.n_parts - 1) / p.n_parts + 1023) & ~1023, from = min(p.V, part * each);
+    return SampleRow<0>{static_cast<const char*>(p.logits) + (row * p.ld + from) * 4, min(each, p.V - from)};
+}
+
+// The parts' largest logits; and the row's sums are cleared, each part a share.
+__global__ __launch_bounds__(kSampleThreads) void sample_parts_largest_kernel(const SampleArgs p) {
+    __shared__ SampleSums s;
+    const int64_t row = blockIdx.x / p.n_parts;
+    const int part = blockIdx.x % p.n_parts;
+    SampleParts* sums = reinterpret_cast<SampleParts*>(p.parts) + row;
+    for (int i = part * kSampleThreads + threadIdx.x; i < kBuckets; i += p.n_parts * kSampleThreads) sums->mass[i] = 0, sums->count[i] = 0;
+    if (part == 0 && threadIdx.x == 0) sums->above = 0;
+    const float m = sample_largest(s, sample_part(p, row, part));
+    if (threadIdx.x == 0) sums->largest[part] = m;
+}
+
+// The row's largest, of its parts'.
+__device__ __forceinline__ float sample_parts_largest(const SampleArgs& p, const SampleParts* sums) {
+    const int lane = threadIdx.x & 63;
+    float m = lane < p.n_parts ? sums->largest[lane] : -INFINITY;
+    const bool none = __any(m != m);
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    return none ? NAN : m;
+}
+
+__global__ __launch_bounds__(kSampleThreads) void sample_parts_fill_kernel(const SampleArgs p) {
+    __shared__ SampleSums s;
+    __shared__ double table[1 << kExpBits];
+    const int64_t row = blockIdx.x / p.n_parts;
+    SampleParts* sums = reinterpret_cast<SampleParts*>(p.parts) + row;
     SampleRule rule;
     rule.read(p, row);
-    sample_by_buckets<0>(p, s, table, SampleRow<0>{static_cast<const char*>(p.logits) + row * p.ld * 4, p.V}, rule, row);
+    rule.sc.m = sample_parts_largest(p, sums);
+    if (!(rule.sc.m > -INFINITY)) return;
+    sample_table(table);
+    const uint64_t above = sample_fill(s, table, sample_part(p, row, blockIdx.x % p.n_parts), rule);
+    for (int i = threadIdx.x; i < kBuckets; i += kSampleThreads) {
+        if (s.mass[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&sums->mass[i]), (unsigned long long)s.mass[i]);
+        if (s.count[i]) atomicAdd(&sums->count[i], s.count[i]);
+    }
+    if (threadIdx.x == 0 && above) atomicAdd(reinterpret_cast<unsigned long long*>(&sums->above), (unsigned long long)above);
+}
+
+__global__ __launch_bounds__(kSampleThreads) void sample_parts_choose_kernel(const SampleArgs p) {
+    __shared__ SampleShared s;
+    __shared__ double table[1 << kExpBits];
+    const int64_t row = blockIdx.x;
+    const SampleParts* sums = reinterpret_cast<const SampleParts*>(p.parts) + row;
+    SampleRule rule;
+    rule.read(p, row);
+    rule.sc.m = sample_parts_largest(p, sums);
+    if (sample_none(p, rule.sc.m, row)) return;
+    sample_table(table);
+    for (int i = threadIdx.x; i < kBuckets; i += kSampleThreads) s.mass[i] = sums->mass[i], s.count[i] = sums->count[i];
+    __syncthreads();
+    sample_by_buckets(p, s, table, SampleRow<0>{static_cast<const char*>(p.logits) + row * p.ld * 4, p.V}, rule, sums->above, row);
+}
+
+// In how many parts.  Two more launches have to pay for themselves, the sooner the fewer rows share the card; a part
+// has 4096 logits at least, and the parts of all rows make up two workgroups a CU.  us by one workgroup a row and in parts
+// (temperature alone): 1 x 16384 17.0, 19.9; 1 x 32768 23.0, 21.1; 1 x 131072 58.0, 26.5; 16 x 32768 24.1, 22.7; 37 x 50001
+// 30.9, 28.2; 64 x 32768 25.4, 27.9; 100 x 131072 67.9, 52.9; 160 x 131072 70.1, 65.5; 250 x 131072 86.4, 93.3.
+static inline int sample_parts(int rows, int V, int dtype) {
+    if (dtype != SF_F32 || V < 28672 + 512 * (int64_t)rows) return 1;
+    return std::max(1, std::min({V / 4096, 512 / rows, kMaxParts}));
 }
 
 // --------------------------------------------------------------- by value
@@ -905,37 +1043,55 @@ template <int KIND>
 __global__ __launch_bounds__(kSampleThreads) void sample_overflow_kernel(const SampleArgs p) {
     __shared__ SampleShared s;
     __shared__ double table[1 << kExpBits];
-    const int64_t row = blockIdx.x;
-    if (p.token[row] != kOverflow) return;
-    sample_table(table);
-    SampleRule rule;
-    rule.read(p, row);
-    sample_by_buckets<KIND>(p, s, table, SampleRow<KIND>{static_cast<const char*>(p.logits) + row * p.ld * 2, p.V}, rule, row);
+    if (p.token[blockIdx.x] == kOverflow) sample_row<KIND>(p, s, table, blockIdx.x);
 }
 
 }  // namespace sfk
 
-extern "C" int sf_sample(const sf_sample_desc* d, void* stream) {
+static int sample_check(const sf_sample_desc* d) {
     if (!d || d->rows < 0 || d->V <= 0) return SF_EINVAL;
     if (d->dtype != SF_F32 && d->dtype != SF_BF16 && d->dtype != SF_F16) return SF_ENOTSUP;
     if (d->V > SF_SAMPLE_MAX_VOCAB || d->rows >= 1 << 22) return SF_ENOTSUP;   // a launch counts its threads in 32 bits
+    return SF_OK;
+}
+
+extern "C" size_t sf_sample_workspace_bytes(const sf_sample_desc* d) {
+    if (sample_check(d) != SF_OK || d->rows == 0 || sfk::sample_parts(d->rows, d->V, d->dtype) == 1) return 0;
+    return (size_t)d->rows * sizeof(sfk::SampleParts);
+}
+
+extern "C" int sf_sample(const sf_sample_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+    const int st = sample_check(d);
+    if (st != SF_OK) return st;
     if (d->rows == 0) return SF_OK;
     if (!d->logits || !d->u || !d->token || d->ld < d->V) return SF_EINVAL;
     if (reinterpret_cast<uintptr_t>(d->logits) & (d->dtype == SF_F32 ? 3 : 1)) return SF_EINVAL;
     for (const void* q : {(const void*)d->u, (const void*)d->temperature, (const void*)d->top_k, (const void*)d->top_p,
                           (const void*)d->min_p, (const void*)d->token, (const void*)d->logprob})
         if (reinterpret_cast<uintptr_t>(q) & 3) return SF_EINVAL;
-    const sfk::SampleArgs p = {d->logits, d->ld, d->u, d->temperature, d->top_p, d->min_p, d->top_k,
-                               d->temperature_all, d->top_p_all, d->min_p_all, d->top_k_all, d->V, d->token, d->logprob};
-    const dim3 grid((unsigned)d->rows), block(sfk::kSampleThreads);
+    const int parts = sfk::sample_parts(d->rows, d->V, d->dtype);
+    if (parts > 1 && (!workspace || workspace_bytes < sf_sample_workspace_bytes(d))) return SF_EWORKSPACE;
+    if (parts > 1 && (reinterpret_cast<uintptr_t>(workspace) & 7)) return SF_EINVAL;
+    const sfk::SampleArgs p = {d->logits, d->ld, d->u, d->temperature, d->top_p, d->min_p, d->top_k, d->temperature_all, d->top_p_all,
+                               d->min_p_all, d->top_k_all, d->V, d->token, d->logprob, static_cast<char*>(workspace), parts};
+    const dim3 grid((unsigned)d->rows), each((unsigned)d->rows * (unsigned)parts), block(sfk::kSampleThreads);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (d->dtype == SF_F32) hipLaunchKernelGGL(sfk::sample_f32_kernel, grid, block, 0, s, p);
-    else if (d->dtype == SF_BF16) hipLaunchKernelGGL(sfk::sample_16_kernel<1>, grid, block, 0, s, p);
-    else hipLaunchKernelGGL(sfk::sample_16_kernel<2>, grid, block, 0, s, p);
-    if (d->dtype != SF_F32 && d->V > 65535) {
+    if (parts > 1) {
+        hipLaunchKernelGGL(sfk::sample_parts_largest_kernel, each, block, 0, s, p);
         if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
-        if (d->dtype == SF_BF16) hipLaunchKernelGGL(sfk::sample_overflow_kernel<1>, grid, block, 0, s, p);
-        else hipLaunchKernelGGL(sfk::sample_overflow_kernel<2>, grid, block, 0, s, p);
+        hipLaunchKernelGGL(sfk::sample_parts_fill_kernel, each, block, 0, s, p);
+        if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
+        hipLaunchKernelGGL(sfk::sample_parts_choose_kernel, grid, block, 0, s, p);
+    } else if (d->dtype == SF_F32) {
+        hipLaunchKernelGGL(sfk::sample_f32_kernel, grid, block, 0, s, p);
+    } else {
+        if (d->dtype == SF_BF16) hipLaunchKernelGGL(sfk::sample_16_kernel<1>, grid, block, 0, s, p);
+        else hipLaunchKernelGGL(sfk::sample_16_kernel<2>, grid, block, 0, s, p);
+        if (d->V > 65535) {
+            if (hipGetLastError() != hipSuccess) return SF_ELAUNCH;
+            if (d->dtype == SF_BF16) hipLaunchKernelGGL(sfk::sample_overflow_kernel<1>, grid, block, 0, s, p);
+            else hipLaunchKernelGGL(sfk::sample_overflow_kernel<2>, grid, block, 0, s, p);
+        }
     }
     return hipGetLastError() == hipSuccess ? SF_OK : SF_ELAUNCH;
 }

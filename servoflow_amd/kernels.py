@@ -538,7 +538,7 @@ def gemm_i8(a, w, w_scale, a_scale=None, bias=None, act=abi.SF_ACT_NONE, out=Non
     return out
 
 
-def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, workspace=None):
     """A token from each row of logits [rows, V] (fp32, bf16 or fp16) by the
     uniform numbers u (fp32 [rows], in [0, 1)): (tokens int32 [rows], logprobs
     fp32 [rows]).  In falling order of logits, ties by index: the first top_k
@@ -547,7 +547,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     running weight exceeds u times what is left, the logprob that of its share.
     temperature 0: the largest logit.  Each parameter is a number or, for a
     value a row, a tensor (top_k int32, the others fp32); None is its default.  -1
-    and NaN for a row with a NaN or with nothing above -infinity."""
+    and NaN for a row with a NaN or with nothing above -infinity.  workspace: for
+    the sums of few long rows, allocated unless given."""
     _check(logits, "logits", _FLOATS, None, 2)
     dev, (rows, V) = logits.device, logits.shape
     ptr, val = [], []
@@ -563,5 +564,16 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     raw = _SAMPLE_DESC.pack(rows, V, logits.data_ptr(), logits.stride(0) if rows > 1 else V, _DT[logits.dtype],
                             _vector(u, "u", torch.float32, rows, dev), *ptr, val[0], val[1], val[2], val[3],
                             token.data_ptr(), logprob.data_ptr())
-    call_on(dev, "sf_sample", abi.lib().sf_sample, ctypes.byref(abi.SampleDesc.from_buffer_copy(raw)))
+    d = ctypes.byref(abi.SampleDesc.from_buffer_copy(raw))
+    ws, n = None, 0
+    if workspace is not None:
+        if workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+        ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    else:
+        n = abi.lib().sf_sample_workspace_bytes(d)
+        if n:
+            workspace = torch.empty(n, dtype=torch.uint8, device=dev)   # needs no init
+            ws = workspace.data_ptr()
+    call_on(dev, "sf_sample", abi.lib().sf_sample, d, ws, n)
     return token, logprob

@@ -82,16 +82,16 @@ def test_attention_refusals():
     assert _attn(Sq=0) == (abi.SF_OK, 0)
 
 
-def _sample(**kw):
+def _sample(ws=None, n=0, **kw):
     d = abi.SampleDesc()
     d.rows, d.V, d.logits, d.ld, d.dtype, d.u, d.token = 2, 100, 256, 100, abi.SF_BF16, 256, 256
     for k, v in kw.items():
         setattr(d, k, v)
-    return abi.lib().sf_sample(ctypes.byref(d), None)
+    return abi.lib().sf_sample(ctypes.byref(d), ws, n, None)
 
 
 def test_sample_refusals():
-    assert abi.lib().sf_sample(None, None) == abi.SF_EINVAL
+    assert abi.lib().sf_sample(None, None, 0, None) == abi.SF_EINVAL
     for kw in ({"rows": -1}, {"V": 0}, {"logits": None}, {"logits": 257}, {"dtype": abi.SF_F32, "logits": 258}, {"u": None},
                {"u": 2}, {"token": None}, {"token": 258}, {"ld": 99}, {"temperature": 2}, {"top_k": 1}, {"top_p": 258},
                {"min_p": 3}, {"logprob": 6}):
@@ -99,6 +99,14 @@ def test_sample_refusals():
     for kw in ({"dtype": abi.SF_I8}, {"V": (1 << 20) + 1, "ld": 1 << 21}, {"rows": 1 << 22}):
         assert _sample(**kw) == abi.SF_ENOTSUP, kw
     assert _sample(rows=0) == abi.SF_OK
+    long = {"dtype": abi.SF_F32, "V": 40000, "ld": 40000}
+    need = abi.lib().sf_sample_workspace_bytes(ctypes.byref(abi.SampleDesc(rows=2, V=40000, dtype=abi.SF_F32)))
+    assert need == 2 * (2048 * 12 + 8 + 64 * 4)
+    assert _sample(**long) == abi.SF_EWORKSPACE and _sample(ws=256, n=need - 1, **long) == abi.SF_EWORKSPACE
+    assert _sample(ws=260, n=need, **long) == abi.SF_EINVAL
+    for kw in ({"rows": 2, "V": 1000, "dtype": abi.SF_F32}, {"rows": 300, "V": 40000, "dtype": abi.SF_F32},
+               {"rows": 2, "V": 40000, "dtype": abi.SF_F16}, {"rows": 0, "V": 40000}):
+        assert abi.lib().sf_sample_workspace_bytes(ctypes.byref(abi.SampleDesc(**kw))) == 0
 
 
 def _quant(x=256, ldx=64, dt=abi.SF_BF16, rows=2, cols=64, codes=256, ldc=64, scale=256):

@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from servoflow_amd import kernels
+from servoflow_amd import abi, kernels
 
 from _drafts import sample as plain
 
@@ -99,7 +99,7 @@ def test_equal_logits(V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
-@pytest.mark.parametrize("V,std", [(131072, 0.01), (131072, 0.3), (60000, 1e-4), (60000, 1e-6)])
+@pytest.mark.parametrize("V,std", [(131072, 0.01), (131072, 0.3), (60000, 1e-4), (60000, 1e-6), (20000, 1e-3)])
 def test_flat_rows(V, dtype, std):
     """Thousands of tokens in one bucket: parts of its keys, down to one value."""
     B = 4
@@ -110,9 +110,9 @@ def test_flat_rows(V, dtype, std):
         _check(x, u, what=f"{r}", **r)
 
 
+@pytest.mark.parametrize("V", [3000, 70000])   # of fp32: by one workgroup, in parts
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
-def test_masked_and_special_logits(dtype):
-    V = 3000
+def test_masked_and_special_logits(dtype, V):
     low = torch.finfo(dtype).min
     x = _logits(9, V, 4, dtype)
     x[0] = -math.inf                       # nothing
@@ -161,6 +161,24 @@ def test_runs_are_equal():
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
     alone = torch.cat([kernels.sample(x[i:i + 1], u[i:i + 1], temperature=1.5, top_p=0.97)[0] for i in range(64)])
     assert torch.equal(first[0], alone)
+
+
+def test_workspace():
+    """Rows in parts: a workspace given, used twice, too small, and the rows alone."""
+    x, u = _logits(3, 100001, 6, F32).to(DEV), _u(3, 6).to(DEV)
+    want = kernels.sample(x, u, top_p=0.95)
+    ws = torch.full((3 * (2048 * 12 + 8 + 64 * 4),), 0xff, dtype=torch.uint8, device=DEV)
+    for _ in range(3):
+        got = kernels.sample(x, u, top_p=0.95, workspace=ws)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(abi.SfError):
+        kernels.sample(x, u, workspace=ws[:-8])
+    with pytest.raises(ValueError):
+        kernels.sample(x, u, workspace=ws[::2])
+    alone = torch.cat([kernels.sample(x[i:i + 1], u[i:i + 1], top_p=0.95)[0] for i in range(3)])
+    assert torch.equal(alone, want[0])
+    many = x.repeat(60, 1)   # so many rows go by one workgroup each
+    assert torch.equal(kernels.sample(many, u.repeat(60), top_p=0.95)[0], want[0].repeat(60))
 
 
 def test_no_rows_and_refusals():
