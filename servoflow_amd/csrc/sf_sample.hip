@@ -552,7 +552,7 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
             if (lo1 <= hi1) atomicMin(&s.lo, lo1), atomicMax(&s.hi, hi1);
             __syncthreads();
             lo = s.lo, hi = s.hi;
-            if (lo == hi) break;   // (of a bucket of one value and no counts the most it can hold is what it holds)
+            if (lo >= hi) break;   // (of a bucket of one value and no counts the most it can hold is what it holds)
             int shift = 0;
             while ((hi - lo) >> shift >= (uint32_t)kBuckets) ++shift;
             for (int i = t; i < kBuckets; i += kSampleThreads) s.part.mass[i] = 0, s.part.count[i] = 0;
@@ -707,7 +707,7 @@ struct SampleValues {
         uint32_t key, rank, equals;
     } hits[3];
     uint64_t above;
-    uint32_t ties, nan, fail, least, none;
+    uint32_t ties, nan, fail, least;
     int token;
 };
 
@@ -747,14 +747,14 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         atomicAdd(reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(s.bins) + (keys << 1 & 0x1fffcu)), 1u << (keys << 4 & 16u));
     };
     // A row's masked logits, -infinity or the lowest number, are counted apart: all in one place they would be added one by
-    // one, and pass 16 bits.
+    // one, and pass 16 bits.  `none`: -infinity, and the NaN behind it.
     uint32_t least = 0, none = 0;
     bool nan = false;
     auto count_any = [&](uint32_t key) __attribute__((always_inline)) {
         if (key < kLeast) count1(key);
         least += key == kLeast;
-        none += key == kNegInf;
-        nan = nan || key > kNegInf;
+        none += key >= kNegInf;
+        nan = nan || key > kNegInf;   // of either sign: the others are below kInf, and counted
     };
     auto count8 = [&](const u32x4& v) __attribute__((always_inline)) {
         uint32_t k[4];
@@ -814,7 +814,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         s.bins[0x4000] &= 0xffff0000u;
         fail = (s.bins[0x3fff] >> 16) + minus > 0xffffu;
         s.bins[0x3fff] += minus << 16;
-        s.above = s.ties = s.nan = s.fail = s.least = s.none = 0;
+        s.above = s.ties = s.nan = s.fail = s.least = 0;
     }
     __syncthreads();
 
@@ -823,8 +823,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     uint32_t tokens = least + none;
     if (__any(tokens != 0)) {
 #pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) least += __shfl_xor(least, d, 64), none += __shfl_xor(none, d, 64);
-        if (lane == 0) atomicAdd(&s.least, least), atomicAdd(&s.none, none);
+        for (int d = 32; d >= 1; d >>= 1) least += __shfl_xor(least, d, 64);
+        if (lane == 0) atomicAdd(&s.least, least);
     }
     auto occur = [](const u32x4& v) __attribute__((always_inline)) {
         uint32_t k = 0;

@@ -129,6 +129,23 @@ def test_masked_and_special_logits(dtype, V):
         assert tok[0] == -1 and tok[3] == -1
 
 
+@pytest.mark.parametrize("V", [1, 9, 3000, 70000])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_nan_of_either_sign(dtype, V):
+    x = _logits(6, V, 5, dtype)
+    bits = {BF: 0x7fc0, FP: 0x7e00, F32: 0x7fc00000}[dtype]
+    whole = x.view(torch.int32 if dtype is F32 else torch.int16)
+    sign = -2 ** (31 if dtype is F32 else 15)
+    whole[0, V // 2] = bits
+    whole[1, V // 2] = bits + sign
+    whole[2, :] = bits + sign
+    whole[3, 0] = -1                       # all bits set
+    whole[4, V - 1] = bits + sign
+    assert x[:5].isnan().any(1).all() and not x[5].isnan().any()
+    tok = _check(x, _u(6, 1))
+    assert (tok[:5] == -1).all() and tok[5] >= 0
+
+
 def test_u_at_its_ends():
     x = _logits(6, 777, 9)
     u = torch.tensor([0.0, 1 - 2.0 ** -24, 2.0 ** -149, 0.5, 2.0 ** -24, 0.0])
