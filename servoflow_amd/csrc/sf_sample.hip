@@ -333,7 +333,7 @@ struct SampleRule {
         top_p = p.top_p ? p.top_p[row] : p.top_p1;
         const float min_p = p.min_p ? p.min_p[row] : p.min_p1;
         if (!(temperature > 0.f)) temperature = 1.f, k = 1;   // the first in order
-        y_min = min_p > 0.f ? 128. * log2((double)min_p) : -INFINITY;
+        y_min = min_p > 0.f ? 128. * (log2((double)min_p) - M_LOG2E * 0x1p-54) : -INFINITY;   // what 64 bits round to min_p reaches it
         sc.octaves = 128. * M_LOG2E / (double)temperature;
         sc.per_bucket = fminf((float)(sc.octaves * (kBuckets / (128. * kOctaves))), 3e38f);
     }

@@ -146,6 +146,15 @@ def test_nan_of_either_sign(dtype, V):
     assert (tok[:5] == -1).all() and tok[5] >= 0
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_min_p_of_one_keeps_equal_weights(dtype):
+    # Logits 1e-20 apart weigh the same in 64 bits (and 2^-44 of the largest, in which they are held, is more); those 1e-3 apart
+    # do not.
+    x = _logits(4, 500, 8) * 1e-20
+    x[1] = x[1] * 1e17
+    _check(x.to(dtype), _u(4, 8), mp=1.0)
+
+
 def test_u_at_its_ends():
     x = _logits(6, 777, 9)
     u = torch.tensor([0.0, 1 - 2.0 ** -24, 2.0 ** -149, 0.5, 2.0 ** -24, 0.0])
