@@ -170,12 +170,20 @@ class DraftTree:
     masks: torch.Tensor     # int32 [1 or B, T, ceil(T / 32)]: a node's ancestors and itself, a bit each
     depth: torch.Tensor     # int32 [1 or B, T]: a node's number of ancestors
 
+    def __post_init__(self):   # the kernels read as much as parents' shape says
+        n, T = self.parents.shape
+        for t, shape in ((self.parents, (n, T)), (self.masks, (n, T, (T + 31) // 32)), (self.depth, (n, T))):
+            if t.shape != shape or t.dtype is not torch.int32 or t.device != self.parents.device or not t.is_contiguous():
+                raise ValueError(f"{tuple(t.shape)} {t.dtype} on {t.device}: contiguous int32 {shape} on "
+                                 f"{self.parents.device} expected")
+
 
 def draft_tree(parents):
     """The tables of trees of drafted tokens.  parents: device int32 [T] or [1,
     T] (one tree for all batch elements) or [B, T]; node 0 is the root, the last
     token already decided, and a node's parent comes before it (-1, or any other
-    value, for none).  A node's position is the root's plus its depth."""
+    value, for none).  A node's position is the root's plus its depth.  The tree
+    holds `parents` itself: it is not changed while the tree is in use."""
     if parents.dim() == 1:
         parents = parents[None]
     if parents.dim() != 2:

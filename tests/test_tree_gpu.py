@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from servoflow_amd import kernels
-from servoflow_amd.attention import Kv4Cache, accept_tree, attention_kv4, draft_tree
+from servoflow_amd.attention import DraftTree, Kv4Cache, accept_tree, attention_kv4, draft_tree
 
 from _drafts import accept, ancestors, attend_see, random_parents, tree_sees
 from _quant4 import half_step, kv4_levels
@@ -59,6 +59,19 @@ def test_chain_star_and_bad_parents():
         assert torch.equal(tree.depth[b].cpu().long(), see.sum(1) - 1)
     one = draft_tree(_int(chain))
     assert one.parents.shape == (1, T) and torch.equal(one.depth[0].cpu().long(), torch.arange(T))
+
+
+def test_a_tree_made_by_hand_is_checked():
+    tree = draft_tree(_int(torch.stack([random_parents(40, i) for i in range(3)])))
+    one = DraftTree(tree.parents[1:2], tree.masks[1:2], tree.depth[1:2])
+    want = draft_tree(tree.parents[1])
+    assert torch.equal(one.masks, want.masks) and torch.equal(one.depth, want.depth)
+    for parents, masks, depth in ((tree.parents, tree.masks[:1], tree.depth), (tree.parents, tree.masks[..., :1], tree.depth),
+                                  (tree.parents, tree.masks.long(), tree.depth), (tree.parents, tree.masks, tree.depth[:, :39]),
+                                  (tree.parents[:, ::2], tree.masks[:, ::2, :1], tree.depth[:, ::2]),
+                                  (tree.parents.cpu(), tree.masks, tree.depth)):
+        with pytest.raises(ValueError):
+            DraftTree(parents, masks, depth)
 
 
 # --- attention ----------------------------------------------------------------
