@@ -193,7 +193,9 @@ def draft_tree(parents):
     masks = torch.empty(n, T, (T + 31) // 32, dtype=torch.int32, device=dev)
     depth = torch.empty(n, T, dtype=torch.int32, device=dev)
     kernels.call_on(dev, "sf_tree_build", abi.lib().sf_tree_build, ptr, n, T, masks.data_ptr(), depth.data_ptr())
-    return DraftTree(parents, masks, depth)
+    tree = object.__new__(DraftTree)   # without the check: these do belong together
+    tree.__dict__.update(parents=parents, masks=masks, depth=depth)
+    return tree
 
 
 def accept_tree(tree, drafted, sampled):
