@@ -17,9 +17,9 @@
 // order, each gets its weight once, and the position is a value and a number among its
 // equals, whose index one more pass over the row finds in registers.
 //
-// 32-bit logits, and rows in which that fails (a value that occurs more than 65535
-// times), are spread over 2048 buckets of (l - m) /
-// temperature, 1 / 44.5 octave each, with count and weight of each; the bucket that
+// 32-bit logits, and rows in which that fails (two values, say, that occur more than
+// 65535 times), are spread over 2048 buckets of (l - m) / temperature, 1 / 44.5
+// octave each, with count and weight of each; the bucket that
 // holds the position is found from their running sums, and only its tokens (with
 // those above it where they are few) are put in order, in LDS.  A bucket of more than
 // 2048 tokens is cut by keys, 2048 parts at a time, until one value is left, of which
@@ -694,6 +694,7 @@ static inline int sample_parts(int rows, int V, int dtype) {
 
 constexpr int kHeld = 16;             // pieces of 16 bytes that a thread keeps: 131072 tokens of a row
 constexpr int kOverflow = -2;         // a token that is still to be found
+constexpr int kCommonFrom = 1024;     // rows of as many are looked over for a value that many tokens share
 constexpr uint32_t kMaxTies = 1024;   // equals that are told apart in a list
 constexpr uint32_t kValueList = 6656;   // values beside the counts
 
@@ -707,7 +708,7 @@ struct SampleValues {
         uint32_t key, rank, equals;
     } hits[3];
     uint64_t above;
-    uint32_t ties, nan, fail, least;
+    uint32_t ties, nan, fail, shared_by, common;
     int token;
 };
 
@@ -728,7 +729,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     } shared;
     __shared__ double table[1 << kExpBits];
     constexpr uint32_t kInf = KIND == 1 ? 0x7fu : 0x3ffu, kNegInf = 0xffffu - kInf;   // falling keys of the infinities
-    constexpr uint32_t kLeast = kNegInf - 1;                                          // of the lowest number
+    constexpr uint32_t kMinusZero = 0x8000, kNoKey = 0x10000;
     SampleValues& s = shared.values;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int64_t row = blockIdx.x;
@@ -736,6 +737,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     const int head = min(p.V, (int)((16 - (reinterpret_cast<uintptr_t>(x.base) & 15)) & 15) / 2);
     const int pieces = (p.V - head) / 8, tail = head + pieces * 8;
     const u32x4* from = reinterpret_cast<const u32x4*>(x.base + head * 2);
+    const uint16_t some = wave == 0 && p.V >= kCommonFrom ? reinterpret_cast<const uint16_t*>(x.base)[(int)((int64_t)lane * p.V >> 6)] : 0;
     u32x4 held[kHeld];
     const bool in_head = t < head, in_tail = t < p.V - tail;
     const uint32_t first = in_head ? reinterpret_cast<const uint16_t*>(x.base)[t] : 0u;
@@ -746,13 +748,15 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     auto count1 = [&](uint32_t keys) __attribute__((always_inline)) {
         atomicAdd(reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(s.bins) + (keys << 1 & 0x1fffcu)), 1u << (keys << 4 & 16u));
     };
-    // A row's masked logits, -infinity or the lowest number, are counted apart: all in one place they would be added one by
-    // one, and pass 16 bits.  `none`: -infinity, and the NaN behind it.
-    uint32_t least = 0, none = 0;
+    // Counted apart: -infinity (`none`, and the NaN behind it), and one value that many tokens share, as a row's masked ones
+    // do (`common`; of 64 tokens from all over the row the first of every fourth one's values that twelve have).  In their
+    // places among the others they would be added one by one, and pass 16 bits: 256 rows of 131072 bf16, all but 2% of them
+    // -10000, take 50 us, and took 186 so.
+    uint32_t common = kNoKey, shared_by = 0, none = 0;
     bool nan = false;
     auto count_any = [&](uint32_t key) __attribute__((always_inline)) {
-        if (key < kLeast) count1(key);
-        least += key == kLeast;
+        if (key < kNegInf && key != common) count1(key);
+        shared_by += key == common;
         none += key >= kNegInf;
         nan = nan || key > kNegInf;   // of either sign: the others are below kInf, and counted
     };
@@ -764,7 +768,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
             k[e] = sample_falling(v[e]);
             most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, k[e]));
         }
-        if (__any(most[0] >= kLeast || most[1] >= kLeast)) {
+        if (common != kNoKey || __any(most[0] >= kNegInf || most[1] >= kNegInf)) {
 #pragma unroll 1
             for (int e = 0; e < 8; ++e) {
                 const uint32_t x01 = e & 2 ? k[1] : k[0], x23 = e & 2 ? k[3] : k[2];
@@ -782,7 +786,21 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         sample_table(table);
 #pragma unroll
         for (int i = 0; i < 8; ++i) reinterpret_cast<u32x4*>(s.bins)[t + i * kSampleThreads] = u32x4{0, 0, 0, 0};
+        if (wave == 0) {
+            if (p.V >= kCommonFrom) {
+                const uint32_t key = sample_falling(some) & 0xffffu;
+                if (__popcll(__ballot(key == dpp_or_0<0x111, 0xf>(key))) >= 2) {   // neighbours: hardly ever without such a value
+#pragma unroll 1
+                    for (int i = 0; i < 64 && common == kNoKey; i += 4) {
+                        const uint32_t k = lane_of(key, i);
+                        if (__popcll(__ballot(key == k)) >= 12 && k < kNegInf && k != kMinusZero) common = k;
+                    }
+                }
+            }
+            if (lane == 0) s.common = common, s.shared_by = 0;
+        }
         lds_barrier();
+        common = __builtin_amdgcn_readfirstlane(s.common);
     };
     if (pieces > kHeld / 2 * kSampleThreads) {   // all loads at once, the last piece again behind it: each is waited for by itself
 #pragma unroll
@@ -807,6 +825,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     }
     if (in_head) count_any(sample_falling(first) & 0xffffu);
     if (in_tail) count_any(sample_falling(last) & 0xffffu);
+    if (common != kNoKey) {
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) shared_by += __shfl_xor(shared_by, d, 64);
+        if (lane == 0) atomicAdd(&s.shared_by, shared_by);
+    }
     __syncthreads();
     bool fail = false;
     if (t == 0) {   // -0, the first of its count, counts as 0, the second of the one before
@@ -814,18 +837,22 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         s.bins[0x4000] &= 0xffff0000u;
         fail = (s.bins[0x3fff] >> 16) + minus > 0xffffu;
         s.bins[0x3fff] += minus << 16;
-        s.above = s.ties = s.nan = s.fail = s.least = 0;
+        s.above = s.ties = s.nan = s.fail = 0;
+        if (s.shared_by) {   // and that value's one, for it to be among those that occur
+            uint32_t& two = s.bins[common >> 1];
+            const int at = 16 * (common & 1);
+            s.shared_by += two >> at & 0xffffu;
+            two = (two & ~(0xffffu << at)) | 1u << at;
+        }
     }
     __syncthreads();
+    const uint32_t many = s.shared_by;
+    auto tokens_of = [&](uint32_t e) __attribute__((always_inline)) { return e >> 16 == common ? many : e & 0xffffu; };
 
     // The values that occur, in order: 128 times 256 counts of two values, which the waves deal.  (Most hold nothing: a
     // row's values are a few thousand, side by side.)
-    uint32_t tokens = least + none;
-    if (__any(tokens != 0)) {
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) least += __shfl_xor(least, d, 64);
-        if (lane == 0) atomicAdd(&s.least, least);
-    }
+    uint32_t tokens = none;
+    if (t == 0 && many) tokens += many - 1;
     auto occur = [](const u32x4& v) __attribute__((always_inline)) {
         uint32_t k = 0;
 #pragma unroll
@@ -856,12 +883,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     before_wave(s.tokens, wave, tokens);
     const uint32_t own0 = s.steps[lane], own1 = s.steps[64 + lane];
     const uint32_t to0 = running64(own0), to1 = running64(own1) + lane_of(to0, 63), n = lane_of(to1, 63);
-    const uint32_t lowest = s.least;   // tokens of the lowest number: behind all that are in the list
     if (s.fail || tokens != (uint32_t)p.V) {   // a count that passed 16 bits: the sum of all is too small
         if (t == 0) p.token[row] = kOverflow;
         return;
     }
-    if (s.nan || n + lowest == 0) {
+    if (s.nan || n == 0) {
         if (t == 0) {
             p.token[row] = -1;
             if (p.logprob) p.logprob[row] = NAN;
@@ -908,9 +934,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         return KIND == 1 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
     };
     SampleScale& sc = rule.sc;
-    uint32_t top = kLeast;   // the largest value's key
+    uint32_t top;   // the largest value's key
     if (listed) {
-        if (n) top = list[0] >> 16;
+        top = list[0] >> 16;
     } else {
         const uint64_t has0 = __ballot(own0 != 0), has1 = __ballot(own1 != 0);
         const int step = has0 ? __builtin_ctzll(has0) : 64 + __builtin_ctzll(has1);
@@ -930,9 +956,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         if (!(e & 0xffffu)) continue;
         const float l = value(e >> 16);
         const double y = sc.exponent(l);
-        c += e & 0xffffu;
+        c += tokens_of(e);
         if (sc.bucket(l) < kBuckets) {
-            const uint64_t one = (e & 0xffffu) * sc.weight_in_play(y, table);
+            const uint64_t one = tokens_of(e) * sc.weight_in_play(y, table);
             w += one;
             above += y >= rule.y_min ? one : 0ull;
         }
@@ -948,28 +974,19 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     __syncthreads();
     c1 += before_wave(s.wave32, wave, all);
     w1 += before_wave(s.wave64, wave, all_mass);
-    const uint32_t c0 = c1 - c, listed_count = all;
-    const uint64_t w0 = w1 - w, listed_mass = all_mass;
-    const float lowest_value = value(kLeast);
-    const uint64_t lowest_weight = lowest && sc.bucket(lowest_value) < kBuckets ? sc.weight(sc.exponent(lowest_value), table) : 0ull;
-    all += lowest;
-    all_mass += lowest * lowest_weight;
-    above = with_min_p ? s.above + (sc.exponent(lowest_value) >= rule.y_min ? lowest * lowest_weight : 0ull) : ~0ull;
+    const uint32_t c0 = c1 - c;
+    const uint64_t w0 = w1 - w;
+    above = with_min_p ? s.above : ~0ull;
     uint32_t equals = 0;
     int asked = 0;
     auto ask = [&](const SampleQuery& q, bool) -> SampleHit {
-        if (!q.at(listed_count, listed_mass) || listed_count == 0) {   // among the lowest
-            const uint32_t r = sample_among_equals(q, lowest, listed_count, listed_mass, lowest_weight);
-            equals = lowest;
-            return SampleHit{listed_mass + r * lowest_weight, kLeast, r, -1};
-        }
         const uint64_t owner = __ballot(c && q.at(c1, w1) && (c0 == 0 || !q.at(c0, w0)));
         SampleValues::Hit& found = s.hits[asked++];   // a place for each question: a slow wave may still read the last one's
         if (owner) {   // this wave's: that thread's values, one a lane
             const int who = __builtin_ctzll(owner);
             const uint32_t i = (64 * wave + who) * each + lane;
             const bool in = (uint32_t)lane < each && i < values;
-            const uint32_t e = in ? entry(i) : 0u, mult = e & 0xffffu;
+            const uint32_t e = in ? entry(i) : 0u, mult = in ? tokens_of(e) : 0u;
             const float l = value(e >> 16);
             const uint64_t one = in && sc.bucket(l) < kBuckets ? sc.weight_in_play(sc.exponent(l), table) : 0ull;
             const uint32_t cs = running64(mult) + lane_of(c0, who), cb = cs - mult;

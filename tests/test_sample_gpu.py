@@ -239,6 +239,26 @@ def test_many_equal_16_bit_logits(V, dtype):
         _check(x, u, what=str(r), **r)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("V", [1023, 1024, 5001, 70000, 200000])
+def test_a_value_that_many_tokens_share(dtype, V):
+    """It is counted apart where it is many tokens' (by itself, as 0 beside -0, beside -infinity); it is drawn as any other."""
+    g = torch.Generator().manual_seed(V)
+    x = _logits(8, V, 3, dtype)
+    some = torch.rand(8, V, generator=g)
+    x[0][some[0] < 0.97] = -1e4
+    x[1][some[1] < 0.5] = 0.0
+    x[2][some[2] < 0.5] = torch.where(torch.rand(V, generator=g) < 0.5, 0.0, -0.0).to(dtype)[some[2] < 0.5]
+    x[3][some[3] < 0.4], x[3][some[3] > 0.6] = -math.inf, 2.0
+    x[4][some[4] < 0.97] = -0.0
+    x[5][some[5] < 0.2] = 1.5
+    x[6, V // 3:] = torch.finfo(dtype).min
+    x[7][some[7] < 0.9] = x[7].max()       # the largest
+    u = torch.tensor([0.999, 0.5, 0.55, 0.8, 0.6, 0.3, 1 - 2.0 ** -24, 0.777])
+    for r in ({}, {"k": V - 3}, {"p": 0.7}, {"mp": 0.3, "t": 3.0}, {"t": 1e6}, {"t": 5.0, "k": 2000, "p": 0.9}, {"t": 0.0}):
+        _check(x, u, what=str(r), **r)
+
+
 def test_only_lowest_numbers_are_left():
     """A row masked by the lowest number but for -infinity: its tokens share the weight."""
     for dtype in (BF, FP, F32):
