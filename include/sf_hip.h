@@ -892,8 +892,9 @@ typedef struct sf_gemm_i8_desc {
     int32_t c_dtype;         /* SF_F32, SF_BF16 or SF_F16 */
     int32_t accumulate;      /* SF_F32 only: C += act(...) */
 } sf_gemm_i8_desc;
-/* Bytes of device workspace (the codes and scales of rows to be quantised, 0 for SF_I8 rows),
- * 16-byte aligned, no initialisation; calls that may run concurrently need separate ones. */
+/* Bytes of device workspace (the codes and scales of rows to be quantised; 0 for SF_I8 rows, and for up to 16
+ * rows of 8192 inputs in all, which are quantised where they are multiplied), 16-byte aligned, no
+ * initialisation; calls that may run concurrently need separate ones. */
 size_t sf_gemm_i8_workspace_bytes(const sf_gemm_i8_desc* desc);
 /* C must not overlap A. */
 int sf_gemm_i8(const sf_gemm_i8_desc* desc, void* workspace, size_t workspace_bytes, void* stream);

@@ -10,6 +10,13 @@
 // lie there in pieces of 16, piece c of row r at c ^ (r / 2 & 7): the 16 rows that a
 // read of 16 bytes takes at a time then lie in different banks.  Few rows: see
 // gemm_i8_rows_kernel.
+//
+// What bounds them (us): 4374 x 8192 x 8192 takes 290, 2.02 POP/s, where the loads into
+// LDS alone take 208, the products with their reads from LDS alone 219 to 227, and a
+// large library product of 8-bit integers runs at 2.4 POP/s (292 for this one); with its
+// quantising, one pass over 72 MB in and 36 out, 306 to 313.  67 x 6144 x 2048 takes 13.4
+// with it, 8.7 without: a chain of launch, first operands, 16 stages and stores.  1 x 8192
+// x 8192 takes 17.7 from memory, 3.8 TB/s of weights.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

@@ -82,7 +82,13 @@ struct KvAttnArgs {
 
 // A tree: the T nodes are the last T tokens, all before them are seen by every row.  Which of
 // the 32 tokens from key0 on the row of node `node` sees, the nodes' first token at key `at`:
-// two words of its ancestors, shifted (about one block in T / 32 + 1 asks).
+// two words of its ancestors, shifted.  Only the T / 32 + 1 blocks that hold nodes ask; all before
+// them run as a call without a tree, so the rows cost what they cost there.  us: 16 x 8 heads x 64
+// rows (16 nodes) over 2048..8192 keys of 128 channels 82, of a floor of 19: the pair's vector
+// work, done for two groups of 32 rows that each unpack the block, and the longest sequence, whose
+// workgroups have a CU each (in equal pieces of 4096, 2048, 1024 keys 96, 98 and 115: a workgroup's
+// start, join and merge cost more than the balance gains); 4 x 32 heads x 64 rows over 1094..4374
+// keys of 64 24, of 5.
 __device__ __forceinline__ uint32_t kv_tree_bits(const KvAttnArgs& p, int b, int node, int key0, int at) {
     const uint32_t* row = p.tree + b * p.tree_stride + (int64_t)node * p.tree_words;
     const int r = key0 - at, w = r >> 5;   // rounded down
