@@ -14,7 +14,7 @@
 // What bounds them (us): 4374 x 8192 x 8192 takes 290, 2.02 POP/s, where the loads into
 // LDS alone take 208, the products with their reads from LDS alone 219 to 227, and a
 // large library product of 8-bit integers runs at 2.4 POP/s (292 for this one); with its
-// quantising, one pass over 72 MB in and 36 out, 306 to 313.  67 x 6144 x 2048 takes 13.4
+// quantising, one pass over 72 MB in and 36 out, 297.  67 x 6144 x 2048 takes 13.4
 // with it, 8.7 without: a chain of launch, first operands, 16 stages and stores.  1 x 8192
 // x 8192 takes 17.7 from memory, 3.8 TB/s of weights.
 #include <hip/hip_runtime.h>
@@ -32,6 +32,8 @@ namespace sfk {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
+constexpr int kI8MaxInputs = 1 << 16;
+
 // ---------------------------------------------------------------- quantising
 
 // Code of x for a step s > 0: |x| <= 127 s but for the step's own rounding.
@@ -45,90 +47,148 @@ __device__ __forceinline__ int i8_code(float x, float s, float inv) {
     return (int)fminf(fmaxf(q, -127.f), 127.f);
 }
 
-template <int KIND>   // 0 fp32, 1 bf16, 2 fp16
-__device__ __forceinline__ void i8_load8(const void* row, int k, float (&x)[8]) {
-    if (KIND == 0) {
-        const f32x4* src = reinterpret_cast<const f32x4*>(static_cast<const float*>(row) + k);
-        const f32x4 a = src[0], b = src[1];
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// Eight inputs of a row.  KIND: 0 fp32, 1 bf16, 2 fp16.
+template <int KIND>
+struct I8Piece {
+    u32x4 v[KIND == 0 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* row, int k) {
+        const u32x4* from = reinterpret_cast<const u32x4*>(static_cast<const char*>(row) + (int64_t)k * (KIND == 0 ? 4 : 2));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
-    } else {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(row) + k);
+        for (int i = 0; i < (KIND == 0 ? 2 : 1); ++i) v[i] = from[i];
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (KIND == 0 ? 2 : 1); ++i) v[i] = u32x4{0, 0, 0, 0};
+    }
+    // The larger of `most` and these without their signs, as whole numbers: an infinity is above all numbers, and a NaN
+    // above that.  16-bit ones two by two.
+    __device__ __forceinline__ uint32_t most(uint32_t most) const {
+#pragma unroll
+        for (int i = 0; i < (KIND == 0 ? 2 : 1); ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (KIND == 0) most = max(most, v[i][e] & 0x7fffffffu);
+                else most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
+                                                                                   __builtin_bit_cast(u16x2, v[i][e] & 0x7fff7fffu)));
+            }
+        return most;
+    }
+    static __device__ __forceinline__ float value(uint32_t h) {   // of 16 bits
+        return KIND == 1 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+    }
+    // What `most` found, as the bits of an fp32 number.
+    static __device__ __forceinline__ uint32_t bits(uint32_t most) {
+        return KIND == 0 ? most : __float_as_uint(value(max(most & 0xffffu, most >> 16)));
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint32_t h = v[e >> 1];
-            if (KIND == 1) x[e] = __uint_as_float(e & 1 ? h & 0xffff0000u : h << 16);
-            else x[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(h >> (16 * (e & 1))));
+            if (KIND == 0) x[e] = __uint_as_float(v[e >> 2 & (KIND == 0)][e & 3]);
+            else x[e] = value(v[0][e >> 1] >> (16 * (e & 1)) & 0xffffu);
         }
     }
-}
+};
 
-// A row's step from its largest |x|, and the same for i8_code where the step's half or reciprocal is no normal number.
+// A row's step from the bits of its largest |x|, and the same for i8_code where the step's half or reciprocal is no normal
+// number.
 struct I8Step {
     float s, step, inv, up;
     bool plain;   // no: codes 0 (a row of zeros; an infinity or a NaN, whose step makes the products NaN)
-    __device__ __forceinline__ explicit I8Step(float big) {
-        s = big / 127.f;
+    __device__ __forceinline__ explicit I8Step(uint32_t big) {
+        s = __uint_as_float(big) / 127.f;
         plain = s > 0.f && s < INFINITY;
         up = s < 0x1p-60f ? 0x1p100f : 1.f;
         step = s * up;
         inv = 1.f / step;
     }
-    __device__ __forceinline__ uint2 codes(const float (&y)[8]) const {
-        uint32_t u[2] = {0u, 0u};
-        if (plain) {
+    // x times the reciprocal is off by less than 127 2^-23 and a rounding: where it is further than 2e-5 from the middle of two
+    // codes the nearer one is right, and one addition of 1.5 2^23 leaves it in the low bits.  False where it is not for one of
+    // these eight (for one in 3000), or the step asks for `up`: slow_codes.
+    __device__ __forceinline__ bool codes(const float (&y)[8], uint2& u) const {
+        constexpr float kWhole = 12582912.f;
+        float far = 0.f;
+        uint32_t z[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) u[e >> 2] |= ((uint32_t)i8_code(y[e] * up, step, inv) & 0xffu) << (8 * (e & 3));
+        for (int e = 0; e < 8; ++e) {
+            const float n = __builtin_fmaf(y[e], inv, kWhole);
+            far = fmaxf(far, fabsf(__builtin_fmaf(y[e], inv, kWhole - n)));
+            z[e] = __float_as_uint(n);
         }
+        auto four = [&](int i) {
+            return __builtin_amdgcn_perm(z[i + 1], z[i], 0x0c0c0400u) | __builtin_amdgcn_perm(z[i + 3], z[i + 2], 0x04000c0cu);
+        };
+        u = plain ? uint2{four(0), four(4)} : uint2{0u, 0u};
+        return !plain || (up == 1.f && far < 0.49998f);
+    }
+    __device__ __forceinline__ uint2 slow_codes(const float (&y)[8]) const {
+        uint32_t u[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e >> 2] |= ((uint32_t)i8_code(y[e] * up, step, inv) & 0xffu) << (8 * (e & 3));
         return uint2{u[0], u[1]};
     }
 };
 
-// One workgroup a row.  Up to 8192 inputs stay in registers between the maximum and the codes.
+// One workgroup a row.  Up to 8192 inputs stay in registers between the maximum and the codes.  4374 rows of 8192 bf16
+// inputs take 22 us (21 at the rate of a copy; 29 with i8_code for all of them), 67 x 2048 6, a launch and a row's chain.
 template <int KIND>
 __global__ __launch_bounds__(256) void quant_i8_kernel(const void* a, int64_t lda, int K, int8_t* codes, int64_t ldc, float* scale) {
     constexpr int kHeld = 4;
-    __shared__ float part[4];
+    __shared__ uint32_t part[4];
     const int64_t m = blockIdx.x;
     const void* row = static_cast<const char*>(a) + m * lda * (KIND == 0 ? 4 : 2);
-    float x[kHeld][8], big = 0.f;
-    bool bad = false;
+    I8Piece<KIND> x[kHeld];
+    uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const int k = 8 * (int)threadIdx.x + 2048 * i;
-        if (k < K) i8_load8<KIND>(row, k, x[i]);
-        else
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[i][e])), bad = bad || x[i][e] != x[i][e];
+        if (k < K) x[i].load(row, k);
+        else x[i].clear();
     }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) most = x[i].most(most);
     for (int k = 8 * (int)threadIdx.x + 2048 * kHeld; k < K; k += 2048) {
-        float y[8];
-        i8_load8<KIND>(row, k, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(y[e])), bad = bad || y[e] != y[e];
+        I8Piece<KIND> y;
+        y.load(row, k);
+        most = y.most(most);
     }
+    most = I8Piece<KIND>::bits(most);
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) big = fmaxf(big, __shfl_xor(big, d, 64));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = big;
-    bad = __syncthreads_or(bad);
-    big = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    const I8Step st(bad ? NAN : big);
+    for (int d = 32; d >= 1; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
+    __syncthreads();
+    const I8Step st(max(max(part[0], part[1]), max(part[2], part[3])));
     if (threadIdx.x == 0) scale[m] = st.s;
     int8_t* dst = codes + m * ldc;
-    auto store = [&](int k, const float (&y)[8]) { *reinterpret_cast<uint2*>(dst + k) = st.codes(y); };
+    uint32_t again = 0;   // pieces of the thread, 32 at most
+    auto store = [&](int i, int k, const I8Piece<KIND>& piece) {
+        float y[8];
+        uint2 u;
+        piece.floats(y);
+        if (!st.codes(y, u)) again |= 1u << i;
+        *reinterpret_cast<uint2*>(dst + k) = u;
+    };
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const int k = 8 * (int)threadIdx.x + 2048 * i;
-        if (k < K) store(k, x[i]);
+        if (k < K) store(i, k, x[i]);
     }
-    for (int k = 8 * (int)threadIdx.x + 2048 * kHeld; k < K; k += 2048) {
+    for (int i = kHeld, k = 8 * (int)threadIdx.x + 2048 * kHeld; k < K; ++i, k += 2048) {
+        I8Piece<KIND> y;
+        y.load(row, k);
+        store(i, k, y);
+    }
+    for (; again; again &= again - 1) {   // from memory once more: few, and the code stays small
+        const int k = 8 * (int)threadIdx.x + 2048 * __builtin_ctz(again);
+        I8Piece<KIND> piece;
         float y[8];
-        i8_load8<KIND>(row, k, y);
-        store(k, y);
+        piece.load(row, k);
+        piece.floats(y);
+        *reinterpret_cast<uint2*>(dst + k) = st.slow_codes(y);
     }
 }
+static_assert(kI8MaxInputs <= 32 * 2048, "a bit for each of a thread's pieces");
 
 // ------------------------------------------------------------------ products
 
@@ -394,7 +454,7 @@ __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(const I8Args p) {
     if constexpr (kFused) {
         constexpr int kChunks = kFusedCodes / 8 / 512;   // of 8 inputs, of a thread
         const int per_row = p.K / 8, all = p.M * per_row;
-        float y[kChunks][8];
+        I8Piece<KIND> y[kChunks];
         int at[kChunks];
         if (threadIdx.x < 16) biggest[threadIdx.x] = 0;
         __syncthreads();
@@ -402,26 +462,25 @@ __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(const I8Args p) {
         for (int i = 0; i < kChunks; ++i) {
             const int c = (int)threadIdx.x + 512 * i, row = c / per_row;
             at[i] = c < all ? row : -1;
-            if (c >= all) continue;
-            i8_load8<KIND>(static_cast<const char*>(p.x) + row * p.ldx * (KIND == 0 ? 4 : 2), 8 * (c % per_row), y[i]);
+            if (c < all) y[i].load(static_cast<const char*>(p.x) + row * p.ldx * (KIND == 0 ? 4 : 2), 8 * (c % per_row));
         }
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            if (at[i] < 0) continue;
-            uint32_t big = 0;   // as whole numbers: an infinity is above all numbers, and a NaN above that
-#pragma unroll
-            for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(y[i][e]) & 0x7fffffffu);
-            atomicMax(&biggest[at[i]], big);
-        }
+        for (int i = 0; i < kChunks; ++i)
+            if (at[i] >= 0) atomicMax(&biggest[at[i]], I8Piece<KIND>::bits(y[i].most(0u)));
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             if (at[i] < 0) continue;
             const int c = (int)threadIdx.x + 512 * i;
-            *reinterpret_cast<uint2*>(held + at[i] * (p.K + 16) + 8 * (c % per_row)) = I8Step(__uint_as_float(biggest[at[i]])).codes(y[i]);
+            const I8Step st(biggest[at[i]]);
+            float x8[8];
+            uint2 u;
+            y[i].floats(x8);
+            if (!st.codes(x8, u)) u = st.slow_codes(x8);
+            *reinterpret_cast<uint2*>(held + at[i] * (p.K + 16) + 8 * (c % per_row)) = u;
         }
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) sm[i] = I8Step(__uint_as_float(biggest[r])).s;   // rows behind the last: 0, not stored
+        for (int i = 0; i < kUnits; ++i) sm[i] = I8Step(biggest[r]).s;   // rows behind the last: 0, not stored
         __syncthreads();
     }
     for (int kb = wave; kb < blocks; kb += DEPTH * NW) {
@@ -545,7 +604,7 @@ static inline bool i8_float(int dtype) { return dtype == SF_F32 || dtype == SF_B
 static inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // Rows, inputs and strides that the kernels' 32-bit offsets take: 256 rows of a tile below 2^31 bytes.
-constexpr int kI8MaxRows = 1 << 22, kI8MaxInputs = 1 << 16;
+constexpr int kI8MaxRows = 1 << 22;
 constexpr int64_t kI8MaxStride = 1 << 22;
 
 static size_t i8_scales_at(const sf_gemm_i8_desc* d) { return ((size_t)d->M * (size_t)d->K + 15) / 16 * 16; }
