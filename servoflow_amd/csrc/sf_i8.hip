@@ -15,8 +15,8 @@
 // LDS alone take 208, the products with their reads from LDS alone 219 to 227, and a
 // large library product of 8-bit integers runs at 2.4 POP/s (292 for this one); with its
 // quantising, one pass over 72 MB in and 36 out, 297.  67 x 6144 x 2048 takes 13.4
-// with it, 8.7 without: a chain of launch, first operands, 16 stages and stores.  1 x 8192
-// x 8192 takes 17.7 from memory, 3.8 TB/s of weights.
+// with it, 8.5 without: a chain of launch, first operands, 16 stages and stores.  1 x 8192
+// x 8192 takes 15.0 from memory, 4.5 TB/s of weights.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -131,7 +131,7 @@ struct I8Step {
 };
 
 // One workgroup a row.  Up to 8192 inputs stay in registers between the maximum and the codes.  4374 rows of 8192 bf16
-// inputs take 22 us (21 at the rate of a copy; 29 with i8_code for all of them), 67 x 2048 6, a launch and a row's chain.
+// inputs take 20 us (21 at the rate of a copy; 27 with i8_code for all of them), 67 x 2048 3.3, a launch and a row's chain.
 template <int KIND>
 __global__ __launch_bounds__(256) void quant_i8_kernel(const void* a, int64_t lda, int K, int8_t* codes, int64_t ldc, float* scale) {
     constexpr int kHeld = 4;
@@ -564,9 +564,9 @@ static int i8_shape(const I8Args& p) {
     return best;
 }
 
-// Few inputs are quantised where they are multiplied.  us in a graph, so and in two launches: 1 x 2048 x 2048 6.4 and 8.5,
-// 1 x 8192 x 8192 17.7 and 22.3, 5 x 2051 x 1152 6.5 and 8.5; of more inputs every workgroup's own quantising counts: 8 x 2048
-// x 2048 10.0 and 9.0, 8 x 8192 x 2048 15.3 and 11.0.
+// Few inputs are quantised where they are multiplied.  us in a graph, so and in two launches: 1 x 2048 x 2048 4.1 and 5.8,
+// 1 x 8192 x 8192 14.2 and 18.9, 5 x 2051 x 1152 4.9 and 6.0, 4 x 8192 x 2048 8.6 and 8.4; of more inputs every workgroup's
+// own quantising counts: 8 x 8192 x 2048 took 4 more.
 static inline bool i8_fused(const sf_gemm_i8_desc* d) {
     return d->a_dtype != SF_I8 && d->M <= 16 && (int64_t)d->M * d->K <= kFusedCodes;
 }

@@ -749,9 +749,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         atomicAdd(reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(s.bins) + (keys << 1 & 0x1fffcu)), 1u << (keys << 4 & 16u));
     };
     // Counted apart: -infinity (`none`, and the NaN behind it), and one value that many tokens share, as a row's masked ones
-    // do (`common`; of 64 tokens from all over the row the first of every fourth one's values that twelve have).  In their
+    // do (`common`; of 64 tokens from all over the row, one that two neighbours and twelve in all have).  In their
     // places among the others they would be added one by one, and pass 16 bits: 256 rows of 131072 bf16, all but 2% of them
-    // -10000, take 50 us, and took 186 so.
+    // -10000, take 48 us, and took 184 so.
     uint32_t common = kNoKey, shared_by = 0, none = 0;
     bool nan = false;
     auto count_any = [&](uint32_t key) __attribute__((always_inline)) {
@@ -789,12 +789,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         if (wave == 0) {
             if (p.V >= kCommonFrom) {
                 const uint32_t key = sample_falling(some) & 0xffffu;
-                if (__popcll(__ballot(key == dpp_or_0<0x111, 0xf>(key))) >= 2) {   // neighbours: hardly ever without such a value
-#pragma unroll 1
-                    for (int i = 0; i < 64 && common == kNoKey; i += 4) {
-                        const uint32_t k = lane_of(key, i);
-                        if (__popcll(__ballot(key == k)) >= 12 && k < kNegInf && k != kMinusZero) common = k;
-                    }
+                uint64_t twice = __ballot(key == dpp_or_0<0x111, 0xf>(key));   // as the lane before: hardly any without such a value
+                for (; twice && common == kNoKey; twice &= twice - 1) {
+                    const uint32_t k = lane_of(key, __builtin_ctzll(twice));
+                    if (__popcll(__ballot(key == k)) >= 12 && k < kNegInf && k != kMinusZero) common = k;
                 }
             }
             if (lane == 0) s.common = common, s.shared_by = 0;
