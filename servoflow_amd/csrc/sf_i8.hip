@@ -14,8 +14,8 @@
 // What bounds them (us): 4374 x 8192 x 8192 takes 290, 2.02 POP/s, where the loads into
 // LDS alone take 208, the products with their reads from LDS alone 219 to 227, and a
 // large library product of 8-bit integers runs at 2.4 POP/s (292 for this one); with its
-// quantising, one pass over 72 MB in and 36 out, 297.  67 x 6144 x 2048 takes 13.4
-// with it, 8.5 without: a chain of launch, first operands, 16 stages and stores.  1 x 8192
+// quantising, one pass over 72 MB in and 36 out, 297.  67 x 6144 x 2048 takes 10.4
+// with it, 7.8 without: a chain of launch, first operands, stages, join and stores.  1 x 8192
 // x 8192 takes 15.0 from memory, 4.5 TB/s of weights.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -273,24 +273,27 @@ __device__ __forceinline__ void i8_tile(const I8Args& p, int& tm, int& tn) {
 // inputs, two to a line, the loads alone took 217 us of 4096 x 8192 x 8192, so 166); STAGES of them in a ring.  A quarter's
 // operands are read under the products of the one before it, those of the next stage's first under the last one's,
 // behind the one barrier of a stage.
-template <int MI, int NI, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(const I8Args p) {
-    constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, NW = WM * WN, kStage = (BM + BN) * 128;
+// KS groups of waves deal the stages, each with a ring of its own, and join in LDS.
+template <int MI, int NI, int WM, int WN, int STAGES, int KS = 1>
+__global__ __launch_bounds__(64 * WM * WN * KS) void gemm_i8_kernel(const I8Args p) {
+    constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, NW = WM * WN, kStage = (BM + BN) * 128;   // NW: of a group
     constexpr int kLoads = (BM + BN) / 8 / NW;   // instructions of a wave, 8 rows each
     static_assert(BM % 8 == 0 && kLoads * 8 * NW == BM + BN, "whole instructions");
     // One array: beside a second one the compiler waits for every load into LDS before each read from it.
-    __shared__ __attribute__((aligned(1024))) int8_t lds[STAGES * kStage + 4 * (BM + 2 * BN)];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ __attribute__((aligned(1024))) int8_t lds[KS * STAGES * kStage + 4 * (BM + 2 * BN)];
+    const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = all_waves / NW, wave = all_waves % NW;
     const int wm = wave / WN, wn = wave % WN, col = lane & 31, g = lane >> 5;
+    int8_t* const ring = lds + group * STAGES * kStage;
     int tm, tn;
     i8_tile(p, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int rows = min(BM, p.M - m0), cols = min(BN, p.N - n0);
     // Scales and bias wait in LDS: read from memory tile by tile at the end they cost 25 us of a 256 x 256 tile.
-    float* w_scale = reinterpret_cast<float*>(lds + STAGES * kStage);
+    float* w_scale = reinterpret_cast<float*>(lds + KS * STAGES * kStage);
     float* bias = w_scale + BN;
     float* a_scale = bias + BN;
-    static_assert(BM <= 64 * NW && BN <= 64 * NW, "a thread for each");
+    static_assert(BM <= 64 * NW * KS && BN <= 64 * NW * KS, "a thread for each");
     if ((int)threadIdx.x < BM) a_scale[threadIdx.x] = (int)threadIdx.x < rows ? p.a_scale[m0 + threadIdx.x] : 0.f;
     if ((int)threadIdx.x < BN) {
         const bool in = (int)threadIdx.x < cols;
@@ -313,7 +316,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(const I8Args p) {
         at[i] = r < (is_a ? rows : cols) ? (uint32_t)r * (uint32_t)(is_a ? p.lda : p.ldw) + (uint32_t)k_lane[piece & 1] : 0x80000000u;
     }
     auto fetch = [&](int s, int8_t* to) __attribute__((always_inline)) {
-        const int k0 = 128 * s;
+        const int k0 = 128 * (KS * s + group);
         auto load = [&](int i, uint32_t off) __attribute__((always_inline)) {
             const int piece = i * NW + wave;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(piece < BM / 8 ? ars : wrs,
@@ -321,7 +324,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(const I8Args p) {
         };
         if (k0 + 128 <= p.K) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) load(i, at[i] + (uint32_t)k0);   // behind the end stays there: k0 is below 2^17
+            for (int i = 0; i < kLoads; ++i) load(i, at[i] + (uint32_t)k0);   // behind the end stays there: k0 is below 2^18
         } else {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
@@ -357,30 +360,47 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(const I8Args p) {
     // the barrier.
     auto meet = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
-        __builtin_amdgcn_s_barrier();
+        if (NW > 1) __builtin_amdgcn_s_barrier();   // a wave alone has its ring to itself
         asm volatile("" ::: "memory");
     };
-    const int steps = (p.K + 127) / 128;
+    const int steps = (p.K + 128 * KS - 1) / (128 * KS);
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) fetch(i, lds + i * kStage);   // behind K: zeros
+    for (int i = 0; i < STAGES - 1; ++i) fetch(i, ring + i * kStage);   // behind K: zeros
+    if (NW == 1) __syncthreads();   // the scales
     meet();
     int here = 0, last = (STAGES - 1) * kStage;   // the stage that is multiplied, and the place of the one before it
-    operands(lds, 0);
+    operands(ring, 0);
     for (int s = 0; s < steps; ++s) {
-        fetch(s + STAGES - 1, lds + last);   // every wave has read what is there
-        operands(lds + here, 1);
+        fetch(s + STAGES - 1, ring + last);   // every wave has read what is there
+        operands(ring + here, 1);
         multiply(0);
-        operands(lds + here, 2);
+        operands(ring + here, 2);
         multiply(1);
-        operands(lds + here, 3);
+        operands(ring + here, 3);
         multiply(2);
         meet();
         last = here;
         here = here == (STAGES - 1) * kStage ? 0 : here + kStage;
-        operands(lds + here, 0);   // behind the last stage: not used
+        operands(ring + here, 0);   // behind the last stage: not used
         multiply(3);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing comes into LDS behind the end
+    // The groups' sums: each stores the quarters q = group, group + KS, ... of every tile.
+    constexpr int kTiles = MI * NI * 4;
+    static_assert(KS == 1 || (4 % KS == 0 && NW * kTiles * 1024 <= STAGES * kStage), "the join takes the rings' place");
+    i32x4* sums = reinterpret_cast<i32x4*>(lds) + (KS * wave * kTiles + group) * 64 + lane;   // [wave][quarter of a tile][group][lane]
+    if constexpr (KS > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    sums[((j * MI + i) * 4 + q) * KS * 64] = i32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+        __syncthreads();
+        sums -= group * 64;
+    }
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
         const int m = 32 * (MI * wm + i) + col;
@@ -388,11 +408,19 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_kernel(const I8Args p) {
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int of = 0; of < 4 / KS; ++of) {
+                const int q = KS * of + (KS > 1 ? group : 0);
                 const int n = 32 * (NI * wn + j) + 8 * q + 4 * g;
+                i32x4 v;
+                if constexpr (KS > 1) {
+                    v = sums[((j * MI + i) * 4 + q) * KS * 64];
+#pragma unroll
+                    for (int k = 1; k < KS; ++k) v += sums[(((j * MI + i) * 4 + q) * KS + k) * 64];
+                } else {
+                    v = i32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+                }
                 const I8Columns c = {*reinterpret_cast<const f32x4*>(w_scale + n), *reinterpret_cast<const f32x4*>(bias + n)};
-                i8_store(p, m0 + m, n0 + n, i32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]},
-                         sm, c);
+                i8_store(p, m0 + m, n0 + n, v, sm, c);
             }
     }
 }
@@ -517,11 +545,11 @@ __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(const I8Args p) {
     }
 }
 
-template <int MI, int NI, int WM, int WN, int STAGES>
+template <int MI, int NI, int WM, int WN, int STAGES, int KS = 1>
 static void launch_i8(I8Args p, hipStream_t s) {
     p.mt = (p.M + 32 * MI * WM - 1) / (32 * MI * WM);
     p.nt = (p.N + 32 * NI * WN - 1) / (32 * NI * WN);
-    hipLaunchKernelGGL((gemm_i8_kernel<MI, NI, WM, WN, STAGES>), dim3((unsigned)(p.mt * p.nt)), dim3(64 * WM * WN), 0, s, p);
+    hipLaunchKernelGGL((gemm_i8_kernel<MI, NI, WM, WN, STAGES, KS>), dim3((unsigned)(p.mt * p.nt)), dim3(64 * WM * WN * KS), 0, s, p);
 }
 
 template <int MB, int NT, int DEPTH>
@@ -532,21 +560,24 @@ static void launch_i8_rows(const I8Args& p, hipStream_t s) {
 
 // The shape whose estimate is the smallest.  A CU takes its share of the workgroups, `resident` at a time; such a round
 // of k of them takes `each` us and for every step max(alone, shared k): a workgroup's own chain, or what the CU fetches
-// and multiplies.  A step is 128 inputs of a tile, 1024 of the forms for few rows (a block for each wave).  Fitted to
-// 270 products of 1..4374 rows, 256..8192 columns and 512..8192 inputs, where the choice costs 0.7% in the mean, and up to
-// 14%, over the fastest of 16 shapes.  us:
-//   1 x 8192 x 8192 14.0 with 16 x 16, 16.5 with 32 x 32 (weights from memory); 67 x 8192 x 8192 21.6 with 64 x 64,
-//   25.3 with 64 x 128, 29.5 with 80 x 32; 1072 x 256 x 8192 18.8 with 64 x 64 and four stages, 33.8 with two; 268 x 8192
-//   x 8192 35.3 with 128 x 128 and 16 waves, 37.0 with 8; 4374 x 2048 x 2048 29.5 with 192 x 256, 36.5 with 128 x 128;
-//   4374 x 8192 x 8192 290 with 192 x 256 (three full rounds of workgroups), 346 with 256 x 256.
+// and multiplies.  A step is 128 inputs of a tile for each group of waves, 1024 of the forms for few rows (a block for each
+// wave).  Fitted to 585 products of 1..4374 rows, 256..8192 columns and 512..8192 inputs, where the choice costs 1% in the
+// mean, and up to 29%, over the fastest of 21 shapes, with weights that mostly come from the memory-side cache; from memory
+// the tiles of 32 rows lose a third where one slab of them reads all weights (1 x 2048 x 8192: 10.3, with 16 x 16 7.6).  us:
+//   1 x 8192 x 8192 14.0 with 16 x 16, 16.5 with 16 x 32 (weights from memory); 67 x 2048 x 8192 8.3 with 32 x 32 in four
+//   groups, 17.0 with 64 x 64 in one; 134 x 2048 x 8192 11.3 with 32 x 64 in four, 14.1 with 64 x 64 in two, 18.7 in one;
+//   536 x 1000 x 8192 14.8 with 64 x 64 in two, 19.0 in one, 21.7 with 32 x 64 in four; 268 x 8192 x 8192 35.3 with
+//   128 x 128 and 16 waves, 37.0 with 8; 4374 x 2048 x 2048 29.5 with 192 x 256, 36.5 with 128 x 128; 4374 x 8192 x 8192
+//   290 with 192 x 256 (three full rounds of workgroups), 346 with 256 x 256.
 struct I8Shape {
     int bm, bn, step, resident;
     double start, alone, shared, each;
 };
 constexpr I8Shape kI8Shapes[] = {
-    {16, 16, 1024, 4, 2.25, 0.94, 0.88, 0.0},  {16, 32, 1024, 4, 2.03, 1.47, 1.26, 0.0},  {32, 32, 1024, 4, 2.19, 1.83, 1.83, 0.0},
-    {64, 64, 128, 2, 1.38, 0.235, 0.19, 2.65}, {64, 128, 128, 1, 0.99, 0.307, 0.0, 3.1},  {128, 128, 128, 2, 0.0, 0.62, 0.54, 4.5},
-    {128, 128, 128, 1, 0.0, 0.41, 0.0, 4.9},   {128, 256, 128, 1, 0.0, 0.71, 0.0, 7.6},   {192, 256, 128, 1, 0.0, 1.05, 0.0, 9.0},
+    {16, 16, 1024, 4, 1.91, 0.0, 0.877, 0.05}, {16, 32, 1024, 4, 1.90, 0.0, 1.337, 0.0},  {32, 32, 512, 1, 1.28, 0.328, 0.0, 2.15},
+    {32, 32, 512, 2, 1.05, 0.468, 0.335, 1.97}, {32, 64, 512, 1, 1.05, 0.509, 0.0, 2.37}, {64, 64, 256, 1, 0.99, 0.357, 0.0, 2.67},
+    {64, 128, 256, 1, 0.05, 0.520, 0.0, 4.25}, {64, 128, 128, 1, 0.58, 0.312, 0.0, 3.10}, {128, 128, 128, 2, 0.0, 0.594, 0.530, 4.42},
+    {128, 128, 128, 1, 0.0, 0.423, 0.0, 4.66}, {128, 256, 128, 1, 0.0, 0.770, 0.0, 7.76}, {192, 256, 128, 1, 0.0, 1.065, 0.0, 9.88},
 };
 
 static int i8_shape(const I8Args& p) {
@@ -555,10 +586,11 @@ static int i8_shape(const I8Args& p) {
     for (int i = 0; i < (int)(sizeof(kI8Shapes) / sizeof(kI8Shapes[0])); ++i) {
         const I8Shape& f = kI8Shapes[i];
         const int64_t slabs = (p.M + f.bm - 1) / f.bm, wgs = slabs * ((p.N + f.bn - 1) / f.bn);
-        if (f.step == 1024 && slabs > 65535) continue;   // the grid's second dimension
+        if ((f.step == 1024 && slabs > 65535) || (wgs >= 1 << 21 && f.bm < 128)) continue;   // a grid's second dimension; its threads
         const int64_t n = (wgs + 255) / 256, steps = (p.K + f.step - 1) / f.step;
         auto round = [&](int64_t k) { return k ? f.each + (double)steps * std::max(f.alone, f.shared * (double)k) : 0.; };
-        const double us = f.start + (double)(n / f.resident) * round(f.resident) + round(n % f.resident);
+        double us = f.start + (double)(n / f.resident) * round(f.resident) + round(n % f.resident);
+        if (f.bm == 32 && slabs == 1) us *= 1.3;
         if (best < 0 || us < least) least = us, best = i;
     }
     return best;
@@ -582,12 +614,15 @@ static void launch_gemm_i8(const I8Args& p, hipStream_t s) {
     switch (i8_shape(p)) {
     case 0: return launch_i8_rows<1, 1, 4>(p, s);
     case 1: return launch_i8_rows<1, 2, 3>(p, s);
-    case 2: return launch_i8_rows<2, 2, 3>(p, s);
-    case 3: return launch_i8<1, 1, 2, 2, 4>(p, s);
-    case 4: return launch_i8<1, 1, 2, 4, 4>(p, s);
-    case 5: return launch_i8<2, 1, 2, 4, 2>(p, s);
-    case 6: return launch_i8<1, 1, 4, 4, 4>(p, s);
-    case 7: return launch_i8<2, 2, 2, 4, 3>(p, s);
+    case 2: return launch_i8<1, 1, 1, 1, 4, 4>(p, s);
+    case 3: return launch_i8<1, 1, 1, 1, 2, 4>(p, s);
+    case 4: return launch_i8<1, 1, 1, 2, 3, 4>(p, s);
+    case 5: return launch_i8<1, 1, 2, 2, 4, 2>(p, s);
+    case 6: return launch_i8<1, 1, 2, 4, 3, 2>(p, s);
+    case 7: return launch_i8<1, 1, 2, 4, 4>(p, s);
+    case 8: return launch_i8<2, 1, 2, 4, 2>(p, s);
+    case 9: return launch_i8<1, 1, 4, 4, 4>(p, s);
+    case 10: return launch_i8<2, 2, 2, 4, 3>(p, s);
     default: return launch_i8<3, 2, 2, 4, 2>(p, s);
     }
 }

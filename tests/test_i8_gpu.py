@@ -115,6 +115,19 @@ def test_rows(M, N, K):
     _check(out, a, s, w, t, bias, what=f"M {M}")
 
 
+@pytest.mark.parametrize("M,N,K", [(20, 300, 528), (20, 2050, 528), (67, 1000, 1040), (134, 1000, 528), (33, 4100, 1040),
+                                   (20, 4100, 1040), (67, 8193, 2064), (67, 8193, 528), (400, 8193, 528), (200, 8193, 528),
+                                   (4374, 1000, 2064), (1072, 8193, 528), (33, 70, 8208), (67, 2050, 8208), (134, 2050, 8176),
+                                   (268, 1000, 4112), (268, 2050, 8208), (536, 1000, 2064), (67, 1000, 65536)])
+def test_tile_shapes(M, N, K):
+    """Of each shape of tile one product at least, ragged in rows, columns and inputs; sums equal those of whole numbers."""
+    a, w = _codes(M, M, K), _codes(N, N, K)
+    one = torch.ones(max(M, N), device=DEV)
+    out = kernels.gemm_i8(a.to(DEV), w.to(DEV), one[:N], one[:M], out_dtype=F32)
+    whole = torch.matmul(a.to(DEV).double(), w.to(DEV).double().t())   # exact: below 2^53
+    assert torch.equal(out, whole.float())
+
+
 @pytest.mark.parametrize("N", [1, 3, 15, 16, 17, 31, 33, 127, 128, 129, 257, 1031])
 @pytest.mark.parametrize("K", [16, 64, 112, 128, 144, 256, 1152, 2064])
 def test_columns_and_inputs(N, K):
