@@ -6,7 +6,8 @@
 // 2^63 for up to 2^20 tokens: their order does not matter, so a row's token depends
 // on the row alone, and neighbours in the running sum differ by far more than it is
 // off -- a vocabulary of 131072 in 32 bits would draw another token than 64 bits do
-// once in some ten rows.  What is below 2^-44 of the largest counts as nothing.
+// once in some ten rows.  What is below 2^-44 of the largest counts as nothing (but in
+// a logprob near 0, which is nothing but what the others weigh: fine_tail).
 //
 // Every filter keeps a prefix of the tokens in falling order, so all that is ever
 // asked of that order is the first position whose running count or running weight
@@ -51,6 +52,8 @@ constexpr uint32_t kListFromTop = 512;              // so many at most of all bu
 constexpr int kExpBits = 7;
 constexpr float kOctaves = 46.f;                    // 2^-46 and below: no weight
 constexpr double kUnit = 8796093022208.;            // 2^43
+constexpr double kFaint = -128. * 80.;              // exponents of what is nothing in any sum
+constexpr double kFineAll = 0x1p70;                 // units of what all others of a row weigh
 
 struct SampleArgs {
     const void* logits;
@@ -70,7 +73,7 @@ constexpr int kMaxParts = 64;
 struct SampleParts {
     uint64_t mass[kBuckets];
     uint32_t count[kBuckets];
-    uint64_t above;
+    uint64_t above, others;   // as sample_fill's
     float largest[kMaxParts];   // a NaN where there is one
 };
 
@@ -202,14 +205,21 @@ struct SampleScale {
         return weight_in_play(fmax(y, -128. * (kOctaves + 1.)), table);
     }
     // y not below -128 (kOctaves + 1): a bucket's.
-    __device__ __forceinline__ uint64_t weight_in_play(double y, const double* table) const {
+    __device__ __forceinline__ uint64_t weight_in_play(double y, const double* table) const { return rounded(power(y, table)); }
+    static __device__ __forceinline__ uint64_t rounded(double w) {
+        return (uint64_t)__double_as_longlong(w + 4503599627370496.) & 0xfffffffffffffull;   // + 2^52
+    }
+    // A weight of a tail, in units of 1 / fine.
+    __device__ __forceinline__ uint64_t fine_weight(double y, const double* table, double fine) const {
+        return y >= kFaint ? (uint64_t)(power(y, table) * (fine * (1. / kUnit))) : 0ull;
+    }
+    static __device__ __forceinline__ double power(double y, const double* table) {   // 2^43 2^(y / 128)
         constexpr double c = M_LN2 / 128., magic = 6755399441055744.;   // 1.5 2^52: the nearest whole number in the low bits
         const double z = y + magic, r = y - (z - magic);
         const uint32_t n = (uint32_t)__double_as_longlong(z);
         const double e = 1. + r * (c + r * (c * c / 2. + r * (c * c * c / 6. + r * (c * c * c * c / 24.))));
         const uint64_t w = (uint64_t)__double_as_longlong(e * table[n & 127u]);   // to be times 2^(n / 128), rounded down
-        const double scaled = __longlong_as_double((long long)((uint64_t)((uint32_t)(w >> 32) + ((n & ~127u) << 13)) << 32 | (uint32_t)w));
-        return (uint64_t)__double_as_longlong(scaled + 4503599627370496.) & 0xfffffffffffffull;   // + 2^52: rounded
+        return __longlong_as_double((long long)((uint64_t)((uint32_t)(w >> 32) + ((n & ~127u) << 13)) << 32 | (uint32_t)w));
     }
 };
 
@@ -307,7 +317,7 @@ __device__ __forceinline__ void sample_find(SampleShared& s, const uint32_t* cou
 struct SampleHit {
     uint64_t mass;
     uint32_t key, rank;
-    int index;   // -1: not known, by rank
+    int index;   // -1: not known, by rank (else the rank says nothing)
 };
 
 // The first of n equal tokens of weight w, behind (c0, m0), that answers q; the last one does.
@@ -340,11 +350,13 @@ struct SampleRule {
     // The three questions that a row's token takes: what top-k keeps, what top-p keeps of that, and where u falls.  What
     // min-p leaves is a beginning of the order too: `above`, its weight.  ask(query, last) answers.
     template <class Ask>
-    __device__ __forceinline__ SampleHit token(uint32_t all, uint64_t all_mass, uint64_t above, float u, uint64_t& kept, Ask ask) const {
+    __device__ __forceinline__ SampleHit token(uint32_t all, uint64_t all_mass, uint64_t above, float u, uint64_t& kept, SampleHit& end,
+                                               Ask ask) const {
         const uint32_t first_k = k <= 0 ? all : min((uint32_t)k, all);
         const bool with_p = top_p < 1.f;
         SampleHit hit = {};
         kept = all_mass;
+        end.rank = 0;
 #pragma unroll 1
         for (int step = 0; step < 3; ++step) {
             SampleQuery q = {0xffffffffu, INFINITY, false};
@@ -362,10 +374,20 @@ struct SampleRule {
                 q.strict = true;
             }
             hit = ask(q, step == 2);
-            if (step < 2) kept = hit.mass;
+            if (step < 2) kept = hit.mass, end = hit;
         }
         return hit;
     }
+    // A largest token's share of nearly all needs what the others weigh to more digits than the questions do: V weights held
+    // to 2^-44 are off by up to V 2^-44 in all, and a logprob of -1e-6 is to be as exact as others.  So where V others at most
+    // weigh less than V 2^-24 they are summed once more, in units of 2^-75, or 2^-67 from 2^-12 on.  `end` is the last token that
+    // top-k and top-p keep (rank 0: all are kept), `top` the largest.  0: the logprob of `kept` will do.
+    __device__ __forceinline__ double fine_tail(const SampleHit& hit, const SampleHit& end, uint32_t top, uint64_t kept, int V) const {
+        const uint64_t others = kept - (uint64_t)kUnit;
+        if (hit.key != top || (end.rank && end.key == top) || others >= (uint64_t)V << 19) return 0.;
+        return others < 1ull << 31 ? 0x1p75 : 0x1p67;
+    }
+    static __device__ __forceinline__ float tail_logprob(uint64_t tail, double fine) { return (float)-log1p((double)tail / fine); }
     __device__ __forceinline__ float logprob(float l, uint64_t kept) const {
         return (float)((l == sc.m ? 0. : ((double)l - (double)sc.m) / (double)temperature) - log((double)kept * (1. / kUnit)));
     }
@@ -419,20 +441,26 @@ __device__ __forceinline__ float sample_largest(SampleSums& s, const SampleRow<K
 }
 
 // Adds a workgroup's logits to the buckets; the weight that min-p leaves of them.  Counts are for top-k alone, and for
-// lists of few tokens; without them a bucket's weight tells how many it holds at most.
+// lists of few tokens; without them a bucket's weight tells how many it holds at most.  others: what all but the largest
+// weigh, of those that min-p leaves, in units of 1 / kFineAll.
 template <int KIND>
-__device__ __forceinline__ uint64_t sample_fill(SampleSums& s, const double* table, const SampleRow<KIND>& x, const SampleRule& rule) {
+__device__ __forceinline__ uint64_t sample_fill(SampleSums& s, const double* table, const SampleRow<KIND>& x, const SampleRule& rule,
+                                                uint64_t& others) {
     const SampleScale& sc = rule.sc;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const bool counted = rule.k > 0, with_min_p = rule.y_min > -INFINITY;
     uint64_t above = 0;
+    double rest = 0.;
     for (int i = t; i < kBuckets; i += kSampleThreads) s.mass[i] = 0, s.count[i] = 0;
     __syncthreads();
     x.template each<2>([&](float l, int) {
         const int b = sc.bucket(l);
-        if (b >= kBuckets) return;
         const double y = sc.exponent(l);
-        const uint64_t w = sc.weight_in_play(y, table);
+        if (!(y >= kFaint)) return;
+        const double exact = sc.power(y, table);
+        if (y >= rule.y_min && l != sc.m) rest += exact;
+        if (b >= kBuckets) return;
+        const uint64_t w = sc.rounded(exact);
         atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), (unsigned long long)w);
         if (counted) atomicAdd(&s.count[b], 1u);
         if (with_min_p) above += y >= rule.y_min ? w : 0ull;
@@ -444,13 +472,18 @@ __device__ __forceinline__ uint64_t sample_fill(SampleSums& s, const double* tab
         before_wave(s.wave64, wave, above);
     }
     __syncthreads();
+    others = running64((uint64_t)fmin(rest * (kFineAll / kUnit), 0x1p63));   // (too many only where it is not used)
+    if (lane == 63) s.wave64[wave] = others;
+    __syncthreads();
+    before_wave(s.wave64, wave, others);
+    __syncthreads();
     return above;
 }
 
 // A row's token from its buckets (rule.sc.m set; above: as sample_fill's).
 template <int KIND>
 __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleShared& s, const double* table, const SampleRow<KIND>& x,
-                                                  const SampleRule& rule, uint64_t above, int64_t row) {
+                                                  const SampleRule& rule, uint64_t above, uint64_t others, int64_t row) {
     const int t = threadIdx.x;
     const SampleScale& sc = rule.sc;
     const bool counted = rule.k > 0;
@@ -535,7 +568,7 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
                 }
             }
             __syncthreads();
-            const SampleHit hit = {s.found_mass, ~(uint32_t)(s.found_entry >> 32), 0, (int)(uint32_t)s.found_entry};
+            const SampleHit hit = {s.found_mass, ~(uint32_t)(s.found_entry >> 32), 1, (int)(uint32_t)s.found_entry};
             __syncthreads();
             return hit;
         }
@@ -581,13 +614,37 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
     };
 
     uint64_t kept;
+    SampleHit end;
     const uint32_t all = counted ? s.count[kBuckets - 1] : 0xffffffffu;
-    const SampleHit hit = rule.token(all, s.mass[kBuckets - 1], above, p.u[row], kept, ask);
+    const SampleHit hit = rule.token(all, s.mass[kBuckets - 1], above, p.u[row], kept, end, ask);
     const int index = hit.index >= 0 ? hit.index : sample_nth(s, x, hit.key, hit.rank);
-    if (t == 0) {
-        p.token[row] = index;
-        if (p.logprob) p.logprob[row] = rule.logprob(sample_value(hit.key), kept);
+    if (t == 0) p.token[row] = index;
+    if (!p.logprob) return;
+    // All others were summed with the buckets; those that top-k or top-p keep take one more pass, which is rare (37 rows of
+    // 50001 with temperature alone take 2 us more for the sums, and took 15 more for such a pass).
+    const double fine = rule.fine_tail(hit, end, sample_key(sc.m), kept, end.rank && counted ? min(rule.k, x.V) : x.V);
+    if (fine == 0. || end.rank == 0) {
+        const float y = fine == 0. || end.rank ? rule.logprob(sample_value(hit.key), kept) : rule.tail_logprob(others, kFineAll);
+        if (t == 0) p.logprob[row] = y;
+        return;
     }
+    uint64_t tail = 0;
+    x.template each<2>([&](float l, int i) {
+        const uint32_t key = sample_key(l);
+        if (l == sc.m || (end.rank && (key < end.key || (key == end.key && i > end.index)))) return;   // (index -1: below)
+        const double y = sc.exponent(l);
+        if (y >= rule.y_min) tail += sc.fine_weight(y, table, fine);
+    });
+    if (t == 0 && end.rank && end.index < 0) {
+        const double y = sc.exponent(sample_value(end.key));
+        if (y >= rule.y_min) tail += end.rank * sc.fine_weight(y, table, fine);
+    }
+    tail = running64(tail);
+    __syncthreads();
+    if ((t & 63) == 63) s.wave64[t >> 6] = tail;
+    __syncthreads();
+    before_wave(s.wave64, __builtin_amdgcn_readfirstlane(t >> 6), tail);
+    if (t == 0) p.logprob[row] = rule.tail_logprob(tail, fine);
 }
 
 // A row that has no token: a NaN, or nothing to take.
@@ -608,8 +665,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& p, SampleShared& s,
     sample_table(table);
     rule.sc.m = sample_largest(s, x);
     if (sample_none(p, rule.sc.m, row)) return;
-    const uint64_t above = sample_fill(s, table, x, rule);
-    sample_by_buckets(p, s, table, x, rule, above, row);
+    uint64_t others;
+    const uint64_t above = sample_fill(s, table, x, rule, others);
+    sample_by_buckets(p, s, table, x, rule, above, others, row);
 }
 
 __global__ __launch_bounds__(kSampleThreads) void sample_f32_kernel(const SampleArgs p) {
@@ -633,7 +691,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_largest_kernel(co
     const int part = blockIdx.x % p.n_parts;
     SampleParts* sums = reinterpret_cast<SampleParts*>(p.parts) + row;
     for (int i = part * kSampleThreads + threadIdx.x; i < kBuckets; i += p.n_parts * kSampleThreads) sums->mass[i] = 0, sums->count[i] = 0;
-    if (part == 0 && threadIdx.x == 0) sums->above = 0;
+    if (part == 0 && threadIdx.x == 0) sums->above = sums->others = 0;
     const float m = sample_largest(s, sample_part(p, row, part));
     if (threadIdx.x == 0) sums->largest[part] = m;
 }
@@ -658,12 +716,16 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_fill_kernel(const
     rule.sc.m = sample_parts_largest(p, sums);
     if (!(rule.sc.m > -INFINITY)) return;
     sample_table(table);
-    const uint64_t above = sample_fill(s, table, sample_part(p, row, blockIdx.x % p.n_parts), rule);
+    uint64_t others;
+    const uint64_t above = sample_fill(s, table, sample_part(p, row, blockIdx.x % p.n_parts), rule, others);
     for (int i = threadIdx.x; i < kBuckets; i += kSampleThreads) {
         if (s.mass[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&sums->mass[i]), (unsigned long long)s.mass[i]);
         if (s.count[i]) atomicAdd(&sums->count[i], s.count[i]);
     }
-    if (threadIdx.x == 0 && above) atomicAdd(reinterpret_cast<unsigned long long*>(&sums->above), (unsigned long long)above);
+    if (threadIdx.x == 0) {
+        if (above) atomicAdd(reinterpret_cast<unsigned long long*>(&sums->above), (unsigned long long)above);
+        if (others) atomicAdd(reinterpret_cast<unsigned long long*>(&sums->others), (unsigned long long)others);
+    }
 }
 
 __global__ __launch_bounds__(kSampleThreads) void sample_parts_choose_kernel(const SampleArgs p) {
@@ -678,7 +740,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_choose_kernel(con
     sample_table(table);
     for (int i = threadIdx.x; i < kBuckets; i += kSampleThreads) s.mass[i] = sums->mass[i], s.count[i] = sums->count[i];
     __syncthreads();
-    sample_by_buckets(p, s, table, SampleRow<0>{static_cast<const char*>(p.logits) + row * p.ld * 4, p.V}, rule, sums->above, row);
+    sample_by_buckets(p, s, table, SampleRow<0>{static_cast<const char*>(p.logits) + row * p.ld * 4, p.V}, rule, sums->above, sums->others, row);
 }
 
 // In how many parts.  Two more launches have to pay for themselves, the sooner the fewer rows share the card; a part
@@ -1001,9 +1063,22 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         equals = found.equals;
         return SampleHit{found.mass, found.key, found.rank, -1};
     };
-    uint64_t kept;
-    const SampleHit hit = rule.token(all, all_mass, above, p.u[row], kept, ask);
+    uint64_t kept, others = 0;
+    SampleHit end;
+    const SampleHit hit = rule.token(all, all_mass, above, p.u[row], kept, end, ask);
+    const double fine = p.logprob ? rule.fine_tail(hit, end, top, kept, p.V) : 0.;
+    if (fine != 0.) {
+        for (uint32_t i = t * each; i < min(values, (t + 1) * each); ++i) {
+            const uint32_t e = entry(i), key = e >> 16;
+            if (!(e & 0xffffu) || key == top || (end.rank && key > end.key)) continue;
+            const double y = sc.exponent(value(key));
+            if (y >= rule.y_min) others += (end.rank && key == end.key ? end.rank : tokens_of(e)) * sc.fine_weight(y, table, fine);
+        }
+        others = running64(others);
+        if (lane == 63) s.wave64[wave] = others;
+    }
     __syncthreads();   // the list of values is spent
+    if (fine != 0.) before_wave(s.wave64, wave, others);
     int index;
     if (equals <= kMaxTies) {
         const uint32_t bits = hit.key & 0x8000u ? hit.key : hit.key ^ 0x7fffu;
@@ -1049,7 +1124,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     }
     if (t == 0) {
         p.token[row] = index;
-        if (p.logprob) p.logprob[row] = rule.logprob(value(hit.key), kept);
+        if (p.logprob) p.logprob[row] = fine != 0. ? rule.tail_logprob(others, fine) : rule.logprob(value(hit.key), kept);
     }
 }
 

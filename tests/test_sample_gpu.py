@@ -146,6 +146,54 @@ def test_nan_of_either_sign(dtype, V):
     assert (tok[:5] == -1).all() and tok[5] >= 0
 
 
+@pytest.mark.parametrize("V", [40, 3000, 50001, 131072])   # of fp32: by one workgroup, in parts
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_logprob_of_a_token_that_has_nearly_all(dtype, V):
+    """-log(1 + what the others weigh), to 1e-6 of itself down to V 2^-75: for one token far above a bulk, for two, with each
+    rule.  The sums of the others are in 64 bits apart from the largest here."""
+    B = 7
+    base = torch.randn(B, V, generator=torch.Generator().manual_seed(V)) * 2
+    u = torch.full((B,), 0.5)
+    for gap in (8.0, 14.0, 20.0, 27.0, 33.0, 40.0):
+        x = base.clone()
+        at = torch.arange(B) * 5 % V
+        x[torch.arange(B), at] = base.max() + gap
+        x[:3, V - 1] = base.max() + gap / 2
+        x = x.to(dtype)
+        for r in ({}, {"t": 0.5}, {"t": 1.5}, {"k": 2}, {"k": 39}, {"mp": 1e-12}, {"k": 30, "mp": 1e-9}, {"p": 1 - 2.0 ** -24},
+                  {"t": 2.0, "k": 1000, "p": 1 - 2.0 ** -23}, {"k": 1}):
+            tok, lp = kernels.sample(x.to(DEV), u.to(DEV), r.get("t", 1.0), r.get("k", 0), r.get("p", 1.0), r.get("mp", 0.0))
+            for b in range(B):
+                order = torch.argsort(-x[b].double(), stable=True)
+                y = (x[b].double()[order] - x[b].double().max()) / r.get("t", 1.0)
+                w = torch.exp(y)
+                n = min(r.get("k", 0) or V, V)
+                if "p" in r:
+                    p = float(torch.tensor(r["p"], dtype=F32))
+                    # reaches p of all: what is left behind is (1 - p) of it at most, summed from the smallest on; V weights
+                    # held to 2^-44 leave the border undecided by V 2^-44
+                    left = torch.flip(torch.cumsum(torch.flip(w[:n], [0]), 0), [0])
+                    edge = (left[1:] / left[0] - (1 - p)).abs() < V * 2.0 ** -44
+                    if edge.any():
+                        continue
+                    n = 1 + int((left[1:] / left[0] > 1 - p).sum())
+                if "mp" in r:
+                    n = min(n, int((w >= float(torch.tensor(r["mp"], dtype=F32))).sum()))
+                rest = float(torch.flip(w[1:n], [0]).sum())
+                if rest >= 0.5:
+                    continue
+                want = -math.log1p(rest)
+                assert int(tok[b]) == int(order[0])
+                # 16 bits: each weight is cut off to a multiple of 2^-75, from 2^-12 on of 2^-67.  fp32: V threads' sums
+                # at most are cut off to 2^-70; what top-k leaves out below 2^-46 of the largest may be in; and k kept weights
+                # are taken as held, to 2^-44, where they are k 2^-24 and more.
+                cut = V * 2.0 ** -75
+                if dtype is F32:
+                    k = min(r.get("k", 0), V)
+                    cut = V * 2.0 ** -70 + (V - k if k else 0) * 2.0 ** -46
+                assert abs(float(lp[b]) - want) <= 1e-6 * abs(want) + cut, (gap, r, b, float(lp[b]), want)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_min_p_of_one_keeps_equal_weights(dtype):
     # Logits 1e-20 apart weigh the same in 64 bits (and 2^-44 of the largest, in which they are held, is more); those 1e-3 apart
@@ -193,7 +241,7 @@ def test_workspace():
     """Rows in parts: a workspace given, used twice, too small, and the rows alone."""
     x, u = _logits(3, 100001, 6, F32).to(DEV), _u(3, 6).to(DEV)
     want = kernels.sample(x, u, top_p=0.95)
-    ws = torch.full((3 * (2048 * 12 + 8 + 64 * 4),), 0xff, dtype=torch.uint8, device=DEV)
+    ws = torch.full((3 * (2048 * 12 + 2 * 8 + 64 * 4),), 0xff, dtype=torch.uint8, device=DEV)
     for _ in range(3):
         got = kernels.sample(x, u, top_p=0.95, workspace=ws)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
