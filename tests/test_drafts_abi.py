@@ -101,7 +101,7 @@ def test_sample_refusals():
     assert _sample(rows=0) == abi.SF_OK
     long = {"dtype": abi.SF_F32, "V": 40000, "ld": 40000}
     need = abi.lib().sf_sample_workspace_bytes(ctypes.byref(abi.SampleDesc(rows=2, V=40000, dtype=abi.SF_F32)))
-    assert need == 2 * (2048 * 12 + 8 + 64 * 4)
+    assert need == 2 * (2048 * 12 + 2 * 8 + 64 * 4)
     assert _sample(**long) == abi.SF_EWORKSPACE and _sample(ws=256, n=need - 1, **long) == abi.SF_EWORKSPACE
     assert _sample(ws=260, n=need, **long) == abi.SF_EINVAL
     for kw in ({"rows": 2, "V": 1000, "dtype": abi.SF_F32}, {"rows": 300, "V": 40000, "dtype": abi.SF_F32},
