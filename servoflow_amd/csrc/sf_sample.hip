@@ -622,7 +622,7 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
     if (!p.logprob) return;
     // All others were summed with the buckets; those that top-k or top-p keep take one more pass, which is rare (37 rows of
     // 50001 with temperature alone take 2 us more for the sums, and took 15 more for such a pass).
-    const double fine = rule.fine_tail(hit, end, sample_key(sc.m), kept, end.rank && counted ? min(rule.k, x.V) : x.V);
+    const double fine = rule.fine_tail(hit, end, sample_key(sc.m), kept, end.rank && counted ? (int)min((int64_t)8 * rule.k, (int64_t)x.V) : x.V);
     if (fine == 0. || end.rank == 0) {
         const float y = fine == 0. || end.rank ? rule.logprob(sample_value(hit.key), kept) : rule.tail_logprob(others, kFineAll);
         if (t == 0) p.logprob[row] = y;
