@@ -53,7 +53,12 @@ constexpr int kExpBits = 7;
 constexpr float kOctaves = 46.f;                    // 2^-46 and below: no weight
 constexpr double kUnit = 8796093022208.;            // 2^43
 constexpr double kFaint = -128. * 80.;              // exponents of what is nothing in any sum
-constexpr double kFineAll = 0x1p70;                 // units of what all others of a row weigh
+// Units of what all others of a row weigh.  They are asked for where they are less than V 2^-24 of the largest (fine_tail),
+// within V 2^-44: below 2^64 in units of 2^-70 up to 2^17 tokens, and in units of 2^-67 up to the most there are.
+constexpr int kFineTokens = 1 << 17;
+constexpr double kFineFew = 0x1p70, kFineMany = 0x1p67;
+constexpr double kFineMost = 0x1p-24 + 0x1p-44;   // of each
+static_assert(kFineFew * kFineTokens * kFineMost < 0x1p64 && kFineMany * SF_SAMPLE_MAX_VOCAB * kFineMost < 0x1p64, "64 bits");
 
 struct SampleArgs {
     const void* logits;
@@ -337,6 +342,7 @@ struct SampleRule {
     int k;
     SampleScale sc;
     double y_min;   // min-p: exponents from here on
+    double fine_all;
     __device__ __forceinline__ void read(const SampleArgs& p, int64_t row) {
         temperature = p.temperature ? p.temperature[row] : p.temperature1;
         k = p.top_k ? p.top_k[row] : p.top_k1;
@@ -344,6 +350,7 @@ struct SampleRule {
         const float min_p = p.min_p ? p.min_p[row] : p.min_p1;
         if (!(temperature > 0.f)) temperature = 1.f, k = 1;   // the first in order
         y_min = min_p > 0.f ? 128. * (log2((double)min_p) - M_LOG2E * 0x1p-54) : -INFINITY;   // what 64 bits round to min_p reaches it
+        fine_all = p.V <= kFineTokens ? kFineFew : kFineMany;
         sc.octaves = 128. * M_LOG2E / (double)temperature;
         sc.per_bucket = fminf((float)(sc.octaves * (kBuckets / (128. * kOctaves))), 3e38f);
     }
@@ -442,7 +449,8 @@ __device__ __forceinline__ float sample_largest(SampleSums& s, const SampleRow<K
 
 // Adds a workgroup's logits to the buckets; the weight that min-p leaves of them.  Counts are for top-k alone, and for
 // lists of few tokens; without them a bucket's weight tells how many it holds at most.  others: what all but the largest
-// weigh, of those that min-p leaves, in units of 1 / kFineAll.
+// weigh, of those that min-p leaves, in units of 1 / rule.fine_all, each thread's to the nearest (of a row in parts V / 4 threads at
+// most: V 2^-70); more than 64 bits hold where it is not used.
 template <int KIND>
 __device__ __forceinline__ uint64_t sample_fill(SampleSums& s, const double* table, const SampleRow<KIND>& x, const SampleRule& rule,
                                                 uint64_t& others) {
@@ -472,7 +480,7 @@ __device__ __forceinline__ uint64_t sample_fill(SampleSums& s, const double* tab
         before_wave(s.wave64, wave, above);
     }
     __syncthreads();
-    others = running64((uint64_t)fmin(rest * (kFineAll / kUnit), 0x1p63));   // (too many only where it is not used)
+    others = running64((uint64_t)(fmin(rest * (rule.fine_all / kUnit), 0x1p63) + 0.5));
     if (lane == 63) s.wave64[wave] = others;
     __syncthreads();
     before_wave(s.wave64, wave, others);
@@ -624,7 +632,7 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
     // 50001 with temperature alone take 2 us more for the sums, and took 15 more for such a pass).
     const double fine = rule.fine_tail(hit, end, sample_key(sc.m), kept, end.rank && counted ? (int)min((int64_t)8 * rule.k, (int64_t)x.V) : x.V);
     if (fine == 0. || end.rank == 0) {
-        const float y = fine == 0. || end.rank ? rule.logprob(sample_value(hit.key), kept) : rule.tail_logprob(others, kFineAll);
+        const float y = fine == 0. || end.rank ? rule.logprob(sample_value(hit.key), kept) : rule.tail_logprob(others, rule.fine_all);
         if (t == 0) p.logprob[row] = y;
         return;
     }

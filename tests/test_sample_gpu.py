@@ -318,3 +318,55 @@ def test_only_lowest_numbers_are_left():
         x[2, 17] = low / 2
         for r in ({}, {"p": 0.5}, {"k": 7}, {"mp": 0.5}, {"t": math.inf}):
             _check(x, torch.tensor([0.77, 0.5, 0.3]), what=str(r), **r)
+
+
+@pytest.mark.parametrize("V", [131072, 131073, 1 << 18, 300001, 1 << 20])
+@pytest.mark.parametrize("rows", [2, 300])   # fp32: in parts, by one workgroup each
+def test_logprob_beside_the_others_of_a_large_vocabulary(V, rows):
+    """One token far above others that weigh up to more than V 2^-24 of it in all, where their sum is not taken any more: flat
+    bulks and broad ones, with temperature alone, min-p that keeps all or some, and rules that keep all."""
+    g = torch.Generator().manual_seed(V)
+    shares = [2.0 ** -9, 2.0 ** -7, 1.02 * 2.0 ** -6, 0.03, 0.99 * V * 2.0 ** -24, 0.999 * V * 2.0 ** -24, 1.05 * V * 2.0 ** -24, 0.1]
+    base = torch.empty(2 * len(shares), V)
+    for i, share in enumerate(shares):
+        base[2 * i] = math.log(share / (V - 1))
+        base[2 * i + 1] = math.log(share / (V - 1)) - 0.125 + 0.5 * torch.randn(V, generator=g)   # exp(randn / 2) is 1.133 in the mean
+    top = torch.randint(0, V, (len(base),), generator=g)
+    base[torch.arange(len(base)), top] = 0.0
+    base = base.to(DEV)
+    w = torch.exp(base.double())
+    w[torch.arange(len(base)), top] = 0.0
+    cut = float(torch.tensor(0.03 / V, dtype=F32))
+    for r, keep in (({}, w), ({"temperature": 0.5}, w), ({"min_p": 1e-12}, w), ({"min_p": cut}, torch.where(w >= cut, w, 0.0)),
+                    ({"top_k": V, "top_p": 1.0}, w)):
+        x = base * r.get("temperature", 1.0)   # (a half: exact)
+        want = torch.log1p(keep.sum(1)).neg().cpu()
+        for at in range(0, len(base), rows):
+            pick = torch.arange(at, at + rows) % len(base)
+            tok, lp = kernels.sample(x[pick.to(DEV)], torch.full((rows,), 0.5, device=DEV), **r)
+            assert torch.equal(tok.cpu().long(), top[pick])
+            # Rounded to fp32 once; the others' sum is cut off by V 2^-70 in all, or each of them is held to 2^-44 where they weigh
+            # V 2^-24 and more (a few that weigh hardly less may be taken so).
+            held = torch.where(torch.expm1(want[pick].neg()) >= 0.9999 * V * 2.0 ** -24, V * 2.0 ** -44, V * 2.0 ** -70)
+            err = (lp.cpu().double() - want[pick]).abs()
+            assert (err <= (2.0 ** -24 + 2.0 ** -40) * want[pick].abs() + held).all(), (r, at, float((err / want[pick].abs()).max()))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("V", [300001, 1 << 20])
+def test_logprob_beside_two_values_that_most_tokens_share(dtype, V):
+    """Each of them more often than 16 bits count: 16-bit rows that go through the buckets."""
+    shares = [2.0 ** -8, 1.02 * 2.0 ** -6, 0.9 * V * 2.0 ** -24]
+    x = torch.empty(len(shares), V, dtype=dtype)
+    for i, share in enumerate(shares):
+        x[i] = math.log(share / V) - 0.2
+        x[i, 1::2] -= 0.125   # a step of both types, or several
+        x[i, 7 * i + 5] = 0.0
+    w = torch.exp(x.double())
+    w[torch.arange(len(shares)), 7 * torch.arange(len(shares)) + 5] = 0.0
+    want = torch.log1p(w.sum(1)).neg()
+    assert (torch.expm1(-want) < 0.999 * V * 2.0 ** -24).all()
+    for r in ({}, {"min_p": 1e-12}):
+        tok, lp = kernels.sample(x.to(DEV), torch.full((len(shares),), 0.5, device=DEV), **r)
+        assert tok.tolist() == [5, 12, 19]
+        assert ((lp.cpu().double() - want).abs() <= (2.0 ** -24 + 2.0 ** -40) * want.abs() + V * 2.0 ** -70).all(), (lp, want)
