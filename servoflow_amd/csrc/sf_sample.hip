@@ -206,11 +206,12 @@ struct SampleScale {
     __device__ __forceinline__ double exponent(float l) const {   // of two, times 128
         return l == m ? 0. : ((double)l - (double)m) * octaves;
     }
-    __device__ __forceinline__ uint64_t weight(double y, const double* table) const {
-        return weight_in_play(fmax(y, -128. * (kOctaves + 1.)), table);
+    static __device__ __forceinline__ bool in_play(double y) { return y >= -128. * kOctaves; }
+    // 0 below the buckets' range.  (A bucket may hold such logits: per_bucket ends at 3e38, so those closer than 7e-36 to the
+    // largest are in one however small the temperature, and `power` has no value for their exponents.)
+    static __device__ __forceinline__ uint64_t weight(double y, const double* table) {
+        return rounded(power(fmax(y, -128. * (kOctaves + 1.)), table));
     }
-    // y not below -128 (kOctaves + 1): a bucket's.
-    __device__ __forceinline__ uint64_t weight_in_play(double y, const double* table) const { return rounded(power(y, table)); }
     static __device__ __forceinline__ uint64_t rounded(double w) {
         return (uint64_t)__double_as_longlong(w + 4503599627370496.) & 0xfffffffffffffull;   // + 2^52
     }
@@ -218,7 +219,7 @@ struct SampleScale {
     __device__ __forceinline__ uint64_t fine_weight(double y, const double* table, double fine) const {
         return y >= kFaint ? (uint64_t)(power(y, table) * (fine * (1. / kUnit))) : 0ull;
     }
-    static __device__ __forceinline__ double power(double y, const double* table) {   // 2^43 2^(y / 128)
+    static __device__ __forceinline__ double power(double y, const double* table) {   // 2^43 2^(y / 128), y from kFaint on
         constexpr double c = M_LN2 / 128., magic = 6755399441055744.;   // 1.5 2^52: the nearest whole number in the low bits
         const double z = y + magic, r = y - (z - magic);
         const uint32_t n = (uint32_t)__double_as_longlong(z);
@@ -522,7 +523,7 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
         for (uint32_t i = t; i < n; i += kSampleThreads) {
             const float l = sample_value(~(uint32_t)(s.list.token[i] >> 32));
             const int b = sc.bucket(l);
-            const uint64_t w = b >= lo && b <= hi ? sc.weight_in_play(sc.exponent(l), table) : 0ull;
+            const uint64_t w = b >= lo && b <= hi ? sc.weight(sc.exponent(l), table) : 0ull;
             const uint32_t part = b >= lo && b <= hi ? min((int)((-sc.below(l) * sc.per_bucket - (float)lo) * finer), kBuckets - 1) : kBuckets;
             s.list.weight[i] = w;
             s.list.part[i] = part;
@@ -543,8 +544,8 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
         const int b = (int)s.found;
         uint32_t c0 = s.found_before, n = 0;
         uint64_t m0 = s.found_mass_before;
-        if (!counted) {   // at most
-            const double least = (double)sc.weight_in_play(-128. * (double)(b + 1) * (kOctaves / kBuckets), table) * (1. - 0x1p-14) - 1.;
+        if (!counted) {   // at most (`collect` counts them where buckets are wider than `least` takes them for, as `weight` says)
+            const double least = (double)sc.weight(-128. * (double)(b + 1) * (kOctaves / kBuckets), table) * (1. - 0x1p-14) - 1.;
             const double most = least > 0. ? (double)(s.mass[b] - m0) / least : 1e9;
             n = most < 1e9 ? (uint32_t)most : 1000000000u;
         } else {
@@ -582,6 +583,7 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
         }
         // More tokens than the list takes: parts of the bucket's keys, from the largest down.
         uint32_t lo = 0, hi = 0xffffffffu;
+        if (!counted) n = (uint32_t)x.V;   // of a bucket of one value: the weight asked for tells which
         while (true) {
             if (t == 0) s.lo = 0xffffffffu, s.hi = 0;
             __syncthreads();
@@ -593,7 +595,7 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
             if (lo1 <= hi1) atomicMin(&s.lo, lo1), atomicMax(&s.hi, hi1);
             __syncthreads();
             lo = s.lo, hi = s.hi;
-            if (lo >= hi) break;   // (of a bucket of one value and no counts the most it can hold is what it holds)
+            if (lo >= hi) break;
             int shift = 0;
             while ((hi - lo) >> shift >= (uint32_t)kBuckets) ++shift;
             for (int i = t; i < kBuckets; i += kSampleThreads) s.part.mass[i] = 0, s.part.count[i] = 0;
@@ -1022,11 +1024,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
     for (uint32_t i = t * each; i < min(values, (t + 1) * each); ++i) {
         const uint32_t e = entry(i);
         if (!(e & 0xffffu)) continue;
-        const float l = value(e >> 16);
-        const double y = sc.exponent(l);
+        const double y = sc.exponent(value(e >> 16));
         c += tokens_of(e);
-        if (sc.bucket(l) < kBuckets) {
-            const uint64_t one = tokens_of(e) * sc.weight_in_play(y, table);
+        if (sc.in_play(y)) {
+            const uint64_t one = tokens_of(e) * sc.rounded(sc.power(y, table));
             w += one;
             above += y >= rule.y_min ? one : 0ull;
         }
@@ -1055,8 +1056,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
             const uint32_t i = (64 * wave + who) * each + lane;
             const bool in = (uint32_t)lane < each && i < values;
             const uint32_t e = in ? entry(i) : 0u, mult = in ? tokens_of(e) : 0u;
-            const float l = value(e >> 16);
-            const uint64_t one = in && sc.bucket(l) < kBuckets ? sc.weight_in_play(sc.exponent(l), table) : 0ull;
+            const double y = sc.exponent(value(e >> 16));
+            const uint64_t one = in && sc.in_play(y) ? sc.rounded(sc.power(y, table)) : 0ull;
             const uint32_t cs = running64(mult) + lane_of(c0, who), cb = cs - mult;
             const uint64_t ws = running64(mult * one) + lane_of(w0, who), wb = ws - mult * one;
             if (mult && q.at(cs, ws) && (cb == 0 || !q.at(cb, wb))) {

@@ -370,3 +370,23 @@ def test_logprob_beside_two_values_that_most_tokens_share(dtype, V):
         tok, lp = kernels.sample(x.to(DEV), torch.full((len(shares),), 0.5, device=DEV), **r)
         assert tok.tolist() == [5, 12, 19]
         assert ((lp.cpu().double() - want).abs() <= (2.0 ** -24 + 2.0 ** -40) * want.abs() + V * 2.0 ** -70).all(), (lp, want)
+
+
+@pytest.mark.parametrize("V", [5, 500, 6000, 60000])   # of fp32: by one workgroup, in parts
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_smallest_logits_and_temperatures(dtype, V):
+    """Logits of the smallest numbers there are: how far below the largest they weigh nothing is then less than a bucket of theirs
+    takes apart."""
+    unit = 2.0 ** -133 if dtype is BF else 2.0 ** -149
+    x = torch.randint(-4, 5, (6, V), generator=torch.Generator().manual_seed(V)).double() * unit
+    x[1] *= 2.0 ** 11
+    x[2] = torch.where(torch.arange(V) % 3 == 0, 0.0, -unit)
+    x[3, ::2] = -math.inf
+    x[4] = torch.rand(V, generator=torch.Generator().manual_seed(V)).double() * 1e-36
+    x[5] = torch.where(torch.arange(V) % 3 == 0, 0.0, -4e-39)   # the second bucket, of one value
+    y = x.to(dtype)
+    if dtype is BF:
+        assert torch.equal(y[:4].double(), x[:4])
+    u = torch.tensor([0.95, 0.5, 0.999, 0.3, 0.97, 0.999])
+    for r in ({"t": 7e-40}, {"t": 2.0 ** -149}, {"t": 1e-44, "k": 3}, {"t": 1e-40}, {"t": 2e-41, "p": 0.9}, {"t": 1e-38, "mp": 0.5}, {"t": 5e-37, "k": V}):
+        _check(y, u, what=str(r), **r)
