@@ -189,16 +189,17 @@ private:
 
 // What a logit counts for.
 struct SampleScale {
-    float m, per_bucket;
+    float m, per_bucket;           // buckets for twice a difference
     double octaves;                // 128 log2 e / temperature
-    __device__ __forceinline__ float below(float l) const { return l == m ? 0.f : l - m; }
+    // Half of how far it lies above the largest: the whole may be beyond fp32.
+    __device__ __forceinline__ float below(float l) const { return l == m ? 0.f : __builtin_fmaf(0.5f, l, -0.5f * m); }
     __device__ __forceinline__ int bucket(float l) const {   // kBuckets and more: no weight
         const float b = -below(l) * per_bucket;
         return b < (float)kBuckets ? (int)b : kBuckets;
     }
     // Bounds of the logits of buckets lo .. hi, 2^-18 of them and of m wider than the roundings of `bucket` ask for.
     __device__ __forceinline__ void range(int lo, int hi, float& from, float& to) const {
-        const double step = 1. / (double)per_bucket, slack = fabs((double)m) * 0x1p-18;
+        const double step = 2. / (double)per_bucket, slack = fabs((double)m) * 0x1p-18;
         from = per_bucket > 0.f ? (float)((double)m - (double)(hi + 1) * step * (1. + 0x1p-18) - slack) : -INFINITY;
         to = per_bucket > 0.f && lo > 0 ? (float)((double)m - (double)lo * step * (1. - 0x1p-18) + slack) : INFINITY;
         if (fabsf(m) == INFINITY) from = m;
@@ -207,7 +208,7 @@ struct SampleScale {
         return l == m ? 0. : ((double)l - (double)m) * octaves;
     }
     static __device__ __forceinline__ bool in_play(double y) { return y >= -128. * kOctaves; }
-    // 0 below the buckets' range.  (A bucket may hold such logits: per_bucket ends at 3e38, so those closer than 7e-36 to the
+    // 0 below the buckets' range.  (A bucket may hold such logits: per_bucket ends at 3e38, so those closer than 1.4e-35 to the
     // largest are in one however small the temperature, and `power` has no value for their exponents.)
     static __device__ __forceinline__ uint64_t weight(double y, const double* table) {
         return rounded(power(fmax(y, -128. * (kOctaves + 1.)), table));
@@ -353,7 +354,7 @@ struct SampleRule {
         y_min = min_p > 0.f ? 128. * (log2((double)min_p) - M_LOG2E * 0x1p-54) : -INFINITY;   // what 64 bits round to min_p reaches it
         fine_all = p.V <= kFineTokens ? kFineFew : kFineMany;
         sc.octaves = 128. * M_LOG2E / (double)temperature;
-        sc.per_bucket = fminf((float)(sc.octaves * (kBuckets / (128. * kOctaves))), 3e38f);
+        sc.per_bucket = (float)fmin(sc.octaves * (kBuckets / (64. * kOctaves)), 3e38);
     }
     // The three questions that a row's token takes: what top-k keeps, what top-p keeps of that, and where u falls.  What
     // min-p leaves is a beginning of the order too: `above`, its weight.  ask(query, last) answers.

@@ -383,10 +383,23 @@ def test_smallest_logits_and_temperatures(dtype, V):
     x[2] = torch.where(torch.arange(V) % 3 == 0, 0.0, -unit)
     x[3, ::2] = -math.inf
     x[4] = torch.rand(V, generator=torch.Generator().manual_seed(V)).double() * 1e-36
-    x[5] = torch.where(torch.arange(V) % 3 == 0, 0.0, -4e-39)   # the second bucket, of one value
+    x[5] = torch.where(torch.arange(V) % 3 == 0, 0.0, -8e-39)   # a bucket of one value
     y = x.to(dtype)
     if dtype is BF:
         assert torch.equal(y[:4].double(), x[:4])
     u = torch.tensor([0.95, 0.5, 0.999, 0.3, 0.97, 0.999])
-    for r in ({"t": 7e-40}, {"t": 2.0 ** -149}, {"t": 1e-44, "k": 3}, {"t": 1e-40}, {"t": 2e-41, "p": 0.9}, {"t": 1e-38, "mp": 0.5}, {"t": 5e-37, "k": V}):
+    for r in ({"t": 1.4e-39}, {"t": 7e-40}, {"t": 2.0 ** -149}, {"t": 1e-44, "k": 3}, {"t": 1e-40}, {"t": 2e-41, "p": 0.9}, {"t": 1e-38, "mp": 0.5}, {"t": 5e-37, "k": V}):
         _check(y, u, what=str(r), **r)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [400, 3000, 60000])   # of fp32: by one workgroup, in parts
+def test_differences_beyond_the_largest_number(dtype, V):
+    """Logits of both ends of the type: their difference has no fp32 value, its quotient by a large temperature has."""
+    g = torch.Generator().manual_seed(V)
+    x = ((torch.rand(4, V, generator=g) * 2 - 1) * 3.3e38).to(dtype)
+    x[1] = torch.where(torch.rand(V, generator=g) < 0.5, -3.3e38, 3.3e38).to(dtype)
+    x[2, ::3] = -math.inf
+    x[3] = torch.finfo(dtype).min
+    x[3, V // 2] = torch.finfo(dtype).max
+    u = torch.tensor([0.95, 0.9, 0.99, 0.999])
+    for r in ({"t": 1e38}, {"t": 3e37, "p": 0.99}, {"t": 2e38, "k": V - 5}, {"t": 3e38, "mp": 0.2}, {"t": math.inf}, {"t": 1.0}):
+        _check(x, u, what=str(r), **r)
