@@ -827,9 +827,9 @@ int sf_kv4_keep(const sf_kv4_cache* cache, const int32_t* nodes, int32_t n, cons
  * held to 2^-44 of the largest.  In falling order of logits, ties by index: the
  * first top_k tokens (0 or less: all); of these the fewest whose weights reach
  * top_p of their sum (1 or more: all; one at least); of these the ones of at
- * least min_p times the largest weight (0: all).  The token is the first whose
- * running weight exceeds u times the sum of what is left, logprob the logarithm of
- * its share of that sum (near 0 to 1.02e-6 of itself, of which 2^-20 is that
+ * least min_p times the largest weight (0: all; one at least).  The token is the
+ * first whose running weight exceeds u times the sum of what is left, logprob the
+ * logarithm of its share of that sum (near 0 to 1.02e-6 of itself, of which 2^-20 is that
  * weights are held to 2^-44, and V 2^-70, for fp32 rows with top_k V 2^-46: they
  * do not tell apart what is below).  temperature 0 or less: the first in order,
  * the lowest index of the largest logits.

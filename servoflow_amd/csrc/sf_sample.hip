@@ -1130,6 +1130,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_16_kernel(const SampleA
         __syncthreads();
         index = s.token;
     } else {
+        __syncthreads();   // the waves' sums are read: sample_nth's memory is theirs, too
         index = sample_nth(shared.nth, x, sample_key(value(hit.key)), hit.rank);
     }
     if (t == 0) {

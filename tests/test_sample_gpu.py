@@ -403,3 +403,19 @@ def test_differences_beyond_the_largest_number(dtype, V):
     u = torch.tensor([0.95, 0.9, 0.99, 0.999])
     for r in ({"t": 1e38}, {"t": 3e37, "p": 0.99}, {"t": 2e38, "k": V - 5}, {"t": 3e38, "mp": 0.2}, {"t": math.inf}, {"t": 1.0}):
         _check(x, u, what=str(r), **r)
+
+
+@pytest.mark.parametrize("V", [1500, 70000, 200001])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_one_of_many_largest(dtype, V):
+    """A min-p above 1 leaves the first of thousands of equals, whose logprob is 0: nothing else weighs; beside lower ones, few and
+    many, and as the whole row."""
+    x = torch.full((4, V), 2.5, dtype=dtype)
+    x[1, :7] = -3.0
+    x[2, ::5] = 1.0
+    x[3, :V // 2] = -math.inf
+    first = [0, 7, 1, V // 2]
+    for u in (0.0, 0.4, 1 - 2.0 ** -24):
+        for r in ({"min_p": 2.0}, {"min_p": 1.5, "top_k": V - 1}, {"min_p": 3.0, "top_p": 0.9}):
+            tok, lp = kernels.sample(x.to(DEV), torch.full((4,), u, device=DEV), **r)
+            assert tok.tolist() == first and (lp == 0).all(), (u, r, tok, lp)
