@@ -520,7 +520,10 @@ __device__ __forceinline__ void sample_by_buckets(const SampleArgs& p, SampleSha
         });
         __syncthreads();
         const uint32_t n = s.lo;   // a few of the buckets beside them among them: they belong to no part
-        if (n > kSampleList) return n;
+        if (n > kSampleList) {
+            __syncthreads();   // s.lo is read: the parts of its keys begin with it
+            return n;
+        }
         for (uint32_t i = t; i < n; i += kSampleThreads) {
             const float l = sample_value(~(uint32_t)(s.list.token[i] >> 32));
             const int b = sc.bucket(l);
