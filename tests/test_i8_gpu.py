@@ -250,3 +250,26 @@ def test_no_rows_and_refusals():
         kernels.gemm_i8(x, w, t, out=torch.zeros(2, 8, dtype=BF, device=DEV), accumulate=True)
     with pytest.raises(abi.SfError):
         kernels.quant_i8(torch.zeros(2, 24, device=DEV))
+
+
+@pytest.mark.parametrize("M", [3, 16, 40, 300])
+@pytest.mark.parametrize("as_codes", [False, True])
+def test_rows_of_the_largest_numbers(M, as_codes):
+    """A row's sums times its scale have no fp32 value where the outputs have one; beside rows of 1 and of the smallest."""
+    N, K = 130, 256
+    x = torch.randn(M, K, generator=_gen(M))
+    big = torch.tensor([1e36, 1.0, 3e38, 1e-36, 3e19, 5e18])[torch.arange(M) % 6]
+    x = x / x.abs().amax(1, keepdim=True) * big[:, None]
+    x[2, 1:] = 0.97 * x[2, 0].abs().clamp_min(1e38)   # sums of 2^22 and more
+    w, t = _codes(K, N, K), _scales(3, N) * 1e-3
+    w[3:7] = 127
+    codes, s = quant(x)
+    assert ((codes.abs() @ w.abs().double().t()).amax() * float(s.max())) > 3.4e38
+    a = (kernels.quant_i8(x.to(DEV))) if as_codes else (x.to(DEV), None)
+    out = kernels.gemm_i8(a[0], w.to(DEV), t.to(DEV), a[1], out_dtype=F32)
+    y = (codes @ w.double().t()) * s.double()[:, None] * t.double()
+    fits = y.abs() < 3.3e38
+    assert fits.any(1).all()
+    y, got = torch.where(fits, y, 0.0), torch.where(fits, out.cpu().double(), 0.0)
+    assert torch.isfinite(got).all()
+    assert ((got - y).abs() <= 5 * 2.0 ** -24 * y.abs() + 2.0 ** -149).all()
