@@ -322,3 +322,80 @@ def test_beyond_32_bits():
     from _drafts import attend_see, tree_sees
     ref = attend_see(q.cpu(), kk.cpu(), vv.cpu(), tree_sees([tree.parents[0].cpu()], n, n, [n] * B))
     assert float((got.cpu().double() - ref).abs().max()) <= 1e-4 * float(vv.abs().max())
+
+
+def test_step_logits_in_64_bits():
+    """Each stage of a verified step, both layers to the logits, from what went into it: norms, 8-bit products, rotated queries, what
+    is cached, attention by the ancestors' mask over the cached values, the residual sum.  The kernels give the same in the step
+    itself, bit for bit.  A norm takes sums of 256 squares, 16 roundings at most; products, rotation and attention: the
+    tolerances of their own tests."""
+    from _drafts import attend_see, quant, tree_sees
+    from _quant4 import half_step, rotate
+    B, S0, T = 2, 40, 24
+    dec = Decoder(B, 128)
+    dec.prompt(torch.randint(0, 1000, (B, S0), generator=torch.Generator().manual_seed(9), dtype=torch.int32).to(DEV))
+    lengths = _int([S0, S0 - 13])
+    parents = torch.stack([random_parents(T, 3 + b) for b in range(B)])
+    assert all(len(set(p.tolist())) < T - 1 for p in parents)   # branches
+    tree = draft_tree(_int(parents))
+    drafted = torch.randint(0, 1000, (B, T), generator=torch.Generator().manual_seed(1), dtype=torch.int32).to(DEV)
+    slots = lengths[:, None] + torch.arange(T, dtype=torch.int32, device=DEV)
+    positions, valid = lengths[:, None] + tree.depth, lengths + T
+    pos, freq = positions.cpu(), dec.freq.cpu()
+    see = tree_sees(list(parents), T, 128, valid.tolist())
+    Hq, H, D = dec.Hq, dec.H, dec.D
+
+    def near(got, ref, tol, what):
+        err = (got.cpu().double() - ref).abs()
+        assert (err <= tol).all(), f"{what}: {float((err / tol.clamp_min(1e-300)).max())} of the tolerance"
+
+    def normed(x, what):
+        h = kernels.rmsnorm(x, dec.ones)
+        y = x.cpu().double()
+        ref = y / torch.sqrt(y.square().mean(1, keepdim=True) + 1e-6)
+        near(h, ref, (2.0 ** -20 + half_step(BF)) * ref.abs(), what)
+        return h
+
+    def product(rows, w, t):
+        codes, s = quant(rows.cpu())
+        ref = (codes @ w.cpu().double().t()) * s.double()[:, None] * t.cpu().double()
+        return ref, 6 * 2.0 ** -24 * ref.abs()
+
+    x = dec.embed[drafted.reshape(-1).long()].clone()
+    for n, (qkv, out, cache) in enumerate(dec.layers):
+        h = normed(x, f"layer {n}: norm")
+        p = kernels.gemm_i8(h, *qkv)
+        ref, tol = product(h, *qkv)
+        near(p, ref, tol + half_step(BF) * (ref.abs() + tol), f"layer {n}: qkv")
+        q, _, _ = kernels.heads_rope(p, T, (Hq, H, H), D, positions=positions, inv_freq=dec.freq, cache=cache, slots=slots)
+        heads = p.cpu().double().reshape(B, T, Hq + 2 * H, D).transpose(1, 2)
+        ref = rotate(heads[:, :Hq], pos, freq, False)
+        turn = 40 * 2.0 ** -24 * 2 * heads.abs().amax(-1, keepdim=True)
+        near(q, ref, turn[:, :Hq] + half_step(BF) * ref.abs(), f"layer {n}: queries")
+        k, v = (t.cpu() for t in cache.read(dtype=F32))
+        for cached, new, what in ((k, rotate(heads[:, Hq:Hq + H], pos, freq, False), "keys"), (v, heads[:, Hq + H:], "values")):
+            got = torch.stack([cached[b, :, lengths[b]:lengths[b] + T] for b in range(B)])
+            top = new.abs().amax(-1, keepdim=True)
+            half = (new.amax(-1, keepdim=True) - new.amin(-1, keepdim=True)) / 2 + 2.0 ** -8 * top   # furthest from the middle, in bf16
+            near(got, new, half * (1 + 2.0 ** -7) / 16 + 2.0 ** -16 * top, f"layer {n}: cached {what}")   # half a step; |value - new|
+        a = torch.empty(B, T, Hq, D, dtype=BF, device=DEV)
+        attention_kv4(q, cache, out=a.transpose(1, 2), valid_len=valid, tree=tree)
+        seen = [slice(0, int(m)) for m in valid]
+        for b in range(B):   # (what no one has written yet reads as NaN)
+            kb, vb = k[b:b + 1, :, seen[b]], v[b:b + 1, :, seen[b]]
+            qb = q[b:b + 1].cpu()
+            ref = attend_see(qb, kb, vb, see[b:b + 1, :, seen[b]])
+            dx = 24 * 2.0 ** -24 / 8 * float(qb.double().abs().sum(-1).max()) * float(kb.abs().max()) * 6
+            rel = 2 * (dx + 2.0 ** -22) + 2.0 ** -16 + (32 + 128 / 32) * 2.0 ** -24 * 16
+            near(a[b:b + 1].transpose(1, 2), ref, rel * float(vb.abs().max()) + half_step(BF) * ref.abs(), f"layer {n}: attention {b}")
+        was = x.cpu().double()
+        rows = a.reshape(B * T, -1)
+        ref, tol = product(rows, *out)
+        kernels.gemm_i8(rows, *out, out=x, accumulate=True)
+        near(x, was + ref, tol + 2.0 ** -24 * (was + ref).abs(), f"layer {n}: sum")
+    h = normed(x, "head: norm")
+    logits = kernels.gemm_i8(h, *dec.head, out_dtype=F32)
+    ref, tol = product(h, *dec.head)
+    near(logits, ref, tol, "logits")
+    again = dec.verify(tree, drafted, lengths, torch.full((B * T,), 0.3, device=DEV))[3]
+    assert torch.equal(again.reshape(B * T, -1), logits)
