@@ -373,7 +373,7 @@ struct SampleRule {
                 if (!with_p || first_k >= all) continue;
                 q.count = first_k;
             } else if (step == 1) {
-                if (!with_p && first_k >= all) continue;
+                if (!with_p && first_k >= all && k != 1) continue;   // (the first alone has it all, whatever lies below the buckets)
                 q.count = first_k;
                 if (with_p) q.mass = (double)top_p * (double)kept;
             } else {

@@ -419,3 +419,16 @@ def test_one_of_many_largest(dtype, V):
         for r in ({"min_p": 2.0}, {"min_p": 1.5, "top_k": V - 1}, {"min_p": 3.0, "top_p": 0.9}):
             tok, lp = kernels.sample(x.to(DEV), torch.full((4,), u, device=DEV), **r)
             assert tok.tolist() == first and (lp == 0).all(), (u, r, tok, lp)
+
+
+@pytest.mark.parametrize("V", [1, 2, 500, 50001])   # of fp32: by one workgroup, in parts
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_the_first_in_order_alone_has_a_logprob_of_0(dtype, V):
+    """Beside others that weigh from e^-60 to e^-1 of it."""
+    x = torch.randn(5, V, generator=torch.Generator().manual_seed(V))
+    for b, gap in enumerate((1.0, 20.0, 33.0, 40.0, 60.0)):
+        x[b, (7 * b + V // 2) % V] = x[b].max() + gap
+    x = x.to(dtype)
+    for r in ({"t": 0.0}, {"k": 1}, {"t": -1.0, "k": 7, "mp": 1e-30}, {"k": 1, "p": 0.5}, {"t": 0.5, "k": 1, "mp": 0.1}):
+        tok, lp = kernels.sample(x.to(DEV), _u(5, V).to(DEV), r.get("t", 1.0), r.get("k", 0), r.get("p", 1.0), r.get("mp", 0.0))
+        assert torch.equal(tok.cpu().long(), x.float().argmax(1)) and (lp == 0).all(), (r, tok, lp)
