@@ -11,10 +11,10 @@
 // read of 16 bytes takes at a time then lie in different banks.  Few rows: see
 // gemm_i8_rows_kernel.
 //
-// What bounds them (us): 4374 x 8192 x 8192 takes 290, 2.02 POP/s, where the loads into
+// What bounds them (us): 4374 x 8192 x 8192 takes 281 to 290, 2.0 to 2.1 POP/s, where the loads into
 // LDS alone take 208, the products with their reads from LDS alone 219 to 227, and a
 // large library product of 8-bit integers runs at 2.4 POP/s (292 for this one); with its
-// quantising, one pass over 72 MB in and 36 out, 297.  67 x 6144 x 2048 takes 10.4
+// quantising, one pass over 72 MB in and 36 out, 296.  67 x 6144 x 2048 takes 10.4
 // with it, 7.8 without: a chain of launch, first operands, stages, join and stores.  1 x 8192
 // x 8192 takes 15.0 from memory, 4.5 TB/s of weights.
 #include <hip/hip_runtime.h>
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void gemm_i8_kernel(const I8Args
 
 // Few rows: MB tiles of 16 rows against NT tiles of 16 columns to a workgroup, whose eight waves deal the inputs, 128 at a
 // time, and join in LDS.  Both operands go straight into registers, DEPTH blocks of inputs ahead; the weights are read once.
-// KIND: of rows that the workgroup quantises itself (as i8_load8; MB 1), -1 for codes.  Up to kFusedCodes inputs in all:
+// KIND: of rows that the workgroup quantises itself (as I8Piece takes it; MB 1), -1 for codes.  Up to kFusedCodes inputs in all:
 // every workgroup does it for itself, while its weights are on their way, and a launch is saved.
 constexpr int kFusedCodes = 8192;
 template <int MB, int NT, int DEPTH, int KIND = -1>

@@ -84,11 +84,11 @@ struct KvAttnArgs {
 // the 32 tokens from key0 on the row of node `node` sees, the nodes' first token at key `at`:
 // two words of its ancestors, shifted.  Only the T / 32 + 1 blocks that hold nodes ask; all before
 // them run as a call without a tree, so the rows cost what they cost there.  us: 16 x 8 heads x 64
-// rows (16 nodes) over 2048..8192 keys of 128 channels 82, of a floor of 19: the pair's vector
+// rows (16 nodes) over 2048..8192 keys of 128 channels 79, of a floor of 19: the pair's vector
 // work, done for two groups of 32 rows that each unpack the block, and the longest sequence, whose
-// workgroups have a CU each (in equal pieces of 4096, 2048, 1024 keys 96, 98 and 115: a workgroup's
+// workgroups have a CU each (in equal pieces of 4096, 2048, 1024 keys 96, 98 and 115, beside 83: a workgroup's
 // start, join and merge cost more than the balance gains); 4 x 32 heads x 64 rows over 1094..4374
-// keys of 64 24, of 5.
+// keys of 64 29, of 5.
 __device__ __forceinline__ uint32_t kv_tree_bits(const KvAttnArgs& p, int b, int node, int key0, int at) {
     const uint32_t* row = p.tree + b * p.tree_stride + (int64_t)node * p.tree_words;
     const int r = key0 - at, w = r >> 5;   // rounded down
@@ -956,7 +956,8 @@ static int kv_column_groups(const sf_attn_kv4_desc* d, int rows, int64_t heads) 
 // with 3; 256 x 67 x 67 9.8 with qt 5, 13.8 with 3.  The (hi, lo) form takes 0.42 us
 // a step, and qt 5 would spill, with three terms qt 4: causal, 12 x 520 rows x 1537
 // keys 16.2 with qt 2, 19.4 with 3, 23 with 4; 16 x 1024 x 2048 26.7 with 4, 35 with
-// 2.  128 channels: 2 tiles are what fits.
+// 2.  128 channels: 2 tiles are what fits; a step of theirs takes about half as long again as `step` (16 x 8 heads of 64
+// rows over up to 8192 keys: 52 by this, 79 measured), which only the splits of few workgroups go by.
 static void kv_tiles(const sf_attn_kv4_desc* d, int64_t R, int64_t heads, KvPlan& k) {
     const bool wide = d->cache.D == 128;
     const int most = wide ? 2 : k.form == kKvExact ? 3 : k.form == kKvPair ? 4 : 5;

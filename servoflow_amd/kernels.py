@@ -499,7 +499,7 @@ def gemm_i8(a, w, w_scale, a_scale=None, bias=None, act=abi.SF_ACT_NONE, out=Non
     scale for each row (w_scale, fp32 [N]); a either codes and their scales
     (quant_i8), or fp32, bf16 or fp16 rows, quantised first (workspace: where,
     allocated unless given).  out_dtype a's unless given, bf16 for codes.
-    accumulate adds into an fp32 `out`."""
+    accumulate adds into an fp32 `out`; out must not overlap a."""
     _check(w, "w", (torch.int8,), None, 2)
     dev, (N, K) = w.device, w.shape
     codes = a.dtype is torch.int8
@@ -543,7 +543,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, workspace=
     uniform numbers u (fp32 [rows], in [0, 1)): (tokens int32 [rows], logprobs
     fp32 [rows]).  In falling order of logits, ties by index: the first top_k
     (0: all), of these the fewest that reach top_p of their weight, of these the
-    ones of at least min_p times the largest; the token is the first whose
+    ones of at least min_p times the largest (one at least); the token is the first whose
     running weight exceeds u times what is left, the logprob that of its share.
     temperature 0: the largest logit.  Each parameter is a number or, for a
     value a row, a tensor (top_k int32, the others fp32); None is its default.  -1
