@@ -226,9 +226,9 @@ __device__ __forceinline__ void i8_store(const I8Args& p, int m, int n, i32x4 ac
     const int64_t at = (int64_t)m * p.ldc + n;
     const int cols = min(4, p.N - n);
     float v[4];
-    // acc is below 2^31: beside a step of 2^64 and more 2^40 of it goes to the other scale, or a sum times the step alone could be
+    // acc is 2^30 at most: beside a step of 2^96 and more 2^30 of it goes to the other scale, or a sum times the step alone could be
     // beyond fp32.
-    const float up = s >= 0x1p64f ? 0x1p40f : 1.f, low = s >= 0x1p64f ? s * 0x1p-40f : s;
+    const float up = s >= 0x1p96f ? 0x1p30f : 1.f, low = s >= 0x1p96f ? s * 0x1p-30f : s;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (float)acc[i] * low * (c4.scale[i] * up) + c4.bias[i];
     if (p.act) {

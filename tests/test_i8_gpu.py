@@ -273,3 +273,16 @@ def test_rows_of_the_largest_numbers(M, as_codes):
     y, got = torch.where(fits, y, 0.0), torch.where(fits, out.cpu().double(), 0.0)
     assert torch.isfinite(got).all()
     assert ((got - y).abs() <= 5 * 2.0 ** -24 * y.abs() + 2.0 ** -149).all()
+
+
+def test_a_sum_of_0_beside_large_scales():
+    """A row of the largest step and a column of a large one: their zeros stay zeros, the bias stays."""
+    M, N, K = 20, 40, 64
+    x = torch.zeros(M, K)
+    x[:, 0] = 3e38
+    w = torch.zeros(N, K, dtype=torch.int8)
+    w[:, 1:] = 5
+    t, bias = torch.full((N,), 1e29), torch.arange(N).float()
+    for rows in (3, M):
+        out = kernels.gemm_i8(x[:rows].to(DEV), w.to(DEV), t.to(DEV), bias=bias.to(DEV), out_dtype=F32)
+        assert torch.equal(out.cpu(), bias.expand(rows, N))
