@@ -301,3 +301,17 @@ def test_keep_any_order_holes_and_places_outside():
     far = _int([2 ** 31 - 1, -2 ** 31, 2 ** 31 - 6, 60])
     c.keep(nodes.to(DEV), far)
     assert all(torch.equal(a.cpu(), b) for a, b in zip(c.read(dtype=F32), (wk, wv)))
+
+
+@pytest.mark.parametrize("D,Hq,H,T,splits", [(128, 32, 8, 8, 0), (128, 8, 2, 16, 5), (64, 8, 8, 64, 0), (64, 16, 4, 3, 7)])
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+def test_runs_are_equal(D, Hq, H, T, splits, out_dtype):
+    """Bit for bit, with other work and other memory between them."""
+    B, Sk = 3, 1500
+    c, _, _ = _filled(B, H, Sk, D, BF, 3)
+    q = _randn(4, B, Hq, T, D, dtype=BF).to(DEV)
+    tree, valid = draft_tree(_int(random_parents(T, 5))), _int([Sk, Sk // 2, T])
+    first = attention_kv4(q, c, valid_len=valid, tree=tree, num_splits=splits, out_dtype=out_dtype)
+    for i in range(6):
+        torch.full((1 << 22,), float(i), device=DEV)
+        assert torch.equal(attention_kv4(q, c, valid_len=valid, tree=tree, num_splits=splits, out_dtype=out_dtype), first)
